@@ -27,6 +27,8 @@ Q4_1_BLOCK = 20
 DOWN_Q4_0, DOWN_Q4_1 = 0, 1     # MOE_DOWN_Q4_0 / MOE_DOWN_Q4_1
 PATH_AUTO, PATH_STREAM, PATH_MFMA = 0, 1, 2
 TYPE_Q4_0, TYPE_Q4_1 = 2, 3     # MOE_TYPE_Q4_0 / MOE_TYPE_Q4_1 (the reference's TensorType ids)
+F32, BF16, F16 = 0, 1, 2        # MOE_F32 / MOE_BF16 / MOE_F16
+E4M3_GROUP = 128                # elements per scale of an e4m3 row
 STAGE_PREPARE, STAGE_GATE_UP, STAGE_DOWN, STAGE_FOLD = 0, 1, 2, 3
 
 
@@ -51,6 +53,7 @@ class ExpertTiming(ctypes.Structure):
 _lib = None
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
 
 
 def library():
@@ -94,6 +97,12 @@ def library():
         lib.moe_linear_forward_q8.argtypes = [_P, _P, _I, _P, _P]
         lib.moe_linear_apply.argtypes = [_P, _P, _I, _P, _P, _P]
         lib.moe_linear_apply_noalloc.argtypes = [_P, _P, _I, _P, _P, _P]
+        lib.moe_quantize_e4m3.argtypes = [_P, _I, _L, _I, _I, _P, _P, _P, _P]
+        lib.moe_fp8_linear_create.argtypes = [_I, _I, _I, _P, _P, _I, _I, ctypes.POINTER(_P)]
+        lib.moe_fp8_linear_destroy.argtypes = [_P]
+        lib.moe_fp8_linear_bytes.argtypes = [_P, ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_fp8_linear_forward.argtypes = [_P, _P, _P, _I, _P, _I, _L, _P]
+        lib.moe_fp8_linear_apply.argtypes = [_P, _P, _I, _L, _I, _P, _I, _L, _P, _P]
         _lib = lib
     return _lib
 
@@ -146,6 +155,49 @@ def _stream(stream):
     import torch
     s = stream if stream is not None else torch.cuda.current_stream()
     return ctypes.c_void_p(s.cuda_stream)
+
+
+def _on_device(device):
+    """Context in which `device` is current, for the calls without a handle."""
+    import torch
+    return torch.cuda.device(device)
+
+
+def _stream_on(stream, device):
+    """The stream handle of a call on tensors of `device`: its current stream
+    when none is given."""
+    import torch
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    return ctypes.c_void_p(s.cuda_stream)
+
+
+def _elem_type(t, name):
+    import torch
+    types = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch tensor")
+    if t.dtype not in types:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return types[t.dtype]
+
+
+def _need_rows(t, name, shape, device=None, dtypes=None):
+    """Check a matrix whose rows may be further apart than they are long (a
+    slice of a wider one): element type, exact shape, unit stride within a row
+    and rows that do not run into each other.  Returns (type id, row stride)."""
+    type_ = _elem_type(t, name)
+    if dtypes is not None and t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {dtypes}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have consecutive elements within a row")
+    stride = t.stride(0) if t.shape[0] > 1 else max(t.shape[1], t.stride(0))
+    if stride < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap (stride {stride} < {t.shape[1]})")
+    if t.device.type != "cuda" or (device is not None and t.device != device):
+        raise ValueError(f"{name} must be on {device if device is not None else 'a GPU'}, got {t.device}")
+    return type_, stride
 
 
 def expert_bytes(hidden, intermediate, down_type=DOWN_Q4_0):
@@ -522,6 +574,149 @@ class MoeLinear:
         _need(error, "error", torch.int32, (1,), dev)
         _check(library().moe_linear_apply_noalloc(self.handle, _ptr(x), n, _ptr(y), _ptr(error), _stream(stream)),
                "moe_linear_apply_noalloc")
+        return y, error
+
+
+def _e4m3(t, name, shape, device=None):
+    """Check e4m3 codes: torch.float8_e4m3fn or uint8, contiguous."""
+    import torch
+    if isinstance(t, torch.Tensor) and t.dtype == torch.uint8:
+        return _need(t, name, torch.uint8, shape, device)
+    return _need(t, name, torch.float8_e4m3fn, shape, device)
+
+
+def _blocks(n):
+    return (n + E4M3_GROUP - 1) // E4M3_GROUP
+
+
+def _e4m3_matrix(codes, scales, rows, cols, name):
+    """(code pointer, scale pointer, on device, kept alive) of a matrix given
+    as torch tensors on a GPU or as numpy arrays."""
+    import torch
+    if isinstance(codes, np.ndarray):
+        c, s = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+        if c.dtype != np.uint8 or s.dtype != np.float32:
+            raise TypeError(f"{name}: numpy codes are uint8 and scales float32, got {c.dtype} and {s.dtype}")
+        if c.shape != (rows, cols) or s.shape != (_blocks(rows), _blocks(cols)):
+            raise ValueError(f"{name}: expected codes {(rows, cols)} and scales {(_blocks(rows), _blocks(cols))}, "
+                             f"got {c.shape} and {s.shape}")
+        return ctypes.c_void_p(c.ctypes.data), ctypes.c_void_p(s.ctypes.data), 0, (c, s)
+    _e4m3(codes, f"{name} codes", (rows, cols))
+    _need(scales, f"{name} scales", torch.float32, (_blocks(rows), _blocks(cols)), codes.device)
+    return _ptr(codes), _ptr(scales), 1, (codes, scales)
+
+
+def quantize_e4m3(x, codes=None, scales=None, error=None, stream=None):
+    """Rows x [n][width] (float32, bfloat16 or float16; rows may be strided)
+    -> (codes float8_e4m3fn [n][width], scales float32 [n][ceil(width/128)],
+    error)."""
+    import torch
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a two-dimensional torch tensor")
+    n, width = x.shape
+    type_, stride = _need_rows(x, "x", (n, width))
+    if codes is None:
+        codes = torch.empty((n, width), dtype=torch.float8_e4m3fn, device=x.device)
+    if scales is None:
+        scales = torch.empty((n, _blocks(width)), dtype=torch.float32, device=x.device)
+    _e4m3(codes, "codes", (n, width), x.device)
+    _need(scales, "scales", torch.float32, (n, _blocks(width)), x.device)
+    if error is None:
+        error = torch.zeros(1, dtype=torch.int32, device=x.device)
+    _need(error, "error", torch.int32, (1,), x.device)
+    with _on_device(x.device):
+        _check(library().moe_quantize_e4m3(_ptr(x), type_, stride, width, n, _ptr(codes), _ptr(scales), _ptr(error),
+                                           _stream_on(stream, x.device)), "moe_quantize_e4m3")
+    return codes, scales, error
+
+
+class MoeFp8Linear:
+    """One resident e4m3 matrix [output][input] with a scale per block of 128 x
+    128 (moe_fp8_linear_create): codes float8_e4m3fn (or uint8) and scales
+    float32 [ceil(output/128)][ceil(input/128)], both torch tensors on a GPU
+    or both numpy arrays.  forward takes e4m3 rows, apply rows of float32,
+    bfloat16 or float16."""
+
+    def __init__(self, input, output, codes, scales, max_columns=0, device=0):
+        import torch
+        self.K, self.M, self.max_columns, self.device = input, output, max_columns, device
+        c, s, on_device, keep = _e4m3_matrix(codes, scales, output, input, "weights")
+        if on_device and keep[0].device != torch.device("cuda", device):
+            raise ValueError(f"weights must be on cuda:{device}, got {keep[0].device}")
+        handle = ctypes.c_void_p()
+        _check(library().moe_fp8_linear_create(input, output, max_columns, c, s, on_device, device,
+                                               ctypes.byref(handle)), "moe_fp8_linear_create")
+        self.handle = handle
+
+    def close(self):
+        if getattr(self, "handle", None):
+            library().moe_fp8_linear_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def weight_bytes(self):
+        n = ctypes.c_size_t()
+        _check(library().moe_fp8_linear_bytes(self.handle, ctypes.byref(n)), "moe_fp8_linear_bytes")
+        return n.value
+
+    def bind_forward(self, x_codes, x_scales, y, stream=None):
+        """Validate the tensors of a forward() once and return a no-argument
+        callable that enqueues it with no per-call checks; the tensors must
+        stay alive and keep their shapes while the callable is used."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x_codes.shape[0]
+        _e4m3(x_codes, "x_codes", (n, self.K), dev)
+        _need(x_scales, "x_scales", torch.float32, (n, _blocks(self.K)), dev)
+        type_, stride = _need_rows(y, "y", (n, self.M), dev)
+        fn, handle = library().moe_fp8_linear_forward, self.handle
+        args = (_ptr(x_codes), _ptr(x_scales), n, _ptr(y), type_, stride, _stream_on(stream, dev))
+
+        def call():
+            st = fn(handle, *args)
+            if st != 0:
+                raise MoeError("moe_fp8_linear_forward", st)
+        return call
+
+    def forward(self, x_codes, x_scales, y=None, dtype=None, stream=None):
+        """y [n][output] (given, or a new tensor of `dtype`, float32 unless
+        said) from e4m3 rows."""
+        import torch
+        if y is None:
+            y = torch.empty((x_codes.shape[0], self.M), dtype=dtype or torch.float32, device=x_codes.device)
+        self.bind_forward(x_codes, x_scales, y, stream)()
+        return y
+
+    def bind_apply(self, x, y, error, stream=None):
+        """bind_forward's counterpart for apply()."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x.shape[0]
+        x_type, x_stride = _need_rows(x, "x", (n, self.K), dev)
+        y_type, y_stride = _need_rows(y, "y", (n, self.M), dev)
+        _need(error, "error", torch.int32, (1,), dev)
+        fn, handle = library().moe_fp8_linear_apply, self.handle
+        args = (_ptr(x), x_type, x_stride, n, _ptr(y), y_type, y_stride, _ptr(error), _stream_on(stream, dev))
+
+        def call():
+            st = fn(handle, *args)
+            if st != 0:
+                raise MoeError("moe_fp8_linear_apply", st)
+        return call
+
+    def apply(self, x, y=None, error=None, dtype=None, stream=None):
+        """(y, error) from rows x [n][input]; y in x's type unless given."""
+        import torch
+        if y is None:
+            y = torch.empty((x.shape[0], self.M), dtype=dtype or x.dtype, device=x.device)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        self.bind_apply(x, y, error, stream)()
         return y, error
 
 

@@ -334,6 +334,66 @@ int moe_linear_apply(moe_linear *linear, const float *x, int columns, float *y, 
 int moe_linear_apply_noalloc(moe_linear *linear, const float *x, int columns, float *y, int *error,
                              void *stream);
 
+/* ------------------------------------------------------------------------
+ * 8-bit floating point: e4m3 values (OCP FP8 E4M3FN: bias 7, at most 448, no
+ * infinities) with one fp32 scale per block, for checkpoints that store their
+ * matrices so.  No counterpart in the reference, whose matrices are Q4.
+ *
+ *   matrix   codes [rows][cols] uint8, scales [ceil(rows/128)][ceil(cols/128)]
+ *            fp32: element (r, c) = e4m3(codes[r][c]) * scales[r/128][c/128]
+ *   rows     (activations) codes [n][width], scales [n][ceil(width/128)]:
+ *            a group x of 128 elements with a = max(|x|max, 2^-100) has the
+ *            scale a / 448 and the codes e4m3(x * (448 / a)), nearest even,
+ *            every operation rounded to fp32
+ * The last block of a row or of the rows may be cut short.
+ * ---------------------------------------------------------------------- */
+
+/* Element types of activations and results. */
+enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_F16 = 2 };
+
+/* x [columns] rows of `width` elements of x_type, x_stride elements apart ->
+ * codes [columns][width], scales [columns][ceil(width/128)].  A group that
+ * holds an infinity or NaN is written as zero codes with scale 0 and sets bit
+ * 1 of `error`.  width 1..16384, columns 1..65536; x, scales and error aligned
+ * to their elements; x_stride >= width.  x may not overlap the outputs. */
+int moe_quantize_e4m3(const void *x, int x_type, int64_t x_stride, int width, int columns, void *codes, float *scales,
+                      int *error, void *stream);
+
+typedef struct moe_fp8_linear moe_fp8_linear;
+
+/* One resident e4m3 matrix [output][input] with its scales, on the host or
+ * (weights_on_device = 1) on `device`; they are copied into the handle's own
+ * layout, so the caller may free them afterwards.  input: multiple of 32,
+ * 32..16384; output 1..262144.  max_columns (0..65536) sizes the workspace of
+ * moe_fp8_linear_apply.  Allocates; waits for the device before it reads the
+ * weights and before it returns. */
+int moe_fp8_linear_create(int input, int output, int max_columns, const void *codes, const float *scales,
+                          int weights_on_device, int device, moe_fp8_linear **out);
+int moe_fp8_linear_destroy(moe_fp8_linear *linear);
+/* Bytes of the codes and scales the handle was created from. */
+int moe_fp8_linear_bytes(const moe_fp8_linear *linear, size_t *weight_bytes);
+
+/* y[n][m] = sum over the matrix row of x * W, for e4m3 rows x_codes
+ * [columns][input] (16-byte aligned) with x_scales; y rows are y_stride
+ * elements of y_type apart.  Each block's sum is multiplied by both scales
+ * into an fp32 sum over the blocks, rounded once to y_type.  The sum within a
+ * block is fp32 when y_type is MOE_F32 or columns <= 64; wider batches with
+ * 16-bit results use the e4m3 matrix instructions, which drop what is more
+ * than about 14 bits below a block's largest product.  columns 1..65536.  No
+ * workspace: calls on one handle may overlap.  The rows between y's columns
+ * and y_stride are left as they are.  NaN codes give NaN results.  Enqueue
+ * only; the handle's device need not be current. */
+int moe_fp8_linear_forward(moe_fp8_linear *linear, const void *x_codes, const float *x_scales, int columns, void *y,
+                           int y_type, int64_t y_stride, void *stream);
+
+/* moe_quantize_e4m3 (same codes, same flags), then forward, with the rows in
+ * the handle's workspace or, for a few columns, in the product's kernel.
+ * columns 1..max_columns.  x and y may overlap: all of x is read before any
+ * of y is written.  Calls on one handle must not overlap (they share the
+ * workspace). */
+int moe_fp8_linear_apply(moe_fp8_linear *linear, const void *x, int x_type, int64_t x_stride, int columns, void *y,
+                         int y_type, int64_t y_stride, int *error, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

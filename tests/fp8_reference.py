@@ -1,0 +1,107 @@
+"""The 8-bit floating point formats and products in 64 bits, for the tests.
+
+Codes and scales are part of the format and are formed as it defines them
+(each operation correctly rounded to fp32); everything after them is float64.
+"""
+import torch
+
+GROUP = 128
+
+
+def e4m3_table():
+    """The value of each code, float64 (OCP E4M3FN: 0x7f and 0xff are NaN)."""
+    c = torch.arange(256)
+    e, m = (c >> 3) & 15, (c & 7).double()
+    v = torch.where(e > 0, (1 + m / 8) * torch.exp2(e.double() - 7), m * 2.0 ** -9)
+    v = torch.where(c >= 128, -v, v)
+    v[0x7f] = v[0xff] = float("nan")
+    return v
+
+
+def codes_to_values(codes):
+    return e4m3_table().to(codes.device)[codes.view(torch.uint8).long()]
+
+
+def blocks(n):
+    return -(-n // GROUP)
+
+
+def spread(scales, dim, size):
+    """A scale per 128 along `dim` -> one per element."""
+    return scales.double().repeat_interleave(GROUP, dim=dim).narrow(dim, 0, size)
+
+
+def matrix(codes, scales):
+    rows, cols = codes.shape
+    return codes_to_values(codes) * spread(spread(scales, 0, rows), 1, cols)
+
+
+def rows(codes, scales):
+    return codes_to_values(codes) * spread(scales, 1, codes.shape[1])
+
+
+def quantise(x):
+    """Finite rows -> (codes uint8, scales float32), nearest even."""
+    n, k = x.shape
+    x = x.float()
+    v = torch.nn.functional.pad(x, (0, blocks(k) * GROUP - k)).view(n, -1, GROUP)
+    a = v.abs().amax(dim=2).clamp_min(2.0 ** -100).double()
+    s, r = (a / 448).float(), (448 / a).float()
+    t = (v * r[..., None]).double()            # one fp32 multiplication
+    e = torch.frexp(t.abs().clamp_min(2.0 ** -20)).exponent.double()
+    step = torch.exp2((e - 4).clamp_min(-9.0))
+    q = (torch.round(t.abs() / step) * step).clamp_max(448.0)
+    mag = torch.searchsorted(e4m3_table()[:0x7f].contiguous().to(x.device), q.contiguous())
+    codes = (mag + 128 * (torch.signbit(t)).long()).to(torch.uint8)
+    return codes.view(n, -1)[:, :k].contiguous(), s
+
+
+def random_matrix(m, k, g, device="cuda"):
+    """Codes of values about N(0, 0.02) and their scales."""
+    codes = (torch.randn((m, k), generator=g, device=device) * 110).clamp(-448, 448).to(torch.float8_e4m3fn)
+    scales = (0.02 / 110) * (0.5 + torch.rand((blocks(m), blocks(k)), generator=g, device=device))
+    return codes, scales
+
+
+def generator(seed, device="cuda"):
+    g = torch.Generator(device=device)
+    g.manual_seed(seed)
+    return g
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def product_bounds(x, w, nb):
+    """(sum of |x w| over K, sum over the blocks of the largest |x w|), per
+    output, for rows x and matrix w in float64."""
+    total = x.abs() @ w.abs().T
+    peak = torch.zeros_like(total)
+    for b in range(nb):
+        xs, ws = x[:, b * GROUP:(b + 1) * GROUP].abs(), w[:, b * GROUP:(b + 1) * GROUP].abs()
+        for n0 in range(0, x.shape[0], 64):
+            part = torch.zeros((min(64, x.shape[0] - n0), w.shape[0]), dtype=torch.float64, device=x.device)
+            for k in range(xs.shape[1]):
+                part = torch.maximum(part, xs[n0:n0 + 64, k, None] * ws[None, :, k])
+            peak[n0:n0 + 64] += part
+    return total, peak
+
+
+def linear_tolerance(x, w, y, dtype, wide):
+    """How far a product may be from y (float64), by arithmetic: within a block
+    the matrix instruction adds 128 products, and the accumulator adds one term
+    per block, each addition off by at most 2^-23 of the sum of magnitudes
+    (truncation included), the two scale products by 2 half steps; then y's own
+    rounding, half a step (fp16: at least half its smallest subnormal).  `wide`: 16-bit
+    results of more than 64 columns come from the e4m3 instruction, in which
+    each of a block's 128 products may lose up to 2^-13 of the largest."""
+    nb = blocks(x.shape[1])
+    if wide and dtype != torch.float32:
+        total, peak = product_bounds(x, w, nb)
+        extra = 128 * 2.0 ** -13 * peak
+    else:
+        total, extra = x.abs() @ w.abs().T, 0.0
+    tol = (128 + nb + 2) * 2.0 ** -23 * total + extra
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    return tol + half_step(dtype) * (y.abs() + tol) + tiny

@@ -1,0 +1,65 @@
+"""The 8-bit floating point and norm entry points refuse bad arguments before
+any HIP call (no GPU here), and the binding refuses tensors that do not fit."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import moe_ffn
+
+F32, BF16 = moe_ffn.F32, moe_ffn.BF16
+
+
+@pytest.fixture()
+def buf():
+    return (ctypes.c_float * 256)()
+
+
+def test_quantise_arguments(buf):
+    q = moe_ffn.library().moe_quantize_e4m3
+    good = [buf, F32, 64, 64, 1, buf, buf, buf, None]
+    for at, bad in ((0, None), (1, 3), (1, -1), (2, 63), (3, 0), (3, 16385), (4, 0), (4, 65537), (5, None), (6, None), (7, None)):
+        args = list(good)
+        args[at] = bad
+        assert q(*args) == 1, (at, bad)
+    odd = ctypes.c_void_p(ctypes.addressof(buf) + 2)
+    assert q(odd, F32, 64, 64, 1, buf, buf, buf, None) == 1      # 4-byte elements on 2 bytes
+    assert q(buf, F32, 64, 64, 1, buf, odd, buf, None) == 1
+    assert q(buf, F32, 64, 64, 1, buf, buf, odd, None) == 1
+    assert q(ctypes.c_void_p(ctypes.addressof(buf) + 1), BF16, 64, 64, 1, buf, buf, buf, None) == 1
+
+
+def test_linear_arguments(buf):
+    lib = moe_ffn.library()
+    h = ctypes.c_void_p(1)
+    for args in ((48, 8, 0), (0, 8, 0), (16416, 8, 0), (64, 0, 0), (64, 262145, 0), (64, 8, -1), (64, 8, 65537)):
+        assert lib.moe_fp8_linear_create(*args, buf, buf, 0, 0, ctypes.byref(h)) == 1, args
+        assert h.value is None   # nothing is left to destroy
+    assert lib.moe_fp8_linear_create(64, 8, 0, None, buf, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_linear_create(64, 8, 0, buf, None, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_linear_create(64, 8, 0, buf, buf, 0, -1, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_linear_create(64, 8, 0, buf, buf, 0, 0, None) == 1
+    assert lib.moe_fp8_linear_forward(None, buf, buf, 1, buf, F32, 8, None) == 1
+    assert lib.moe_fp8_linear_apply(None, buf, F32, 64, 1, buf, F32, 8, buf, None) == 1
+    assert lib.moe_fp8_linear_destroy(None) == 1
+    n = ctypes.c_size_t()
+    assert lib.moe_fp8_linear_bytes(None, ctypes.byref(n)) == 1
+
+
+def test_binding_checks_weights():
+    c, s = np.zeros((130, 256), np.uint8), np.ones((2, 2), np.float32)
+    for codes, scales in ((c[:129], s), (c, s[:1]), (c.T, s)):
+        with pytest.raises(ValueError):
+            moe_ffn.MoeFp8Linear(256, 130, codes, scales)
+    for codes, scales in ((c.astype(np.int8), s), (c, s.astype(np.float64))):
+        with pytest.raises(TypeError):
+            moe_ffn.MoeFp8Linear(256, 130, codes, scales)
+
+
+def test_row_checks():
+    torch = pytest.importorskip("torch")
+    x = torch.zeros((4, 64))
+    for bad, exc in ((x.double(), TypeError), (x[:3], ValueError), (x.t(), ValueError), (x[:1].expand(4, 64), ValueError),
+                     (x, ValueError)):   # the last: on the CPU
+        with pytest.raises(exc):
+            moe_ffn._need_rows(bad, "x", (4, 64))
