@@ -77,10 +77,15 @@ __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ 
 
 hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, hipStream_t s) {
     const int nb = (cols + kFp8Block - 1) / kFp8Block;
-    const size_t chunks = (rows + kFp8TileRows - 1) / kFp8TileRows * nb * (kFp8TileBytes / 16);
-    // Grids of at most 2^30 workgroups: the largest bank has 2^31 chunks.
-    k_fp8_repack<<<dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, s>>>(
-        codes, reinterpret_cast<uint4 *>(tiles), rows, cols, nb, chunks);
+    // A grid holds fewer than 2^32 threads: at most 2^30 chunks a launch.
+    const size_t rows_at_once = (size_t{1} << 30) / (static_cast<size_t>(nb) * kFp8TileBytes / 16) * kFp8TileRows;
+    for (size_t first = 0; first < rows; first += rows_at_once) {
+        const size_t n = std::min(rows_at_once, rows - first);
+        const size_t chunks = (n + kFp8TileRows - 1) / kFp8TileRows * nb * (kFp8TileBytes / 16);
+        k_fp8_repack<<<dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, s>>>(
+            codes + first * cols, reinterpret_cast<uint4 *>(tiles + first / kFp8TileRows * nb * kFp8TileBytes), n, cols, nb,
+            chunks);
+    }
     return hipGetLastError();
 }
 

@@ -44,6 +44,17 @@ class Config(ctypes.Structure):
                 ("down_type", ctypes.c_int)]
 
 
+class Fp8LayerConfig(ctypes.Structure):
+    """moe_fp8_layer_config."""
+    _fields_ = [("hidden", ctypes.c_int), ("intermediate", ctypes.c_int), ("experts", ctypes.c_int),
+                ("top_k", ctypes.c_int), ("has_shared", ctypes.c_int), ("max_tokens", ctypes.c_int)]
+
+
+class Fp8Matrix(ctypes.Structure):
+    """moe_fp8_matrix."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
 class ExpertTiming(ctypes.Structure):
     """moe_expert_timing (ExpertTiming, src/gpu_expert.hpp:6)."""
     _fields_ = [("upload_ms", ctypes.c_double), ("resident_ms", ctypes.c_double),
@@ -103,6 +114,12 @@ def library():
         lib.moe_fp8_linear_bytes.argtypes = [_P, ctypes.POINTER(ctypes.c_size_t)]
         lib.moe_fp8_linear_forward.argtypes = [_P, _P, _P, _I, _P, _I, _L, _P]
         lib.moe_fp8_linear_apply.argtypes = [_P, _P, _I, _L, _I, _P, _I, _L, _P, _P]
+        lib.moe_fp8_layer_memory_bytes.argtypes = [ctypes.POINTER(Fp8LayerConfig), ctypes.POINTER(ctypes.c_size_t),
+                                                   ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_fp8_layer_create.argtypes = [ctypes.POINTER(Fp8LayerConfig), ctypes.POINTER(Fp8Matrix),
+                                             ctypes.POINTER(Fp8Matrix), _I, _I, ctypes.POINTER(_P)]
+        lib.moe_fp8_layer_destroy.argtypes = [_P]
+        lib.moe_fp8_layer_forward.argtypes = [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P]
         _lib = lib
     return _lib
 
@@ -589,20 +606,22 @@ def _blocks(n):
     return (n + E4M3_GROUP - 1) // E4M3_GROUP
 
 
-def _e4m3_matrix(codes, scales, rows, cols, name):
-    """(code pointer, scale pointer, on device, kept alive) of a matrix given
-    as torch tensors on a GPU or as numpy arrays."""
+def _e4m3_matrices(codes, scales, shape, name, device):
+    """(code pointer, scale pointer, on device, kept alive) of e4m3 matrices of
+    `shape` [..][rows][cols], torch tensors on `device` or numpy arrays."""
     import torch
+    shape = tuple(shape)
+    blocks = (*shape[:-2], _blocks(shape[-2]), _blocks(shape[-1]))
     if isinstance(codes, np.ndarray):
         c, s = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
         if c.dtype != np.uint8 or s.dtype != np.float32:
             raise TypeError(f"{name}: numpy codes are uint8 and scales float32, got {c.dtype} and {s.dtype}")
-        if c.shape != (rows, cols) or s.shape != (_blocks(rows), _blocks(cols)):
-            raise ValueError(f"{name}: expected codes {(rows, cols)} and scales {(_blocks(rows), _blocks(cols))}, "
-                             f"got {c.shape} and {s.shape}")
+        if c.shape != shape or s.shape != blocks:
+            raise ValueError(f"{name}: expected codes {shape} and scales {blocks}, got {c.shape} and {s.shape}")
         return ctypes.c_void_p(c.ctypes.data), ctypes.c_void_p(s.ctypes.data), 0, (c, s)
-    _e4m3(codes, f"{name} codes", (rows, cols))
-    _need(scales, f"{name} scales", torch.float32, (_blocks(rows), _blocks(cols)), codes.device)
+    dev = torch.device("cuda", device)
+    _e4m3(codes, f"{name} codes", shape, dev)
+    _need(scales, f"{name} scales", torch.float32, blocks, dev)
     return _ptr(codes), _ptr(scales), 1, (codes, scales)
 
 
@@ -638,11 +657,8 @@ class MoeFp8Linear:
     bfloat16 or float16."""
 
     def __init__(self, input, output, codes, scales, max_columns=0, device=0):
-        import torch
         self.K, self.M, self.max_columns, self.device = input, output, max_columns, device
-        c, s, on_device, keep = _e4m3_matrix(codes, scales, output, input, "weights")
-        if on_device and keep[0].device != torch.device("cuda", device):
-            raise ValueError(f"weights must be on cuda:{device}, got {keep[0].device}")
+        c, s, on_device, _keep = _e4m3_matrices(codes, scales, (output, input), "weights", device)
         handle = ctypes.c_void_p()
         _check(library().moe_fp8_linear_create(input, output, max_columns, c, s, on_device, device,
                                                ctypes.byref(handle)), "moe_fp8_linear_create")
@@ -717,6 +733,83 @@ class MoeFp8Linear:
         if error is None:
             error = torch.zeros(1, dtype=torch.int32, device=x.device)
         self.bind_apply(x, y, error, stream)()
+        return y, error
+
+
+class MoeFp8Layer:
+    """One MoE layer of e4m3 matrices for batches of up to 64 tokens
+    (moe_fp8_layer_create).  gate and up are (codes [E][I][H], scales
+    [E][ceil(I/128)][ceil(H/128)]), down is (codes [E][H][I], scales
+    [E][ceil(H/128)][ceil(I/128)]) and shared, for a layer with a shared
+    expert, its (gate, up, down) of the same without E; all torch tensors on
+    the layer's GPU (float8_e4m3fn or uint8 codes) or all numpy arrays."""
+
+    def __init__(self, hidden, intermediate, experts, top_k, has_shared, max_tokens, gate, up, down, shared=None, device=0):
+        self.cfg = Fp8LayerConfig(hidden, intermediate, experts, top_k, 1 if has_shared else 0, max_tokens)
+        self.H, self.I, self.E, self.k = hidden, intermediate, experts, top_k
+        self.has_shared, self.max_tokens, self.device = bool(has_shared), max_tokens, device
+        if self.has_shared and shared is None:
+            raise ValueError("a layer with a shared expert needs its matrices")
+        gate_up, down_shape = (intermediate, hidden), (hidden, intermediate)
+        parts = [_e4m3_matrices(*m, (experts, *shape), name, device)
+                 for m, shape, name in ((gate, gate_up, "gate"), (up, gate_up, "up"), (down, down_shape, "down"))]
+        if self.has_shared:
+            parts += [_e4m3_matrices(*m, shape, f"shared {name}", device)
+                      for m, shape, name in zip(shared, (gate_up, gate_up, down_shape), ("gate", "up", "down"))]
+        if len({p[2] for p in parts}) != 1:
+            raise ValueError("the matrices must be all torch tensors or all numpy arrays")
+        banks = [(Fp8Matrix * 3)(*[Fp8Matrix(p[0], p[1]) for p in parts[i:i + 3]]) for i in range(0, len(parts), 3)]
+        handle = ctypes.c_void_p()
+        _check(library().moe_fp8_layer_create(ctypes.byref(self.cfg), banks[0], banks[1] if self.has_shared else None,
+                                              parts[0][2], device, ctypes.byref(handle)), "moe_fp8_layer_create")
+        self.handle = handle
+
+    def close(self):
+        if getattr(self, "handle", None):
+            library().moe_fp8_layer_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def bind_forward(self, x, ids, weights, y, error, shared_gate=None, stream=None):
+        """Validate the tensors of a forward() once and return a no-argument
+        callable that enqueues it with no per-call checks (as
+        MoeLayer.bind_forward)."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x.shape[0]
+        if not 1 <= n <= self.max_tokens:
+            raise ValueError(f"tokens {n} outside 1..{self.max_tokens}")
+        type_ = _elem_type(x, "x")
+        _need(x, "x", x.dtype, (n, self.H), dev)
+        _routes_check(ids, weights, n, self.k, dev)
+        if shared_gate is not None:
+            _need(shared_gate, "shared_gate", torch.float32, (n,), dev)
+        _need(y, "y", x.dtype, (n, self.H), dev)
+        _need(error, "error", torch.int32, (1,), dev)
+        fn, handle = library().moe_fp8_layer_forward, self.handle
+        args = (_ptr(x), type_, _ptr(ids), _ptr(weights), n, _ptr(shared_gate), _ptr(y), _ptr(error),
+                _stream_on(stream, dev))
+
+        def call():
+            st = fn(handle, *args)
+            if st != 0:
+                raise MoeError("moe_fp8_layer_forward", st)
+        return call
+
+    def forward(self, x, ids, weights, shared_gate=None, y=None, error=None, stream=None):
+        """(y, error) for x [n][H] of float32, bfloat16 or float16; y has x's
+        type."""
+        import torch
+        if y is None:
+            y = torch.empty_like(x)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        self.bind_forward(x, ids, weights, y, error, shared_gate, stream)()
         return y, error
 
 

@@ -394,6 +394,54 @@ int moe_fp8_linear_forward(moe_fp8_linear *linear, const void *x_codes, const fl
 int moe_fp8_linear_apply(moe_fp8_linear *linear, const void *x, int x_type, int64_t x_stride, int columns, void *y,
                          int y_type, int64_t y_stride, int *error, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A routed-expert layer of e4m3 matrices for a few tokens: moe_ffn_forward's
+ * operator for decode batches of an e4m3 checkpoint, in two launches.
+ * ---------------------------------------------------------------------- */
+
+typedef struct moe_fp8_layer_config {
+    int hidden;        /* H: multiple of 32, 32..16384 */
+    int intermediate;  /* I: multiple of 32, 32..16384 */
+    int experts;       /* E: routed experts, 1..4096 */
+    int top_k;         /* routes per token, 1..32, <= experts */
+    int has_shared;    /* 1: one shared expert, always routed */
+    int max_tokens;    /* capacity of forward(), 1..64 */
+} moe_fp8_layer_config;
+
+/* e4m3 matrices of one kind, one after the other: codes [n][rows][cols],
+ * scales [n][ceil(rows/128)][ceil(cols/128)]. */
+typedef struct moe_fp8_matrix {
+    const void *codes;
+    const float *scales;
+} moe_fp8_matrix;
+
+typedef struct moe_fp8_layer moe_fp8_layer;
+
+/* Device bytes held by a layer (weights, workspace for max_tokens). */
+int moe_fp8_layer_memory_bytes(const moe_fp8_layer_config *config, size_t *weight_bytes, size_t *workspace_bytes);
+
+/* `experts` = gate [E][I][H], up [E][I][H], down [E][H][I]; `shared` = the
+ * shared expert's three matrices (n = 1), NULL when the layer has none.  All
+ * on the host or all on `device`; they are copied into the handle's own
+ * layout.  Allocates; waits for the device before it reads the weights and
+ * before it returns. */
+int moe_fp8_layer_create(const moe_fp8_layer_config *config, const moe_fp8_matrix *experts, const moe_fp8_matrix *shared,
+                         int weights_on_device, int device, moe_fp8_layer **layer);
+int moe_fp8_layer_destroy(moe_fp8_layer *layer);
+
+/* x, y [tokens][H] of `type` (MOE_F32, MOE_BF16, MOE_F16); ids, weights,
+ * shared_gate and the sum as in moe_ffn_forward.  x's rows and the experts'
+ * middle rows SiLU(gate) * up are quantised as moe_quantize_e4m3 does; sums
+ * are fp32, y is rounded once.  Flags in `error` as in moe_ffn_forward:
+ * routes with a bad id or an id of an earlier rank are dropped and set bit 1,
+ * as do a negative or nonfinite weight (which stays in the sum, a nonfinite
+ * one as 0) and nonfinite input, whose group of 128 counts as zeros.  x is
+ * aligned to 16 bytes and may not overlap y.  tokens in 1..max_tokens.
+ * Enqueue only; calls on one layer must not overlap (they share the
+ * workspace).  The layer's device need not be current. */
+int moe_fp8_layer_forward(moe_fp8_layer *layer, const void *x, int type, const int32_t *ids, const float *weights,
+                          int tokens, const float *shared_gate, void *y, int *error, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -105,3 +105,73 @@ def linear_tolerance(x, w, y, dtype, wide):
     tol = (128 + nb + 2) * 2.0 ** -23 * total + extra
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
     return tol + half_step(dtype) * (y.abs() + tol) + tiny
+
+
+def quantise_with_slack(m, slack):
+    """Rows m (float64) as e4m3 values, and how far each may be from what a
+    kernel gives whose m is off by up to `slack`: one step where the scaled
+    value lies within the slack of a rounding boundary, else the slack of the
+    scale alone."""
+    codes, s = quantise(m)
+    v = rows(codes, s)
+    n, k = m.shape
+    pad = lambda t: torch.nn.functional.pad(t, (0, blocks(k) * GROUP - k)).view(n, -1, GROUP)  # noqa: E731
+    a = pad(m.abs()).amax(dim=2).clamp_min(2.0 ** -100)
+    rel = spread(pad(slack).amax(dim=2) / a + 2.0 ** -22, 1, k)      # of the scale
+    sd = spread(s, 1, k)
+    t, dt = m / sd, slack / sd + (m / sd).abs() * rel
+    # The two values next to t: a kernel's code may be any between the
+    # roundings of t - dt and t + dt.
+    r = lambda z: _round(z.clamp(-448, 448))  # noqa: E731
+    spread_ = torch.maximum((r(t + dt) - v / sd).abs(), (r(t - dt) - v / sd).abs())
+    return v, spread_ * sd + v.abs() * rel
+
+
+def _round(t):
+    e = torch.frexp(t.abs().clamp_min(2.0 ** -20)).exponent.double()
+    step = torch.exp2((e - 4).clamp_min(-9.0))
+    return torch.round(t / step) * step
+
+
+def expert(x, gate, up, down):
+    """(output, tolerance) of one expert for rows x (e4m3 values), float64:
+    the tolerance is that of fp32 sums, carried through SiLU(g) u (slope of
+    SiLU at most 1.1) and the rounding of the middle."""
+    g, u = x @ gate.T, x @ up.T
+    dg, du = (linear_tolerance(x, w, y, torch.float32, False) for w, y in ((gate, g), (up, u)))
+    silu = g * torch.sigmoid(g)
+    m = silu * u
+    dm = 1.1 * dg * (u.abs() + du) + silu.abs() * du + 8 * 2.0 ** -24 * m.abs()
+    v, dv = quantise_with_slack(m, dm)
+    y = v @ down.T
+    return y, dv @ down.abs().T + linear_tolerance(v, down, y, torch.float32, False)
+
+
+def layer(x, ids, weights, experts, shared=None, gate=None):
+    """(output, tolerance) of a layer, float64; routes with a bad id or a
+    repeated one are dropped.  experts[e] = (gate, up, down) in float64."""
+    codes, s = quantise(x)
+    q = rows(codes, s)
+    n, k = ids.shape
+    y = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(y)
+    size = torch.zeros_like(y)
+    use = {}
+    for t, row in enumerate(ids.tolist()):
+        for r, e in enumerate(row):
+            if 0 <= e < len(experts) and e not in row[:r]:
+                use.setdefault(e, []).append((t, r))
+    for e, where in use.items():
+        t, r = (torch.tensor(i, device=q.device) for i in zip(*where))
+        out, d = expert(q[t], *experts[e])
+        w = weights[t, r].double()[:, None]
+        y.index_add_(0, t, w * out)
+        tol.index_add_(0, t, w.abs() * d)
+        size.index_add_(0, t, (w * out).abs())
+    if shared is not None:
+        out, d = expert(q, *shared)
+        w = torch.ones(n, device=q.device).double() if gate is None else torch.sigmoid(gate.double())
+        y += w[:, None] * out
+        tol += w[:, None] * (d + 4 * 2.0 ** -24 * out.abs())
+        size += (w[:, None] * out).abs()
+    return y, tol + (k + 3) * 2.0 ** -24 * size

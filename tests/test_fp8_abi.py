@@ -63,3 +63,31 @@ def test_row_checks():
                      (x, ValueError)):   # the last: on the CPU
         with pytest.raises(exc):
             moe_ffn._need_rows(bad, "x", (4, 64))
+
+
+def test_layer_arguments(buf):
+    lib = moe_ffn.library()
+    good = dict(hidden=64, intermediate=32, experts=4, top_k=2, has_shared=1, max_tokens=8)
+    bank = (moe_ffn.Fp8Matrix * 3)(*[moe_ffn.Fp8Matrix(ctypes.addressof(buf), ctypes.addressof(buf))] * 3)
+    h, w, s = ctypes.c_void_p(1), ctypes.c_size_t(), ctypes.c_size_t()
+    cfg = lambda **c: ctypes.byref(moe_ffn.Fp8LayerConfig(*{**good, **c}.values()))  # noqa: E731
+    for bad in (dict(hidden=48), dict(hidden=0), dict(hidden=16416), dict(intermediate=16), dict(intermediate=16416),
+                dict(experts=0), dict(experts=4097), dict(top_k=0), dict(top_k=5), dict(experts=64, top_k=33),
+                dict(has_shared=2), dict(max_tokens=0), dict(max_tokens=65)):
+        assert lib.moe_fp8_layer_create(cfg(**bad), bank, bank, 0, 0, ctypes.byref(h)) == 1, bad
+        assert h.value is None
+        assert lib.moe_fp8_layer_memory_bytes(cfg(**bad), ctypes.byref(w), ctypes.byref(s)) == 1, bad
+    assert lib.moe_fp8_layer_create(None, bank, bank, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_layer_create(cfg(), None, bank, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_layer_create(cfg(), bank, None, 0, 0, ctypes.byref(h)) == 1
+    hole = (moe_ffn.Fp8Matrix * 3)(bank[0], moe_ffn.Fp8Matrix(ctypes.addressof(buf), None), bank[2])
+    assert lib.moe_fp8_layer_create(cfg(), hole, bank, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_layer_create(cfg(), bank, hole, 0, 0, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_layer_create(cfg(), bank, bank, 0, -1, ctypes.byref(h)) == 1
+    assert lib.moe_fp8_layer_destroy(None) == 1
+    assert lib.moe_fp8_layer_forward(None, buf, F32, buf, buf, 1, None, buf, buf, None) == 1
+    assert lib.moe_fp8_layer_memory_bytes(cfg(hidden=2048, intermediate=512, experts=512, top_k=10), ctypes.byref(w),
+                                          ctypes.byref(s)) == 0
+    scales = 513 * 3 * 64 * 4
+    assert 513 * 3 * 2048 * 512 + scales <= w.value < 513 * 3 * 2048 * 512 + scales + 6 * 256
+    assert s.value == 8 * 11 * 512 * 4
