@@ -1,0 +1,343 @@
+// The norms after one block and before the next with the gate, the scales and
+// the residual sum between them (moe_block_norm), one pass over the rows:
+//   b = post_weight ? rms(block) (offset + post_weight) : block
+//   h = residual_scale residual + block_scale gate b
+//   n = rms(h) (offset + pre_weight),   rms(v) = v / sqrt(mean(v^2) + eps)
+// n may be written as values, as Q8_1 rows and as e4m3 rows at once: the
+// router reads values and the experts' products read quantised rows.
+#include "moe_ffn.h"
+#include "moe_fp8.hpp"
+
+#include <algorithm>
+
+namespace moe {
+namespace {
+
+struct NormArgs {
+    const void *residual, *block, *gate;
+    void *residual_out, *out;
+    int64_t residual_stride, block_stride, gate_stride, residual_out_stride, out_stride;
+    const float *post_weight, *pre_weight;
+    uint32_t *q8;
+    uint8_t *codes;
+    float *scales;
+    int *error;
+    float eps, offset, residual_scale, block_scale;
+    int hidden, tokens, gate_form, gate_sigmoid;
+    bool vec;   // every row takes 8-element accesses
+};
+
+template<int T>
+__device__ __forceinline__ void load8_any(const void *p, size_t at, int valid, bool vec, float (&v)[8]) {
+    if (vec) {
+        Raw8 raw{};
+        if (valid > 0) raw = load8_raw<T>(p, at);
+        unpack8<T>(raw, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? load1<T>(p, at + i) : 0.0f;
+    }
+}
+template<int T>
+__device__ __forceinline__ void store8_any(void *p, size_t at, int valid, bool vec, const float (&v)[8]) {
+    if (vec) {
+        if (valid <= 0) return;
+        if constexpr (T == kF32) {
+            float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
+            q[0] = make_float4(v[0], v[1], v[2], v[3]);
+            q[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            const auto pack = [](float a, float b) { return T == kBF16 ? pack_bf16(a, b) : pack_f16(a, b); };
+            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) =
+                make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) store1<T>(p, at + i, v[i]);
+    }
+}
+
+// The sum over the workgroup, by a butterfly in each wave and then in wave
+// order.  Consecutive sums alternate between two slots: a wave writes a slot
+// again only after the barrier of the sum between, which no wave reaches
+// before it has read the slot.
+__device__ __forceinline__ float group_sum(float v, float (*slot)[16], int &which) {
+    v = xor_sum_from<32>(v);
+    const int W = blockDim.x >> 6;
+    if (W == 1) return v;
+    which ^= 1;
+    if ((threadIdx.x & 63) == 0) slot[which][threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = slot[which][0];
+    for (int w = 1; w < W; ++w) s = s + slot[which][w];
+    return s;
+}
+
+// A Q8_1 block from four neighbouring lanes with 8 elements each: the bytes
+// and flags of moe_quantize_q8_1 for the same fp32 row (its pairwise sum is a
+// subtree of the raw sum's XOR butterfly in every lane, combined in order).
+__device__ __forceinline__ void store_q8(uint32_t *q8, size_t block, int part, float (&v)[8], bool in, int &flags) {
+    int bad = 0;
+    float amax = 0.0f, t[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if (!isfinite(v[i])) { bad = 1; v[i] = 0.0f; }
+        amax = fmaxf(amax, fabsf(v[i]));
+        t[i] = v[i];
+    }
+#pragma unroll
+    for (int w = 4; w >= 1; w >>= 1)
+#pragma unroll
+        for (int i = 0; i < w; ++i) t[i] = t[2 * i] + t[2 * i + 1];
+    amax = fmaxf(amax, lane_xor<1>(amax));
+    amax = fmaxf(amax, lane_xor<2>(amax));
+    bad |= lane_xor<1>(bad);
+    bad |= lane_xor<2>(bad);
+    const float sum = xor_sum<2>(xor_sum<1>(t[0])), d = amax / 127.0f;
+    const uint32_t hd = f2h(d), hs = f2h(sum);
+    const bool representable = isfinite(sum) && (hs & 0x7c00u) != 0x7c00u && (hd & 0x7c00u) != 0x7c00u &&
+                               (amax == 0.0f || d > 0.0f);
+    const bool quant = !bad && representable && amax != 0.0f;
+    uint32_t words[2];
+    int bad_code = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        words[w] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const float c = quant ? roundf(v[4 * w + b] / d) : 0.0f;
+            bad_code |= !isfinite(c) || c < -127.0f || c > 127.0f;
+            words[w] |= (static_cast<uint32_t>(static_cast<int>(c)) & 0xffu) << (8 * b);
+        }
+    }
+    bad_code |= lane_xor<1>(bad_code);
+    bad_code |= lane_xor<2>(bad_code);
+    const bool valid = !bad && representable && !bad_code;
+    if (!in) return;
+    uint32_t *out = q8 + block * 9;
+    if (part == 0) out[0] = valid && amax != 0.0f ? hd | (hs << 16) : 0u;
+    out[1 + 2 * part] = valid ? words[0] : 0u;
+    out[2 + 2 * part] = valid ? words[1] : 0u;
+    flags |= (bad ? 1 : 0) | ((representable && !bad_code) ? 0 : 2);
+}
+
+// An e4m3 group from 16 neighbouring lanes, as k_quantize_e4m3 forms it.
+__device__ __forceinline__ void store_e4m3(uint8_t *codes, size_t at, float *scale, int part, const float (&v)[8], int valid,
+                                           bool vec, int &flags) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i]));
+    m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
+    m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
+    m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
+    m = max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
+    const GroupScale g = group_scale(m);
+    uint2 c = make_uint2(pack_e4m3(v[0] * g.r, v[1] * g.r, v[2] * g.r, v[3] * g.r),
+                         pack_e4m3(v[4] * g.r, v[5] * g.r, v[6] * g.r, v[7] * g.r));
+    if (g.bad) c = make_uint2(0u, 0u);
+    if (vec) {
+        if (valid > 0) *reinterpret_cast<uint2 *>(codes + at) = c;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) codes[at + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+    }
+    if (part == 0 && valid > 0) *scale = g.s;
+    if (g.bad) flags |= 1;
+}
+
+// A workgroup per row, 8 NV elements a thread, all of the row in registers.
+// TB: type of block, out and an element gate; TR: of the residual.
+template<int TB, int TR, int NV>
+__global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
+    __shared__ float slots[2][16];
+    const int tid = threadIdx.x, H = a.hidden, nb = (H + kFp8Block - 1) / kFp8Block;
+    const bool vec = a.vec;
+    int col[NV], valid[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        col[j] = (j * static_cast<int>(blockDim.x) + tid) * 8;
+        valid[j] = min(8, H - col[j]);   // <= 0 past the row's end
+    }
+    int flags = 0, which = 0;
+    for (int n = blockIdx.x; n < a.tokens; n += gridDim.x) {
+        float r[NV][8], b[NV][8];
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            load8_any<TR>(a.residual, static_cast<size_t>(n) * a.residual_stride + col[j], valid[j], vec, r[j]);
+            if (a.block) load8_any<TB>(a.block, static_cast<size_t>(n) * a.block_stride + col[j], valid[j], vec, b[j]);
+        }
+        if (a.block) {
+            float g[NV][8];
+            if (a.gate_form == MOE_GATE_TOKEN) {
+                const float v = static_cast<const float *>(a.gate)[n];
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) g[j][i] = v;
+            } else if (a.gate_form == MOE_GATE_CHANNEL) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) load8_any<kF32>(a.gate, col[j], valid[j], vec, g[j]);
+            } else if (a.gate_form == MOE_GATE_ELEMENT) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    load8_any<TB>(a.gate, static_cast<size_t>(n) * a.gate_stride + col[j], valid[j], vec, g[j]);
+            }
+            if (a.post_weight) {
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s = fmaf(b[j][i], b[j][i], s);
+                s = group_sum(s, slots, which);
+                const float scale = 1.0f / sqrtf(s / static_cast<float>(H) + a.eps);
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    float w[8];
+                    load8_any<kF32>(a.post_weight, col[j], valid[j], vec, w);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[j][i] = b[j][i] * scale * (a.offset + w[i]);
+                }
+            }
+            if (a.gate_form != MOE_GATE_NONE) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        b[j][i] = a.gate_sigmoid ? b[j][i] / (1.0f + moe_expf(-g[j][i])) : b[j][i] * g[j][i];
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[j][i] = fmaf(a.residual_scale, r[j][i], a.block_scale * b[j][i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[j][i] = a.residual_scale * r[j][i];
+        }
+        if (a.residual_out) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                store8_any<TR>(a.residual_out, static_cast<size_t>(n) * a.residual_out_stride + col[j], valid[j], vec, r[j]);
+        }
+        if (!a.pre_weight) continue;
+        // The norm takes the sum as it is, not as a 16-bit residual_out rounds it.
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s = fmaf(r[j][i], r[j][i], s);
+        s = group_sum(s, slots, which);
+        const float scale = 1.0f / sqrtf(s / static_cast<float>(H) + a.eps);
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float w[8];
+            load8_any<kF32>(a.pre_weight, col[j], valid[j], vec, w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[j][i] = r[j][i] * scale * (a.offset + w[i]);
+            if (a.out) store8_any<TB>(a.out, static_cast<size_t>(n) * a.out_stride + col[j], valid[j], vec, r[j]);
+            if (a.codes) {
+                if (valid[j] < 8) {   // 0 weights past the end would leave NaN of a NaN row there
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i >= valid[j]) r[j][i] = 0.0f;
+                }
+                store_e4m3(a.codes, static_cast<size_t>(n) * H + col[j], a.scales + static_cast<size_t>(n) * nb + col[j] / kFp8Block,
+                           tid & 15, r[j], valid[j], vec, flags);
+            }
+            if (a.q8) store_q8(a.q8, static_cast<size_t>(n) * (H / 32) + col[j] / 32, tid & 3, r[j], valid[j] > 0, flags);
+        }
+    }
+    if (flags) atomicOr(a.error, flags);
+}
+
+template<int TB, int TR>
+hipError_t launch_norm(const NormArgs &a, hipStream_t s) {
+    const int nv = a.hidden > 8192 ? 2 : 1, waves = (a.hidden + 512 * nv - 1) / (512 * nv);
+    const dim3 grid(std::min(a.tokens, 256 * std::max(1, 16 / waves))), block(64 * waves);
+    if (nv == 1) k_block_norm<TB, TR, 1><<<grid, block, 0, s>>>(a);
+    else k_block_norm<TB, TR, 2><<<grid, block, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+bool aligned(const void *p, size_t n) { return p && reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+}  // namespace moe
+
+extern "C" int moe_block_norm(const moe_block_norm_args *p, void *stream) {
+    constexpr int kInvalid = hipErrorInvalidValue;
+    if (!p) return kInvalid;
+    const moe_block_norm_args &n = *p;
+    const auto is_type = [](int t) { return t == MOE_F32 || t == MOE_BF16 || t == MOE_F16; };
+    if (n.hidden < 1 || n.hidden > 16384 || n.tokens < 1 || n.tokens > 65536 || !is_type(n.type) ||
+        (n.residual_type != n.type && n.residual_type != MOE_F32) || !(n.eps > 0.0f) || n.eps > 3.4e38f)
+        return kInvalid;
+    const int es = moe::elem_bytes(n.type), rs = moe::elem_bytes(n.residual_type);
+    bool vec = n.hidden % 8 == 0;
+    // Rows of `size`-byte elements; false: cannot be taken.
+    const auto rows = [&](const void *q, int64_t stride, int size) {
+        vec = vec && moe::aligned(q, 16) && stride * size % 16 == 0;
+        return moe::aligned(q, size) && stride >= n.hidden && stride <= (int64_t{1} << 40);
+    };
+    if (!rows(n.residual, n.residual_stride, rs)) return kInvalid;
+    if (n.residual_out && !rows(n.residual_out, n.residual_out_stride, rs)) return kInvalid;
+    if (n.block) {
+        if (!rows(n.block, n.block_stride, es)) return kInvalid;
+        if (n.gate_form < MOE_GATE_NONE || n.gate_form > MOE_GATE_ELEMENT) return kInvalid;
+        if (n.gate_form == MOE_GATE_ELEMENT && !rows(n.gate, n.gate_stride, es)) return kInvalid;
+        if ((n.gate_form == MOE_GATE_TOKEN || n.gate_form == MOE_GATE_CHANNEL) && !moe::aligned(n.gate, 4)) return kInvalid;
+        if (n.gate_form == MOE_GATE_CHANNEL) vec = vec && moe::aligned(n.gate, 16);
+        if (n.post_weight) {
+            if (!moe::aligned(n.post_weight, 4)) return kInvalid;
+            vec = vec && moe::aligned(n.post_weight, 16);
+        }
+    } else if (n.gate_form != MOE_GATE_NONE || n.post_weight) {
+        return kInvalid;
+    }
+    const bool next = n.out || n.q8 || n.codes || n.scales;
+    if (n.pre_weight ? !next : next) return kInvalid;
+    if (!n.pre_weight && !n.residual_out) return kInvalid;   // nothing to write
+    if (n.pre_weight) {
+        if (!moe::aligned(n.pre_weight, 4)) return kInvalid;
+        vec = vec && moe::aligned(n.pre_weight, 16);
+        if (n.out && !rows(n.out, n.out_stride, es)) return kInvalid;
+        if ((n.codes != nullptr) != (n.scales != nullptr) || (n.scales && !moe::aligned(n.scales, 4))) return kInvalid;
+        if (n.codes) vec = vec && moe::aligned(n.codes, 8);
+        if (n.q8 && (n.hidden % 32 || !moe::aligned(n.q8, 4))) return kInvalid;
+        if ((n.q8 || n.codes) && !moe::aligned(n.error, 4)) return kInvalid;
+    }
+    moe::NormArgs a{};
+    a.residual = n.residual;
+    a.block = n.block;
+    a.gate = n.gate;
+    a.residual_out = n.residual_out;
+    a.out = n.out;
+    a.residual_stride = n.residual_stride;
+    a.block_stride = n.block_stride;
+    a.gate_stride = n.gate_stride;
+    a.residual_out_stride = n.residual_out_stride;
+    a.out_stride = n.out_stride;
+    a.post_weight = n.post_weight;
+    a.pre_weight = n.pre_weight;
+    a.q8 = static_cast<uint32_t *>(n.q8);
+    a.codes = static_cast<uint8_t *>(n.codes);
+    a.scales = n.scales;
+    a.error = n.error;
+    a.eps = n.eps;
+    a.offset = n.weight_offset;
+    a.residual_scale = n.residual_scale;
+    a.block_scale = n.block_scale;
+    a.hidden = n.hidden;
+    a.tokens = n.tokens;
+    a.gate_form = n.block ? n.gate_form : MOE_GATE_NONE;
+    a.gate_sigmoid = n.gate_sigmoid;
+    a.vec = vec;
+    const auto s = static_cast<hipStream_t>(stream);
+    if (n.type == MOE_F32) return moe::launch_norm<moe::kF32, moe::kF32>(a, s);
+    if (n.type == MOE_BF16)
+        return n.residual_type == MOE_F32 ? moe::launch_norm<moe::kBF16, moe::kF32>(a, s) : moe::launch_norm<moe::kBF16, moe::kBF16>(a, s);
+    return n.residual_type == MOE_F32 ? moe::launch_norm<moe::kF16, moe::kF32>(a, s) : moe::launch_norm<moe::kF16, moe::kF16>(a, s);
+}

@@ -28,6 +28,7 @@ DOWN_Q4_0, DOWN_Q4_1 = 0, 1     # MOE_DOWN_Q4_0 / MOE_DOWN_Q4_1
 PATH_AUTO, PATH_STREAM, PATH_MFMA = 0, 1, 2
 TYPE_Q4_0, TYPE_Q4_1 = 2, 3     # MOE_TYPE_Q4_0 / MOE_TYPE_Q4_1 (the reference's TensorType ids)
 F32, BF16, F16 = 0, 1, 2        # MOE_F32 / MOE_BF16 / MOE_F16
+GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_ELEMENT = 0, 1, 2, 3   # MOE_GATE_*
 E4M3_GROUP = 128                # elements per scale of an e4m3 row
 STAGE_PREPARE, STAGE_GATE_UP, STAGE_DOWN, STAGE_FOLD = 0, 1, 2, 3
 
@@ -53,6 +54,19 @@ class Fp8LayerConfig(ctypes.Structure):
 class Fp8Matrix(ctypes.Structure):
     """moe_fp8_matrix."""
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
+class BlockNormArgs(ctypes.Structure):
+    """moe_block_norm_args."""
+    _fields_ = ([(n, ctypes.c_int) for n in ("hidden", "tokens", "type", "residual_type")] +
+                [(n, ctypes.c_float) for n in ("eps", "weight_offset", "residual_scale", "block_scale")] +
+                [("residual", ctypes.c_void_p), ("residual_stride", ctypes.c_int64), ("block", ctypes.c_void_p),
+                 ("block_stride", ctypes.c_int64), ("post_weight", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                 ("gate_stride", ctypes.c_int64), ("gate_form", ctypes.c_int), ("gate_sigmoid", ctypes.c_int),
+                 ("residual_out", ctypes.c_void_p), ("residual_out_stride", ctypes.c_int64),
+                 ("pre_weight", ctypes.c_void_p), ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+                 ("q8", ctypes.c_void_p), ("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                 ("error", ctypes.c_void_p)])
 
 
 class ExpertTiming(ctypes.Structure):
@@ -120,6 +134,7 @@ def library():
                                              ctypes.POINTER(Fp8Matrix), _I, _I, ctypes.POINTER(_P)]
         lib.moe_fp8_layer_destroy.argtypes = [_P]
         lib.moe_fp8_layer_forward.argtypes = [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P]
+        lib.moe_block_norm.argtypes = [ctypes.POINTER(BlockNormArgs), _P]
         _lib = lib
     return _lib
 
@@ -811,6 +826,146 @@ class MoeFp8Layer:
             error = torch.zeros(1, dtype=torch.int32, device=x.device)
         self.bind_forward(x, ids, weights, y, error, shared_gate, stream)()
         return y, error
+
+
+class BlockNorm:
+    """The norm after a block and the norm before the next one, with the gate,
+    the scales and the residual sum between them (moe_block_norm):
+
+        b = rms(block) * (weight_offset + post_weight)   (post_weight None: block)
+        h = residual_scale * residual + block_scale * gate(b)
+        n = rms(h) * (weight_offset + pre_weight)
+
+    Weights are float32 [hidden] tensors on a GPU.  pre_weight None: only h.
+    gate(b) multiplies by the gate given to a call, or by its sigmoid with
+    gate_sigmoid."""
+
+    def __init__(self, hidden, pre_weight=None, post_weight=None, eps=1e-6, weight_offset=0.0, residual_scale=1.0,
+                 block_scale=1.0, gate_sigmoid=False):
+        import torch
+        if pre_weight is None and post_weight is None:
+            raise ValueError("pre_weight or post_weight is required")
+        self.hidden, self.pre_weight, self.post_weight = hidden, pre_weight, post_weight
+        self.device = (pre_weight if pre_weight is not None else post_weight).device
+        for name, w in (("pre_weight", pre_weight), ("post_weight", post_weight)):
+            if w is not None:
+                _need(w, name, torch.float32, (hidden,), self.device)
+        if not eps > 0:
+            raise ValueError("eps must be positive")
+        self.eps, self.weight_offset, self.gate_sigmoid = eps, weight_offset, gate_sigmoid
+        self.residual_scale, self.block_scale = residual_scale, block_scale
+
+    def bind(self, residual, block=None, gate=None, residual_out=None, out=None, q8=None, codes=None, scales=None,
+             error=None, stream=None):
+        """Validate the tensors of a call once and return a no-argument
+        callable that enqueues it; the tensors must stay alive and keep their
+        shapes while the callable is used.
+
+        residual, residual_out [n][hidden] of the block's type or float32;
+        block, out [n][hidden] float32, bfloat16 or float16; gate float32 [n, 1]
+        (one value a row), float32 [hidden] (one a channel) or [n][hidden] of
+        the block's type; q8 uint8 [n][hidden/32*36]; codes float8_e4m3fn
+        [n][hidden] with scales float32 [n][ceil(hidden/128)].  Rows of the
+        [n][hidden] tensors other than codes may be strided.  Without a block
+        the norm of the residual alone is taken."""
+        import torch
+        h = self.hidden
+        if not isinstance(residual, torch.Tensor) or residual.dim() != 2:
+            raise ValueError("residual must be a two-dimensional torch tensor")
+        n, dev = residual.shape[0], self.device
+        a = BlockNormArgs(hidden=h, tokens=n, eps=self.eps, weight_offset=self.weight_offset,
+                          residual_scale=self.residual_scale, block_scale=self.block_scale,
+                          gate_sigmoid=1 if self.gate_sigmoid else 0)
+        a.residual_type, a.residual_stride = _need_rows(residual, "residual", (n, h), dev)
+        a.residual = residual.data_ptr()
+        like = block if block is not None else out if out is not None else residual
+        a.type = _elem_type(like, "block")
+        if residual.dtype not in (torch.float32, like.dtype):
+            raise TypeError(f"residual must be float32 or {like.dtype}, got {residual.dtype}")
+        if block is not None:
+            _, a.block_stride = _need_rows(block, "block", (n, h), dev)
+            a.block = block.data_ptr()
+            if self.post_weight is not None:
+                a.post_weight = self.post_weight.data_ptr()
+        if gate is not None:
+            if block is None:
+                raise ValueError("a gate needs a block")
+            if not isinstance(gate, torch.Tensor):
+                raise TypeError("gate must be a torch tensor")
+            if tuple(gate.shape) == (n, 1) and (h > 1 or gate.dtype != like.dtype):
+                a.gate_form = GATE_TOKEN
+                _need(gate, "gate", torch.float32, (n, 1), dev)
+            elif gate.dim() == 1:
+                a.gate_form = GATE_CHANNEL
+                _need(gate, "gate", torch.float32, (h,), dev)
+            else:
+                a.gate_form = GATE_ELEMENT
+                _, a.gate_stride = _need_rows(gate, "gate", (n, h), dev, dtypes=(like.dtype,))
+            a.gate = gate.data_ptr()
+        if residual_out is not None:
+            _, a.residual_out_stride = _need_rows(residual_out, "residual_out", (n, h), dev, dtypes=(residual.dtype,))
+            a.residual_out = residual_out.data_ptr()
+        if (codes is None) != (scales is None):
+            raise ValueError("codes and scales come together")
+        if self.pre_weight is None:
+            if out is not None or q8 is not None or codes is not None:
+                raise ValueError("out, q8 and codes need a pre_weight")
+            if residual_out is None:
+                raise ValueError("residual_out is required without a pre_weight")
+        elif out is not None or q8 is not None or codes is not None:
+            a.pre_weight = self.pre_weight.data_ptr()
+        elif residual_out is None:
+            raise ValueError("one of residual_out, out, q8 and codes is required")
+        if out is not None:
+            _, a.out_stride = _need_rows(out, "out", (n, h), dev, dtypes=(like.dtype,))
+            a.out = out.data_ptr()
+        if q8 is not None:
+            if h % 32:
+                raise ValueError("q8 needs a multiple of 32 channels")
+            a.q8 = _need(q8, "q8", torch.uint8, (n, h // 32 * Q8_BLOCK), dev).data_ptr()
+        if codes is not None:
+            a.codes = _e4m3(codes, "codes", (n, h), dev).data_ptr()
+            a.scales = _need(scales, "scales", torch.float32, (n, _blocks(h)), dev).data_ptr()
+        if q8 is not None or codes is not None:
+            a.error = _need(error, "error", torch.int32, (1,), dev).data_ptr()
+        fn, arg, s = library().moe_block_norm, ctypes.byref(a), _stream_on(stream, dev)
+        current, switch = torch.cuda.current_device, dev.index
+
+        def call():
+            if current() != switch:
+                with _on_device(dev):
+                    st = fn(arg, s)
+            else:
+                st = fn(arg, s)
+            if st != 0:
+                raise MoeError("moe_block_norm", st)
+        return call
+
+    def __call__(self, residual, block=None, gate=None, outputs=("residual", "out"), error=None, stream=None):
+        """One call into new tensors: `outputs` names which of residual, out,
+        q8 and e4m3 are wanted.  Returns a dict of them (e4m3 as codes and
+        scales) and the error word."""
+        import torch
+        unknown = set(outputs) - {"residual", "out", "q8", "e4m3"}
+        if unknown:
+            raise ValueError(f"unknown outputs {sorted(unknown)}")
+        n, h, dev = residual.shape[0], self.hidden, residual.device
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=dev)
+        made = {}
+        if "residual" in outputs:
+            made["residual_out"] = torch.empty((n, h), dtype=residual.dtype, device=dev)
+        if "out" in outputs and self.pre_weight is not None:
+            made["out"] = torch.empty((n, h), dtype=(block if block is not None else residual).dtype, device=dev)
+        if "q8" in outputs:
+            made["q8"] = torch.empty((n, h // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+        if "e4m3" in outputs:
+            made["codes"] = torch.empty((n, h), dtype=torch.float8_e4m3fn, device=dev)
+            made["scales"] = torch.empty((n, _blocks(h)), dtype=torch.float32, device=dev)
+        self.bind(residual, block=block, gate=gate, error=error, stream=stream, **made)()
+        if "residual_out" in made:
+            made["residual"] = made.pop("residual_out")
+        return dict(made, error=error)
 
 
 class MoeStack:

@@ -442,6 +442,58 @@ int moe_fp8_layer_destroy(moe_fp8_layer *layer);
 int moe_fp8_layer_forward(moe_fp8_layer *layer, const void *x, int type, const int32_t *ids, const float *weights,
                           int tokens, const float *shared_gate, void *y, int *error, void *stream);
 
+/* ------------------------------------------------------------------------
+ * The norms around a block, with its gate, the scales and the residual sum.
+ * ---------------------------------------------------------------------- */
+
+/* Form of `gate`: [tokens] fp32, one value a row; [hidden] fp32, one a
+ * channel; [tokens][hidden] of `type`. */
+enum { MOE_GATE_NONE = 0, MOE_GATE_TOKEN = 1, MOE_GATE_CHANNEL = 2, MOE_GATE_ELEMENT = 3 };
+
+/* All pointers are device memory; strides are the elements between rows.
+ *   b = post_weight ? rms(block) * (weight_offset + post_weight) : block
+ *   b = b * gate, or b * sigmoid(gate) with gate_sigmoid
+ *   h = residual_scale * residual + block_scale * b   (no block: the first term)
+ *   n = rms(h) * (weight_offset + pre_weight)
+ * with rms(v) = v / sqrt(mean(v^2) + eps) over a row, in fp32 throughout.
+ * h goes to residual_out and n, of the unrounded h, to whichever of out, q8
+ * and codes / scales are given. */
+typedef struct moe_block_norm_args {
+    int hidden;              /* 1..16384; a multiple of 32 for q8 */
+    int tokens;              /* 1..65536 */
+    int type;                /* of block, out and an element gate: MOE_F32, MOE_BF16, MOE_F16 */
+    int residual_type;       /* of residual and residual_out: `type` or MOE_F32 */
+    float eps;               /* > 0 */
+    float weight_offset;     /* 0, or 1 for weights stored about zero */
+    float residual_scale, block_scale;
+    const void *residual;    /* [tokens][hidden] */
+    int64_t residual_stride;
+    const void *block;       /* [tokens][hidden], or NULL: the norm before a first block */
+    int64_t block_stride;
+    const float *post_weight;   /* [hidden], or NULL: no norm after the block */
+    const void *gate;
+    int64_t gate_stride;     /* element gates */
+    int gate_form;           /* MOE_GATE_* */
+    int gate_sigmoid;
+    void *residual_out;      /* [tokens][hidden], or NULL: h is not written */
+    int64_t residual_out_stride;
+    const float *pre_weight; /* [hidden], or NULL: h only */
+    void *out;               /* [tokens][hidden], or NULL */
+    int64_t out_stride;
+    void *q8;                /* canonical Q8_1 rows [tokens][hidden/32], 4-byte aligned, or NULL */
+    void *codes;             /* e4m3 rows [tokens][hidden] with their scales, or both NULL */
+    float *scales;           /* [tokens][ceil(hidden/128)] */
+    int *error;              /* needed for q8 and codes */
+} moe_block_norm_args;
+
+/* One launch; no workspace, so calls may overlap.  q8 rows and flags are
+ * those of moe_quantize_q8_1, codes, scales and flags those of
+ * moe_quantize_e4m3, for the fp32 n.  Values that are not finite carry
+ * through to h and n.  residual_out may be residual and out may be block, with
+ * the same stride; other overlaps are not allowed.  A block's post_weight and
+ * gate need a block; pre_weight needs an output, and an output pre_weight. */
+int moe_block_norm(const moe_block_norm_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

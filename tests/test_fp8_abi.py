@@ -91,3 +91,22 @@ def test_layer_arguments(buf):
     scales = 513 * 3 * 64 * 4
     assert 513 * 3 * 2048 * 512 + scales <= w.value < 513 * 3 * 2048 * 512 + scales + 6 * 256
     assert s.value == 8 * 11 * 512 * 4
+
+
+def test_norm_arguments(buf):
+    lib, at = moe_ffn.library(), ctypes.addressof(buf)
+    good = dict(hidden=64, tokens=1, type=F32, residual_type=F32, eps=1e-6, residual=at, residual_stride=64, block=at,
+                block_stride=64, gate=at, gate_stride=64, gate_form=moe_ffn.GATE_ELEMENT, residual_out=at,
+                residual_out_stride=64, pre_weight=at, post_weight=at, out=at, out_stride=64, codes=at, scales=at, error=at)
+    assert lib.moe_block_norm(None, None) == 1
+    for bad in (dict(hidden=0), dict(hidden=16385), dict(tokens=0), dict(tokens=65537), dict(type=3), dict(residual_type=BF16),
+                dict(type=BF16, residual_type=moe_ffn.F16), dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")),
+                dict(eps=float("inf")), dict(residual=None), dict(residual=at + 2), dict(residual_stride=63),
+                dict(block_stride=63), dict(gate_form=4), dict(gate_form=-1), dict(gate=None), dict(gate_stride=0),
+                dict(gate_form=moe_ffn.GATE_TOKEN, gate=at + 1), dict(post_weight=at + 1), dict(pre_weight=at + 2),
+                dict(residual_out_stride=1), dict(out_stride=1), dict(out=at + 1), dict(scales=None), dict(codes=None),
+                dict(scales=at + 1), dict(error=None), dict(error=at + 1), dict(pre_weight=None),
+                dict(out=None, codes=None, scales=None), dict(block=None), dict(block=None, post_weight=None),
+                dict(q8=at + 2), dict(hidden=48, q8=at),
+                dict(pre_weight=None, out=None, codes=None, scales=None, residual_out=None)):
+        assert lib.moe_block_norm(ctypes.byref(moe_ffn.BlockNormArgs(**{**good, **bad})), None) == 1, bad
