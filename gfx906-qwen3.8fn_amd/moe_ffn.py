@@ -973,28 +973,63 @@ class MoeStack:
     or replayed from one captured HIP graph (torch.cuda.CUDAGraph over the
     library's launches).
 
-    Layer l takes its own input batch x[l] (fp32 [N_l][H], device).  With
-    `projections` (MoeLinear H -> H per layer) the layer input is
-    h = projection.apply(x); with `routers` (MoeLinear H -> E per layer) the
-    routes are chosen on the device from router.apply(h) by router_select;
-    otherwise fixed device ids / weights are given to bind().  Every buffer is
-    allocated by bind(), so run() allocates nothing and can be captured."""
+    Layers, projections and routers may be Q4 (MoeLayer, MoeLinear) or e4m3
+    (MoeFp8Layer, MoeFp8Linear) handles.
 
-    def __init__(self, layers, projections=None, routers=None):
+    Without `norms`, layer l takes its own input batch x[l] (fp32 [N_l][H],
+    device; e4m3 layers also bfloat16 or float16).  With `projections` (H -> H
+    per layer) the layer input is h = projection.apply(x); with `routers` (H ->
+    E per layer) the routes are chosen on the device from router.apply(h) by
+    router_select; otherwise fixed device ids / weights are given to bind().
+
+    With `norms` (len(layers) + 1 BlockNorms) the layers run on one residual
+    stream, xs = [x]: norms[0] makes the first layer's input from x, norms[l]
+    adds layer l - 1's output to the stream and makes layer l's input, and the
+    last one closes the stack (with a pre_weight: the final norm as well).  An
+    e4m3 projection takes its input as the e4m3 rows that the norm writes, and
+    a Q4 layer without a projection as its Q8_1 rows.
+
+    Every buffer is allocated by bind(), so run() allocates nothing and can be
+    captured."""
+
+    def __init__(self, layers, projections=None, routers=None, norms=None):
         self.layers = list(layers)
         self.projections = projections
         self.routers = routers
+        self.norms = norms
+        if norms is not None:
+            if len(norms) != len(self.layers) + 1:
+                raise ValueError("norms: one before the first layer and one after each")
+            if any(n.pre_weight is None for n in norms[:-1]):
+                raise ValueError("norms before a layer need a pre_weight")
         self.graph = None
 
-    def bind(self, xs, ids=None, weights=None):
+    def bind(self, xs, ids=None, weights=None, dtype=None):
+        """Allocate every buffer for the input batches xs.  dtype (with norms):
+        type of the layers' inputs and outputs, that of x unless said."""
         import torch
         dev = xs[0].device
         self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         self.steps = []
-        for l, (L, x) in enumerate(zip(self.layers, xs)):
-            n = x.shape[0]
-            st = {"x": x, "y": torch.empty((n, L.H), dtype=torch.float32, device=dev)}
-            st["h"] = torch.empty((n, L.H), dtype=torch.float32, device=dev) if self.projections else x
+        if self.norms is not None and len(xs) != 1:
+            raise ValueError("a stack with norms takes one input batch")
+        for l, L in enumerate(self.layers):
+            x = xs[0] if self.norms is not None else xs[l]
+            n, kind = x.shape[0], x.dtype if dtype is None or self.norms is None else dtype
+            st = {"y": torch.empty((n, L.H), dtype=kind, device=dev)}
+            if self.norms is not None:
+                st["x"] = torch.empty((n, L.H), dtype=kind, device=dev)
+                st["norm"] = {"out": st["x"]}
+                if self.projections and isinstance(self.projections[l], MoeFp8Linear):
+                    st["codes"] = torch.empty((n, L.H), dtype=torch.float8_e4m3fn, device=dev)
+                    st["scales"] = torch.empty((n, _blocks(L.H)), dtype=torch.float32, device=dev)
+                    st["norm"] = {"codes": st["codes"], "scales": st["scales"]}
+                elif not self.projections and isinstance(L, MoeLayer):
+                    st["q8"] = torch.empty((n, L.H // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+                    st["norm"]["q8"] = st["q8"]
+            else:
+                st["x"] = x
+            st["h"] = torch.empty((n, L.H), dtype=kind, device=dev) if self.projections else st["x"]
             if self.routers:
                 st["logits"] = torch.empty((n, L.E), dtype=torch.float32, device=dev)
                 st["ids"] = torch.empty((n, L.k), dtype=torch.int32, device=dev)
@@ -1002,17 +1037,40 @@ class MoeStack:
             else:
                 st["ids"], st["w"] = ids[l], weights[l]
             self.steps.append(st)
+        if self.norms is not None:
+            self.x = xs[0]
+            self.residual = torch.empty_like(self.x)
+            self.last = {"residual_out": self.residual}
+            if self.norms[-1].pre_weight is not None:
+                self.last["out"] = torch.empty_like(self.steps[-1]["y"])
         self.graph = None
 
     def run(self, stream=None):
         for l, (L, st) in enumerate(zip(self.layers, self.steps)):
+            if self.norms is not None:
+                self._norm(l, st["norm"], stream)
             if self.projections:
-                self.projections[l].apply(st["x"], y=st["h"], error=self.error, stream=stream)
+                if "codes" in st:
+                    self.projections[l].forward(st["codes"], st["scales"], y=st["h"], stream=stream)
+                else:
+                    self.projections[l].apply(st["x"], y=st["h"], error=self.error, stream=stream)
             if self.routers:
                 self.routers[l].apply(st["h"], y=st["logits"], error=self.error, stream=stream)
                 router_select(st["logits"], top_k=L.k, error=self.error, stream=stream, ids=st["ids"],
                               weights=st["w"])
-            L.forward(st["h"], st["ids"], st["w"], y=st["y"], error=self.error, stream=stream)
+            if "q8" in st:
+                L.forward_q8(st["q8"], st["ids"], st["w"], y=st["y"], error=self.error, stream=stream)
+            else:
+                L.forward(st["h"], st["ids"], st["w"], y=st["y"], error=self.error, stream=stream)
+        if self.norms is not None:
+            self._norm(len(self.layers), self.last, stream)
+
+    def _norm(self, l, outputs, stream):
+        """norms[l]: the stream starts as x and is self.residual from the first
+        layer's output on."""
+        if l > 0:
+            outputs = dict(outputs, block=self.steps[l - 1]["y"], residual_out=self.residual)
+        self.norms[l].bind(self.x if l <= 1 else self.residual, error=self.error, stream=stream, **outputs)()
 
     def capture(self):
         """Record one run() into a HIP graph (after one eager run as warm-up)."""
@@ -1032,4 +1090,8 @@ class MoeStack:
         self.graph.replay()
 
     def outputs(self):
+        """Each layer's output; with norms the residual stream at the end and,
+        where the last norm has a pre_weight, the final norm."""
+        if self.norms is not None:
+            return [self.residual] + ([self.last["out"]] if "out" in self.last else [])
         return [st["y"] for st in self.steps]
