@@ -24,11 +24,12 @@ inline constexpr int kFp8TileBytes = kFp8TileRows * kFp8Block;
 // Element types of the entry points (MOE_F32, MOE_BF16, MOE_F16).
 inline constexpr int kF32 = 0, kBF16 = 1, kF16 = 2;
 __host__ __device__ constexpr int elem_bytes(int type) { return type == kF32 ? 4 : 2; }
-// Any source of e4m3 rows: quantised before the call.
-inline constexpr int kCodes = 3;
+// Sources of e4m3 columns that are quantised before a product: rows and tiles.
+inline constexpr int kCodes = 3, kTiles = 4;
 
-// Canonical e4m3 codes [rows][cols] -> tiles.  cols % 16 == 0.
-hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, hipStream_t s);
+// Canonical e4m3 codes [rows][cols] -> tiles, `stride` tiles from one 16 rows
+// to the next (zeros past the row's own).  cols % 16 == 0.
+hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, int stride, hipStream_t s);
 // Rows of `type` -> codes [columns][width] and scales [columns][ceil(width/128)].
 hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
                                 float *scales, int *error, hipStream_t s);
@@ -156,6 +157,26 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
     return static_cast<uint32_t>(w);
 }
 
+// The largest magnitude of 16 neighbouring lanes' eight values.
+__device__ __forceinline__ uint32_t max16(const float (&v)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i]));
+    m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
+    m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
+    m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
+    return max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
+}
+__device__ __forceinline__ uint2 quantize8(const float (&v)[8], const GroupScale &s) {
+    if (s.bad) return make_uint2(0u, 0u);
+    return make_uint2(pack_e4m3(v[0] * s.r, v[1] * s.r, v[2] * s.r, v[3] * s.r),
+                      pack_e4m3(v[4] * s.r, v[5] * s.r, v[6] * s.r, v[7] * s.r));
+}
+// Where a tile holds elements 8 part .. + 7 of a row's block.
+__device__ __forceinline__ int tile_offset(int part, int row) {
+    return ((part >> 1) & 1) * 1024 + ((part >> 2) * 16 + row) * 16 + (part & 1) * 8;
+}
+
 // ---------------------------------------------------------------- products ---
 // Eight e4m3 codes as fp16, which holds every e4m3 value exactly (NaN too).
 __device__ __forceinline__ f16x8 e4m3_to_f16(uint32_t lo, uint32_t hi) {
@@ -175,6 +196,12 @@ struct FragF16 {
 __device__ __forceinline__ FragF16 to_f16(const Frag &f) {
     return FragF16{{e4m3_to_f16(f.c0.x, f.c0.y), e4m3_to_f16(f.c0.z, f.c0.w), e4m3_to_f16(f.c1.x, f.c1.y),
                     e4m3_to_f16(f.c1.z, f.c1.w)}};
+}
+// A fragment as the operand of block_dot.
+template<class Operand>
+__device__ __forceinline__ Operand operand(const Frag &f) {
+    if constexpr (sizeof(Operand) == sizeof(Frag)) return f;
+    else return to_f16(f);
 }
 // One block's products summed from zero: lane l gets rows 4 (l / 16) + i of
 // the tile against token l % 16.
@@ -201,11 +228,19 @@ __device__ __forceinline__ Frag load_tile(const uint8_t *tile, int lane) {
     return Frag{p[0], p[64]};
 }
 
-// 16 bytes a lane from memory straight into LDS, lane i's at dst + 16 i (dst
-// is the same for the whole wave).
-__device__ __forceinline__ void load_to_lds(const void *src, void *dst) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
-                                     (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
+// 16 bytes a lane from memory (base r, byte offset off, zero past r's end)
+// straight into LDS, lane i's at byte 16 i from `lds`, which is the same for
+// the whole wave.  Written in assembly, without output registers: the compiler
+// orders every LDS read behind such a load that it knows of, where here only
+// the wait and the barrier before a buffer's first read have to.  Nothing but
+// those may read what it writes.
+__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                 :: "s"(lds), "v"(off), "s"(r) : "memory");
+}
+__device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_offset(const void *p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
 }
 
 }  // namespace

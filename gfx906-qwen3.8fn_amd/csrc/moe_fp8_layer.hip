@@ -111,20 +111,8 @@ __global__ __launch_bounds__(512) void k_fp8_gate_up(Fp8LayerArgs a) {
                 if (col < a.H) raw = load8_raw<T_>(a.x, static_cast<size_t>(token[c0 + c]) * a.H + col);
                 float v[8];
                 unpack8<T_>(raw, v);
-                uint32_t m = 0;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) m = max(m, magnitude(v[q]));
-                m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
-                m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
-                m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
-                m = max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
-                const GroupScale g = group_scale(m);
-                uint2 w = make_uint2(pack_e4m3(v[0] * g.r, v[1] * g.r, v[2] * g.r, v[3] * g.r),
-                                     pack_e4m3(v[4] * g.r, v[5] * g.r, v[6] * g.r, v[7] * g.r));
-                if (g.bad) w = make_uint2(0u, 0u);
-                // Elements 8 part .. + 7 are half of a chunk of lane 16 (part / 4) + c.
-                *reinterpret_cast<uint2 *>(lds + b * kFp8TileBytes + ((part >> 1) & 1) * 1024 + ((part >> 2) * 16 + c) * 16 +
-                                           (part & 1) * 8) = w;
+                const GroupScale g = group_scale(max16(v));
+                *reinterpret_cast<uint2 *>(lds + b * kFp8TileBytes + tile_offset(part, c)) = quantize8(v, g);
                 if (part == 0) xs[b * 16 + c] = g.s;
             }
             __syncthreads();
@@ -231,18 +219,9 @@ __global__ __launch_bounds__(1024) void k_fp8_down_fold(Fp8LayerArgs a) {
             if (col < a.I) raw = load8_raw<kF32>(mid, col);
             float v[8];
             unpack8<kF32>(raw, v);
-            uint32_t m = 0;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) m = max(m, magnitude(v[q]));
-            m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
-            m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
-            m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
-            m = max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
-            const GroupScale g = group_scale(m);
+            const GroupScale g = group_scale(max16(v));
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last round's reads are done
-            *reinterpret_cast<uint2 *>(&codes[wave][lane * 8]) =
-                make_uint2(pack_e4m3(v[0] * g.r, v[1] * g.r, v[2] * g.r, v[3] * g.r),
-                           pack_e4m3(v[4] * g.r, v[5] * g.r, v[6] * g.r, v[7] * g.r));
+            *reinterpret_cast<uint2 *>(&codes[wave][lane * 8]) = quantize8(v, g);
             if ((lane & 15) == 0) scales[wave][lane >> 4] = g.s;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -391,7 +370,7 @@ hipError_t upload(moe_fp8_layer *L, const Part &p, const moe_fp8_matrix &m, size
     }
     if (r == hipSuccess)
         r = moe::launch_fp8_repack(static_cast<const uint8_t *>(codes), L->mem + p.tiles_at + first * p.tiles, count * p.rows,
-                                   p.cols, nullptr);
+                                   p.cols, blocks(p.cols), nullptr);
     if (r == hipSuccess)
         r = hipMemcpy(L->mem + p.scales_at + first * p.scales * 4, m.scales, count * p.scales * 4,
                       on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);

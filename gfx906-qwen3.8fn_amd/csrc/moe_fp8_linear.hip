@@ -8,6 +8,7 @@
 
 #include <algorithm>
 #include <new>
+#include <type_traits>
 
 namespace moe {
 namespace {
@@ -15,13 +16,13 @@ namespace {
 // --------------------------------------------------------------- layout ---
 // One thread per 16-byte chunk of the tiles.
 __global__ __launch_bounds__(256) void k_fp8_repack(const uint8_t *__restrict__ codes, uint4 *__restrict__ tiles,
-                                                    size_t rows, int cols, int nb, size_t chunks) {
+                                                    size_t rows, int cols, int stride, size_t chunks) {
     const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= chunks) return;
     const int lane = static_cast<int>(i & 63), half = static_cast<int>(i >> 6) & 1;
     const size_t tile = i >> 7;
-    const size_t row = tile / nb * kFp8TileRows + (lane & 15);
-    const int col = static_cast<int>(tile % nb) * kFp8Block + (lane >> 4) * 32 + half * 16;
+    const size_t row = tile / stride * kFp8TileRows + (lane & 15);
+    const int col = static_cast<int>(tile % stride) * kFp8Block + (lane >> 4) * 32 + half * 16;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows && col < cols) __builtin_memcpy(&v, codes + row * cols + col, 16);
     tiles[i] = v;
@@ -29,15 +30,25 @@ __global__ __launch_bounds__(256) void k_fp8_repack(const uint8_t *__restrict__ 
 
 // ------------------------------------------------------------- quantiser ---
 // 16 lanes per group of 128, 8 elements each; memory bound.
-template<int T>
+// Tiles: a workgroup writes one tile (16 rows, one block) of the products'
+// operand layout, and scales [block][row]; otherwise the canonical rows.
+template<int T, bool Tiles>
 __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ x, int64_t stride, int width, int nb,
-                                                       size_t groups, bool vec, uint8_t *__restrict__ codes,
-                                                       float *__restrict__ scales, int *error) {
-    const size_t g = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
-    if (g >= groups) return;   // whole groups of 16 lanes
+                                                       int columns, bool vec, uint8_t *__restrict__ codes, int tile_stride,
+                                                       float *__restrict__ scales, int64_t scale_stride, int *error) {
+    size_t n;
+    int b;
     const int part = threadIdx.x & 15;
-    const size_t n = g / nb;
-    const int k = static_cast<int>(g % nb) * kFp8Block + part * 8;
+    if constexpr (Tiles) {
+        n = static_cast<size_t>(blockIdx.x / nb) * 16 + (threadIdx.x >> 4);
+        b = blockIdx.x % nb;
+    } else {
+        const size_t g = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
+        n = g / nb;
+        b = static_cast<int>(g % nb);
+    }
+    if (n >= static_cast<size_t>(columns)) return;   // whole groups of 16 lanes
+    const int k = b * kFp8Block + part * 8;
     const size_t at = n * static_cast<size_t>(stride) + k;
     float v[8];
     if (vec) {
@@ -48,97 +59,105 @@ __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ 
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = k + i < width ? load1<T>(x, at + i) : 0.0f;
     }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i]));
-    m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
-    const GroupScale s = group_scale(m);
-    uint2 c = make_uint2(pack_e4m3(v[0] * s.r, v[1] * s.r, v[2] * s.r, v[3] * s.r),
-                         pack_e4m3(v[4] * s.r, v[5] * s.r, v[6] * s.r, v[7] * s.r));
-    if (s.bad) c = make_uint2(0u, 0u);
-    uint8_t *out = codes + n * width + k;
-    if (vec) {
-        if (k < width) *reinterpret_cast<uint2 *>(out) = c;
+    const GroupScale s = group_scale(max16(v));
+    const uint2 c = quantize8(v, s);
+    if constexpr (Tiles) {
+        // Elements 8 part .. + 7: half of a chunk of lane 16 (part / 4) + n % 16.
+        uint8_t *tile = codes + (n / 16 * tile_stride + b) * kFp8TileBytes;
+        *reinterpret_cast<uint2 *>(tile + tile_offset(part, static_cast<int>(n & 15))) = c;
+        if (part == 0) scales[b * scale_stride + n] = s.s;
     } else {
+        uint8_t *out = codes + n * width + k;
+        if (vec) {
+            if (k < width) *reinterpret_cast<uint2 *>(out) = c;
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (k + i < width) out[i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+            for (int i = 0; i < 8; ++i)
+                if (k + i < width) out[i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+        }
+        if (part == 0) scales[n * nb + b] = s.s;
     }
-    if (part == 0) {
-        scales[g] = s.s;
-        if (s.bad) atomicOr(error, 1);
-    }
+    if (part == 0 && s.bad) atomicOr(error, 1);
 }
 
 }  // namespace
 
-hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, hipStream_t s) {
-    const int nb = (cols + kFp8Block - 1) / kFp8Block;
+hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, int stride, hipStream_t s) {
     // A grid holds fewer than 2^32 threads: at most 2^30 chunks a launch.
-    const size_t rows_at_once = (size_t{1} << 30) / (static_cast<size_t>(nb) * kFp8TileBytes / 16) * kFp8TileRows;
+    const size_t row_chunks = static_cast<size_t>(stride) * kFp8TileBytes / 16;   // of 16 rows
+    const size_t rows_at_once = (size_t{1} << 30) / row_chunks * kFp8TileRows;
     for (size_t first = 0; first < rows; first += rows_at_once) {
         const size_t n = std::min(rows_at_once, rows - first);
-        const size_t chunks = (n + kFp8TileRows - 1) / kFp8TileRows * nb * (kFp8TileBytes / 16);
+        const size_t chunks = (n + kFp8TileRows - 1) / kFp8TileRows * row_chunks;
         k_fp8_repack<<<dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, s>>>(
-            codes + first * cols, reinterpret_cast<uint4 *>(tiles + first / kFp8TileRows * nb * kFp8TileBytes), n, cols, nb,
-            chunks);
-    }
-    return hipGetLastError();
-}
-
-hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
-                                float *scales, int *error, hipStream_t s) {
-    const int nb = (width + kFp8Block - 1) / kFp8Block;
-    const size_t groups = static_cast<size_t>(columns) * nb;
-    const dim3 grid(static_cast<unsigned>((groups + 15) / 16)), block(256);
-    const bool vec = width % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * elem_bytes(type) % 16 == 0 &&
-                     reinterpret_cast<uintptr_t>(codes) % 8 == 0;
-    switch (type) {
-    case kF32: k_quantize_e4m3<kF32><<<grid, block, 0, s>>>(x, stride, width, nb, groups, vec, codes, scales, error); break;
-    case kBF16: k_quantize_e4m3<kBF16><<<grid, block, 0, s>>>(x, stride, width, nb, groups, vec, codes, scales, error); break;
-    default: k_quantize_e4m3<kF16><<<grid, block, 0, s>>>(x, stride, width, nb, groups, vec, codes, scales, error); break;
+            codes + first * cols, reinterpret_cast<uint4 *>(tiles + first / kFp8TileRows * stride * kFp8TileBytes), n, cols,
+            stride, chunks);
     }
     return hipGetLastError();
 }
 
 namespace {
 
+template<bool Tiles>
+hipError_t launch_quantize(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes, int tile_stride,
+                           float *scales, int64_t scale_stride, int *error, hipStream_t s) {
+    const int nb = (width + kFp8Block - 1) / kFp8Block;
+    const size_t groups = Tiles ? static_cast<size_t>((columns + 15) / 16) * nb : (static_cast<size_t>(columns) * nb + 15) / 16;
+    const dim3 grid(static_cast<unsigned>(groups)), block(256);
+    const bool vec = width % 8 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0 && stride * elem_bytes(type) % 16 == 0 &&
+                     reinterpret_cast<uintptr_t>(codes) % 8 == 0;
+    const auto launch = [&](auto kernel) {
+        kernel<<<grid, block, 0, s>>>(x, stride, width, nb, columns, vec, codes, tile_stride, scales, scale_stride, error);
+    };
+    if (type == kF32) launch(k_quantize_e4m3<kF32, Tiles>);
+    else if (type == kBF16) launch(k_quantize_e4m3<kBF16, Tiles>);
+    else launch(k_quantize_e4m3<kF16, Tiles>);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
+                                float *scales, int *error, hipStream_t s) {
+    return launch_quantize<false>(x, type, stride, width, columns, codes, 0, scales, 0, error, s);
+}
+
+namespace {
+
 struct Fp8LinearArgs {
-    const uint8_t *tiles;    // [ceil(M/16)][nb] tiles
+    const uint8_t *tiles;    // [ceil(M/16)][tile_stride] tiles, nb of each used
     const float *wscale;     // [ceil(M/128)][nb]
     const void *x;           // rows of a type (few columns), or unused
     int64_t x_stride;
-    const uint8_t *codes;    // [N][K] e4m3 rows
-    const float *xscale;     // [N][nb]
-    const uint8_t *zero;     // 16 bytes of zeros
+    const uint8_t *codes;    // e4m3 columns: rows [N][K], or tiles [ceil(N/16)][tile_stride]
+    const float *xscale;     // scale of column n, block b at n scale_n + b scale_b
+    int scale_n, scale_b;
     void *y;
     int64_t y_stride;
     int y_type;
     int y_vec;               // rows of y take 4-element stores
     int x_vec;               // rows of x take 8-element loads
     int M, N, K, nb;
+    int tile_stride;         // tiles from one 16 rows to the next: nb, made odd
     int *error;
 };
 
 // Four results of one token, rows m .. m + 3.
+template<int Y>
 __device__ __forceinline__ void store_rows(const Fp8LinearArgs &a, int n, int m, const float (&v)[4]) {
     const size_t at = static_cast<size_t>(n) * a.y_stride + m;
     if (a.y_vec && m + 3 < a.M) {
-        if (a.y_type == kF32) store4<kF32>(a.y, at, v);
-        else if (a.y_type == kBF16) store4<kBF16>(a.y, at, v);
-        else store4<kF16>(a.y, at, v);
+        store4<Y>(a.y, at, v);
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (m + i >= a.M) break;
-        if (a.y_type == kF32) store1<kF32>(a.y, at + i, v[i]);
-        else if (a.y_type == kBF16) store1<kBF16>(a.y, at + i, v[i]);
-        else store1<kF16>(a.y, at + i, v[i]);
-    }
+    for (int i = 0; i < 4; ++i)
+        if (m + i < a.M) store1<Y>(a.y, at + i, v[i]);
+}
+__device__ __forceinline__ void store_rows(const Fp8LinearArgs &a, int n, int m, const float (&v)[4]) {
+    if (a.y_type == kF32) store_rows<kF32>(a, n, m, v);
+    else if (a.y_type == kBF16) store_rows<kBF16>(a, n, m, v);
+    else store_rows<kF16>(a, n, m, v);
 }
 
 // A token's 32 elements at k as its fragment, quantised here: the four lanes
@@ -187,13 +206,13 @@ __device__ __forceinline__ Frag quantize_frag(const Fp8LinearArgs &a, int n, int
 // out the blocks of the row (wave w: blocks w, w + W, ..) and add up through
 // LDS in wave order.  The matrix streams from memory straight into registers,
 // each tile once per column tile group.
-// IN: the columns' type, quantised here (NT = 1), or kCodes.
+// IN: the columns' type, quantised here (NT = 1), or kCodes (rows), kTiles.
 template<int IN, int NT>
 __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
     __shared__ f32x4 red[8][NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int W = blockDim.x >> 6, mt = blockIdx.x, n0 = blockIdx.y * 16 * NT;
-    const uint8_t *row = a.tiles + static_cast<size_t>(mt) * a.nb * kFp8TileBytes;
+    const uint8_t *row = a.tiles + static_cast<size_t>(mt) * a.tile_stride * kFp8TileBytes;
     const float *wscale = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
     const int kl = (lane >> 4) * 32;
     int token[NT];
@@ -223,17 +242,21 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
             for (int t = 0; t < NT; ++t) {
                 Frag x;
                 float sx;
-                if constexpr (IN == kCodes) {
+                if constexpr (IN == kTiles) {
+                    const int tile = min(n0 / 16 + t, (a.N - 1) / 16);
+                    x = load_tile(a.codes + (static_cast<size_t>(tile) * a.tile_stride + b) * kFp8TileBytes, lane);
+                } else if constexpr (IN == kCodes) {
                     const int k = b * kFp8Block + kl;
                     x = Frag{};
                     if (k < a.K) {
                         const uint4 *p = reinterpret_cast<const uint4 *>(a.codes + static_cast<size_t>(token[t]) * a.K + k);
                         x = Frag{p[0], p[1]};
                     }
-                    sx = a.xscale[static_cast<size_t>(token[t]) * a.nb + b];
                 } else {
                     x = quantize_frag<IN>(a, token[t], b * kFp8Block + kl, sx, flags);
                 }
+                if constexpr (IN == kCodes || IN == kTiles)
+                    sx = a.xscale[static_cast<size_t>(token[t]) * a.scale_n + static_cast<size_t>(b) * a.scale_b];
                 const f32x4 p = block_dot(wf, to_f16(x));
                 const float s = sx * sw;
 #pragma unroll
@@ -241,7 +264,7 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
             }
         }
     }
-    if constexpr (IN != kCodes) {
+    if constexpr (IN != kCodes && IN != kTiles) {
         if (mt == 0 && flags) atomicOr(a.error, flags);   // every row tile quantises the same columns
     }
 #pragma unroll
@@ -261,120 +284,246 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
     }
 }
 
-// Many columns: a workgroup of WR x WC waves takes 16 TM WR rows and 16 TN WC
-// columns, and steps through the blocks of K with both operands' next step on
-// the way to LDS (two buffers) while it multiplies the current one.
-template<int WR, int WC, int TM, int TN, bool F16>
-__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m, int tiles_n) {
-    constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
+// ---------------------------------------------------------- many columns ---
+// A workgroup of WR x WC waves takes 16 TM WR rows and 16 TN WC columns, and
+// steps through the blocks of K with both operands' next step on the way to
+// LDS (two buffers) while it multiplies the current one.
+// Tiles: the columns lie in tiles as the rows do.  Otherwise they are canonical
+// rows: at a power-of-two width the 256 rows of a step lie a multiple of the
+// L2's channel period apart and queue up at one channel (8192 x 8192 at 16,384
+// columns: 1.31 ms from rows, 1.02 from tiles with their quantiser), which is also why the tiles of
+// 16 rows are an odd number of tiles apart.
+template<int WR, int WC, int TM, int TN, bool Tiles>
+struct GemmTile {
+    static constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
+    static constexpr int ABytes = BM * kFp8Block, BBytes = BN * kFp8Block, Buffer = ABytes + BBytes;
+    static constexpr int ALoads = BM / 8 / W, BLoads = BN / 8 / W;   // 1 KiB loads of a wave and step
     static_assert(kFp8Block % (16 * TM) == 0, "a wave's rows share one scale block");
-    constexpr int ABytes = BM * kFp8Block, BBytes = BN * kFp8Block;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][ABytes + BBytes];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wr = wave / WC, wc = wave % WC;
-    const int pm = blockIdx.x % tiles_m, pn = blockIdx.x / tiles_m;
-    const int m0 = pm * BM, n0 = pn * BN, row_tiles = (a.M + 15) / 16;
+    static_assert(BM / 8 % W == 0 && BN / 8 % W == 0 && W % 2 == 0, "every wave issues the same loads");
 
-    // Staging, 1 KiB (64 lanes x 16 bytes) a load.  Rows of the matrix past
-    // its end and columns past N read the last one again; they are not stored.
-    // Columns: 8 rows of 128 bytes a load, each row's eight chunks permuted by
-    // its index so that the fragment reads below spread over the LDS banks.
-    constexpr int ALoads = BM / 8, BLoads = BN / 8;
-    static_assert(ALoads % W == 0 && BLoads % W == 0, "every wave issues the same number of loads");
-    const uint8_t *ap[ALoads / W];
-    const uint8_t *bp[BLoads / W];
-    int bk[BLoads / W];
-#pragma unroll
-    for (int i = 0; i < ALoads / W; ++i) {
-        const int c = i * W + wave;
-        const int tile = min(m0 / 16 + (c >> 1), row_tiles - 1);
-        ap[i] = a.tiles + static_cast<size_t>(tile) * a.nb * kFp8TileBytes + (c & 1) * 1024 + lane * 16;
-    }
-#pragma unroll
-    for (int i = 0; i < BLoads / W; ++i) {
-        const int c = i * W + wave, t = lane >> 3;
-        bk[i] = ((lane & 7) ^ t ^ (c & 1)) * 16;
-        bp[i] = a.codes + static_cast<size_t>(min(n0 + 8 * c + t, a.N - 1)) * a.K + bk[i];
-    }
-    auto stage = [&](int b, uint8_t *buf) {
-#pragma unroll
-        for (int i = 0; i < ALoads / W; ++i)
-            load_to_lds(ap[i] + static_cast<size_t>(b) * kFp8TileBytes, buf + (i * W + wave) * 1024);
-#pragma unroll
-        for (int i = 0; i < BLoads / W; ++i) {
-            const uint8_t *p = b * kFp8Block + bk[i] < a.K ? bp[i] + b * kFp8Block : a.zero;
-            load_to_lds(p, buf + ABytes + (i * W + wave) * 1024);
+    int lane, wave, wr, wc, m0, n0, K, nb, scale_b;
+    __amdgpu_buffer_rsrc_t ar, br;
+    uint32_t tile_row, aoff, boff, boff_last, lds0;
+    const float *wscale, *xscale;
+    uint32_t xs[TN];
+    int b0off, b1off, aread, bread;
+
+    __device__ __forceinline__ GemmTile(const Fp8LinearArgs &a, int pm, int pn, const void *lds) {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wr = wave / WC;
+        wc = wave % WC;
+        m0 = pm * BM;
+        n0 = pn * BN;
+        K = a.K;
+        nb = a.nb;
+        // Rows of the matrix and columns past the end are read as zeros.
+        const int row_tiles = (a.M + 15) / 16;
+        tile_row = static_cast<uint32_t>(a.tile_stride) * kFp8TileBytes;   // bytes of 16 rows
+        ar = buffer_rsrc(a.tiles + static_cast<size_t>(m0 / 16) * tile_row,
+                         static_cast<uint32_t>(min(row_tiles - m0 / 16, BM / 16)) * tile_row);
+        aoff = lane * 16;
+        if constexpr (Tiles) {
+            br = buffer_rsrc(a.codes + static_cast<size_t>(n0 / 16) * tile_row,
+                             static_cast<uint32_t>(min((a.N + 15) / 16 - n0 / 16, BN / 16)) * tile_row);
+        } else {
+            // 8 rows of 128 bytes a load, each row's eight chunks permuted by
+            // its index so that the fragment reads spread over the LDS banks.
+            br = buffer_rsrc(a.codes + static_cast<size_t>(n0) * a.K, static_cast<uint32_t>(min(a.N - n0, BN)) * a.K);
+            const int bt = lane >> 3, bk = ((lane & 7) ^ bt ^ (wave & 1)) * 16;   // row and byte of the lane's chunk
+            boff = static_cast<uint32_t>(bt) * a.K + bk;
+            boff_last = (a.nb - 1) * kFp8Block + bk < a.K ? boff : 0xff000000u;   // past the row's end: zeros
         }
-    };
-
-    const float *wscale = a.wscale + static_cast<size_t>(min(m0 + wr * 16 * TM, a.M - 1) / kFp8Block) * a.nb;
-    const float *xs[TN];
+        lds0 = lds_offset(lds);
+        wscale = a.wscale + static_cast<size_t>(min(m0 + wr * 16 * TM, a.M - 1) / kFp8Block) * a.nb;
+        xscale = a.xscale;
+        scale_b = a.scale_b;
 #pragma unroll
-    for (int t = 0; t < TN; ++t)
-        xs[t] = a.xscale + static_cast<size_t>(min(n0 + (wc * TN + t) * 16 + (lane & 15), a.N - 1)) * a.nb;
+        for (int t = 0; t < TN; ++t)   // the lane's columns' scales
+            xs[t] = static_cast<uint32_t>(min(n0 + (wc * TN + t) * 16 + (lane & 15), a.N - 1)) * a.scale_n;
+        if constexpr (!Tiles) {
+            // Fragment of column l % 16, chunks 2 (l / 16) and + 1, in the permuted order.
+            const int tok = lane & 15, swz = (tok & 7) ^ (tok >> 3), frag = (tok >> 3) * 1024 + (tok & 7) * 128;
+            b0off = frag + (((lane >> 4) * 2) ^ swz) * 16;
+            b1off = frag + (((lane >> 4) * 2 + 1) ^ swz) * 16;
+        }
+        aread = wr * TM * 2048;
+        bread = ABytes + wc * TN * 2048;
+    }
+    // Start block b's loads into its buffer.
+    __device__ __forceinline__ void stage(int b) const {
+        const uint32_t to = lds0 + (b & 1) * Buffer + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < ALoads; ++i) {
+            const int c = i * W + wave;
+            load_to_lds(ar, aoff + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + i * W * 1024);
+        }
+        if constexpr (Tiles) {
+#pragma unroll
+            for (int i = 0; i < BLoads; ++i) {
+                const int c = i * W + wave;
+                load_to_lds(br, aoff + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + ABytes + i * W * 1024);
+            }
+        } else {
+            const uint32_t lane_off = b + 1 < nb ? boff : boff_last;
+#pragma unroll
+            for (int i = 0; i < BLoads; ++i)
+                load_to_lds(br, lane_off + (8 * (i * W + wave) * K + b * kFp8Block), to + ABytes + i * W * 1024);
+        }
+    }
+    __device__ __forceinline__ float scale(int t, int b) const { return xscale[xs[t] + static_cast<uint32_t>(b * scale_b)]; }
+    __device__ __forceinline__ Frag column(const uint8_t *buf, int t) const {
+        const uint8_t *p = buf + bread + t * 2048;
+        if constexpr (Tiles) return load_tile(p, lane);
+        else return Frag{*reinterpret_cast<const uint4 *>(p + b0off), *reinterpret_cast<const uint4 *>(p + b1off)};
+    }
+    __device__ __forceinline__ Frag row(const uint8_t *buf, int i) const { return load_tile(buf + aread + i * 2048, lane); }
+    template<int Y>
+    __device__ __forceinline__ void store(const Fp8LinearArgs &a, const f32x4 (&acc)[TM][TN]) const {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            const int n = n0 + (wc * TN + t) * 16 + (lane & 15);
+            if (n >= a.N) continue;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const float v[4] = {acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
+                store_rows<Y>(a, n, m0 + (wr * TM + i) * 16 + (lane >> 4) * 4, v);
+            }
+        }
+    }
+};
+
+// Y: type of y; fp32 results on fp16 operands, the others on e4m3 ones.
+template<int WR, int WC, int TM, int TN, bool Tiles, int Y>
+__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m) {
+    using Tile = GemmTile<WR, WC, TM, TN, Tiles>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][Tile::Buffer];
+    const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds);
     f32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int t = 0; t < TN; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    // Fragment of column l % 16, chunks 2 (l / 16) and + 1, in the permuted order.
-    const int tok = lane & 15, swz = (tok & 7) ^ (tok >> 3);
-    const int boff = (tok >> 3) * 1024 + (tok & 7) * 128;
-    const int b0off = boff + (((lane >> 4) * 2) ^ swz) * 16, b1off = boff + (((lane >> 4) * 2 + 1) ^ swz) * 16;
-
-    stage(0, lds[0]);
+    // The scales of a step are loaded during the step before it, and used
+    // before the next loads to LDS are issued: memory answers in order.
+    float sw = g.wscale[0], sx[TN];
+#pragma unroll
+    for (int t = 0; t < TN; ++t) sx[t] = g.scale(t, 0);
+    g.stage(0);
     for (int b = 0; b < a.nb; ++b) {
+        wait_for_lds_loads();
         __syncthreads();
-        uint8_t *buf = lds[b & 1];
-        const float sw = wscale[b];
         float s[TN];
 #pragma unroll
-        for (int t = 0; t < TN; ++t) s[t] = xs[t][b] * sw;
-        if (b + 1 < a.nb) stage(b + 1, lds[(b + 1) & 1]);
-        const uint8_t *bb = buf + ABytes + wc * TN * 2048;
-        Frag x[TN];
+        for (int t = 0; t < TN; ++t) s[t] = sx[t] * sw;
+        __builtin_amdgcn_sched_barrier(0);
+        const uint8_t *buf = lds[b & 1];
+        if (b + 1 < a.nb) {
+            g.stage(b + 1);
+            sw = g.wscale[b + 1];
 #pragma unroll
-        for (int t = 0; t < TN; ++t)
-            x[t] = Frag{*reinterpret_cast<const uint4 *>(bb + t * 2048 + b0off), *reinterpret_cast<const uint4 *>(bb + t * 2048 + b1off)};
-        const uint8_t *ab = buf + wr * TM * 2048;
-        if constexpr (F16) {
-            FragF16 xf[TN];
-#pragma unroll
-            for (int t = 0; t < TN; ++t) xf[t] = to_f16(x[t]);
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const FragF16 w = to_f16(load_tile(ab + i * 2048, lane));
-#pragma unroll
-                for (int t = 0; t < TN; ++t) {
-                    const f32x4 p = block_dot(w, xf[t]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(p[e], s[t], acc[i][t][e]);
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < TM; ++i) {
-                const Frag w = load_tile(ab + i * 2048, lane);
-#pragma unroll
-                for (int t = 0; t < TN; ++t) {
-                    const f32x4 p = block_dot(w, x[t]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(p[e], s[t], acc[i][t][e]);
-                }
-            }
+            for (int t = 0; t < TN; ++t) sx[t] = g.scale(t, b + 1);
         }
-    }
+        using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
+        Operand x[TN];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
-        const int n = n0 + (wc * TN + t) * 16 + (lane & 15);
-        if (n >= a.N) continue;
+        for (int t = 0; t < TN; ++t) x[t] = operand<Operand>(g.column(buf, t));
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-            const float v[4] = {acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
-            store_rows(a, n, m0 + (wr * TM + i) * 16 + (lane >> 4) * 4, v);
+            const Operand w = operand<Operand>(g.row(buf, i));
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const f32x4 p = block_dot(w, x[t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(p[e], s[t], acc[i][t][e]);
+            }
         }
     }
+    g.template store<Y>(a, acc);
+}
+
+// The largest batches: 256 x 256 a workgroup, eight waves of 128 x 64, two on
+// each SIMD that take turns, one at the MFMAs of half a step (four row tiles
+// against four column tiles) while the other reads its next operands from LDS.
+// A barrier ends each turn.  With turn p of waves 0 .. 3 at
+//   4 b: read columns, rows 0 .. 3 | 4 b + 1: multiply | 4 b + 2: read rows
+//   4 .. 7 | 4 b + 3: multiply
+// and waves 4 .. 7 one turn behind, block b's buffer is last read in turn 4 b
+// + 3; block b + 1's loads start in turns 4 b and 4 b + 1, into the buffer last
+// read in turn 4 b - 1, and each wave waits for its own before the barrier
+// that ends its second read of block b, turn 4 b + 3 at the latest.
+template<bool Tiles, int Y>
+__global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tiles_m) {
+    using Tile = GemmTile<2, 4, 8, 4, Tiles>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][Tile::Buffer];
+    const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds);
+    f32x4 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    // Everything issued before it is done and nothing moves across it.
+    const auto turn = [](bool loads) {
+        __builtin_amdgcn_sched_barrier(0);
+        if (loads) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    float sw = g.wscale[0], sx[4], s[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) sx[t] = g.scale(t, 0);
+    g.stage(0);
+    turn(true);
+    if (g.wr == 1) turn(false);   // waves 4 .. 7: one turn behind
+    const auto multiply = [&](const Frag (&w)[4], const Frag (&x)[4], int i0) {
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const f32x4 p = block_dot(w[i], x[t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i0 + i][t][e] = fmaf(p[e], s[t], acc[i0 + i][t][e]);
+            }
+        // Four MFMAs ahead, so that no product is waited for.
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
+#pragma unroll
+        for (int q = 0; q < 12; ++q) {
+            __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);   // VALU
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);   // MFMA
+        }
+        __builtin_amdgcn_sched_group_barrier(0x2, 16, 0);
+        __builtin_amdgcn_s_setprio(0);
+    };
+    for (int b = 0; b < a.nb; ++b) {
+        const uint8_t *buf = lds[b & 1];
+        Frag x[4], w[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[t] = sx[t] * sw;
+        __builtin_amdgcn_sched_barrier(0);
+        if (b + 1 < a.nb) {
+            g.stage(b + 1);
+            sw = g.wscale[b + 1];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) sx[t] = g.scale(t, b + 1);
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[t] = g.column(buf, t);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = g.row(buf, i);
+        turn(false);
+        multiply(w, x, 0);
+        turn(false);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = g.row(buf, 4 + i);
+        turn(true);
+        multiply(w, x, 4);
+        turn(false);
+    }
+    if (g.wr == 0) turn(false);   // as many turns for every wave
+    g.template store<Y>(a, acc);
 }
 
 }  // namespace
@@ -383,11 +532,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int 
 // ------------------------------------------------------------------ C ABI ---
 struct moe_fp8_linear {
     int input = 0, output = 0, max_columns = 0, device = 0;
-    int nb = 0;
-    uint8_t *mem = nullptr;       // tiles, scales, 16 bytes of zeros
+    int nb = 0, tile_stride = 0;
+    uint8_t *mem = nullptr;       // tiles, scales
     const float *scales = nullptr;
-    const uint8_t *zero = nullptr;
-    uint8_t *ws = nullptr;        // codes [max_columns][input], then scales [max_columns][nb]
+    uint8_t *ws = nullptr;        // columns as tiles, then scales [nb][columns]
 };
 
 namespace {
@@ -412,7 +560,6 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     moe::Fp8LinearArgs a{};
     a.tiles = L->mem;
     a.wscale = L->scales;
-    a.zero = L->zero;
     a.y = y;
     a.y_type = y_type;
     a.y_stride = y_stride;
@@ -422,16 +569,27 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     a.N = columns;
     a.K = L->input;
     a.nb = L->nb;
+    a.tile_stride = L->tile_stride;
     return a;
 }
 
-template<int WR, int WC, int TM, int TN>
+template<int WR, int WC, int TM, int TN, bool Tiles>
 int launch_gemm(const moe::Fp8LinearArgs &a, hipStream_t s) {
-    constexpr int BM = 16 * TM * WR, BN = 16 * TN * WC;
-    const int tm = (a.M + BM - 1) / BM, tn = (a.N + BN - 1) / BN;
-    const dim3 grid(static_cast<unsigned>(static_cast<size_t>(tm) * tn)), block(64 * WR * WC);
-    if (a.y_type == MOE_F32) moe::k_fp8_gemm<WR, WC, TM, TN, true><<<grid, block, 0, s>>>(a, tm, tn);
-    else moe::k_fp8_gemm<WR, WC, TM, TN, false><<<grid, block, 0, s>>>(a, tm, tn);
+    using Tile = moe::GemmTile<WR, WC, TM, TN, Tiles>;
+    const int tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
+    const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * Tile::W);
+    if (a.y_type == MOE_F32) moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
+    else if (a.y_type == MOE_BF16) moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
+    else moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
+    return hipGetLastError();
+}
+
+template<bool Tiles>
+int launch_gemm_wide(const moe::Fp8LinearArgs &a, hipStream_t s) {
+    const int tm = (a.M + 255) / 256, tn = (a.N + 255) / 256;
+    const dim3 grid(static_cast<unsigned>(tm) * tn), block(512);
+    if (a.y_type == MOE_BF16) moe::k_fp8_gemm_wide<Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
+    else moe::k_fp8_gemm_wide<Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
     return hipGetLastError();
 }
 
@@ -443,17 +601,18 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-int launch_rows(moe::Fp8LinearArgs a, const uint8_t *codes, const float *scales, hipStream_t s) {
-    a.codes = codes;
-    a.xscale = scales;
-    if (a.N <= 16) return launch_stream<moe::kCodes, 1>(a, s);
-    if (a.N <= 32) return launch_stream<moe::kCodes, 2>(a, s);
-    if (a.N <= 64) return launch_stream<moe::kCodes, 4>(a, s);
+// The product for quantised columns: canonical rows, or Tiles.
+template<bool Tiles>
+int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
+    constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
+    if (a.N <= 16) return launch_stream<IN, 1>(a, s);
+    if (a.N <= 32) return launch_stream<IN, 2>(a, s);
+    if (a.N <= 64) return launch_stream<IN, 4>(a, s);
     const long big = static_cast<long>((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if (big >= 200) return launch_gemm<2, 4, 8, 4>(a, s);
+    if (big >= 200) return a.y_type == MOE_F32 ? launch_gemm<2, 4, 8, 4, Tiles>(a, s) : launch_gemm_wide<Tiles>(a, s);
     const long mid = static_cast<long>((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (mid >= 200) return launch_gemm<2, 2, 4, 4>(a, s);
-    return launch_gemm<2, 2, 2, 2>(a, s);
+    if (mid >= 200) return launch_gemm<2, 2, 4, 4, Tiles>(a, s);
+    return launch_gemm<2, 2, 2, 2, Tiles>(a, s);
 }
 
 }  // namespace
@@ -487,29 +646,30 @@ int moe_fp8_linear_create(int input, int output, int max_columns, const void *co
     L->nb = (input + moe::kFp8Block - 1) / moe::kFp8Block;
     const size_t code_bytes = static_cast<size_t>(output) * input;
     const size_t scale_bytes = static_cast<size_t>((output + 127) / 128) * L->nb * 4;
-    const size_t tiles = static_cast<size_t>((output + 15) / 16) * L->nb * moe::kFp8TileBytes;
-    const size_t scale_at = round_up(tiles, 256), zero_at = scale_at + round_up(scale_bytes, 256);
+    L->tile_stride = L->nb | 1;
+    const auto tile_bytes = [&](int rows) { return static_cast<size_t>((rows + 15) / 16) * L->tile_stride * moe::kFp8TileBytes; };
+    const size_t tiles = tile_bytes(output);
+    const size_t scale_at = round_up(tiles, 256);
     void *staging = nullptr;
     // Weights that another stream is still writing are complete after this.
     hipError_t r = hipDeviceSynchronize();
-    if (r == hipSuccess) r = hipMalloc(&L->mem, zero_at + 256);
+    if (r == hipSuccess) r = hipMalloc(&L->mem, scale_at + scale_bytes);
     if (r == hipSuccess && max_columns > 0)
-        r = hipMalloc(&L->ws, static_cast<size_t>(max_columns) * (static_cast<size_t>(input) + L->nb * 4));
+        r = hipMalloc(&L->ws, tile_bytes(max_columns) + static_cast<size_t>(L->nb) * max_columns * 4);
     const void *device_codes = codes;
     if (r == hipSuccess && !weights_on_device) {
         r = hipMalloc(&staging, code_bytes);
         if (r == hipSuccess) r = hipMemcpy(staging, codes, code_bytes, hipMemcpyHostToDevice);
         device_codes = staging;
     }
-    if (r == hipSuccess) r = moe::launch_fp8_repack(static_cast<const uint8_t *>(device_codes), L->mem, output, input, nullptr);
+    if (r == hipSuccess) r = moe::launch_fp8_repack(static_cast<const uint8_t *>(device_codes), L->mem, output, input,
+                                                       L->tile_stride, nullptr);
     if (r == hipSuccess)
         r = hipMemcpy(L->mem + scale_at, scales, scale_bytes, weights_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);
-    if (r == hipSuccess) r = hipMemset(L->mem + zero_at, 0, 256);
     if (r == hipSuccess) r = hipDeviceSynchronize();
     if (staging) (void)hipFree(staging);
     if (r != hipSuccess) { release(L); return r; }
     L->scales = reinterpret_cast<const float *>(L->mem + scale_at);
-    L->zero = L->mem + zero_at;
     *out = L;
     return 0;
 }
@@ -534,8 +694,12 @@ int moe_fp8_linear_forward(moe_fp8_linear *L, const void *x_codes, const float *
         return kInvalid;
     moe::LaunchDevice device(L->device);
     if (!device.ok()) return hipErrorInvalidDevice;
-    return launch_rows(base_args(L, columns, y, y_type, y_stride), static_cast<const uint8_t *>(x_codes), x_scales,
-                       static_cast<hipStream_t>(stream));
+    moe::Fp8LinearArgs a = base_args(L, columns, y, y_type, y_stride);
+    a.codes = static_cast<const uint8_t *>(x_codes);
+    a.xscale = x_scales;
+    a.scale_n = L->nb;
+    a.scale_b = 1;
+    return launch_product<false>(a, static_cast<hipStream_t>(stream));
 }
 
 int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x_stride, int columns, void *y, int y_type,
@@ -561,10 +725,15 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
         if (x_type == MOE_BF16) return launch_stream<moe::kBF16, 1>(a, s);
         return launch_stream<moe::kF16, 1>(a, s);
     }
-    auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>(L->max_columns) * L->input);
-    const hipError_t r = moe::launch_quantize_e4m3(x, x_type, x_stride, L->input, columns, L->ws, scales, error, s);
+    auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>((columns + 15) / 16) * L->tile_stride * moe::kFp8TileBytes);
+    const hipError_t r = moe::launch_quantize<true>(x, x_type, x_stride, L->input, columns, L->ws, L->tile_stride, scales, columns,
+                                                    error, s);
     if (r != hipSuccess) return r;
-    return launch_rows(a, L->ws, scales, s);
+    a.codes = L->ws;
+    a.xscale = scales;
+    a.scale_n = 1;
+    a.scale_b = columns;
+    return launch_product<true>(a, s);
 }
 
 }  // extern "C"

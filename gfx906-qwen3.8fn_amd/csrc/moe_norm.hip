@@ -125,17 +125,8 @@ __device__ __forceinline__ void store_q8(uint32_t *q8, size_t block, int part, f
 // An e4m3 group from 16 neighbouring lanes, as k_quantize_e4m3 forms it.
 __device__ __forceinline__ void store_e4m3(uint8_t *codes, size_t at, float *scale, int part, const float (&v)[8], int valid,
                                            bool vec, int &flags) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, magnitude(v[i]));
-    m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<4>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<8>(static_cast<int>(m))));
-    const GroupScale g = group_scale(m);
-    uint2 c = make_uint2(pack_e4m3(v[0] * g.r, v[1] * g.r, v[2] * g.r, v[3] * g.r),
-                         pack_e4m3(v[4] * g.r, v[5] * g.r, v[6] * g.r, v[7] * g.r));
-    if (g.bad) c = make_uint2(0u, 0u);
+    const GroupScale g = group_scale(max16(v));
+    const uint2 c = quantize8(v, g);
     if (vec) {
         if (valid > 0) *reinterpret_cast<uint2 *>(codes + at) = c;
     } else {
