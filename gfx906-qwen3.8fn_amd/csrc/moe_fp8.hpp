@@ -238,7 +238,17 @@ __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t o
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                  :: "s"(lds), "v"(off), "s"(r) : "memory");
 }
-__device__ __forceinline__ void wait_for_lds_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void load_word_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+                 :: "s"(lds), "v"(off), "s"(r) : "memory");
+}
+// Until at most N of the wave's loads are outstanding.
+template<int N>
+__device__ __forceinline__ void wait_for_lds_loads() {
+    static_assert(N < 64);
+    asm volatile("s_waitcnt vmcnt(%0)" :: "i"(N) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_offset(const void *p) {
     return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((const __attribute__((address_space(3))) void *)p));
 }

@@ -286,31 +286,34 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
 
 // ---------------------------------------------------------- many columns ---
 // A workgroup of WR x WC waves takes 16 TM WR rows and 16 TN WC columns, and
-// steps through the blocks of K with both operands' next step on the way to
-// LDS (two buffers) while it multiplies the current one.
+// steps through the blocks of K with the next steps' operands and column
+// scales on the way to a ring of S buffers in LDS.
+//
 // Tiles: the columns lie in tiles as the rows do.  Otherwise they are canonical
 // rows: at a power-of-two width the 256 rows of a step lie a multiple of the
 // L2's channel period apart and queue up at one channel (8192 x 8192 at 16,384
-// columns: 1.31 ms from rows, 1.02 from tiles with their quantiser), which is also why the tiles of
-// 16 rows are an odd number of tiles apart.
-template<int WR, int WC, int TM, int TN, bool Tiles>
+// columns: 1.31 ms from rows, 1.02 from tiles with their quantiser), which is
+// also why the tiles of 16 rows are an odd number of tiles apart.
+template<int WR, int WC, int TM, int TN, int S, bool Tiles>
 struct GemmTile {
     static constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
-    static constexpr int ABytes = BM * kFp8Block, BBytes = BN * kFp8Block, Buffer = ABytes + BBytes;
+    static constexpr int ABytes = BM * kFp8Block, BBytes = BN * kFp8Block, Buffer = ABytes + BBytes + BN * 4;
     static constexpr int ALoads = BM / 8 / W, BLoads = BN / 8 / W;   // 1 KiB loads of a wave and step
+    static constexpr int Loads = ALoads + BLoads + 1;                // and one of scales
     static_assert(kFp8Block % (16 * TM) == 0, "a wave's rows share one scale block");
-    static_assert(BM / 8 % W == 0 && BN / 8 % W == 0 && W % 2 == 0, "every wave issues the same loads");
+    static_assert(BM / 8 % W == 0 && BN / 8 % W == 0 && W % 2 == 0 && BN % 64 == 0 && W % (BN / 64) == 0,
+                  "every wave issues the same loads");
 
-    int lane, wave, wr, wc, m0, n0, K, nb, scale_b;
-    __amdgpu_buffer_rsrc_t ar, br;
-    uint32_t tile_row, aoff, boff, boff_last, lds0;
-    const float *wscale, *xscale;
-    uint32_t xs[TN];
-    int b0off, b1off, aread, bread;
+    int lane, wave, wr, wc, m0, n0, K, nb;
+    __amdgpu_buffer_rsrc_t ar, br, sr;
+    uint32_t tile_row, aoff, boff, boff_last, soff, sstep, lds0;
+    // In the constant address space: scalar loads, which the waits above do not count.
+    const __attribute__((address_space(4))) float *wscale;
+    int b0off, b1off, aread, bread, sread;
 
     __device__ __forceinline__ GemmTile(const Fp8LinearArgs &a, int pm, int pn, const void *lds) {
         lane = threadIdx.x & 63;
-        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
         wr = wave / WC;
         wc = wave % WC;
         m0 = pm * BM;
@@ -318,29 +321,29 @@ struct GemmTile {
         K = a.K;
         nb = a.nb;
         // Rows of the matrix and columns past the end are read as zeros.
-        const int row_tiles = (a.M + 15) / 16;
+        const int row_tiles = (a.M + 15) / 16, cols = min(a.N - n0, BN);
         tile_row = static_cast<uint32_t>(a.tile_stride) * kFp8TileBytes;   // bytes of 16 rows
         ar = buffer_rsrc(a.tiles + static_cast<size_t>(m0 / 16) * tile_row,
                          static_cast<uint32_t>(min(row_tiles - m0 / 16, BM / 16)) * tile_row);
         aoff = lane * 16;
         if constexpr (Tiles) {
-            br = buffer_rsrc(a.codes + static_cast<size_t>(n0 / 16) * tile_row,
-                             static_cast<uint32_t>(min((a.N + 15) / 16 - n0 / 16, BN / 16)) * tile_row);
+            br = buffer_rsrc(a.codes + static_cast<size_t>(n0 / 16) * tile_row, static_cast<uint32_t>((cols + 15) / 16) * tile_row);
         } else {
             // 8 rows of 128 bytes a load, each row's eight chunks permuted by
             // its index so that the fragment reads spread over the LDS banks.
-            br = buffer_rsrc(a.codes + static_cast<size_t>(n0) * a.K, static_cast<uint32_t>(min(a.N - n0, BN)) * a.K);
+            br = buffer_rsrc(a.codes + static_cast<size_t>(n0) * a.K, static_cast<uint32_t>(cols) * a.K);
             const int bt = lane >> 3, bk = ((lane & 7) ^ bt ^ (wave & 1)) * 16;   // row and byte of the lane's chunk
             boff = static_cast<uint32_t>(bt) * a.K + bk;
-            boff_last = (a.nb - 1) * kFp8Block + bk < a.K ? boff : 0xff000000u;   // past the row's end: zeros
+            boff_last = (a.nb - 1) * kFp8Block + bk < a.K ? boff : kPastEnd;   // past the row's end: zeros
         }
+        // Scales of 64 columns a wave; waves beyond the columns load the same again.
+        sr = buffer_rsrc(a.xscale + static_cast<size_t>(n0) * a.scale_n,
+                         (static_cast<uint32_t>(cols - 1) * a.scale_n + static_cast<uint32_t>(a.nb - 1) * a.scale_b + 1) * 4);
+        soff = static_cast<uint32_t>(wave % (BN / 64) * 64 + lane) * a.scale_n * 4;
+        sstep = static_cast<uint32_t>(a.scale_b) * 4;
+        if (wave % (BN / 64) * 64 + lane >= cols) soff = kPastEnd;
         lds0 = lds_offset(lds);
-        wscale = a.wscale + static_cast<size_t>(min(m0 + wr * 16 * TM, a.M - 1) / kFp8Block) * a.nb;
-        xscale = a.xscale;
-        scale_b = a.scale_b;
-#pragma unroll
-        for (int t = 0; t < TN; ++t)   // the lane's columns' scales
-            xs[t] = static_cast<uint32_t>(min(n0 + (wc * TN + t) * 16 + (lane & 15), a.N - 1)) * a.scale_n;
+        wscale = (const __attribute__((address_space(4))) float *)(a.wscale + static_cast<size_t>(min(m0 + wr * 16 * TM, a.M - 1) / kFp8Block) * a.nb);
         if constexpr (!Tiles) {
             // Fragment of column l % 16, chunks 2 (l / 16) and + 1, in the permuted order.
             const int tok = lane & 15, swz = (tok & 7) ^ (tok >> 3), frag = (tok >> 3) * 1024 + (tok & 7) * 128;
@@ -349,29 +352,38 @@ struct GemmTile {
         }
         aread = wr * TM * 2048;
         bread = ABytes + wc * TN * 2048;
+        sread = ABytes + BBytes + (wc * TN * 16 + (lane & 15)) * 4;
     }
-    // Start block b's loads into its buffer.
-    __device__ __forceinline__ void stage(int b) const {
-        const uint32_t to = lds0 + (b & 1) * Buffer + wave * 1024;
+    static constexpr uint32_t kPastEnd = 0xc0000000u;   // past every resource here, and no sum with it wraps
+
+    // Start block b's loads into buffer `buf`: the rows, then the columns and
+    // their scales.  Past the last block nothing is read (zeros are stored).
+    __device__ __forceinline__ void stage_rows(int b, int buf) const {
+        const uint32_t to = lds0 + buf * Buffer + wave * 1024;
+        const uint32_t off = b < nb ? aoff : kPastEnd;
 #pragma unroll
         for (int i = 0; i < ALoads; ++i) {
             const int c = i * W + wave;
-            load_to_lds(ar, aoff + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + i * W * 1024);
-        }
-        if constexpr (Tiles) {
-#pragma unroll
-            for (int i = 0; i < BLoads; ++i) {
-                const int c = i * W + wave;
-                load_to_lds(br, aoff + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + ABytes + i * W * 1024);
-            }
-        } else {
-            const uint32_t lane_off = b + 1 < nb ? boff : boff_last;
-#pragma unroll
-            for (int i = 0; i < BLoads; ++i)
-                load_to_lds(br, lane_off + (8 * (i * W + wave) * K + b * kFp8Block), to + ABytes + i * W * 1024);
+            load_to_lds(ar, off + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + i * W * 1024);
         }
     }
-    __device__ __forceinline__ float scale(int t, int b) const { return xscale[xs[t] + static_cast<uint32_t>(b * scale_b)]; }
+    __device__ __forceinline__ void stage_columns(int b, int buf) const {
+        const uint32_t to = lds0 + buf * Buffer + ABytes + wave * 1024;
+        const uint32_t off = b >= nb ? kPastEnd : Tiles ? aoff : b + 1 < nb ? boff : boff_last;
+#pragma unroll
+        for (int i = 0; i < BLoads; ++i) {
+            const int c = i * W + wave;
+            if constexpr (Tiles)
+                load_to_lds(br, off + ((c >> 1) * tile_row + b * kFp8TileBytes + (c & 1) * 1024), to + i * W * 1024);
+            else
+                load_to_lds(br, off + (8 * c * K + b * kFp8Block), to + i * W * 1024);
+        }
+        load_word_to_lds(sr, b < nb ? soff + b * sstep : kPastEnd, lds0 + buf * Buffer + ABytes + BBytes + wave % (BN / 64) * 256);
+    }
+    // The scale of column l % 16 of column tile t.
+    __device__ __forceinline__ float scale(const uint8_t *buf, int t) const {
+        return *reinterpret_cast<const float *>(buf + sread + t * 64);
+    }
     __device__ __forceinline__ Frag column(const uint8_t *buf, int t) const {
         const uint8_t *p = buf + bread + t * 2048;
         if constexpr (Tiles) return load_tile(p, lane);
@@ -393,42 +405,48 @@ struct GemmTile {
     }
 };
 
+// G groups of WR x WC waves share the tile, group g taking blocks g, g + G, ..
+// through a ring of its own; their sums meet in LDS at the end, in group order.
 // Y: type of y; fp32 results on fp16 operands, the others on e4m3 ones.
-template<int WR, int WC, int TM, int TN, bool Tiles, int Y>
-__global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m) {
-    using Tile = GemmTile<WR, WC, TM, TN, Tiles>;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][Tile::Buffer];
-    const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds);
+template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, int Y>
+__global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m) {
+    using Tile = GemmTile<WR, WC, TM, TN, S, Tiles>;
+    constexpr int Sums = TM * TN * Tile::W * 64 * 16;   // bytes of one group's sums
+    static_assert(G == 1 || Sums <= G * S * Tile::Buffer);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[G][S][Tile::Buffer];
+    const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / Tile::W;
+    const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds[group]);
     f32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int t = 0; t < TN; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-
-    // The scales of a step are loaded during the step before it, and used
-    // before the next loads to LDS are issued: memory answers in order.
-    float sw = g.wscale[0], sx[TN];
 #pragma unroll
-    for (int t = 0; t < TN; ++t) sx[t] = g.scale(t, 0);
-    g.stage(0);
-    for (int b = 0; b < a.nb; ++b) {
-        wait_for_lds_loads();
+    for (int b = 0; b < S - 1; ++b) {
+        g.stage_rows(b * G + group, b);
+        g.stage_columns(b * G + group, b);
+    }
+    int at = 0;   // the step's buffer, step % S
+    for (int b = group; b - group < a.nb; b += G) {
+        // Block b's loads are all but the last S - 2 steps'; memory answers in
+        // order, and past the last block a step still issues as many.
+        wait_for_lds_loads<(S - 2) * Tile::Loads>();
         __syncthreads();
-        float s[TN];
-#pragma unroll
-        for (int t = 0; t < TN; ++t) s[t] = sx[t] * sw;
-        __builtin_amdgcn_sched_barrier(0);
-        const uint8_t *buf = lds[b & 1];
-        if (b + 1 < a.nb) {
-            g.stage(b + 1);
-            sw = g.wscale[b + 1];
-#pragma unroll
-            for (int t = 0; t < TN; ++t) sx[t] = g.scale(t, b + 1);
-        }
+        // Every wave is done with the last step: its buffer takes the one S - 1 ahead.
+        const int next = at == 0 ? S - 1 : at - 1;
+        g.stage_rows(b + (S - 1) * G, next);
+        g.stage_columns(b + (S - 1) * G, next);
+        const uint8_t *buf = lds[group][at];
+        at = at + 1 == S ? 0 : at + 1;
+        const float sw = g.wscale[G == 1 ? b : min(b, a.nb - 1)];   // a group's block past the last: zeros
         using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
         Operand x[TN];
+        float s[TN];
 #pragma unroll
-        for (int t = 0; t < TN; ++t) x[t] = operand<Operand>(g.column(buf, t));
+        for (int t = 0; t < TN; ++t) {
+            x[t] = operand<Operand>(g.column(buf, t));
+            s[t] = g.scale(buf, t) * sw;
+        }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const Operand w = operand<Operand>(g.row(buf, i));
@@ -440,6 +458,28 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int 
             }
         }
     }
+    wait_for_lds_loads<0>();   // no load may outlive the buffers
+    if constexpr (G > 1) {
+        f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + g.wave * 64 + g.lane;   // [tile][wave][lane]
+#pragma unroll
+        for (int q = 1; q < G; ++q) {
+            __syncthreads();
+            if (group == q) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int t = 0; t < TN; ++t) sums[(i * TN + t) * Tile::W * 64] = acc[i][t];
+            }
+            __syncthreads();
+            if (group == 0) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int t = 0; t < TN; ++t) acc[i][t] += sums[(i * TN + t) * Tile::W * 64];
+            }
+        }
+        if (group > 0) return;
+    }
     g.template store<Y>(a, acc);
 }
 
@@ -450,12 +490,12 @@ __global__ __launch_bounds__(64 * WR * WC) void k_fp8_gemm(Fp8LinearArgs a, int 
 //   4 b: read columns, rows 0 .. 3 | 4 b + 1: multiply | 4 b + 2: read rows
 //   4 .. 7 | 4 b + 3: multiply
 // and waves 4 .. 7 one turn behind, block b's buffer is last read in turn 4 b
-// + 3; block b + 1's loads start in turns 4 b and 4 b + 1, into the buffer last
+// + 3; block b + 1's loads start in turns 4 b to 4 b + 2, into the buffer last
 // read in turn 4 b - 1, and each wave waits for its own before the barrier
 // that ends its second read of block b, turn 4 b + 3 at the latest.
 template<bool Tiles, int Y>
 __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tiles_m) {
-    using Tile = GemmTile<2, 4, 8, 4, Tiles>;
+    using Tile = GemmTile<2, 4, 8, 4, 2, Tiles>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][Tile::Buffer];
     const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds);
     f32x4 acc[8][4];
@@ -471,10 +511,9 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    float sw = g.wscale[0], sx[4], s[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) sx[t] = g.scale(t, 0);
-    g.stage(0);
+    float s[4];
+    g.stage_rows(0, 0);
+    g.stage_columns(0, 0);
     turn(true);
     if (g.wr == 1) turn(false);   // waves 4 .. 7: one turn behind
     const auto multiply = [&](const Frag (&w)[4], const Frag (&x)[4], int i0) {
@@ -499,21 +538,18 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
     };
     for (int b = 0; b < a.nb; ++b) {
         const uint8_t *buf = lds[b & 1];
+        const float sw = g.wscale[b];
         Frag x[4], w[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) s[t] = sx[t] * sw;
-        __builtin_amdgcn_sched_barrier(0);
-        if (b + 1 < a.nb) {
-            g.stage(b + 1);
-            sw = g.wscale[b + 1];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) sx[t] = g.scale(t, b + 1);
-        }
 #pragma unroll
         for (int t = 0; t < 4; ++t) x[t] = g.column(buf, t);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = g.row(buf, i);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) s[t] = g.scale(buf, t) * sw;
+        __builtin_amdgcn_sched_barrier(0);
+        if (b + 1 < a.nb) g.stage_rows(b + 1, (b + 1) & 1);
         turn(false);
+        if (b + 1 < a.nb) g.stage_columns(b + 1, (b + 1) & 1);
         multiply(w, x, 0);
         turn(false);
 #pragma unroll
@@ -573,14 +609,14 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     return a;
 }
 
-template<int WR, int WC, int TM, int TN, bool Tiles>
+template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, bool F32>
 int launch_gemm(const moe::Fp8LinearArgs &a, hipStream_t s) {
-    using Tile = moe::GemmTile<WR, WC, TM, TN, Tiles>;
+    using Tile = moe::GemmTile<WR, WC, TM, TN, S, Tiles>;
     const int tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
-    const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * Tile::W);
-    if (a.y_type == MOE_F32) moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
-    else if (a.y_type == MOE_BF16) moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
-    else moe::k_fp8_gemm<WR, WC, TM, TN, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
+    const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * Tile::W * G);
+    if constexpr (F32) moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
+    else if (a.y_type == MOE_BF16) moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
+    else moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
     return hipGetLastError();
 }
 
@@ -602,17 +638,46 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 }
 
 // The product for quantised columns: canonical rows, or Tiles.
+//
+// Small products stream the matrix (16 rows a workgroup, K shared out among
+// its waves); beyond that the output tile grows with the number of tiles, and
+// where there are few the tile's K is shared among groups of waves.  us for
+// apply with bf16 columns, as 64 x 64 tiles in two groups / in two of half as
+// many waves / 128 x 64 / 128 x 128 / 256 x 256 (MI355X, launches in a row):
+//   bf16  2048 x 2048 at   96:   8.7 /  9.4 / 12.5 / 15.9 /  30, streamed 7.2
+//         8192 x 8192 at   96:  20.9 / 24.7 / 37.8 / 47.1 /  94, streamed 33.7
+//         2048 x 2048 at  512:  10.2 / 10.7 / 13.7 / 17.4 /  35
+//         8192 x 8192 at  256:  44.0 / 30.0 / 41.0 / 50.6 / 100
+//         2048 x 2048 at 1032:  21.3 / 18.8 / 16.2 / 19.4 /  36
+//         2048 x 2048 at 4096:  52.3 / 39.5 / 36.7 / 32.9 /  42
+//         2048 x 2048 at 8192, 128 x 128 against 256 x 256: 61.2 / 52.2
+//         8192 x 8192 at 2048 / 4096: 158 / 184 and 331 / 300
+//   fp32, 64 x 64 in four groups / in two of half as many waves / 128 x 128 in
+//         two groups / 128 x 128:
+//         8192 x 8192 at   96:  26.7 / 28.4 / 63.5 / 73.3, streamed 34.4
+//         2048 x 2048 at 1032:  28.7 / 24.1 / 25.8 / 27.3
+//         8192 x 8192 at  512:  98.1 / 85.8 / 70.3 / 78.7
+//         2048 x 2048 at 4096:  72.3 / 56.8 / 54.1 / 47.4; 256 x 256 76.0
 template<bool Tiles>
 int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
     constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
     if (a.N <= 16) return launch_stream<IN, 1>(a, s);
     if (a.N <= 32) return launch_stream<IN, 2>(a, s);
     if (a.N <= 64) return launch_stream<IN, 4>(a, s);
-    const long big = static_cast<long>((a.M + 255) / 256) * ((a.N + 255) / 256);
-    if (big >= 200) return a.y_type == MOE_F32 ? launch_gemm<2, 4, 8, 4, Tiles>(a, s) : launch_gemm_wide<Tiles>(a, s);
-    const long mid = static_cast<long>((a.M + 127) / 128) * ((a.N + 127) / 128);
-    if (mid >= 200) return launch_gemm<2, 2, 4, 4, Tiles>(a, s);
-    return launch_gemm<2, 2, 2, 2, Tiles>(a, s);
+    const auto tiles = [&](long m, long n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
+    if (static_cast<long>(a.M) * a.N <= 320 * 1024)
+        return tiles(16, 64) >= 256 ? launch_stream<IN, 4>(a, s) : launch_stream<IN, 2>(a, s);
+    if (a.y_type == MOE_F32) {
+        if (tiles(64, 64) <= 256) return launch_gemm<2, 2, 2, 2, 2, 4, Tiles, true>(a, s);
+        if (tiles(64, 64) <= 800) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, true>(a, s);
+        if (tiles(128, 128) <= 400) return launch_gemm<2, 2, 4, 4, 2, 2, Tiles, true>(a, s);
+        return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, true>(a, s);
+    }
+    if (tiles(64, 64) <= 256) return launch_gemm<2, 2, 2, 2, 3, 2, Tiles, false>(a, s);
+    if (tiles(64, 64) <= 512) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, false>(a, s);
+    if (tiles(128, 128) < 256) return launch_gemm<2, 2, 4, 2, 2, 1, Tiles, false>(a, s);
+    if (tiles(256, 256) < 240 || (tiles(256, 256) < 512 && a.nb > 32)) return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, false>(a, s);
+    return launch_gemm_wide<Tiles>(a, s);
 }
 
 }  // namespace

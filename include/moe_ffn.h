@@ -377,7 +377,7 @@ int moe_fp8_linear_bytes(const moe_fp8_linear *linear, size_t *weight_bytes);
  * [columns][input] (16-byte aligned) with x_scales; y rows are y_stride
  * elements of y_type apart.  Each block's sum is multiplied by both scales
  * into an fp32 sum over the blocks, rounded once to y_type.  The sum within a
- * block is fp32 when y_type is MOE_F32 or columns <= 64; wider batches with
+ * block is fp32 when y_type is MOE_F32 or columns <= 64; larger products with
  * 16-bit results use the e4m3 matrix instructions, which drop what is more
  * than about 14 bits below a block's largest product.  columns 1..65536.  No
  * workspace: calls on one handle may overlap.  The rows between y's columns
