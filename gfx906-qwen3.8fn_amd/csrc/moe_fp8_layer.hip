@@ -1,14 +1,15 @@
 // A routed-expert layer of e4m3 matrices for a few tokens (moe_fp8_layer_*),
 // in two launches:
-//   gate_up    per (expert that a token reaches, 16 intermediate rows): the
-//              tokens' rows quantised to e4m3, gate and up products, SiLU(g) u
-//   down_fold  per (token, 16 or 32 output rows): each rank's middle row
+//   gate_up    per (expert that a token reaches, slice of intermediate rows):
+//              the tokens' rows quantised to e4m3, gate and up products, SiLU(g) u
+//   down_fold  per (token, slice of output rows): each rank's middle row
 //              quantised, its down product, and the weighted sum in rank order
 //              with the shared expert
 // Both are bound by the experts' bytes (6 H I flops a token and expert against
-// 3 H I bytes an expert): every byte of a reached expert's gate and up is read
-// once however many tokens share it; down rows that tokens share are read by
-// workgroups of one XCD at about the same time, so that its L2 serves them.
+// 3 H I bytes an expert).  gate_up reads every byte of a reached expert once
+// however many tokens share it; down_fold reads an expert's rows for each of
+// its tokens, by workgroups of one XCD at about the same time, so that its L2
+// serves all but the first.
 #include "moe_ffn.h"
 #include "moe_fp8.hpp"
 
@@ -17,7 +18,7 @@
 
 namespace moe {
 
-inline constexpr int kFp8LayerTokens = 64;   // tokens of one forward: one lane each in the grouping
+inline constexpr int kFp8LayerTokens = 64;   // tokens of one forward: a lane each in the grouping
 
 namespace {
 
@@ -35,267 +36,427 @@ struct Fp8LayerArgs {
     int nbh, nbi;
 };
 
-inline constexpr int kChunk = 24;   // blocks of K whose rows a gate/up workgroup holds in LDS: 50 KB
+inline constexpr int kTileWaves = 4, kRowTiles = 8 / kTileWaves;   // waves of a row tile, row tiles of a gate_up item
+inline constexpr int kGateUpGroups = 512;   // workgroups of gate_up: two a CU
+inline constexpr int kChunk = 24;   // blocks of K whose columns a workgroup holds in LDS: 50 KB
 
-// ------------------------------------------------------------ gate and up ---
-// Workgroup (p, s): route p = t k + r (p = T k: the shared expert), rows 16 s
-// .. + 15.  It goes on if no earlier route names the same expert and takes all
-// tokens that do, in columns of 16.  Wave w multiplies blocks w, w + W, ..;
-// the partial sums meet in LDS, in wave order.
-template<int T_>
-__global__ __launch_bounds__(512) void k_fp8_gate_up(Fp8LayerArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // x codes [blocks][2048], scales [blocks][16]; then the sums
-    __shared__ int rank_of[kFp8LayerTokens], token[kFp8LayerTokens], rank[kFp8LayerTokens], counted;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
-    const int S = a.I / 16, s = blockIdx.x % S, p = blockIdx.x / S, routes = a.T * a.k;
-    const bool shared = p == routes;
-    if (s == 0 && !shared && p % a.k == 0) {
-        // The token's input flags, whatever becomes of its routes.
-        const size_t row = static_cast<size_t>(p / a.k) * a.H;
-        bool bad = false;
-        for (int i = threadIdx.x; i < a.H; i += blockDim.x) bad |= !isfinite(load1<T_>(a.x, row + i));
-        if (bad) atomicOr(a.error, 1);
-    }
-    const int e = shared ? a.E : a.ids[p];
-    if (!shared && (e < 0 || e >= a.E)) return;   // flagged by down_fold
-    if (threadIdx.x < kFp8LayerTokens) rank_of[threadIdx.x] = shared && static_cast<int>(threadIdx.x) < a.T ? a.k : INT_MAX;
-    __syncthreads();
-    int earlier = 0;
-    if (!shared) {
-        for (int q = threadIdx.x; q < routes; q += blockDim.x) {
-            if (a.ids[q] != e) continue;
-            if (q < p) earlier = 1;
-            atomicMin(&rank_of[q / a.k], q % a.k);
+// The routes of the batch, in the registers of a workgroup of 512 threads:
+// thread i holds ids i, i + 512, .. (-1 past the last, and for bad ids).
+struct Routes {
+    static constexpr int Own = kFp8LayerTokens * 32 / 512;
+    int id[Own];
+    __device__ __forceinline__ explicit Routes(const Fp8LayerArgs &a) {
+        const int routes = a.T * a.k;
+#pragma unroll
+        for (int i = 0; i < Own; ++i) {
+            const int q = threadIdx.x + i * 512;
+            const int e = q < routes ? a.ids[q] : -1;
+            id[i] = e < a.E ? e : -1;
         }
     }
-    if (__syncthreads_or(earlier)) return;
-    if (wave == 0) {
-        const int r = rank_of[lane];
+};
+
+// The experts that the batch reaches, each once: the shared expert, then the
+// others in the order of their first routes.  Returns their number.
+// first [E]: scratch in LDS; list: up to 1 + T k.
+__device__ __forceinline__ int list_experts(const Fp8LayerArgs &a, const Routes &q, int *first, int *list) {
+    __shared__ int counts[Routes::Own * 8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, shared = a.P1 > a.k ? 1 : 0;
+    if (a.T * a.k <= 64) {
+        // Every wave on its own, a route a lane.
+        int mine = lane < a.T * a.k ? a.ids[lane] : -1;
+        if (mine >= a.E) mine = -1;
+        bool later = mine < 0;
+        for (int i = 0; i + 1 < a.T * a.k; ++i) later |= lane > i && mine == __builtin_amdgcn_readlane(mine, i);
+        const uint64_t is_first = __builtin_amdgcn_ballot_w64(!later);
+        if (wave == 0) {
+            if (lane == 0 && shared) list[0] = a.E;
+            if (!later) list[shared + __builtin_popcountll(is_first & ((uint64_t{1} << lane) - 1))] = mine;
+        }
+        __syncthreads();
+        return shared + __builtin_popcountll(is_first);
+    }
+    for (int i = threadIdx.x; i < a.E; i += 512) first[i] = INT_MAX;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < Routes::Own; ++i)
+        if (q.id[i] >= 0) atomicMin(&first[q.id[i]], static_cast<int>(threadIdx.x) + i * 512);
+    __syncthreads();
+    uint64_t is_first[Routes::Own];
+#pragma unroll
+    for (int i = 0; i < Routes::Own; ++i) {
+        is_first[i] = __builtin_amdgcn_ballot_w64(q.id[i] >= 0 && first[q.id[i] >= 0 ? q.id[i] : 0] ==
+                                                                      static_cast<int>(threadIdx.x) + i * 512);
+        if (lane == 0) counts[i * 8 + wave] = __builtin_popcountll(is_first[i]);
+    }
+    if (threadIdx.x == 0 && shared) list[0] = a.E;
+    __syncthreads();
+    int before = shared, total = shared;
+    for (int i = 0; i < Routes::Own * 8; ++i) total += counts[i];
+#pragma unroll
+    for (int i = 0; i < Routes::Own; ++i) {
+        before = shared;
+        for (int j = 0; j < i * 8 + wave; ++j) before += counts[j];
+        if (is_first[i] >> lane & 1) list[before + __builtin_popcountll(is_first[i] & ((uint64_t{1} << lane) - 1))] = q.id[i];
+    }
+    __syncthreads();
+    return total;
+}
+
+// The tokens of one expert and its rank in each, in token order; a token's
+// repeat of an id counts at its first rank.
+struct Members {
+    int rank_of[kFp8LayerTokens];
+    int token[kFp8LayerTokens], rank[kFp8LayerTokens];
+    int count;
+};
+__device__ __forceinline__ int find_members(const Fp8LayerArgs &a, const Routes &q, int e, Members &m) {
+    const int lane = threadIdx.x & 63;
+    if (a.T == 1) {
+        if (threadIdx.x < 64) {
+            const uint64_t at = __builtin_amdgcn_ballot_w64(q.id[0] == e);   // e of the batch's own, or the shared one
+            if (lane == 0) {
+                m.token[0] = 0;
+                m.rank[0] = e == a.E ? a.k : __builtin_ctzll(at);
+            }
+        }
+        __syncthreads();
+        return 1;
+    }
+    if (threadIdx.x < kFp8LayerTokens)
+        m.rank_of[threadIdx.x] = e == a.E && static_cast<int>(threadIdx.x) < a.T ? a.k : INT_MAX;
+    __syncthreads();
+    if (e < a.E) {
+#pragma unroll
+        for (int i = 0; i < Routes::Own; ++i) {
+            const int r = threadIdx.x + i * 512;
+            if (q.id[i] == e) atomicMin(&m.rank_of[r / a.k], r % a.k);
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x < 64) {
+        const int r = m.rank_of[lane];
         const uint64_t in = __builtin_amdgcn_ballot_w64(r != INT_MAX);
         if (r != INT_MAX) {
             const int at = __builtin_popcountll(in & ((uint64_t{1} << lane) - 1));
-            token[at] = lane;
-            rank[at] = r;
+            m.token[at] = lane;
+            m.rank[at] = r;
         }
-        if (lane == 0) counted = __builtin_popcountll(in);
+        if (lane == 0) m.count = __builtin_popcountll(in);
     }
-    const size_t tile0 = (static_cast<size_t>(e) * S + s) * a.nbh;
-    const uint8_t *gw = a.gate + tile0 * kFp8TileBytes, *uw = a.up + tile0 * kFp8TileBytes;
-    const size_t scale0 = (static_cast<size_t>(e) * ((a.I + kFp8Block - 1) / kFp8Block) + s * 16 / kFp8Block) * a.nbh;
-    const float *gs = a.gate_s + scale0, *us = a.up_s + scale0;
-    constexpr int U = 2;   // blocks whose loads are in flight together
     __syncthreads();
-    const int count = __builtin_amdgcn_readfirstlane(counted);
+    return __builtin_amdgcn_readfirstlane(m.count);
+}
 
-    for (int c0 = 0; c0 < count; c0 += 16) {
-        const int cols = min(16, count - c0);
-        f32x4 ga = {0.0f, 0.0f, 0.0f, 0.0f}, ua = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < a.nbh; k0 += kChunk) {
-            const int kb = min(kChunk, a.nbh - k0);
-            float *xs = reinterpret_cast<float *>(lds + kb * kFp8TileBytes);
-            Frag gf[U], uf[U];
-            auto load = [&](int b0) {
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    // Past the chunk: the round's first block again, not used below.
-                    const int b = k0 + (b0 + u * W < kb ? b0 + u * W : b0);
-                    gf[u] = load_tile(gw + static_cast<size_t>(b) * kFp8TileBytes, lane);
-                    uf[u] = load_tile(uw + static_cast<size_t>(b) * kFp8TileBytes, lane);
-                }
-            };
-            if (wave < kb) load(wave);
-            // The columns' blocks, 16 threads each.
-            for (int i = threadIdx.x >> 4; i < cols * kb; i += blockDim.x >> 4) {
-                const int c = i / kb, b = i % kb, part = threadIdx.x & 15, col = (k0 + b) * kFp8Block + part * 8;
-                Raw8 raw{};
-                if (col < a.H) raw = load8_raw<T_>(a.x, static_cast<size_t>(token[c0 + c]) * a.H + col);
-                float v[8];
-                unpack8<T_>(raw, v);
-                const GroupScale g = group_scale(max16(v));
-                *reinterpret_cast<uint2 *>(lds + b * kFp8TileBytes + tile_offset(part, c)) = quantize8(v, g);
-                if (part == 0) xs[b * 16 + c] = g.s;
-            }
-            __syncthreads();
-            for (int b0 = wave; b0 < kb; b0 += W * U) {
-                if (b0 != wave) load(b0);
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int b = b0 + u * W;
-                    if (b >= kb) break;
-                    const FragF16 x = to_f16(load_tile(lds + b * kFp8TileBytes, lane));
-                    const float sx = xs[b * 16 + (lane & 15)];
-                    const f32x4 gp = block_dot(to_f16(gf[u]), x), upr = block_dot(to_f16(uf[u]), x);
-                    const float sg = sx * gs[k0 + b], su = sx * us[k0 + b];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        ga[q] = fmaf(gp[q], sg, ga[q]);
-                        ua[q] = fmaf(upr[q], su, ua[q]);
-                    }
-                }
-            }
-            __syncthreads();   // the rows are used up
-        }
-        f32x4 *red = reinterpret_cast<f32x4 *>(lds);   // [wave][gate, up][lane]
-        red[(wave * 2 + 0) * 64 + lane] = ga;
-        red[(wave * 2 + 1) * 64 + lane] = ua;
-        __syncthreads();
-        // Sum i: row 4 (lane / 16) + i % 4 of column lane % 16, lane = i / 4.
-        const float *sum = reinterpret_cast<const float *>(lds);
-        int flags = 0;
-        for (int i = threadIdx.x; i < 256; i += blockDim.x) {
-            const int c = (i >> 2) & 15, row = (i >> 6) * 4 + (i & 3);
-            if (c >= cols) continue;
-            float g = sum[i], u = sum[256 + i];
-            for (int q = 1; q < W; ++q) {
-                g = g + sum[q * 512 + i];
-                u = u + sum[q * 512 + 256 + i];
-            }
-            const size_t pair = static_cast<size_t>(token[c0 + c]) * a.P1 + rank[c0 + c];
-            a.middle[pair * a.I + s * 16 + row] = silu_mul(g, u, flags);
-        }
-        if (flags) atomicOr(a.error, flags);
-        __syncthreads();   // the sums are used up
+// Blocks k0 .. k0 + kb - 1 of `cols` rows of x (row i at rows(i), K elements
+// of type T_) as one operand tile a block in LDS, and their scales [block][16].
+// 16 threads a block.
+template<int T_, class Rows>
+__device__ __forceinline__ void quantize_columns(const void *x, Rows rows, int cols, int K, int k0, int kb, uint8_t *tiles,
+                                                 float *scales) {
+    const int part = threadIdx.x & 15;
+    for (int i = threadIdx.x >> 4; i < cols * kb; i += 512 / 16) {
+        const int c = i / kb, b = i % kb, col = (k0 + b) * kFp8Block + part * 8;
+        Raw8 raw{};
+        if (col < K) raw = load8_raw<T_>(x, rows(c) + col);
+        float v[8];
+        unpack8<T_>(raw, v);
+        const GroupScale g = group_scale(max16(v));
+        *reinterpret_cast<uint2 *>(tiles + b * kFp8TileBytes + tile_offset(part, c)) = quantize8(v, g);
+        if (part == 0) scales[b * 16 + c] = g.s;
     }
 }
 
+// ------------------------------------------------------------ gate and up ---
+// Work item (expert, s): two tiles of 16 rows, four waves a tile, of which wave
+// w multiplies blocks w, w + 4, .. of all of the expert's tokens, 16 at a time;
+// the sums meet in LDS, in wave order.  A workgroup lists the experts and takes
+// items in turn, each with its first tiles on their way before the last one's
+// sums are done.  64 tokens, 2048/512, layer time in us with top-10 of 512
+// uniform / Zipf(1.1): 274 / 205 with a workgroup per route and slice, of
+// which those of an expert's later routes end at once, 244 / 170 so; with
+// eight or two waves a tile 258 / 191 and 251 / 178.  Four waves a SIMD (two
+// workgroups a CU): with two blocks a round in flight the kernel needs 167
+// registers and one fits (268 / 185).
+template<int T_>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k_fp8_gate_up(Fp8LayerArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];   // column tiles [blocks][2048], scales [blocks][16]; then the sums
+    __shared__ Members m;
+    __shared__ int list[1 + kFp8LayerTokens * 32];
+    constexpr int KW = kTileWaves, RW = kRowTiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kw = wave % KW, rw = wave / KW;
+    const int row_tiles = a.I / 16, S = (row_tiles + RW - 1) / RW;
+    for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
+        // A token's input flags, whatever becomes of its routes.
+        bool bad = false;
+        for (int i = threadIdx.x; i < a.H; i += 512) bad |= !isfinite(load1<T_>(a.x, static_cast<size_t>(t) * a.H + i));
+        if (bad) atomicOr(a.error, 1);
+    }
+    const Routes routes(a);
+    const int items = list_experts(a, routes, reinterpret_cast<int *>(lds), list) * S;
+    constexpr int U = 1;   // blocks a round; the next round's loads are on their way during one
+    Frag gf[2][U], uf[2][U];
+    const uint8_t *gw = a.gate, *uw = a.up;
+    // Blocks k0 + b0, + KW, .. of an item's tile; past the chunk its last block again, not used.
+    auto load = [&](int k0, int kb, int b0, Frag (&g)[U], Frag (&v)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t b = k0 + min(b0 + u * KW, kb - 1);
+            g[u] = load_tile(gw + b * kFp8TileBytes, lane);
+            v[u] = load_tile(uw + b * kFp8TileBytes, lane);
+        }
+    };
+    // The last slice may have fewer tiles: its other waves take the last one again.
+    auto select = [&](int item) {
+        const int e = __builtin_amdgcn_readfirstlane(list[item / S]), tile = min(item % S * RW + rw, row_tiles - 1);
+        const size_t at = (static_cast<size_t>(e) * row_tiles + tile) * a.nbh * kFp8TileBytes;
+        gw = a.gate + at;
+        uw = a.up + at;
+        load(0, min(kChunk, a.nbh), kw, gf[0], uf[0]);
+        return e;
+    };
+    int flags = 0, e = static_cast<int>(blockIdx.x) < items ? select(blockIdx.x) : 0;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int s = item % S, tile = min(s * RW + rw, row_tiles - 1);
+        const int count = find_members(a, routes, e, m);
+        const size_t scale0 = (static_cast<size_t>(e) * ((a.I + kFp8Block - 1) / kFp8Block) + tile * 16 / kFp8Block) * a.nbh;
+        const float *gs = a.gate_s + scale0, *us = a.up_s + scale0;
+        for (int c0 = 0; c0 < count; c0 += 16) {
+            const int cols = min(16, count - c0);
+            f32x4 ga = {0.0f, 0.0f, 0.0f, 0.0f}, ua = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int k0 = 0; k0 < a.nbh; k0 += kChunk) {
+                const int kb = min(kChunk, a.nbh - k0);
+                float *xs = reinterpret_cast<float *>(lds + kb * kFp8TileBytes);
+                auto multiply = [&](int b0, const Frag (&g)[U], const Frag (&v)[U]) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int b = b0 + u * KW;
+                        if (b >= kb) break;
+                        const FragF16 x = to_f16(load_tile(lds + b * kFp8TileBytes, lane));
+                        const float sx = xs[b * 16 + (lane & 15)];
+                        const f32x4 gp = block_dot(to_f16(g[u]), x), up = block_dot(to_f16(v[u]), x);
+                        const float sg = sx * gs[k0 + b], su = sx * us[k0 + b];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            ga[q] = fmaf(gp[q], sg, ga[q]);
+                            ua[q] = fmaf(up[q], su, ua[q]);
+                        }
+                    }
+                };
+                if (c0 > 0 || k0 > 0) load(k0, kb, kw, gf[0], uf[0]);
+                quantize_columns<T_>(a.x, [&](int c) { return static_cast<size_t>(m.token[c0 + c]) * a.H; }, cols, a.H, k0, kb, lds, xs);
+                __syncthreads();
+                for (int b0 = kw; b0 < kb; b0 += 2 * KW * U) {
+                    if (b0 + KW * U < kb) load(k0, kb, b0 + KW * U, gf[1], uf[1]);
+                    multiply(b0, gf[0], uf[0]);
+                    if (b0 + 2 * KW * U < kb) load(k0, kb, b0 + 2 * KW * U, gf[0], uf[0]);
+                    multiply(b0 + KW * U, gf[1], uf[1]);
+                }
+                __syncthreads();   // the columns are used up
+            }
+            f32x4 *red = reinterpret_cast<f32x4 *>(lds);   // [wave][gate, up][lane]
+            red[(wave * 2 + 0) * 64 + lane] = ga;
+            red[(wave * 2 + 1) * 64 + lane] = ua;
+            if (c0 + 16 >= count && item + static_cast<int>(gridDim.x) < items) e = select(item + gridDim.x);
+            __syncthreads();
+            // Sum i of a row tile: row 4 (lane / 16) + i % 4 of column lane % 16, lane = i / 4.
+            const float *sum = reinterpret_cast<const float *>(lds);
+            for (int i = threadIdx.x; i < 256 * RW; i += 512) {
+                const int r = i >> 8, j = i & 255, c = (j >> 2) & 15, row = (s * RW + r) * 16 + (j >> 6) * 4 + (j & 3);
+                if (c >= cols || row >= a.I) continue;
+                const float *w = sum + r * KW * 512 + j;
+                float g = w[0], u = w[256];
+#pragma unroll
+                for (int q = 1; q < KW; ++q) {
+                    g = g + w[q * 512];
+                    u = u + w[q * 512 + 256];
+                }
+                const size_t pair = static_cast<size_t>(m.token[c0 + c]) * a.P1 + m.rank[c0 + c];
+                a.middle[pair * a.I + row] = silu_mul(g, u, flags);
+            }
+            __syncthreads();   // the sums are used up
+        }
+    }
+    if (flags) atomicOr(a.error, flags);
+}
+
+// y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags
+// of moe_ffn_forward's sum.  c(r): rank r's output, of the routes that count.
+template<class C>
+__device__ __forceinline__ float fold(int k, bool shared, bool gated, const int *valid, const float *weight, C c, int &flags) {
+    int f = 0;
+    float v = 0.0f;
+    for (int r = 0; r < k; ++r) {
+        if (!valid[r]) continue;
+        float x = c(r), w = weight[r];
+        if (!isfinite(x)) { f |= 1; x = 0.0f; }
+        if (!isfinite(w)) { f |= 1; w = 0.0f; }
+        float q = w * x;
+        if (!isfinite(q)) { f |= 2; q = 0.0f; }
+        v = v + q;
+        if (!isfinite(v)) { f |= 2; v = 0.0f; }
+    }
+    if (f) v = 0.0f;
+    int sf = 0;
+    if (shared) {
+        float x = c(k), scale = 1.0f;
+        if (!isfinite(x)) { sf |= 1; x = 0.0f; }
+        if (gated) {
+            float g = weight[k];
+            if (!isfinite(g)) { sf |= 1; g = 0.0f; }
+            scale = 1.0f / (1.0f + moe_expf(-g));
+            if (!isfinite(scale)) { sf |= 2; scale = 0.0f; }
+        }
+        v = v + scale * x;
+        if (!isfinite(v)) { sf |= 2; v = 0.0f; }
+    }
+    flags |= f | sf;
+    return sf ? 0.0f : v;
+}
+
+inline constexpr int kMaxPairs = 33;   // 32 routes and the shared expert
+
+// Route r of token t, by a whole wave: its expert (the shared one for r = k),
+// -1 for a bad id or a repeat of an earlier rank; its weight or gate.
+__device__ __forceinline__ int route(const Fp8LayerArgs &a, int t, int r, float &w, int &flags) {
+    if (r == a.k) {
+        w = a.shared_gate ? a.shared_gate[t] : 1.0f;
+        return a.E;
+    }
+    const int lane = threadIdx.x & 63;
+    const int mine = lane < a.k ? a.ids[t * a.k + lane] : -1;
+    w = a.weights[t * a.k + r];
+    const int e = __builtin_amdgcn_readlane(mine, r);
+    if (!isfinite(w) || w < 0.0f) flags |= 1;
+    if (e < 0 || e >= a.E || __builtin_amdgcn_ballot_w64(lane < r && mine == e)) {
+        flags |= 1;
+        return -1;
+    }
+    return e;
+}
+
 // ------------------------------------------------------- down and the sum ---
-// Workgroup (t, slice of 16 RT rows); wave w takes ranks w, w + W, ..  All 16
-// columns of its MFMA hold the one token, so every lane has its results.
-template<int T_, int RT>
-__global__ __launch_bounds__(1024) void k_fp8_down_fold(Fp8LayerArgs a) {
-    constexpr int R = 16 * RT, MaxPairs = 33;
-    constexpr int KB = 4;   // blocks in flight together: 64 lanes x 8 elements
-    __shared__ __attribute__((aligned(16))) uint8_t codes[16][KB * kFp8Block];
-    __shared__ float scales[16][KB];
-    __shared__ float part[MaxPairs][R];
-    __shared__ float weight[MaxPairs];
-    __shared__ int valid[MaxPairs];
+// Workgroup (t, slice of 16 `tiles` rows); wave w takes ranks w, w + W, ..  It
+// quantises the rank's middle row in pieces of eight blocks and streams the
+// expert's row tiles past it, U blocks a round with the next round's loads on
+// their way.  All 16 columns of its MFMA hold the one token, so every lane has
+// its results.
+// Six waves a SIMD: two workgroups of eleven waves (top-10 and the shared
+// expert) fit a CU, one streaming while the other starts or sums up.
+inline constexpr int kDownPiece = 8, kDownTiles = 16;
+template<int T_>
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(6))) void k_fp8_down_fold(Fp8LayerArgs a, int tiles) {
+    extern __shared__ __attribute__((aligned(16))) float part[];   // [rank][16 tiles]
+    __shared__ __attribute__((aligned(16))) uint8_t codes[16][kDownPiece * kFp8Block];
+    __shared__ float scales[16][kDownPiece];
+    constexpr int U = 2;
+    const int R = 16 * tiles;
+    __shared__ float weight[kMaxPairs];
+    __shared__ int valid[kMaxPairs];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
     // Workgroup i runs on XCD i % 8: all tokens of one slice on one XCD, one
     // after the other, so that experts they share come from its L2.
-    const int S = a.H / R, j = blockIdx.x >> 3, t = j % a.T, s = (blockIdx.x & 7) + 8 * (j / a.T);
+    const int row_tiles = a.H / 16, S = (row_tiles + tiles - 1) / tiles;
+    const int j = blockIdx.x >> 3, t = j % a.T, s = (blockIdx.x & 7) + 8 * (j / a.T);
     if (s >= S) return;
-    const int m0 = s * R;
+    const int tile0 = s * tiles, here = min(tiles, row_tiles - tile0);   // this slice's tiles
     int flags = 0;
     for (int r = wave; r < a.P1; r += W) {
-        // The route: a bad id and a repeat of an earlier rank are dropped.
-        int e = a.E;
-        float w = 1.0f;
-        if (r < a.k) {
-            const int mine = lane < a.k ? a.ids[t * a.k + lane] : -1;
-            w = a.weights[t * a.k + r];
-            e = __builtin_amdgcn_readlane(mine, r);
-            if (!isfinite(w) || w < 0.0f) flags |= 1;
-            if (e < 0 || e >= a.E || __builtin_amdgcn_ballot_w64(lane < r && mine == e)) {
-                flags |= 1;
-                e = -1;
-            }
-        } else if (a.shared_gate) {
-            w = a.shared_gate[t];
-        }
+        float w;
+        const int e = route(a, t, r, w, flags);
         if (lane == 0) {
             weight[r] = w;
             valid[r] = e >= 0;
         }
         if (e < 0) continue;
-        const uint8_t *dw = a.down + (static_cast<size_t>(e) * (a.H / 16) + m0 / 16) * a.nbi * kFp8TileBytes;
-        const float *ds = a.down_s + (static_cast<size_t>(e) * ((a.H + kFp8Block - 1) / kFp8Block) + m0 / kFp8Block) * a.nbi;
+        const uint8_t *dw = a.down + (static_cast<size_t>(e) * row_tiles + tile0) * a.nbi * kFp8TileBytes;
+        const float *ds = a.down_s + static_cast<size_t>(e) * ((a.H + kFp8Block - 1) / kFp8Block) * a.nbi;
         const float *mid = a.middle + (static_cast<size_t>(t) * a.P1 + r) * a.I;
-        f32x4 acc[RT];
+        for (int k0 = 0; k0 < a.nbi; k0 += kDownPiece) {
+            const int kb = min(kDownPiece, a.nbi - k0), rounds = (kb + U - 1) / U, n1 = here * rounds;
+            Frag wf[2][U];
+            // Round n: tile n / rounds, blocks U (n % rounds) .. of the piece.
+            const auto load = [&](int n, Frag (&f)[U]) {
+                const size_t tile = min(n / rounds, here - 1);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k0 = 0; k0 < a.nbi; k0 += KB) {
-            const int kb = min(KB, a.nbi - k0);
-            Frag wf[KB][RT];
+                for (int u = 0; u < U; ++u)   // past the piece: its last block again, not used
+                    f[u] = load_tile(dw + (tile * a.nbi + k0 + min(n % rounds * U + u, kb - 1)) * kFp8TileBytes, lane);
+            };
+            load(0, wf[0]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last piece's reads are done
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                const int at = k0 + min(b, kb - 1);   // past the row's end: its last block again, not used
-#pragma unroll
-                for (int i = 0; i < RT; ++i) wf[b][i] = load_tile(dw + (static_cast<size_t>(i) * a.nbi + at) * kFp8TileBytes, lane);
+            for (int h = 0; h < kDownPiece / 4; ++h) {
+                // Lane l: elements 8 l .. + 7 of 512.
+                const int col = (k0 + 4 * h) * kFp8Block + lane * 8;
+                if (4 * h >= kb) break;
+                Raw8 raw{};
+                if (col < a.I) raw = load8_raw<kF32>(mid, col);
+                float v[8];
+                unpack8<kF32>(raw, v);
+                const GroupScale g = group_scale(max16(v));
+                *reinterpret_cast<uint2 *>(&codes[wave][h * 512 + lane * 8]) = quantize8(v, g);
+                if ((lane & 15) == 0) scales[wave][4 * h + (lane >> 4)] = g.s;
             }
-            // Lane l: elements 8 l .. + 7 of the row's next 512.
-            const int col = k0 * kFp8Block + lane * 8;
-            Raw8 raw{};
-            if (col < a.I) raw = load8_raw<kF32>(mid, col);
-            float v[8];
-            unpack8<kF32>(raw, v);
-            const GroupScale g = group_scale(max16(v));
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last round's reads are done
-            *reinterpret_cast<uint2 *>(&codes[wave][lane * 8]) = quantize8(v, g);
-            if ((lane & 15) == 0) scales[wave][lane >> 4] = g.s;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+            f32x4 acc;
+            const auto multiply = [&](int n, const Frag (&f)[U]) {
+                const int tile = n / rounds, q = n % rounds;
+                const float *sw = ds + (tile0 + tile) * 16 / kFp8Block * a.nbi + k0;
+                f32x4 *out = reinterpret_cast<f32x4 *>(&part[r * R + 16 * tile + (lane >> 4) * 4]);
+                if (q == 0) acc = k0 > 0 ? *out : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int b = 0; b < KB; ++b) {
-                if (b >= kb) break;
-                const uint4 *c = reinterpret_cast<const uint4 *>(&codes[wave][b * kFp8Block + (lane >> 4) * 32]);
-                const FragF16 x = to_f16(Frag{c[0], c[1]});
-                const float sc = scales[wave][b] * ds[k0 + b];
+                for (int u = 0; u < U; ++u) {
+                    const int b = q * U + u;
+                    if (b >= kb) break;
+                    const uint4 *c = reinterpret_cast<const uint4 *>(&codes[wave][b * kFp8Block + (lane >> 4) * 32]);
+                    const f32x4 p = block_dot(to_f16(f[u]), to_f16(Frag{c[0], c[1]}));
+                    const float sc = scales[wave][b] * sw[b];
 #pragma unroll
-                for (int i = 0; i < RT; ++i) {
-                    const f32x4 p = block_dot(to_f16(wf[b][i]), x);
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) acc[i][q] = fmaf(p[q], sc, acc[i][q]);
+                    for (int i = 0; i < 4; ++i) acc[i] = fmaf(p[i], sc, acc[i]);
                 }
+                if (q == rounds - 1 && (lane & 15) == 0) *out = acc;
+            };
+            for (int n = 0; n < n1; n += 2) {
+                load(n + 1, wf[1]);
+                multiply(n, wf[0]);
+                if (n + 1 >= n1) break;
+                load(n + 2, wf[0]);
+                multiply(n + 1, wf[1]);
             }
-        }
-        if ((lane & 15) == 0) {
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) part[r][16 * i + (lane >> 4) * 4 + q] = acc[i][q];
         }
     }
     if (s == 0 && flags && lane == 0) atomicOr(a.error, flags);
     __syncthreads();
-    if (threadIdx.x < R) {
-        // y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the
-        // flags of moe_ffn_forward's sum.
-        const int row = threadIdx.x;
+    for (int row = threadIdx.x; row < here * 16; row += blockDim.x) {
         int f = 0;
-        float v = 0.0f;
-        for (int r = 0; r < a.k; ++r) {
-            if (!valid[r]) continue;
-            float c = part[r][row], w = weight[r];
-            if (!isfinite(c)) { f |= 1; c = 0.0f; }
-            if (!isfinite(w)) { f |= 1; w = 0.0f; }
-            float q = w * c;
-            if (!isfinite(q)) { f |= 2; q = 0.0f; }
-            v = v + q;
-            if (!isfinite(v)) { f |= 2; v = 0.0f; }
-        }
-        if (f) v = 0.0f;
-        int sf = 0;
-        if (a.P1 > a.k) {
-            float c = part[a.k][row], scale = 1.0f;
-            if (!isfinite(c)) { sf |= 1; c = 0.0f; }
-            if (a.shared_gate) {
-                float g = weight[a.k];
-                if (!isfinite(g)) { sf |= 1; g = 0.0f; }
-                scale = 1.0f / (1.0f + moe_expf(-g));
-                if (!isfinite(scale)) { sf |= 2; scale = 0.0f; }
-            }
-            const float q = scale * c;
-            v = v + q;
-            if (!isfinite(v)) { sf |= 2; v = 0.0f; }
-        }
-        store1<T_>(a.y, static_cast<size_t>(t) * a.H + m0 + row, sf ? 0.0f : v);
-        if (f | sf) atomicOr(a.error, f | sf);
+        const float v = fold(a.k, a.P1 > a.k, a.shared_gate != nullptr, valid, weight, [&](int r) { return part[r * R + row]; }, f);
+        store1<T_>(a.y, static_cast<size_t>(t) * a.H + tile0 * 16 + row, v);
+        if (f) atomicOr(a.error, f);
     }
+}
+
+size_t column_bytes(int blocks) { return static_cast<size_t>(std::min(blocks, kChunk)) * (kFp8TileBytes + 64); }
+
+template<int T_>
+hipError_t launch_gate_up(const Fp8LayerArgs &a, hipStream_t s) {
+    const int experts = std::min(a.T * a.k, a.E) + (a.P1 > a.k ? 1 : 0);   // at most
+    const int slices = (a.I / 16 + kRowTiles - 1) / kRowTiles, grid = std::min(experts * slices, kGateUpGroups);
+    const size_t lds = std::max({column_bytes(a.nbh), size_t{8 * 2048}, static_cast<size_t>(a.E) * 4});
+    k_fp8_gate_up<T_><<<dim3(grid), dim3(512), lds, s>>>(a);
+    return hipGetLastError();
 }
 
 template<int T_>
 hipError_t launch_layer(const Fp8LayerArgs &a, hipStream_t s) {
-    const int pairs = a.T * a.k + (a.P1 > a.k ? 1 : 0), W = std::min(8, a.nbh);
-    const size_t rows = static_cast<size_t>(std::min(a.nbh, kChunk)) * (kFp8TileBytes + 64);
-    const size_t lds = std::max<size_t>(rows, static_cast<size_t>(W) * 2048);
-    k_fp8_gate_up<T_><<<dim3(static_cast<unsigned>(pairs) * (a.I / 16)), dim3(64 * W), lds, s>>>(a);
-    hipError_t r = hipGetLastError();
+    const hipError_t r = launch_gate_up<T_>(a, s);
     if (r != hipSuccess) return r;
-    const int W2 = std::min(16, a.P1);
-    const auto grid = [&](int rows_) { return dim3(static_cast<unsigned>((a.H / rows_ + 7) / 8 * 8) * a.T); };
-    if (a.T >= 4) k_fp8_down_fold<T_, 2><<<grid(32), dim3(64 * W2), 0, s>>>(a);
-    else k_fp8_down_fold<T_, 1><<<grid(16), dim3(64 * W2), 0, s>>>(a);
+    const int row_tiles = a.H / 16;
+    int tiles = 1;
+    while (tiles < kDownTiles && a.T * ((row_tiles + tiles - 1) / tiles) > (a.T <= 8 ? 256 : 512)) tiles *= 2;
+    const dim3 grid(static_cast<unsigned>((row_tiles + tiles - 1) / tiles + 7) / 8 * 8 * a.T), block(64 * std::min(16, a.P1));
+    k_fp8_down_fold<T_><<<grid, block, static_cast<size_t>(a.P1) * tiles * 64, s>>>(a, tiles);
     return hipGetLastError();
 }
 
