@@ -13,6 +13,10 @@
 namespace moe {
 namespace {
 
+// Waves a CU of a long batch (16,384 rows, us at 16 / 24 / 32: 2,560 bf16
+// channels with an element gate 88 / 101 / 112, 2,048 fp32 ones 104 / 106 / 103).
+inline constexpr int kNormWaves = 16;
+
 struct NormArgs {
     const void *residual, *block, *gate;
     void *residual_out, *out;
@@ -24,38 +28,57 @@ struct NormArgs {
     int *error;
     float eps, offset, residual_scale, block_scale;
     int hidden, tokens, gate_form, gate_sigmoid;
-    bool vec;   // every row takes 8-element accesses
 };
 
+// Eight elements at any alignment of their type (the hardware takes such 16-byte
+// accesses), of which the first `valid` are the row's; 0 after those.
 template<int T>
-__device__ __forceinline__ void load8_any(const void *p, size_t at, int valid, bool vec, float (&v)[8]) {
-    if (vec) {
-        Raw8 raw{};
-        if (valid > 0) raw = load8_raw<T>(p, at);
-        unpack8<T>(raw, v);
-    } else {
+__device__ __forceinline__ Raw8 load8_any(const void *p, size_t at, int valid) {
+    Raw8 r{};
+    const char *q = static_cast<const char *>(p) + at * elem_bytes(T);
+    if (valid >= 8) {
+        __builtin_memcpy(&r.lo, q, 16);
+        if constexpr (T == kF32) __builtin_memcpy(&r.hi, q + 16, 16);
+    } else if (valid > 0) {
+        uint32_t w[8] = {};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? load1<T>(p, at + i) : 0.0f;
+        for (int i = 0; i < 7; ++i) {
+            if (i >= valid) break;
+            if constexpr (T == kF32) w[i] = reinterpret_cast<const uint32_t *>(q)[i];
+            else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(q)[i]) << (16 * (i & 1));
+        }
+        r.lo = make_uint4(w[0], w[1], w[2], w[3]);
+        if constexpr (T == kF32) r.hi = make_uint4(w[4], w[5], w[6], w[7]);
     }
+    return r;
 }
 template<int T>
-__device__ __forceinline__ void store8_any(void *p, size_t at, int valid, bool vec, const float (&v)[8]) {
-    if (vec) {
-        if (valid <= 0) return;
+__device__ __forceinline__ void store8_any(void *p, size_t at, int valid, const float (&v)[8]) {
+    char *q = static_cast<char *>(p) + at * elem_bytes(T);
+    if (valid >= 8) {
         if constexpr (T == kF32) {
-            float4 *q = reinterpret_cast<float4 *>(static_cast<float *>(p) + at);
-            q[0] = make_float4(v[0], v[1], v[2], v[3]);
-            q[1] = make_float4(v[4], v[5], v[6], v[7]);
+            __builtin_memcpy(q, v, 32);
         } else {
             const auto pack = [](float a, float b) { return T == kBF16 ? pack_bf16(a, b) : pack_f16(a, b); };
-            *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + at) =
-                make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+            const uint4 w = make_uint4(pack(v[0], v[1]), pack(v[2], v[3]), pack(v[4], v[5]), pack(v[6], v[7]));
+            __builtin_memcpy(q, &w, 16);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            if (i < valid) store1<T>(p, at + i, v[i]);
+        for (int i = 0; i < 7; ++i)
+            if (i < valid) store1<T>(q, i, v[i]);
     }
+}
+
+// 1 / (1 + e^-g).  e^-g = 2^t (1 + r ln 2) with t the rounded product -g log2 e
+// and r what rounding it left out; 2^t and the quotient are the hardware's, an
+// ulp each, so that the whole is within 8 half ulps.  Infinite g: 0 or 1.
+__device__ __forceinline__ float sigmoid(float g) {
+    constexpr float log2e = 0x1.715476p+0f, log2e_rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;
+    const float t = -g * log2e;
+    float e = __builtin_amdgcn_exp2f(t);
+    if (fabsf(t) < 200.0f) e = fmaf(e, fmaf(-g, log2e_rest, fmaf(-g, log2e, -t)) * ln2, e);
+    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
 // The sum over the workgroup, by a butterfly in each wave and then in wave
@@ -124,57 +147,73 @@ __device__ __forceinline__ void store_q8(uint32_t *q8, size_t block, int part, f
 
 // An e4m3 group from 16 neighbouring lanes, as k_quantize_e4m3 forms it.
 __device__ __forceinline__ void store_e4m3(uint8_t *codes, size_t at, float *scale, int part, const float (&v)[8], int valid,
-                                           bool vec, int &flags) {
+                                           int &flags) {
     const GroupScale g = group_scale(max16(v));
     const uint2 c = quantize8(v, g);
-    if (vec) {
-        if (valid > 0) *reinterpret_cast<uint2 *>(codes + at) = c;
+    if (valid >= 8) {
+        __builtin_memcpy(codes + at, &c, 8);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 7; ++i)
             if (i < valid) codes[at + i] = static_cast<uint8_t>((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
     }
     if (part == 0 && valid > 0) *scale = g.s;
     if (g.bad) flags |= 1;
 }
 
-// A workgroup per row, 8 NV elements a thread, all of the row in registers.
+// A workgroup takes rows blockIdx.x, + gridDim.x, .., 8 NV elements a thread
+// and all of a row in registers.  Weights and a gate per channel stay in
+// registers and a row is on its way while the last one is reduced (NV = 1; with
+// 16 elements a thread the registers do not suffice for that).
 // TB: type of block, out and an element gate; TR: of the residual.
 template<int TB, int TR, int NV>
 __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
     __shared__ float slots[2][16];
     const int tid = threadIdx.x, H = a.hidden, nb = (H + kFp8Block - 1) / kFp8Block;
-    const bool vec = a.vec;
     int col[NV], valid[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         col[j] = (j * static_cast<int>(blockDim.x) + tid) * 8;
         valid[j] = min(8, H - col[j]);   // <= 0 past the row's end
     }
-    int flags = 0, which = 0;
-    for (int n = blockIdx.x; n < a.tokens; n += gridDim.x) {
-        float r[NV][8], b[NV][8];
+    const auto channels = [&](const void *p, int j, float (&w)[8]) { unpack8<kF32>(load8_any<kF32>(p, col[j], valid[j]), w); };
+    float post[8], pre[8], gate[8];   // NV = 1
+    if constexpr (NV == 1) {
+        if (a.post_weight) channels(a.post_weight, 0, post);
+        if (a.pre_weight) channels(a.pre_weight, 0, pre);
+        if (a.gate_form == MOE_GATE_CHANNEL) {
+            channels(a.gate, 0, gate);
+            if (a.gate_sigmoid) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) gate[i] = sigmoid(gate[i]);
+            }
+        }
+    }
+    Raw8 nr[NV], nblk[NV], ng[NV];   // the next row
+    float token_gate = 0.0f;
+    const auto load = [&](size_t n) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            load8_any<TR>(a.residual, static_cast<size_t>(n) * a.residual_stride + col[j], valid[j], vec, r[j]);
-            if (a.block) load8_any<TB>(a.block, static_cast<size_t>(n) * a.block_stride + col[j], valid[j], vec, b[j]);
+            nr[j] = load8_any<TR>(a.residual, n * a.residual_stride + col[j], valid[j]);
+            if (a.block) nblk[j] = load8_any<TB>(a.block, n * a.block_stride + col[j], valid[j]);
+            if (a.gate_form == MOE_GATE_ELEMENT) ng[j] = load8_any<TB>(a.gate, n * a.gate_stride + col[j], valid[j]);
         }
+        if (a.gate_form == MOE_GATE_TOKEN) token_gate = static_cast<const float *>(a.gate)[n];
+    };
+    int flags = 0, which = 0;
+    if constexpr (NV == 1) load(blockIdx.x);
+    for (int n = blockIdx.x; n < a.tokens; n += gridDim.x) {
+        float r[NV][8], b[NV][8], g[NV][8];
+        if constexpr (NV > 1) load(n);
+        float row_gate = token_gate;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            unpack8<TR>(nr[j], r[j]);
+            if (a.block) unpack8<TB>(nblk[j], b[j]);
+            if (a.gate_form == MOE_GATE_ELEMENT) unpack8<TB>(ng[j], g[j]);
+        }
+        if (NV == 1 && n + static_cast<int>(gridDim.x) < a.tokens) load(n + gridDim.x);
         if (a.block) {
-            float g[NV][8];
-            if (a.gate_form == MOE_GATE_TOKEN) {
-                const float v = static_cast<const float *>(a.gate)[n];
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) g[j][i] = v;
-            } else if (a.gate_form == MOE_GATE_CHANNEL) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j) load8_any<kF32>(a.gate, col[j], valid[j], vec, g[j]);
-            } else if (a.gate_form == MOE_GATE_ELEMENT) {
-#pragma unroll
-                for (int j = 0; j < NV; ++j)
-                    load8_any<TB>(a.gate, static_cast<size_t>(n) * a.gate_stride + col[j], valid[j], vec, g[j]);
-            }
             if (a.post_weight) {
                 float s = 0.0f;
 #pragma unroll
@@ -185,18 +224,35 @@ __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
                 const float scale = 1.0f / sqrtf(s / static_cast<float>(H) + a.eps);
 #pragma unroll
                 for (int j = 0; j < NV; ++j) {
-                    float w[8];
-                    load8_any<kF32>(a.post_weight, col[j], valid[j], vec, w);
+                    if constexpr (NV > 1) channels(a.post_weight, j, post);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) b[j][i] = b[j][i] * scale * (a.offset + w[i]);
+                    for (int i = 0; i < 8; ++i) b[j][i] = b[j][i] * scale * (a.offset + post[i]);
                 }
             }
-            if (a.gate_form != MOE_GATE_NONE) {
+            if (a.gate_form == MOE_GATE_TOKEN) {
+                const float v = a.gate_sigmoid ? sigmoid(row_gate) : row_gate;
 #pragma unroll
                 for (int j = 0; j < NV; ++j)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        b[j][i] = a.gate_sigmoid ? b[j][i] / (1.0f + moe_expf(-g[j][i])) : b[j][i] * g[j][i];
+                    for (int i = 0; i < 8; ++i) b[j][i] *= v;
+            } else if (a.gate_form == MOE_GATE_CHANNEL) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j) {
+                    if constexpr (NV > 1) {
+                        channels(a.gate, j, gate);
+                        if (a.gate_sigmoid) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) gate[i] = sigmoid(gate[i]);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[j][i] *= gate[i];
+                }
+            } else if (a.gate_form == MOE_GATE_ELEMENT) {
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) b[j][i] *= a.gate_sigmoid ? sigmoid(g[j][i]) : g[j][i];
             }
 #pragma unroll
             for (int j = 0; j < NV; ++j)
@@ -211,7 +267,7 @@ __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
         if (a.residual_out) {
 #pragma unroll
             for (int j = 0; j < NV; ++j)
-                store8_any<TR>(a.residual_out, static_cast<size_t>(n) * a.residual_out_stride + col[j], valid[j], vec, r[j]);
+                store8_any<TR>(a.residual_out, static_cast<size_t>(n) * a.residual_out_stride + col[j], valid[j], r[j]);
         }
         if (!a.pre_weight) continue;
         // The norm takes the sum as it is, not as a 16-bit residual_out rounds it.
@@ -219,25 +275,18 @@ __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(r[j][i], r[j][i], s);
+            for (int i = 0; i < 8; ++i) s = fmaf(i < valid[j] ? r[j][i] : 0.0f, r[j][i], s);
         s = group_sum(s, slots, which);
         const float scale = 1.0f / sqrtf(s / static_cast<float>(H) + a.eps);
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            float w[8];
-            load8_any<kF32>(a.pre_weight, col[j], valid[j], vec, w);
+            if constexpr (NV > 1) channels(a.pre_weight, j, pre);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[j][i] = r[j][i] * scale * (a.offset + w[i]);
-            if (a.out) store8_any<TB>(a.out, static_cast<size_t>(n) * a.out_stride + col[j], valid[j], vec, r[j]);
-            if (a.codes) {
-                if (valid[j] < 8) {   // 0 weights past the end would leave NaN of a NaN row there
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (i >= valid[j]) r[j][i] = 0.0f;
-                }
+            for (int i = 0; i < 8; ++i) r[j][i] = i < valid[j] ? r[j][i] * scale * (a.offset + pre[i]) : 0.0f;
+            if (a.out) store8_any<TB>(a.out, static_cast<size_t>(n) * a.out_stride + col[j], valid[j], r[j]);
+            if (a.codes)
                 store_e4m3(a.codes, static_cast<size_t>(n) * H + col[j], a.scales + static_cast<size_t>(n) * nb + col[j] / kFp8Block,
-                           tid & 15, r[j], valid[j], vec, flags);
-            }
+                           tid & 15, r[j], valid[j], flags);
             if (a.q8) store_q8(a.q8, static_cast<size_t>(n) * (H / 32) + col[j] / 32, tid & 3, r[j], valid[j] > 0, flags);
         }
     }
@@ -247,7 +296,7 @@ __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
 template<int TB, int TR>
 hipError_t launch_norm(const NormArgs &a, hipStream_t s) {
     const int nv = a.hidden > 8192 ? 2 : 1, waves = (a.hidden + 512 * nv - 1) / (512 * nv);
-    const dim3 grid(std::min(a.tokens, 256 * std::max(1, 16 / waves))), block(64 * waves);
+    const dim3 grid(std::min(a.tokens, 256 * std::max(1, kNormWaves / waves))), block(64 * waves);
     if (nv == 1) k_block_norm<TB, TR, 1><<<grid, block, 0, s>>>(a);
     else k_block_norm<TB, TR, 2><<<grid, block, 0, s>>>(a);
     return hipGetLastError();
@@ -267,10 +316,7 @@ extern "C" int moe_block_norm(const moe_block_norm_args *p, void *stream) {
         (n.residual_type != n.type && n.residual_type != MOE_F32) || !(n.eps > 0.0f) || n.eps > 3.4e38f)
         return kInvalid;
     const int es = moe::elem_bytes(n.type), rs = moe::elem_bytes(n.residual_type);
-    bool vec = n.hidden % 8 == 0;
-    // Rows of `size`-byte elements; false: cannot be taken.
     const auto rows = [&](const void *q, int64_t stride, int size) {
-        vec = vec && moe::aligned(q, 16) && stride * size % 16 == 0;
         return moe::aligned(q, size) && stride >= n.hidden && stride <= (int64_t{1} << 40);
     };
     if (!rows(n.residual, n.residual_stride, rs)) return kInvalid;
@@ -280,11 +326,7 @@ extern "C" int moe_block_norm(const moe_block_norm_args *p, void *stream) {
         if (n.gate_form < MOE_GATE_NONE || n.gate_form > MOE_GATE_ELEMENT) return kInvalid;
         if (n.gate_form == MOE_GATE_ELEMENT && !rows(n.gate, n.gate_stride, es)) return kInvalid;
         if ((n.gate_form == MOE_GATE_TOKEN || n.gate_form == MOE_GATE_CHANNEL) && !moe::aligned(n.gate, 4)) return kInvalid;
-        if (n.gate_form == MOE_GATE_CHANNEL) vec = vec && moe::aligned(n.gate, 16);
-        if (n.post_weight) {
-            if (!moe::aligned(n.post_weight, 4)) return kInvalid;
-            vec = vec && moe::aligned(n.post_weight, 16);
-        }
+        if (n.post_weight && !moe::aligned(n.post_weight, 4)) return kInvalid;
     } else if (n.gate_form != MOE_GATE_NONE || n.post_weight) {
         return kInvalid;
     }
@@ -293,10 +335,8 @@ extern "C" int moe_block_norm(const moe_block_norm_args *p, void *stream) {
     if (!n.pre_weight && !n.residual_out) return kInvalid;   // nothing to write
     if (n.pre_weight) {
         if (!moe::aligned(n.pre_weight, 4)) return kInvalid;
-        vec = vec && moe::aligned(n.pre_weight, 16);
         if (n.out && !rows(n.out, n.out_stride, es)) return kInvalid;
         if ((n.codes != nullptr) != (n.scales != nullptr) || (n.scales && !moe::aligned(n.scales, 4))) return kInvalid;
-        if (n.codes) vec = vec && moe::aligned(n.codes, 8);
         if (n.q8 && (n.hidden % 32 || !moe::aligned(n.q8, 4))) return kInvalid;
         if ((n.q8 || n.codes) && !moe::aligned(n.error, 4)) return kInvalid;
     }
@@ -325,7 +365,6 @@ extern "C" int moe_block_norm(const moe_block_norm_args *p, void *stream) {
     a.tokens = n.tokens;
     a.gate_form = n.block ? n.gate_form : MOE_GATE_NONE;
     a.gate_sigmoid = n.gate_sigmoid;
-    a.vec = vec;
     const auto s = static_cast<hipStream_t>(stream);
     if (n.type == MOE_F32) return moe::launch_norm<moe::kF32, moe::kF32>(a, s);
     if (n.type == MOE_BF16)

@@ -34,8 +34,8 @@ def reference(norm, residual, block, gate):
     """(h, dh, n, dn): values and bounds of a fp32 evaluation, float64.  A sum
     of squares passes through at most 16 + 6 + 16 additions (elements of a
     thread, lanes, waves), each off by U of a sum of positive terms; mean, eps,
-    root and quotient add 4 U; a product or quotient U each; expf 2 U of a
-    sigmoid at most."""
+    root and quotient add 4 U; a product or quotient U each; a sigmoid is within
+    8 U (exponential and reciprocal 2 U each, the sum, the argument)."""
     sums = 40 * U
     r = residual.double() * norm.residual_scale
     h, dh = r, U * r.abs()
@@ -49,7 +49,7 @@ def reference(norm, residual, block, gate):
         if gate is not None:
             g = gate.double()
             b = b * (torch.sigmoid(g) if norm.gate_sigmoid else g)
-            rel = rel + 6 * U
+            rel = rel + 10 * U
         b = b * norm.block_scale
         h = r + b
         dh = b.abs() * (rel + 2 * U) + U * r.abs() + U * h.abs()
