@@ -289,17 +289,22 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
 // steps through the blocks of K with the next steps' operands and column
 // scales on the way to a ring of S buffers in LDS.
 //
-// Tiles: the columns lie in tiles as the rows do.  Otherwise they are canonical
-// rows: at a power-of-two width the 256 rows of a step lie a multiple of the
-// L2's channel period apart and queue up at one channel (8192 x 8192 at 16,384
-// columns: 1.31 ms from rows, 1.02 from tiles with their quantiser), which is
-// also why the tiles of 16 rows are an odd number of tiles apart.
-template<int WR, int WC, int TM, int TN, int S, bool Tiles>
+// Tiles: the columns lie in tiles as the rows do, their scales [block][column].
+// Otherwise they are canonical rows with scales [column][block], of which four
+// blocks' are loaded at once where a row's lie on 16 bytes: a block at a time,
+// the columns' scales take as many memory requests as their codes (8192 x 8192
+// at 16,384 columns 1.15 ms, in fours 1.08).  The tiles of 16 rows are an odd
+// number of tiles apart: at a power-of-two width a step's rows would lie a
+// multiple of the L2's channel period apart and queue up at one channel (1.31
+// against 1.15 ms).
+template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles>
 struct GemmTile {
     static constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
     static constexpr int ABytes = BM * kFp8Block, BBytes = BN * kFp8Block, Buffer = ABytes + BBytes + BN * 4;
     static constexpr int ALoads = BM / 8 / W, BLoads = BN / 8 / W;   // 1 KiB loads of a wave and step
-    static constexpr int Loads = ALoads + BLoads + 1;                // and one of scales
+    static constexpr int Loads = ALoads + BLoads + (Tiles ? 1 : 0);  // at least: and one of scales
+    static constexpr int Fours = Tiles ? 0 : 2 * BN * 16;            // two sets of four blocks' scales
+    static constexpr int Lds = S * Buffer + Fours;
     static_assert(kFp8Block % (16 * TM) == 0, "a wave's rows share one scale block");
     static_assert(BM / 8 % W == 0 && BN / 8 % W == 0 && W % 2 == 0 && BN % 64 == 0 && W % (BN / 64) == 0,
                   "every wave issues the same loads");
@@ -310,6 +315,7 @@ struct GemmTile {
     // In the constant address space: scalar loads, which the waits above do not count.
     const __attribute__((address_space(4))) float *wscale;
     int b0off, b1off, aread, bread, sread;
+    bool fours;   // scales in fours
 
     __device__ __forceinline__ GemmTile(const Fp8LinearArgs &a, int pm, int pn, const void *lds) {
         lane = threadIdx.x & 63;
@@ -340,6 +346,7 @@ struct GemmTile {
         sr = buffer_rsrc(a.xscale + static_cast<size_t>(n0) * a.scale_n,
                          (static_cast<uint32_t>(cols - 1) * a.scale_n + static_cast<uint32_t>(a.nb - 1) * a.scale_b + 1) * 4);
         soff = static_cast<uint32_t>(wave % (BN / 64) * 64 + lane) * a.scale_n * 4;
+        fours = !Tiles && a.nb % 4 == 0 && reinterpret_cast<uintptr_t>(a.xscale) % 16 == 0;
         sstep = static_cast<uint32_t>(a.scale_b) * 4;
         if (wave % (BN / 64) * 64 + lane >= cols) soff = kPastEnd;
         lds0 = lds_offset(lds);
@@ -378,10 +385,19 @@ struct GemmTile {
             else
                 load_to_lds(br, off + (8 * c * K + b * kFp8Block), to + i * W * 1024);
         }
-        load_word_to_lds(sr, b < nb ? soff + b * sstep : kPastEnd, lds0 + buf * Buffer + ABytes + BBytes + wave % (BN / 64) * 256);
+        const int part = wave % (BN / 64);
+        if (!Tiles && fours) {
+            // Of the group's blocks b, b + G, .. the first of each four.
+            if ((b & 3) < G)
+                load_to_lds(sr, b < nb ? soff + (b & ~3) * 4 : kPastEnd, lds0 + S * Buffer + (b >> 2 & 1) * (BN * 16) + part * 1024);
+        } else {
+            load_word_to_lds(sr, b < nb ? soff + b * sstep : kPastEnd, lds0 + buf * Buffer + ABytes + BBytes + part * 256);
+        }
     }
-    // The scale of column l % 16 of column tile t.
-    __device__ __forceinline__ float scale(const uint8_t *buf, int t) const {
+    // The scale of column l % 16 of column tile t in block b, whose buffer is buf of lds.
+    __device__ __forceinline__ float scale(const uint8_t *lds, const uint8_t *buf, int b, int t) const {
+        if (!Tiles && fours)
+            return *reinterpret_cast<const float *>(lds + S * Buffer + (b >> 2 & 1) * (BN * 16) + (wc * TN * 16 + t * 16 + (lane & 15)) * 16 + (b & 3) * 4);
         return *reinterpret_cast<const float *>(buf + sread + t * 64);
     }
     __device__ __forceinline__ Frag column(const uint8_t *buf, int t) const {
@@ -410,10 +426,10 @@ struct GemmTile {
 // Y: type of y; fp32 results on fp16 operands, the others on e4m3 ones.
 template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, int Y>
 __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m) {
-    using Tile = GemmTile<WR, WC, TM, TN, S, Tiles>;
+    using Tile = GemmTile<WR, WC, TM, TN, S, G, Tiles>;
     constexpr int Sums = TM * TN * Tile::W * 64 * 16;   // bytes of one group's sums
-    static_assert(G == 1 || Sums <= G * S * Tile::Buffer);
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[G][S][Tile::Buffer];
+    static_assert(G == 1 || Sums <= G * Tile::Lds);
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[G][Tile::Lds];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / Tile::W;
     const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds[group]);
     f32x4 acc[TM][TN];
@@ -429,14 +445,15 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
     int at = 0;   // the step's buffer, step % S
     for (int b = group; b - group < a.nb; b += G) {
         // Block b's loads are all but the last S - 2 steps'; memory answers in
-        // order, and past the last block a step still issues as many.
+        // order, and past the last block a step still issues as many (of scales
+        // in fours, most steps load none: Loads counts the fewest).
         wait_for_lds_loads<(S - 2) * Tile::Loads>();
         __syncthreads();
         // Every wave is done with the last step: its buffer takes the one S - 1 ahead.
         const int next = at == 0 ? S - 1 : at - 1;
         g.stage_rows(b + (S - 1) * G, next);
         g.stage_columns(b + (S - 1) * G, next);
-        const uint8_t *buf = lds[group][at];
+        const uint8_t *buf = lds[group] + at * Tile::Buffer;
         at = at + 1 == S ? 0 : at + 1;
         const float sw = g.wscale[G == 1 ? b : min(b, a.nb - 1)];   // a group's block past the last: zeros
         using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
@@ -445,7 +462,7 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
 #pragma unroll
         for (int t = 0; t < TN; ++t) {
             x[t] = operand<Operand>(g.column(buf, t));
-            s[t] = g.scale(buf, t) * sw;
+            s[t] = g.scale(lds[group], buf, b, t) * sw;
         }
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
@@ -495,8 +512,8 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
 // that ends its second read of block b, turn 4 b + 3 at the latest.
 template<bool Tiles, int Y>
 __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tiles_m) {
-    using Tile = GemmTile<2, 4, 8, 4, 2, Tiles>;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][Tile::Buffer];
+    using Tile = GemmTile<2, 4, 8, 4, 2, 1, Tiles>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::Lds];
     const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds);
     f32x4 acc[8][4];
 #pragma unroll
@@ -537,7 +554,7 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
         __builtin_amdgcn_s_setprio(0);
     };
     for (int b = 0; b < a.nb; ++b) {
-        const uint8_t *buf = lds[b & 1];
+        const uint8_t *buf = lds + (b & 1) * Tile::Buffer;
         const float sw = g.wscale[b];
         Frag x[4], w[4];
 #pragma unroll
@@ -545,7 +562,7 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = g.row(buf, i);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) s[t] = g.scale(buf, t) * sw;
+        for (int t = 0; t < 4; ++t) s[t] = g.scale(lds, buf, b, t) * sw;
         __builtin_amdgcn_sched_barrier(0);
         if (b + 1 < a.nb) g.stage_rows(b + 1, (b + 1) & 1);
         turn(false);
@@ -611,7 +628,7 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
 
 template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, bool F32>
 int launch_gemm(const moe::Fp8LinearArgs &a, hipStream_t s) {
-    using Tile = moe::GemmTile<WR, WC, TM, TN, S, Tiles>;
+    using Tile = moe::GemmTile<WR, WC, TM, TN, S, G, Tiles>;
     const int tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
     const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * Tile::W * G);
     if constexpr (F32) moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
