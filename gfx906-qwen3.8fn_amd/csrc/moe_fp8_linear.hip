@@ -202,42 +202,52 @@ __device__ __forceinline__ Frag quantize_frag(const Fp8LinearArgs &a, int n, int
     return Frag{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
 
-// Few columns: a workgroup takes 16 rows and 16 NT columns, its waves share
+// Few columns: a workgroup takes 16 RT rows and 16 NT columns, its waves share
 // out the blocks of the row (wave w: blocks w, w + W, ..) and add up through
 // LDS in wave order.  The matrix streams from memory straight into registers,
-// each tile once per column tile group.
+// each tile once per column tile group; with more than one column tile the
+// columns' codes are most of what is read (from L2), which RT = 2 halves.
 // IN: the columns' type, quantised here (NT = 1), or kCodes (rows), kTiles.
-template<int IN, int NT>
+template<int IN, int NT, int RT>
 __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
-    __shared__ f32x4 red[8][NT][64];
+    __shared__ f32x4 red[8][RT * NT][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int W = blockDim.x >> 6, mt = blockIdx.x, n0 = blockIdx.y * 16 * NT;
-    const uint8_t *row = a.tiles + static_cast<size_t>(mt) * a.tile_stride * kFp8TileBytes;
-    const float *wscale = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
+    const int W = blockDim.x >> 6, n0 = blockIdx.y * 16 * NT, row_tiles = (a.M + 15) / 16;
+    const uint8_t *row[RT];
+    const float *wscale[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int mt = min(static_cast<int>(blockIdx.x) * RT + r, row_tiles - 1);   // past the end: the last one again
+        row[r] = a.tiles + static_cast<size_t>(mt) * a.tile_stride * kFp8TileBytes;
+        wscale[r] = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
+    }
     const int kl = (lane >> 4) * 32;
     int token[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) token[t] = min(n0 + 16 * t + (lane & 15), a.N - 1);
-    f32x4 acc[NT];
+    f32x4 acc[RT][NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int flags = 0;
     constexpr int U = NT == 1 ? 4 : 2;   // blocks whose loads are in flight together
     for (int b0 = wave; b0 < a.nb; b0 += W * U) {
-        Frag w[U];
+        Frag w[U][RT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            // Past the last block: the first one of the round again, with a scale of 0 below.
+            // Past the last block: the first one of the round again, not used below.
             const int b = b0 + u * W < a.nb ? b0 + u * W : b0;
-            w[u] = load_tile(row + static_cast<size_t>(b) * kFp8TileBytes, lane);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) w[u][r] = load_tile(row[r] + static_cast<size_t>(b) * kFp8TileBytes, lane);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const bool in = b0 + u * W < a.nb;
-            if (!in) break;
             const int b = b0 + u * W;
-            const FragF16 wf = to_f16(w[u]);
-            const float sw = wscale[b];
+            if (b >= a.nb) break;
+            FragF16 wf[RT];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) wf[r] = to_f16(w[u][r]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 Frag x;
@@ -257,30 +267,36 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
                 }
                 if constexpr (IN == kCodes || IN == kTiles)
                     sx = a.xscale[static_cast<size_t>(token[t]) * a.scale_n + static_cast<size_t>(b) * a.scale_b];
-                const f32x4 p = block_dot(wf, to_f16(x));
-                const float s = sx * sw;
+                const FragF16 xf = to_f16(x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(p[i], s, acc[t][i]);
+                for (int r = 0; r < RT; ++r) {
+                    const f32x4 p = block_dot(wf[r], xf);
+                    const float s = sx * wscale[r][b];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[r][t][i] = fmaf(p[i], s, acc[r][t][i]);
+                }
             }
         }
     }
     if constexpr (IN != kCodes && IN != kTiles) {
-        if (mt == 0 && flags) atomicOr(a.error, flags);   // every row tile quantises the same columns
+        if (blockIdx.x == 0 && flags) atomicOr(a.error, flags);   // every workgroup quantises the same columns
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) red[wave][t][lane] = acc[t];
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) red[wave][r * NT + t][lane] = acc[r][t];
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * NT; i += blockDim.x) {
-        const int t = i >> 6, l = i & 63;
-        f32x4 s = red[0][t][l];
-        for (int q = 1; q < W; ++q) {
-            const f32x4 v = red[q][t][l];
+    for (int i = threadIdx.x; i < 64 * RT * NT; i += blockDim.x) {
+        const int q = i >> 6, r = q / NT, t = q % NT, l = i & 63;
+        f32x4 s = red[0][q][l];
+        for (int j = 1; j < W; ++j) {
+            const f32x4 v = red[j][q][l];
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[e] = s[e] + v[e];
         }
         const int n = n0 + 16 * t + (l & 15);
         const float v[4] = {s[0], s[1], s[2], s[3]};
-        if (n < a.N) store_rows(a, n, mt * kFp8TileRows + (l >> 4) * 4, v);
+        if (n < a.N) store_rows(a, n, (static_cast<int>(blockIdx.x) * RT + r) * kFp8TileRows + (l >> 4) * 4, v);
     }
 }
 
@@ -646,21 +662,28 @@ int launch_gemm_wide(const moe::Fp8LinearArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
-// The stream kernel's launch for 16 NT columns a workgroup; IN as there.
-template<int IN, int NT>
+// The stream kernel's launch; IN, NT and RT as there.
+template<int IN, int NT, int RT>
 int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
-    const dim3 grid((a.M + 15) / 16, (a.N + 16 * NT - 1) / (16 * NT)), block(64 * std::min(8, a.nb));
-    moe::k_fp8_stream<IN, NT><<<grid, block, 0, s>>>(a);
+    const dim3 grid((a.M + 16 * RT - 1) / (16 * RT), (a.N + 16 * NT - 1) / (16 * NT)), block(64 * std::min(8, a.nb));
+    moe::k_fp8_stream<IN, NT, RT><<<grid, block, 0, s>>>(a);
     return hipGetLastError();
 }
 
 // The product for quantised columns: canonical rows, or Tiles.
 //
-// Small products stream the matrix (16 rows a workgroup, K shared out among
-// its waves); beyond that the output tile grows with the number of tiles, and
-// where there are few the tile's K is shared among groups of waves.  us for
-// apply with bf16 columns, as 64 x 64 tiles in two groups / in two of half as
-// many waves / 128 x 64 / 128 x 128 / 256 x 256 (MI355X, launches in a row):
+// Small products stream the matrix (16 RT rows and 16 NT columns a workgroup, K
+// shared out among its waves); beyond that the output tile grows with the
+// number of tiles, and where there are few the tile's K is shared among groups
+// of waves.  us for apply with bf16 columns (MI355X, launches in a row),
+// streamed with NT, RT = 1, 1 / 2, 1 / 2, 2 / 2, 4, then as 64 x 64 tiles:
+//         2048 x 2048 at 32 / 64:  5.9 / 6.2 / 6.8 / 7.8; 8.3 and
+//                                  6.5 / 6.4 / 6.9 / 8.0; 8.6
+//         8192 x 8192 at 32 / 64:  22.9 / 16.3 / 15.4 / 17.5; 19.1 and
+//                                  40.4 / 26.7 / 22.8 / 18.0; 19.7
+//         8192 x 2048 at 100:      16.8 / 14.7 / 12.3 / 15.5; 18.5
+// As 64 x 64 tiles in two groups / in two of half as many waves / 128 x 64 /
+// 128 x 128 / 256 x 256:
 //   bf16  2048 x 2048 at   96:   8.7 /  9.4 / 12.5 / 15.9 /  30, streamed 7.2
 //         8192 x 8192 at   96:  20.9 / 24.7 / 37.8 / 47.1 /  94, streamed 33.7
 //         2048 x 2048 at  512:  10.2 / 10.7 / 13.7 / 17.4 /  35
@@ -678,12 +701,13 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 template<bool Tiles>
 int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
     constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
-    if (a.N <= 16) return launch_stream<IN, 1>(a, s);
-    if (a.N <= 32) return launch_stream<IN, 2>(a, s);
-    if (a.N <= 64) return launch_stream<IN, 4>(a, s);
     const auto tiles = [&](long m, long n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
-    if (static_cast<long>(a.M) * a.N <= 320 * 1024)
-        return tiles(16, 64) >= 256 ? launch_stream<IN, 4>(a, s) : launch_stream<IN, 2>(a, s);
+    if (a.N <= 64 || static_cast<long>(a.M) * a.N <= 320 * 1024) {
+        const int row_tiles = (a.M + 15) / 16;
+        if (a.N <= 16 || (a.N <= 32 && row_tiles <= 160)) return launch_stream<IN, 1, 1>(a, s);
+        if (row_tiles >= 512) return a.N <= 32 ? launch_stream<IN, 2, 2>(a, s) : launch_stream<IN, 2, 4>(a, s);
+        return a.N <= 64 ? launch_stream<IN, 2, 1>(a, s) : launch_stream<IN, 2, 2>(a, s);
+    }
     if (a.y_type == MOE_F32) {
         if (tiles(64, 64) <= 256) return launch_gemm<2, 2, 2, 2, 2, 4, Tiles, true>(a, s);
         if (tiles(64, 64) <= 800) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, true>(a, s);
@@ -803,9 +827,9 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
         a.x_stride = x_stride;
         a.x_vec = aligned(x, 16) && x_stride * moe::elem_bytes(x_type) % 16 == 0;
         a.error = error;
-        if (x_type == MOE_F32) return launch_stream<moe::kF32, 1>(a, s);
-        if (x_type == MOE_BF16) return launch_stream<moe::kBF16, 1>(a, s);
-        return launch_stream<moe::kF16, 1>(a, s);
+        if (x_type == MOE_F32) return launch_stream<moe::kF32, 1, 1>(a, s);
+        if (x_type == MOE_BF16) return launch_stream<moe::kBF16, 1, 1>(a, s);
+        return launch_stream<moe::kF16, 1, 1>(a, s);
     }
     auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>((columns + 15) / 16) * L->tile_stride * moe::kFp8TileBytes);
     const hipError_t r = moe::launch_quantize<true>(x, x_type, x_stride, L->input, columns, L->ws, L->tile_stride, scales, columns,
