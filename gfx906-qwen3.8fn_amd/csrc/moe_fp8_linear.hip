@@ -160,46 +160,29 @@ __device__ __forceinline__ void store_rows(const Fp8LinearArgs &a, int n, int m,
     else store_rows<kF16>(a, n, m, v);
 }
 
-// A token's 32 elements at k as its fragment, quantised here: the four lanes
-// l, l ^ 16, l ^ 32, l ^ 48 hold the token's block.  Elements past the row's
-// end count as zero.
+// All of the columns (at most 16) quantised by the whole workgroup into LDS:
+// codes [block][32-element part][column][32 B], scales [block][column], 16
+// threads a block.  Elements past a row's end count as zero.
 template<int T>
-__device__ __forceinline__ Frag quantize_frag(const Fp8LinearArgs &a, int n, int k, float &scale, int &flags) {
-    const size_t at = static_cast<size_t>(n) * a.x_stride + k;
-    const bool in = k < a.K;
-    float v[32];
-    if (a.x_vec) {
-        Raw8 raw[4] = {};
-        if (in) {
+__device__ __forceinline__ void quantize_to_lds(const Fp8LinearArgs &a, uint8_t *codes, float *scales, int &flags) {
+    const int part = threadIdx.x & 15;
+    for (int i = threadIdx.x >> 4; i < a.N * a.nb; i += blockDim.x >> 4) {
+        const int n = i / a.nb, b = i % a.nb, k = b * kFp8Block + part * 8;
+        const size_t at = static_cast<size_t>(n) * a.x_stride + k;
+        float v[8];
+        if (a.x_vec) {
+            Raw8 raw{};
+            if (k < a.K) raw = load8_raw<T>(a.x, at);
+            unpack8<T>(raw, v);
+        } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) raw[q] = load8_raw<T>(a.x, at + 8 * q);
+            for (int j = 0; j < 8; ++j) v[j] = k < a.K ? load1<T>(a.x, at + j) : 0.0f;
         }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float u[8];
-            unpack8<T>(raw[q], u);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[8 * q + i] = u[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = in ? load1<T>(a.x, at + i) : 0.0f;
+        const GroupScale s = group_scale(max16(v));
+        *reinterpret_cast<uint2 *>(codes + ((b * 4 + (part >> 2)) * a.N + n) * 32 + (part & 3) * 8) = quantize8(v, s);
+        if (part == 0) scales[b * a.N + n] = s.s;
+        if (s.bad) flags |= 1;
     }
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 32; ++i) m = max(m, magnitude(v[i]));
-    m = max(m, static_cast<uint32_t>(lane_xor<16>(static_cast<int>(m))));
-    m = max(m, static_cast<uint32_t>(lane_xor<32>(static_cast<int>(m))));
-    const GroupScale s = group_scale(m);
-    uint32_t w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        w[i] = pack_e4m3(v[4 * i] * s.r, v[4 * i + 1] * s.r, v[4 * i + 2] * s.r, v[4 * i + 3] * s.r);
-        if (s.bad) w[i] = 0u;
-    }
-    if (s.bad) flags |= 1;
-    scale = s.s;
-    return Frag{make_uint4(w[0], w[1], w[2], w[3]), make_uint4(w[4], w[5], w[6], w[7])};
 }
 
 // Few columns: a workgroup takes 16 RT rows and 16 NT columns, its waves share
@@ -207,10 +190,13 @@ __device__ __forceinline__ Frag quantize_frag(const Fp8LinearArgs &a, int n, int
 // LDS in wave order.  The matrix streams from memory straight into registers,
 // each tile once per column tile group; with more than one column tile the
 // columns' codes are most of what is read (from L2), which RT = 2 halves.
-// IN: the columns' type, quantised here (NT = 1), or kCodes (rows), kTiles.
+// IN: the columns' type, quantised here (one column tile), or kCodes (rows), kTiles.
 template<int IN, int NT, int RT>
 __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
+    constexpr bool Quantize = IN != kCodes && IN != kTiles;
+    static_assert(!Quantize || NT == 1);
     __shared__ f32x4 red[8][RT * NT][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t columns[];   // Quantize: codes, then scales
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int W = blockDim.x >> 6, n0 = blockIdx.y * 16 * NT, row_tiles = (a.M + 15) / 16;
     const uint8_t *row[RT];
@@ -232,8 +218,9 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
         for (int t = 0; t < NT; ++t) acc[r][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     int flags = 0;
     constexpr int U = NT == 1 ? 4 : 2;   // blocks whose loads are in flight together
-    for (int b0 = wave; b0 < a.nb; b0 += W * U) {
-        Frag w[U][RT];
+    const float *scales = reinterpret_cast<const float *>(columns + static_cast<size_t>(a.N) * a.nb * kFp8Block);
+    Frag w[U][RT];
+    const auto load = [&](int b0) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             // Past the last block: the first one of the round again, not used below.
@@ -241,6 +228,14 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
 #pragma unroll
             for (int r = 0; r < RT; ++r) w[u][r] = load_tile(row[r] + static_cast<size_t>(b) * kFp8TileBytes, lane);
         }
+    };
+    if constexpr (Quantize) {
+        load(wave);
+        quantize_to_lds<IN>(a, columns, const_cast<float *>(scales), flags);
+        __syncthreads();
+    }
+    for (int b0 = wave; b0 < a.nb; b0 += W * U) {
+        if (!Quantize || b0 != wave) load(b0);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int b = b0 + u * W;
@@ -263,9 +258,12 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
                         x = Frag{p[0], p[1]};
                     }
                 } else {
-                    x = quantize_frag<IN>(a, token[t], b * kFp8Block + kl, sx, flags);
+                    const int n = min(lane & 15, a.N - 1);
+                    const uint4 *p = reinterpret_cast<const uint4 *>(columns + ((b * 4 + (lane >> 4)) * a.N + n) * 32);
+                    x = Frag{p[0], p[1]};
+                    sx = scales[b * a.N + n];
                 }
-                if constexpr (IN == kCodes || IN == kTiles)
+                if constexpr (!Quantize)
                     sx = a.xscale[static_cast<size_t>(token[t]) * a.scale_n + static_cast<size_t>(b) * a.scale_b];
                 const FragF16 xf = to_f16(x);
 #pragma unroll
@@ -278,7 +276,7 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
             }
         }
     }
-    if constexpr (IN != kCodes && IN != kTiles) {
+    if constexpr (Quantize) {
         if (blockIdx.x == 0 && flags) atomicOr(a.error, flags);   // every workgroup quantises the same columns
     }
 #pragma unroll
@@ -662,11 +660,15 @@ int launch_gemm_wide(const moe::Fp8LinearArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// LDS of a stream kernel that quantises its columns.
+size_t quantize_lds(const moe::Fp8LinearArgs &a) { return static_cast<size_t>(a.N) * a.nb * (moe::kFp8Block + 4); }
+
 // The stream kernel's launch; IN, NT and RT as there.
 template<int IN, int NT, int RT>
 int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
     const dim3 grid((a.M + 16 * RT - 1) / (16 * RT), (a.N + 16 * NT - 1) / (16 * NT)), block(64 * std::min(8, a.nb));
-    moe::k_fp8_stream<IN, NT, RT><<<grid, block, 0, s>>>(a);
+    const size_t lds = IN == moe::kCodes || IN == moe::kTiles ? 0 : quantize_lds(a);
+    moe::k_fp8_stream<IN, NT, RT><<<grid, block, lds, s>>>(a);
     return hipGetLastError();
 }
 
@@ -822,7 +824,13 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
     };
     const char *xb = static_cast<const char *>(x), *yb = static_cast<const char *>(y);
     const bool apart = xb + extent(x_stride, L->input, x_type) <= yb || yb + extent(y_stride, L->output, y_type) <= xb;
-    if (columns <= 16 && apart) {
+    // Every workgroup (16 rows) quantises all of the columns: in its own kernel
+    // where that is up to four passes of its threads, or two where a CU takes
+    // more than one workgroup (us, in the product's kernel / in two launches:
+    // 2048 x 2048 at 1, 4, 8, 16 columns 3.6 / 5.7, 4.4 / 5.6, 5.5 / 5.7, 7.7 /
+    // 5.8; 8192 x 8192 at 1, 2 14.2 / 14.4, 16.5 / 14.4; rows of 2,048 of 8,192
+    // at 4, 8 6.0 / 6.3, 7.7 / 6.3).
+    if (columns <= 16 && apart && columns * L->nb <= (L->output <= 4096 ? 128 : 64)) {
         a.x = x;
         a.x_stride = x_stride;
         a.x_vec = aligned(x, 16) && x_stride * moe::elem_bytes(x_type) % 16 == 0;
