@@ -236,12 +236,12 @@ __device__ __forceinline__ Frag load_tile(const uint8_t *tile, int lane) {
 // those may read what it writes.
 __device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-                 :: "s"(lds), "v"(off), "s"(r) : "memory");
+                 :: "s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 // The same with 4 bytes a lane.
 __device__ __forceinline__ void load_word_to_lds(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
-                 :: "s"(lds), "v"(off), "s"(r) : "memory");
+                 :: "s"(lds), "v"(off), "s"(r) : "memory", "m0");
 }
 // Until at most N of the wave's loads are outstanding.
 template<int N>

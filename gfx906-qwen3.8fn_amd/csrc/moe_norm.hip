@@ -275,7 +275,10 @@ __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s = fmaf(i < valid[j] ? r[j][i] : 0.0f, r[j][i], s);
+            for (int i = 0; i < 8; ++i) {
+                if (i >= valid[j]) r[j][i] = 0.0f;   // 0 there, but NaN with an infinite factor
+                s = fmaf(r[j][i], r[j][i], s);
+            }
         s = group_sum(s, slots, which);
         const float scale = 1.0f / sqrtf(s / static_cast<float>(H) + a.eps);
 #pragma unroll

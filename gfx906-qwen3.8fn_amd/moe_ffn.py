@@ -698,18 +698,19 @@ class MoeFp8Linear:
     def bind_forward(self, x_codes, x_scales, y, stream=None):
         """Validate the tensors of a forward() once and return a no-argument
         callable that enqueues it with no per-call checks; the tensors must
-        stay alive and keep their shapes while the callable is used."""
+        stay alive and keep their shapes while the callable is used.  It keeps
+        the matrix alive, and raises after close()."""
         import torch
         dev = torch.device("cuda", self.device)
         n = x_codes.shape[0]
         _e4m3(x_codes, "x_codes", (n, self.K), dev)
         _need(x_scales, "x_scales", torch.float32, (n, _blocks(self.K)), dev)
         type_, stride = _need_rows(y, "y", (n, self.M), dev)
-        fn, handle = library().moe_fp8_linear_forward, self.handle
+        fn = library().moe_fp8_linear_forward
         args = (_ptr(x_codes), _ptr(x_scales), n, _ptr(y), type_, stride, _stream_on(stream, dev))
 
         def call():
-            st = fn(handle, *args)
+            st = fn(self.handle, *args)
             if st != 0:
                 raise MoeError("moe_fp8_linear_forward", st)
         return call
@@ -731,11 +732,11 @@ class MoeFp8Linear:
         x_type, x_stride = _need_rows(x, "x", (n, self.K), dev)
         y_type, y_stride = _need_rows(y, "y", (n, self.M), dev)
         _need(error, "error", torch.int32, (1,), dev)
-        fn, handle = library().moe_fp8_linear_apply, self.handle
+        fn = library().moe_fp8_linear_apply
         args = (_ptr(x), x_type, x_stride, n, _ptr(y), y_type, y_stride, _ptr(error), _stream_on(stream, dev))
 
         def call():
-            st = fn(handle, *args)
+            st = fn(self.handle, *args)
             if st != 0:
                 raise MoeError("moe_fp8_linear_apply", st)
         return call
@@ -763,8 +764,8 @@ class MoeFp8Layer:
         self.cfg = Fp8LayerConfig(hidden, intermediate, experts, top_k, 1 if has_shared else 0, max_tokens)
         self.H, self.I, self.E, self.k = hidden, intermediate, experts, top_k
         self.has_shared, self.max_tokens, self.device = bool(has_shared), max_tokens, device
-        if self.has_shared and shared is None:
-            raise ValueError("a layer with a shared expert needs its matrices")
+        if self.has_shared != (shared is not None) or (self.has_shared and len(shared) != 3):
+            raise ValueError("shared: three matrices where the layer has a shared expert, None where not")
         gate_up, down_shape = (intermediate, hidden), (hidden, intermediate)
         parts = [_e4m3_matrices(*m, (experts, *shape), name, device)
                  for m, shape, name in ((gate, gate_up, "gate"), (up, gate_up, "up"), (down, down_shape, "down"))]
@@ -793,7 +794,8 @@ class MoeFp8Layer:
     def bind_forward(self, x, ids, weights, y, error, shared_gate=None, stream=None):
         """Validate the tensors of a forward() once and return a no-argument
         callable that enqueues it with no per-call checks (as
-        MoeLayer.bind_forward)."""
+        MoeLayer.bind_forward); it keeps the layer alive, and raises after
+        close()."""
         import torch
         dev = torch.device("cuda", self.device)
         n = x.shape[0]
@@ -806,12 +808,12 @@ class MoeFp8Layer:
             _need(shared_gate, "shared_gate", torch.float32, (n,), dev)
         _need(y, "y", x.dtype, (n, self.H), dev)
         _need(error, "error", torch.int32, (1,), dev)
-        fn, handle = library().moe_fp8_layer_forward, self.handle
+        fn = library().moe_fp8_layer_forward
         args = (_ptr(x), type_, _ptr(ids), _ptr(weights), n, _ptr(shared_gate), _ptr(y), _ptr(error),
                 _stream_on(stream, dev))
 
         def call():
-            st = fn(handle, *args)
+            st = fn(self.handle, *args)
             if st != 0:
                 raise MoeError("moe_fp8_layer_forward", st)
         return call
@@ -928,6 +930,7 @@ class BlockNorm:
             a.scales = _need(scales, "scales", torch.float32, (n, _blocks(h)), dev).data_ptr()
         if q8 is not None or codes is not None:
             a.error = _need(error, "error", torch.int32, (1,), dev).data_ptr()
+        a.weights = self.pre_weight, self.post_weight   # alive while the callable is
         fn, arg, s = library().moe_block_norm, ctypes.byref(a), _stream_on(stream, dev)
         current, switch = torch.cuda.current_device, dev.index
 

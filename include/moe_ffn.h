@@ -345,7 +345,9 @@ int moe_linear_apply_noalloc(moe_linear *linear, const float *x, int columns, fl
  *            a group x of 128 elements with a = max(|x|max, 2^-100) has the
  *            scale a / 448 and the codes e4m3(x * (448 / a)), nearest even,
  *            every operation rounded to fp32
- * The last block of a row or of the rows may be cut short.
+ * The last block of a row or of the rows may be cut short.  Products multiply
+ * a group's scale by a matrix's first: where that leaves fp32's normal range
+ * (beyond 2^128, below 2^-126) so do the results.
  * ---------------------------------------------------------------------- */
 
 /* Element types of activations and results. */
@@ -380,9 +382,9 @@ int moe_fp8_linear_bytes(const moe_fp8_linear *linear, size_t *weight_bytes);
  * block is fp32 when y_type is MOE_F32 or columns <= 64; larger products with
  * 16-bit results use the e4m3 matrix instructions, which drop what is more
  * than about 14 bits below a block's largest product.  columns 1..65536.  No
- * workspace: calls on one handle may overlap.  The rows between y's columns
- * and y_stride are left as they are.  NaN codes give NaN results.  Enqueue
- * only; the handle's device need not be current. */
+ * workspace: calls on one handle may overlap.  What lies between y's rows is
+ * left as it is.  y may not overlap the rows or their scales.  NaN codes give
+ * NaN results.  Enqueue only; the handle's device need not be current. */
 int moe_fp8_linear_forward(moe_fp8_linear *linear, const void *x_codes, const float *x_scales, int columns, void *y,
                            int y_type, int64_t y_stride, void *stream);
 

@@ -110,3 +110,12 @@ def test_norm_arguments(buf):
                 dict(q8=at + 2), dict(hidden=48, q8=at),
                 dict(pre_weight=None, out=None, codes=None, scales=None, residual_out=None)):
         assert lib.moe_block_norm(ctypes.byref(moe_ffn.BlockNormArgs(**{**good, **bad})), None) == 1, bad
+
+
+def test_binding_checks_shared():
+    """A shared expert's three matrices where the layer has one, none where not."""
+    kinds = [(np.zeros((2, r, c), np.uint8), np.ones((2, 1, 1), np.float32)) for r, c in ((32, 64), (32, 64), (64, 32))]
+    shared = [(c[0], s[0]) for c, s in kinds]
+    for has, given in ((False, shared), (True, None), (True, shared[:2])):
+        with pytest.raises(ValueError):
+            moe_ffn.MoeFp8Layer(64, 32, 2, 1, has, 4, *kinds, shared=given)

@@ -268,3 +268,51 @@ def test_refusals():
     with pytest.raises(moe_ffn.MoeError):
         moe_ffn.MoeFp8Layer(64, 32, 4, 2, True, 65, *bank.experts, shared=bank.shared)
     layer.close()
+
+
+def test_bank_past_32_bits():
+    """Matrices of 17 GB a kind, which also take more than one launch to lay
+    out: every expert's tiles are where the products look for them."""
+    H, I, E, k, T = 2048, 2080, 4096, 4, 5
+    g = R.generator(10)
+    codes = torch.empty((E, I, H), dtype=torch.uint8, device=DEV)
+    codes.random_(generator=g).bitwise_and_(0xBF)   # below 2: no NaN
+    parts = [(codes, torch.rand((E, 17, 16), generator=g, device=DEV) * 0.02) for _ in range(2)]
+    parts.append((codes.view(E, H, I), torch.rand((E, 16, 17), generator=g, device=DEV) * 0.02))
+    layer = moe_ffn.MoeFp8Layer(H, I, E, k, False, T, *parts)
+    x = torch.randn((T, H), generator=g, device=DEV).to(BF16)
+    ids, w = routes(T, E, k, g)
+    ids[0] = torch.tensor([E - 1, 0, E // 2, E - 2], device=DEV)
+    ids[1] = torch.tensor([4032, 4033, 1024, 1023], device=DEV)
+
+    class Experts:
+        def __len__(self):
+            return E
+
+        def __getitem__(self, e):
+            return tuple(R.matrix(c[e], s[e]) for c, s in parts)
+
+    y, e = layer.forward(x, ids, w)
+    ref, tol = R.layer(x, ids, w, Experts())
+    tol = tol + R.half_step(BF16) * (ref.abs() + tol)
+    assert flag(e) == 0 and bool(((y.double() - ref).abs() <= tol).all())
+    layer.close()
+
+
+def test_bound_call_keeps_the_layer():
+    g = R.generator(12)
+    bank = Bank(64, 32, 4, True, g)
+    layer = bank.layer(2, 3)
+    x = torch.randn((3, 64), generator=g, device=DEV)
+    ids, w = routes(3, 4, 2, g)
+    y, e = torch.empty_like(x), torch.zeros(1, dtype=torch.int32, device=DEV)
+    want, _ = layer.forward(x, ids, w)
+    call = layer.bind_forward(x, ids, w, y, e)
+    del layer
+    call()
+    assert same(y, want)
+    layer = bank.layer(2, 3)
+    call = layer.bind_forward(x, ids, w, y, e)
+    layer.close()
+    with pytest.raises(moe_ffn.MoeError):
+        call()

@@ -280,3 +280,63 @@ def test_refusals():
     with pytest.raises(ValueError):
         moe_ffn.MoeFp8Linear(K, M, codes, scales.expand(2, 1).contiguous())
     lin.close()
+
+
+@pytest.mark.parametrize("N", [1, 20, 100, 2000])
+def test_matrix_past_32_bits(N):
+    """The largest matrix: its codes and its tiles pass 2^32 bytes."""
+    K, M = 16384, 262144
+    g = R.generator(19)
+    codes = torch.empty((M, K), dtype=torch.uint8, device=DEV)
+    codes.random_(generator=g).bitwise_and_(0xBF)   # below 2: no NaN
+    scales = torch.rand((M // 128, K // 128), generator=g, device=DEV) * 0.02
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales)
+    x = torch.randn((N, K), generator=g, device=DEV)
+    qc, qs = R.quantise(x)
+    y = lin.forward(qc, qs, dtype=BF16)
+    cols = torch.cat([torch.arange(40, device=DEV), M // 2 + torch.arange(40, device=DEV), M - 1 - torch.arange(120, device=DEV)])
+    rows = torch.unique(torch.tensor([0, N // 3, N - 1], device=DEV))
+    w = R.codes_to_values(codes[cols]) * R.spread(scales[cols // 128], 1, K)
+    check(y[rows][:, cols], qc[rows], qs[rows], w, BF16, N > 64)
+    assert bool(y.isfinite().all())
+    lin.close()
+
+
+def test_rows_past_32_bits():
+    """65,536 rows of x and of y inside a buffer of more than 2^32 elements."""
+    K, M, N = 32, 40, 65536
+    g = R.generator(23)
+    codes, scales = R.random_matrix(M, K, g)
+    buf = torch.full((N, 65700), 3.0, dtype=BF16, device=DEV)
+    x, y = buf[:, 7:7 + K], buf[:, 65600:65600 + M]
+    x.normal_(generator=g)
+    qc, qs = R.quantise(x)
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales, max_columns=N)
+    got = moe_ffn.quantize_e4m3(x)
+    assert torch.equal(got[0].view(torch.uint8), qc) and torch.equal(got[1], qs) and flag(got[2]) == 0
+    e = torch.zeros(1, dtype=torch.int32, device=DEV)
+    lin.apply(x, y=y, error=e)
+    check(y, qc, qs, R.matrix(codes, scales), BF16, True)
+    assert flag(e) == 0 and bool((buf[:, :7] == 3).all()) and bool((buf[:, 7 + K:65600] == 3).all())
+    lin.close()
+
+
+def test_bound_calls_keep_the_matrix():
+    """A bound call outlives the caller's last reference to the handle, and
+    raises once the handle is closed."""
+    K, M = 128, 64
+    g = R.generator(29)
+    codes, scales = R.random_matrix(M, K, g)
+    x = torch.randn((3, K), generator=g, device=DEV)
+    y, e = torch.empty((3, M), device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales, max_columns=3)
+    want, _ = lin.apply(x)
+    call = lin.bind_apply(x, y, e)
+    del lin
+    call()
+    assert same(y, want)
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales)
+    call = lin.bind_forward(*moe_ffn.quantize_e4m3(x)[:2], y)
+    lin.close()
+    with pytest.raises(moe_ffn.MoeError):
+        call()

@@ -238,3 +238,33 @@ def test_refusals():
         make(g, 64, eps=0.0)
     with pytest.raises(moe_ffn.MoeError):
         norm.bind(x[:0], out=out[:0])()
+
+
+def test_rows_past_32_bits():
+    """65,536 rows of residual, block and outputs inside a buffer of more than
+    2^32 elements."""
+    n, h = 65536, 96
+    g = R.generator(6)
+    norm = make(g, h)
+    buf = torch.full((n, 65700), 3.0, dtype=BF16, device=DEV)
+    residual, block = buf[:, 65600:65600 + h], buf[:, 5:5 + h]
+    residual.normal_(generator=g)
+    block.normal_(generator=g)
+    want = norm(residual.contiguous(), block=block.contiguous())
+    norm.bind(residual, block=block, residual_out=residual, out=block)()
+    assert same(residual, want["residual"]) and same(block, want["out"])
+    assert bool((buf[:, 5 + h:65600] == 3).all()) and bool((buf[:, 65600 + h:] == 3).all())
+
+
+def test_bound_call_keeps_the_weights():
+    n, h = 3, 256
+    g = R.generator(7)
+    norm = make(g, h)
+    x = torch.randn((n, h), generator=g, device=DEV)
+    want = norm(x, block=x)["out"]
+    out = torch.empty_like(x)
+    call = norm.bind(x, block=x, out=out)
+    del norm
+    other = [torch.full((h,), 9.0, device=DEV) for _ in range(64)]   # would take the weights' memory
+    call()
+    assert same(out, want) and len(other) == 64
