@@ -298,6 +298,102 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
     }
 }
 
+// Few tiles: W waves share the blocks of 16 TM rows x 16 TN columns (wave w:
+// blocks w, w + W, ..), each with its operands straight from memory into
+// registers, the next block's on their way during a block, and no barrier
+// before the sums meet in LDS in wave order.  Nothing but the sums is shared, so
+// that every operand crosses the L1 once for each tile: this pays while a CU's
+// tiles are few (2080 x 1000 at 333 canonical rows, bf16 results: 7.8 us as 64 x 64
+// tiles through LDS, 5.9 so) and, on tiles of columns, for fp32 results, whose
+// conversions leave the L1 the time (the table at launch_product).  Canonical
+// rows, a power of two apart and with a scale load each, do not come fast enough
+// for more: 2048 x 2048 at 1,032 columns, fp32, in 32 x 48 tiles 34.5 us against
+// 20.9.
+template<int TM, int TN, int W, bool Tiles, int Y>
+__global__ __launch_bounds__(64 * W) void k_fp8_split(Fp8LinearArgs a, int tiles_m) {
+    static_assert(kFp8Block % (16 * TM) == 0, "the rows share one scale block");
+    using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
+    __shared__ f32x4 red[W][TM * TN][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int mt = static_cast<int>(blockIdx.x) % tiles_m * TM, nt = static_cast<int>(blockIdx.x) / tiles_m * TN;
+    const int row_tiles = (a.M + 15) / 16, col_tiles = (a.N + 15) / 16, kl = (lane >> 4) * 32;
+    // Tiles past the end: the last one again, not stored.
+    const uint8_t *row[TM], *col[TN];
+    const float *xscale[TN], *wscale = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+        row[i] = a.tiles + static_cast<size_t>(min(mt + i, row_tiles - 1)) * a.tile_stride * kFp8TileBytes;
+#pragma unroll
+    for (int t = 0; t < TN; ++t) {
+        const int n = min((nt + t) * 16 + (lane & 15), a.N - 1);
+        if constexpr (Tiles) col[t] = a.codes + static_cast<size_t>(min(nt + t, col_tiles - 1)) * a.tile_stride * kFp8TileBytes;
+        else col[t] = a.codes + static_cast<size_t>(n) * a.K + kl;
+        xscale[t] = a.xscale + static_cast<size_t>(n) * a.scale_n;
+    }
+    f32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) acc[i][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    Frag w[TM], x[TN];   // of the next block
+    float sx[TN];
+    const auto load_row = [&](int i, int b) { w[i] = load_tile(row[i] + static_cast<size_t>(b) * kFp8TileBytes, lane); };
+    const auto load_column = [&](int t, int b) {
+        if constexpr (Tiles) {
+            x[t] = load_tile(col[t] + static_cast<size_t>(b) * kFp8TileBytes, lane);
+        } else {
+            x[t] = Frag{};
+            if (b * kFp8Block + kl < a.K) {
+                const uint4 *p = reinterpret_cast<const uint4 *>(col[t] + b * kFp8Block);
+                x[t] = Frag{p[0], p[1]};
+            }
+        }
+        sx[t] = xscale[t][static_cast<size_t>(b) * a.scale_b];
+    };
+    if (wave < a.nb) {
+#pragma unroll
+        for (int t = 0; t < TN; ++t) load_column(t, wave);
+#pragma unroll
+        for (int i = 0; i < TM; ++i) load_row(i, wave);
+    }
+    for (int b = wave; b < a.nb; b += W) {
+        const int next = b + W < a.nb ? b + W : b;   // past the last block: it again, not used
+        const float sw = wscale[b];
+        Operand xo[TN];
+        float s[TN];
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+            xo[t] = operand<Operand>(x[t]);
+            s[t] = sx[t] * sw;
+            load_column(t, next);
+        }
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const Operand wo = operand<Operand>(w[i]);
+            load_row(i, next);
+#pragma unroll
+            for (int t = 0; t < TN; ++t) {
+                const f32x4 p = block_dot(wo, xo[t]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][t][e] = fmaf(p[e], s[t], acc[i][t][e]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int t = 0; t < TN; ++t) red[wave][i * TN + t][lane] = acc[i][t];
+    __syncthreads();
+    for (int q = wave; q < TM * TN; q += W) {
+        f32x4 v = red[0][q][lane];
+#pragma unroll
+        for (int j = 1; j < W; ++j) v += red[j][q][lane];
+        const int n = (nt + q % TN) * 16 + (lane & 15);
+        const float out[4] = {v[0], v[1], v[2], v[3]};
+        if (n < a.N) store_rows<Y>(a, n, (mt + q / TN) * kFp8TileRows + (lane >> 4) * 4, out);
+    }
+}
+
 // ---------------------------------------------------------- many columns ---
 // A workgroup of WR x WC waves takes 16 TM WR rows and 16 TN WC columns, and
 // steps through the blocks of K with the next steps' operands and column
@@ -651,6 +747,16 @@ int launch_gemm(const moe::Fp8LinearArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template<int TM, int TN, int W, bool Tiles, bool F32>
+int launch_split(const moe::Fp8LinearArgs &a, hipStream_t s) {
+    const int tm = (a.M + 16 * TM - 1) / (16 * TM), tn = (a.N + 16 * TN - 1) / (16 * TN);
+    const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * W);
+    if constexpr (F32) moe::k_fp8_split<TM, TN, W, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
+    else if (a.y_type == MOE_BF16) moe::k_fp8_split<TM, TN, W, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
+    else moe::k_fp8_split<TM, TN, W, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
+    return hipGetLastError();
+}
+
 template<bool Tiles>
 int launch_gemm_wide(const moe::Fp8LinearArgs &a, hipStream_t s) {
     const int tm = (a.M + 255) / 256, tn = (a.N + 255) / 256;
@@ -676,9 +782,9 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 //
 // Small products stream the matrix (16 RT rows and 16 NT columns a workgroup, K
 // shared out among its waves); beyond that the output tile grows with the
-// number of tiles, and where there are few the tile's K is shared among groups
-// of waves.  us for apply with bf16 columns (MI355X, launches in a row),
-// streamed with NT, RT = 1, 1 / 2, 1 / 2, 2 / 2, 4, then as 64 x 64 tiles:
+// number of tiles, and where there are few the tile's K is split among waves or
+// shared among groups of them.  us for apply (MI355X, launches in a row), with
+// bf16 columns, streamed with NT, RT = 1, 1 / 2, 1 / 2, 2 / 2, 4, then as 64 x 64 tiles:
 //         2048 x 2048 at 32 / 64:  5.9 / 6.2 / 6.8 / 7.8; 8.3 and
 //                                  6.5 / 6.4 / 6.9 / 8.0; 8.6
 //         8192 x 8192 at 32 / 64:  22.9 / 16.3 / 15.4 / 17.5; 19.1 and
@@ -694,12 +800,23 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 //         2048 x 2048 at 4096:  52.3 / 39.5 / 36.7 / 32.9 /  42
 //         2048 x 2048 at 8192, 128 x 128 against 256 x 256: 61.2 / 52.2
 //         8192 x 8192 at 2048 / 4096: 158 / 184 and 331 / 300
-//   fp32, 64 x 64 in four groups / in two of half as many waves / 128 x 128 in
-//         two groups / 128 x 128:
-//         8192 x 8192 at   96:  26.7 / 28.4 / 63.5 / 73.3, streamed 34.4
-//         2048 x 2048 at 1032:  28.7 / 24.1 / 25.8 / 27.3
-//         8192 x 8192 at  512:  98.1 / 85.8 / 70.3 / 78.7
-//         2048 x 2048 at 4096:  72.3 / 56.8 / 54.1 / 47.4; 256 x 256 76.0
+//         64 x 32 split among eight waves against 64 x 64 in two groups, 2048 x
+//         2048 at 170 / 256 / 333: 7.7, 8.1, 9.9 and 8.9, 9.2, 9.5
+//   fp32, 64 x 32 split among eight waves / 32 x 48 among four / among two / 64 x
+//         64 in four groups / in two of half as many waves / 128 x 128 in two
+//         groups / 128 x 128:
+//         2048 x 2048 at  256:   8.8 /  9.8 /  ..  / 12.0
+//                         333:  12.7 / 10.3 / 12.6 / 12.6 / 12.8 / 23.9 / 25.5
+//                         700:  16.9 / 15.1 / 14.4 / 20.6 / 17.1 / 24.6 / 26.4
+//                        1000:  20.9 / 18.8 / 19.8 / 20.9 / 17.9 / 25.2 / 26.8
+//                        1032:  23.7 / 19.2 / 19.9 / 27.2 / 22.8 / 25.0 / 26.7
+//                        2500:  45.8 / 36.2 / 36.7 / 46.6 / 37.2 / 46.4 / 42.3
+//                        3700:  66.1 / 51.1 / 50.0 / 69.9 / 53.5 / 50.3 / 44.8
+//         8192 x 8192 at   96:  30.2 / 21.4 / 29.3 / 27.2 / 30.2 / 63.2 / 73.7
+//                         512:   108 /  106 /  94  /  98  /  88  / 75.7 / 81.4
+//                         700:   148 /  147 /  130 /  144 /  124 /  131 /  120
+// So the larger tiles take what fills the CUs (128 x 128 in rounds of 256 tiles,
+// 64 x 64 in one or two), and the split ones the rest.
 template<bool Tiles>
 int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
     constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
@@ -710,15 +827,26 @@ int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
         if (row_tiles >= 512) return a.N <= 32 ? launch_stream<IN, 2, 2>(a, s) : launch_stream<IN, 2, 4>(a, s);
         return a.N <= 64 ? launch_stream<IN, 2, 1>(a, s) : launch_stream<IN, 2, 2>(a, s);
     }
+    const long t64 = tiles(64, 64), t128 = tiles(128, 128), rounds128 = (t128 + 255) / 256;
     if (a.y_type == MOE_F32) {
-        if (tiles(64, 64) <= 256) return launch_gemm<2, 2, 2, 2, 2, 4, Tiles, true>(a, s);
-        if (tiles(64, 64) <= 800) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, true>(a, s);
-        if (tiles(128, 128) <= 400) return launch_gemm<2, 2, 4, 4, 2, 2, Tiles, true>(a, s);
-        return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, true>(a, s);
+        if (tiles(64, 32) <= 256) return launch_split<4, 2, 8, Tiles, true>(a, s);
+        // The two forms of a number of groups give the same sums, and so do apply and forward.
+        const bool fills = t64 <= 512 && 10 * static_cast<long>(a.M) * a.N >= 9 * 4096 * 256 * ((t64 + 255) / 256);
+        if (t64 <= 256) {
+            if constexpr (Tiles)
+                if (!fills) return launch_split<2, 3, 4, true, true>(a, s);
+            return launch_gemm<2, 2, 2, 2, 2, 4, Tiles, true>(a, s);
+        }
+        if (rounds128 > 2 || t128 * 10 >= 256 * rounds128 * (rounds128 == 1 ? 8 : 7))
+            return rounds128 == 1 ? launch_gemm<2, 2, 4, 4, 2, 2, Tiles, true>(a, s) : launch_gemm<2, 2, 4, 4, 2, 1, Tiles, true>(a, s);
+        if constexpr (Tiles)
+            if (!fills) return launch_split<2, 3, 2, true, true>(a, s);
+        return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, true>(a, s);
     }
-    if (tiles(64, 64) <= 256) return launch_gemm<2, 2, 2, 2, 3, 2, Tiles, false>(a, s);
-    if (tiles(64, 64) <= 512) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, false>(a, s);
-    if (tiles(128, 128) < 256) return launch_gemm<2, 2, 4, 2, 2, 1, Tiles, false>(a, s);
+    if (tiles(64, 32) <= 256) return launch_split<4, 2, 8, Tiles, false>(a, s);
+    if (t64 <= 256) return launch_gemm<2, 2, 2, 2, 3, 2, Tiles, false>(a, s);
+    if (t64 <= 512) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, false>(a, s);
+    if (t128 < 256) return launch_gemm<2, 2, 4, 2, 2, 1, Tiles, false>(a, s);
     if (tiles(256, 256) < 240 || (tiles(256, 256) < 512 && a.nb > 32)) return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, false>(a, s);
     return launch_gemm_wide<Tiles>(a, s);
 }
