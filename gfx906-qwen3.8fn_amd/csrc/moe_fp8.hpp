@@ -121,15 +121,18 @@ __device__ __forceinline__ void unpack8(const Raw8 &r, float (&v)[8]) {
         }
     }
 }
-// Four consecutive results, 16 or 8 bytes (aligned to that).
+// Four consecutive results, 16 or 8 bytes at any alignment of their type (the
+// hardware takes such stores).
 template<int T>
 __device__ __forceinline__ void store4(void *p, size_t i, const float (&v)[4]) {
-    if constexpr (T == kF32)
-        *reinterpret_cast<float4 *>(static_cast<float *>(p) + i) = make_float4(v[0], v[1], v[2], v[3]);
-    else if constexpr (T == kBF16)
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + i) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-    else
-        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + i) = make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+    char *q = static_cast<char *>(p) + i * elem_bytes(T);
+    if constexpr (T == kF32) {
+        __builtin_memcpy(q, v, 16);
+    } else {
+        const uint2 w = T == kBF16 ? make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]))
+                                   : make_uint2(pack_f16(v[0], v[1]), pack_f16(v[2], v[3]));
+        __builtin_memcpy(q, &w, 8);
+    }
 }
 
 // ---------------------------------------------------------- quantisation ---

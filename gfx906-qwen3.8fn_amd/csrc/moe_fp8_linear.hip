@@ -135,7 +135,6 @@ struct Fp8LinearArgs {
     void *y;
     int64_t y_stride;
     int y_type;
-    int y_vec;               // rows of y take 4-element stores
     int x_vec;               // rows of x take 8-element loads
     int M, N, K, nb;
     int tile_stride;         // tiles from one 16 rows to the next: nb, made odd
@@ -146,7 +145,7 @@ struct Fp8LinearArgs {
 template<int Y>
 __device__ __forceinline__ void store_rows(const Fp8LinearArgs &a, int n, int m, const float (&v)[4]) {
     const size_t at = static_cast<size_t>(n) * a.y_stride + m;
-    if (a.y_vec && m + 3 < a.M) {
+    if (m + 3 < a.M) {
         store4<Y>(a.y, at, v);
         return;
     }
@@ -726,8 +725,6 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     a.y = y;
     a.y_type = y_type;
     a.y_stride = y_stride;
-    const int four = 4 * moe::elem_bytes(y_type);
-    a.y_vec = aligned(y, four) && y_stride * moe::elem_bytes(y_type) % four == 0;
     a.M = L->output;
     a.N = columns;
     a.K = L->input;
