@@ -787,33 +787,36 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 //         8192 x 8192 at 32 / 64:  22.9 / 16.3 / 15.4 / 17.5; 19.1 and
 //                                  40.4 / 26.7 / 22.8 / 18.0; 19.7
 //         8192 x 2048 at 100:      16.8 / 14.7 / 12.3 / 15.5; 18.5
-// As 64 x 64 tiles in two groups / in two of half as many waves / 128 x 64 /
-// 128 x 128 / 256 x 256:
-//   bf16  2048 x 2048 at   96:   8.7 /  9.4 / 12.5 / 15.9 /  30, streamed 7.2
-//         8192 x 8192 at   96:  20.9 / 24.7 / 37.8 / 47.1 /  94, streamed 33.7
-//         2048 x 2048 at  512:  10.2 / 10.7 / 13.7 / 17.4 /  35
-//         8192 x 8192 at  256:  44.0 / 30.0 / 41.0 / 50.6 / 100
-//         2048 x 2048 at 1032:  21.3 / 18.8 / 16.2 / 19.4 /  36
-//         2048 x 2048 at 4096:  52.3 / 39.5 / 36.7 / 32.9 /  42
-//         2048 x 2048 at 8192, 128 x 128 against 256 x 256: 61.2 / 52.2
-//         8192 x 8192 at 2048 / 4096: 158 / 184 and 331 / 300
-//         64 x 32 split among eight waves against 64 x 64 in two groups, 2048 x
-//         2048 at 170 / 256 / 333: 7.7, 8.1, 9.9 and 8.9, 9.2, 9.5
-//   fp32, 64 x 32 split among eight waves / 32 x 48 among four / among two / 64 x
-//         64 in four groups / in two of half as many waves / 128 x 128 in two
-//         groups / 128 x 128:
-//         2048 x 2048 at  256:   8.8 /  9.8 /  ..  / 12.0
-//                         333:  12.7 / 10.3 / 12.6 / 12.6 / 12.8 / 23.9 / 25.5
-//                         700:  16.9 / 15.1 / 14.4 / 20.6 / 17.1 / 24.6 / 26.4
-//                        1000:  20.9 / 18.8 / 19.8 / 20.9 / 17.9 / 25.2 / 26.8
-//                        1032:  23.7 / 19.2 / 19.9 / 27.2 / 22.8 / 25.0 / 26.7
-//                        2500:  45.8 / 36.2 / 36.7 / 46.6 / 37.2 / 46.4 / 42.3
-//                        3700:  66.1 / 51.1 / 50.0 / 69.9 / 53.5 / 50.3 / 44.8
-//         8192 x 8192 at   96:  30.2 / 21.4 / 29.3 / 27.2 / 30.2 / 63.2 / 73.7
-//                         512:   108 /  106 /  94  /  98  /  88  / 75.7 / 81.4
-//                         700:   148 /  147 /  130 /  144 /  124 /  131 /  120
-// So the larger tiles take what fills the CUs (128 x 128 in rounds of 256 tiles,
-// 64 x 64 in one or two), and the split ones the rest.
+// 16-bit results, 64 x 32 split among eight waves / 64 x 64 in two groups / in
+// two of half as many waves / 128 x 64 / 128 x 128 / 256 x 256:
+//         2048 x 2048 at  256:   8.2 /  9.3 /  9.9 / 13.1 / 16.9 / 34.1
+//                         333:  10.0 /  9.7 / 10.2 / 13.5 / 17.7 / 34.9
+//                        1000:  15.1 / 15.2 / 12.4 / 14.3 / 17.8 / 34.9
+//                        2500:  30.1 / 31.9 / 27.1 / 24.6 / 25.6 / 37.7
+//                        3700:  41.5 / 47.4 / 35.4 / 31.3 / 28.6 / 39.4
+//         8192 x 8192 at   96:  24.5 / 19.4 / 24.0 / 36.3 / 46.4 / 93.5, streamed 33.7
+//                         200:  43.9 / 35.3 / 28.7 / 38.0 / 48.2 / 97.0
+//                         700:   120 /   97 /  80  / 70.9 / 75.3 / 115
+//                        2048:   331 /  281 /  217 /  183 /  164 / 139
+//                        2800 / 3300 / 4300, the last two: 224 / 223, 263 / 236, 329 / 336
+//         2048 x 2048 at 7000 / 9000 / 12000, the last two: 49.4 / 46.0, 65.2 / 78.3, 80.9 / 86.4
+// fp32, 64 x 32 split among eight waves / 32 x 48 among four / among two / 64 x
+// 64 in four groups / in two of half as many waves / 128 x 128 in two groups /
+// 128 x 128:
+//         2048 x 2048 at  256:   8.7 /  9.8 / 12.1 / 11.7 / 11.9 / 21.6 / 23.3
+//                         333:  12.4 / 10.2 / 12.4 / 12.2 / 12.2 / 22.2 / 23.8
+//                         700:  16.6 / 14.3 / 14.0 / 19.8 / 15.9 / 22.5 / 24.2
+//                        1000:  20.8 / 18.4 / 19.4 / 20.4 / 17.0 / 23.6 / 25.3
+//                        1032:  23.3 / 18.2 / 19.3 / 26.4 / 21.8 / 23.4 / 25.1
+//                        2000:  36.3 / 29.4 / 28.9 / 35.6 / 28.6 / 26.5 / 28.1
+//                        2500:  45.0 / 35.1 / 37.5 / 44.3 / 36.5 / 43.0 / 39.4
+//                        3000:  52.8 / 40.2 / 40.7 / 52.1 / 40.4 / 44.0 / 39.7
+//         8192 x 8192 at   96:  29.2 / 21.2 / 29.1 / 26.0 / 29.4 / 61.7 / 71.1
+//                         128:  29.8 / 30.0 / 31.9 / 26.8 / 30.2 / 63.0 / 73.0
+//                         512:   107 /  108 /  95  /  96  /  89  / 78.0 / 83.9
+//                         700:   146 /  147 /  132 /  139 /  125 /  128 /  117
+// So the larger tiles take what fills the CUs, by how much of their last round of
+// 256 tiles is used, and the smaller ones the rest.
 template<bool Tiles>
 int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
     constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
@@ -843,8 +846,9 @@ int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
     if (tiles(64, 32) <= 256) return launch_split<4, 2, 8, Tiles, false>(a, s);
     if (t64 <= 256) return launch_gemm<2, 2, 2, 2, 3, 2, Tiles, false>(a, s);
     if (t64 <= 512) return launch_gemm<1, 2, 4, 2, 2, 2, Tiles, false>(a, s);
-    if (t128 < 256) return launch_gemm<2, 2, 4, 2, 2, 1, Tiles, false>(a, s);
-    if (tiles(256, 256) < 240 || (tiles(256, 256) < 512 && a.nb > 32)) return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, false>(a, s);
+    if (t128 < 400) return launch_gemm<2, 2, 4, 2, 2, 1, Tiles, false>(a, s);
+    const long t256 = tiles(256, 256);
+    if (t256 * 5 < 4 * 256 * ((t256 + 255) / 256)) return launch_gemm<2, 2, 4, 4, 2, 1, Tiles, false>(a, s);
     return launch_gemm_wide<Tiles>(a, s);
 }
 

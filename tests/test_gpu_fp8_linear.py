@@ -99,7 +99,8 @@ def check(y, codes_x, scales_x, w, dtype, wide):
 SHAPES = [(32, 1, 1), (96, 17, 3), (160, 130, 16), (1056, 100, 14), (8192, 4200, 1), (2048, 33, 16), (2048, 512, 1), (2048, 2048, 17), (1056, 300, 33), (16384, 48, 5),
           (640, 2560, 65), (352, 8200, 20), (288, 8210, 50), (3200, 77, 1500), (8192, 1500, 70), (2048, 5000, 66), (2080, 1000, 333), (128, 40, 700), (512, 2047, 1500), (8192, 200, 130),
           (1056, 1500, 1300), (64, 2100, 1100), (320, 2100, 1100), (192, 3000, 2100), (128, 4100, 4000), (416, 4000, 4090), (1024, 4000, 4090),
-          (160, 1500, 300), (1056, 1000, 900), (96, 1000, 900), (16384, 700, 1111), (416, 1020, 1000), (256, 2040, 2000)]
+          (160, 1500, 300), (1056, 1000, 900), (96, 1000, 900), (16384, 700, 1111), (416, 1020, 1000), (256, 2040, 2000),
+          (352, 4000, 4090), (64, 4090, 4000)]
 
 
 @pytest.mark.parametrize("K,M,N", SHAPES)
