@@ -515,6 +515,36 @@ struct GemmTile {
         else return Frag{*reinterpret_cast<const uint4 *>(p + b0off), *reinterpret_cast<const uint4 *>(p + b1off)};
     }
     __device__ __forceinline__ Frag row(const uint8_t *buf, int i) const { return load_tile(buf + aread + i * 2048, lane); }
+    // 16-bit results by way of LDS (lds: the buffers, which no wave reads or
+    // fills any more), so that a wave's stores run along the rows of y.
+    template<int Y>
+    __device__ __forceinline__ void store_along_rows(const Fp8LinearArgs &a, const f32x4 (&acc)[TM][TN], uint8_t *lds) const {
+        constexpr int Pitch = BM * 2 + 8, Lanes = BM / 4;   // lanes of a row
+        static_assert(G == 1 && Y != kF32 && BN * Pitch <= Lds && 64 * W % Lanes == 0);
+#pragma unroll
+        for (int t = 0; t < TN; ++t)
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const float v[4] = {acc[i][t][0], acc[i][t][1], acc[i][t][2], acc[i][t][3]};
+                store4<Y>(lds + ((wc * TN + t) * 16 + (lane & 15)) * Pitch, (wr * TM + i) * 16 + (lane >> 4) * 4, v);
+            }
+        __syncthreads();
+        const int c = static_cast<int>(threadIdx.x) % Lanes * 4;
+#pragma unroll 4
+        for (int n = static_cast<int>(threadIdx.x) / Lanes; n < min(a.N - n0, BN); n += 64 * W / Lanes) {
+            uint2 w;
+            __builtin_memcpy(&w, lds + n * Pitch + c * 2, 8);
+            const size_t at = static_cast<size_t>(n0 + n) * a.y_stride + m0 + c;
+            uint16_t *y = static_cast<uint16_t *>(a.y) + at;
+            if (m0 + c + 3 < a.M) {
+                __builtin_memcpy(y, &w, 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (m0 + c + i < a.M) y[i] = static_cast<uint16_t>((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
+            }
+        }
+    }
     template<int Y>
     __device__ __forceinline__ void store(const Fp8LinearArgs &a, const f32x4 (&acc)[TM][TN]) const {
 #pragma unroll
@@ -606,7 +636,12 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
         }
         if (group > 0) return;
     }
-    g.template store<Y>(a, acc);
+    if constexpr (G == 1 && Y != kF32) {
+        __syncthreads();
+        g.template store_along_rows<Y>(a, acc, lds[0]);
+    } else {
+        g.template store<Y>(a, acc);
+    }
 }
 
 // The largest batches: 256 x 256 a workgroup, eight waves of 128 x 64, two on
@@ -685,7 +720,7 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
         turn(false);
     }
     if (g.wr == 0) turn(false);   // as many turns for every wave
-    g.template store<Y>(a, acc);
+    g.template store_along_rows<Y>(a, acc, lds);
 }
 
 }  // namespace
