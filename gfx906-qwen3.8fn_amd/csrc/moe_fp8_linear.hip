@@ -516,7 +516,10 @@ struct GemmTile {
     }
     __device__ __forceinline__ Frag row(const uint8_t *buf, int i) const { return load_tile(buf + aread + i * 2048, lane); }
     // 16-bit results by way of LDS (lds: the buffers, which no wave reads or
-    // fills any more), so that a wave's stores run along the rows of y.
+    // fills any more), so that a wave's stores run along the rows of y: straight
+    // from the accumulators they are pieces of four elements of 16 rows each
+    // (96 x 2047 at 16,000 columns 41 us, 22 so; 96 x 2048 26 and 21; 8192 x 8192 at
+    // 16,384 1,012 and 985).  fp32 pieces are twice as long and gain nothing.
     template<int Y>
     __device__ __forceinline__ void store_along_rows(const Fp8LinearArgs &a, const f32x4 (&acc)[TM][TN], uint8_t *lds) const {
         constexpr int Pitch = BM * 2 + 8, Lanes = BM / 4;   // lanes of a row
@@ -824,17 +827,17 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 //         8192 x 2048 at 100:      16.8 / 14.7 / 12.3 / 15.5; 18.5
 // 16-bit results, 64 x 32 split among eight waves / 64 x 64 in two groups / in
 // two of half as many waves / 128 x 64 / 128 x 128 / 256 x 256:
-//         2048 x 2048 at  256:   8.2 /  9.3 /  9.9 / 13.1 / 16.9 / 34.1
-//                         333:  10.0 /  9.7 / 10.2 / 13.5 / 17.7 / 34.9
-//                        1000:  15.1 / 15.2 / 12.4 / 14.3 / 17.8 / 34.9
-//                        2500:  30.1 / 31.9 / 27.1 / 24.6 / 25.6 / 37.7
-//                        3700:  41.5 / 47.4 / 35.4 / 31.3 / 28.6 / 39.4
-//         8192 x 8192 at   96:  24.5 / 19.4 / 24.0 / 36.3 / 46.4 / 93.5, streamed 33.7
-//                         200:  43.9 / 35.3 / 28.7 / 38.0 / 48.2 / 97.0
-//                         700:   120 /   97 /  80  / 70.9 / 75.3 / 115
-//                        2048:   331 /  281 /  217 /  183 /  164 / 139
-//                        2800 / 3300 / 4300, the last two: 224 / 223, 263 / 236, 329 / 336
-//         2048 x 2048 at 7000 / 9000 / 12000, the last two: 49.4 / 46.0, 65.2 / 78.3, 80.9 / 86.4
+//         2048 x 2048 at  256:   8.3 /  9.4 / 10.0 / 12.9 / 16.4 / 29.7
+//                         333:  10.0 /  9.7 / 10.3 / 13.3 / 16.7 / 30.1
+//                        1000:  15.4 / 15.3 / 12.5 / 14.3 / 18.0 / 30.6
+//                        2500:  30.4 / 31.8 / 27.4 / 24.0 / 24.4 / 34.2
+//                        3700:  41.4 / 47.4 / 35.5 / 30.7 / 26.9 / 35.5
+//         8192 x 8192 at   96:  24.5 / 19.7 / 24.2 / 36.2 / 46.1 / 91.0, streamed 33.7
+//                         200:  44.0 / 35.4 / 27.9 / 38.1 / 48.2 / 94.1
+//                         700:   133 /   97 /  79  / 73.5 / 74.3 / 111
+//                        2048:   331 /  273 /  219 /  187 /  163 / 141
+//                        2800 / 3300 / 4300, the last two: 223 / 221, 260 / 244, 327 / 333
+//         2048 x 2048 at 7000 / 9000 / 12000, the last two: 46.4 / 45.1, 60.8 / 70.8, 76.1 / 79.5
 // fp32, 64 x 32 split among eight waves / 32 x 48 among four / among two / 64 x
 // 64 in four groups / in two of half as many waves / 128 x 128 in two groups /
 // 128 x 128:
