@@ -30,28 +30,7 @@ struct NormArgs {
     int hidden, tokens, gate_form, gate_sigmoid;
 };
 
-// Eight elements at any alignment of their type (the hardware takes such 16-byte
-// accesses), of which the first `valid` are the row's; 0 after those.
-template<int T>
-__device__ __forceinline__ Raw8 load8_any(const void *p, size_t at, int valid) {
-    Raw8 r{};
-    const char *q = static_cast<const char *>(p) + at * elem_bytes(T);
-    if (valid >= 8) {
-        __builtin_memcpy(&r.lo, q, 16);
-        if constexpr (T == kF32) __builtin_memcpy(&r.hi, q + 16, 16);
-    } else if (valid > 0) {
-        uint32_t w[8] = {};
-#pragma unroll
-        for (int i = 0; i < 7; ++i) {
-            if (i >= valid) break;
-            if constexpr (T == kF32) w[i] = reinterpret_cast<const uint32_t *>(q)[i];
-            else w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t *>(q)[i]) << (16 * (i & 1));
-        }
-        r.lo = make_uint4(w[0], w[1], w[2], w[3]);
-        if constexpr (T == kF32) r.hi = make_uint4(w[4], w[5], w[6], w[7]);
-    }
-    return r;
-}
+// The counterpart of load8_any.
 template<int T>
 __device__ __forceinline__ void store8_any(void *p, size_t at, int valid, const float (&v)[8]) {
     char *q = static_cast<char *>(p) + at * elem_bytes(T);
