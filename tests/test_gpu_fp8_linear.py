@@ -342,3 +342,47 @@ def test_bound_calls_keep_the_matrix():
     lin.close()
     with pytest.raises(moe_ffn.MoeError):
         call()
+
+
+# The tiles of test_forward_and_apply's wider shapes, with a last row tile of few rows.
+@pytest.mark.parametrize("K,M,N", [(160, 1501, 300), (1056, 1001, 900), (512, 2047, 1500), (64, 2101, 1100), (192, 3003, 2100),
+                                   (352, 4090, 4090)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_strided_rows_of_wide_batches(K, M, N, dtype):
+    """Rows of x and y inside wider tensors at odd starts: the results of
+    contiguous ones, and nothing between them touched."""
+    g = R.generator(K + M)
+    codes, scales = R.random_matrix(M, K, g)
+    x = torch.randn((N, K + 5), generator=g, device=DEV).to(dtype)[:, 3:3 + K]
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales, max_columns=N)
+    want, e = lin.apply(x.contiguous())
+    out = torch.full((N + 1, M + 6), 7.0, dtype=dtype, device=DEV)
+    y = out[:N, 1:1 + M]
+    lin.apply(x, y=y, error=e)
+    assert same(y, want) and flag(e) == 0
+    y.fill_(7.0)
+    assert bool((out == 7.0).all())
+    lin.forward(*R.quantise(x), y=y)
+    assert same(y, want)
+    y.fill_(7.0)
+    assert bool((out == 7.0).all())
+    lin.close()
+
+
+def test_overlapping_forwards_of_one_handle():
+    K, M = 1024, 1000
+    g = R.generator(31)
+    codes, scales = R.random_matrix(M, K, g)
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales)
+    rows = [R.quantise(torch.randn((n, K), generator=g, device=DEV)) for n in (7, 900)]
+    want = [lin.forward(*r, dtype=BF16) for r in rows]
+    streams = [torch.cuda.Stream() for _ in rows]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for r, s in zip(rows, streams):
+            with torch.cuda.stream(s):
+                got.append(lin.forward(*r, dtype=BF16))
+    torch.cuda.synchronize()
+    assert all(same(y, want[i % 2]) for i, y in enumerate(got))
+    lin.close()
