@@ -27,9 +27,8 @@ __host__ __device__ constexpr int elem_bytes(int type) { return type == kF32 ? 4
 // Sources of e4m3 columns that are quantised before a product: rows and tiles.
 inline constexpr int kCodes = 3, kTiles = 4;
 
-// Canonical e4m3 codes [rows][cols] -> tiles, `stride` tiles from one 16 rows
-// to the next (zeros past the row's own).  cols % 16 == 0.
-hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, int stride, hipStream_t s);
+// Canonical e4m3 codes [rows][cols] -> tiles.  cols % 16 == 0.
+hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, hipStream_t s);
 // Rows of `type` -> codes [columns][width] and scales [columns][ceil(width/128)].
 hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
                                 float *scales, int *error, hipStream_t s);

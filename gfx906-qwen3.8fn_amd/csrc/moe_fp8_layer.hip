@@ -544,7 +544,7 @@ hipError_t upload(moe_fp8_layer *L, const Part &p, const moe_fp8_matrix &m, size
     }
     if (r == hipSuccess)
         r = moe::launch_fp8_repack(static_cast<const uint8_t *>(codes), L->mem + p.tiles_at + first * p.tiles, count * p.rows,
-                                   p.cols, blocks(p.cols), nullptr);
+                                   p.cols, nullptr);
     if (r == hipSuccess)
         r = hipMemcpy(L->mem + p.scales_at + first * p.scales * 4, m.scales, count * p.scales * 4,
                       on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);

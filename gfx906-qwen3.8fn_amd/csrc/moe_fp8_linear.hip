@@ -16,13 +16,13 @@ namespace {
 // --------------------------------------------------------------- layout ---
 // One thread per 16-byte chunk of the tiles.
 __global__ __launch_bounds__(256) void k_fp8_repack(const uint8_t *__restrict__ codes, uint4 *__restrict__ tiles,
-                                                    size_t rows, int cols, int stride, size_t chunks) {
+                                                    size_t rows, int cols, int nb, size_t chunks) {
     const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
     if (i >= chunks) return;
     const int lane = static_cast<int>(i & 63), half = static_cast<int>(i >> 6) & 1;
     const size_t tile = i >> 7;
-    const size_t row = tile / stride * kFp8TileRows + (lane & 15);
-    const int col = static_cast<int>(tile % stride) * kFp8Block + (lane >> 4) * 32 + half * 16;
+    const size_t row = tile / nb * kFp8TileRows + (lane & 15);
+    const int col = static_cast<int>(tile % nb) * kFp8Block + (lane >> 4) * 32 + half * 16;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows && col < cols) __builtin_memcpy(&v, codes + row * cols + col, 16);
     tiles[i] = v;
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void k_fp8_repack(const uint8_t *__restrict__ 
 // operand layout, and scales [block][row]; otherwise the canonical rows.
 template<int T, bool Tiles>
 __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ x, int64_t stride, int width, int nb,
-                                                       int columns, uint8_t *__restrict__ codes, int tile_stride,
+                                                       int columns, uint8_t *__restrict__ codes,
                                                        float *__restrict__ scales, int64_t scale_stride, int *error) {
     size_t n;
     int b;
@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ 
     const uint2 c = quantize8(v, s);
     if constexpr (Tiles) {
         // Elements 8 part .. + 7: half of a chunk of lane 16 (part / 4) + n % 16.
-        uint8_t *tile = codes + (n / 16 * tile_stride + b) * kFp8TileBytes;
+        uint8_t *tile = codes + (n / 16 * nb + b) * kFp8TileBytes;
         *reinterpret_cast<uint2 *>(tile + tile_offset(part, static_cast<int>(n & 15))) = c;
         if (part == 0) scales[b * scale_stride + n] = s.s;
     } else {
@@ -77,16 +77,17 @@ __global__ __launch_bounds__(256) void k_quantize_e4m3(const void *__restrict__ 
 
 }  // namespace
 
-hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, int stride, hipStream_t s) {
+hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, int cols, hipStream_t s) {
+    const int nb = (cols + kFp8Block - 1) / kFp8Block;
     // A grid holds fewer than 2^32 threads: at most 2^30 chunks a launch.
-    const size_t row_chunks = static_cast<size_t>(stride) * kFp8TileBytes / 16;   // of 16 rows
+    const size_t row_chunks = static_cast<size_t>(nb) * kFp8TileBytes / 16;   // of 16 rows
     const size_t rows_at_once = (size_t{1} << 30) / row_chunks * kFp8TileRows;
     for (size_t first = 0; first < rows; first += rows_at_once) {
         const size_t n = std::min(rows_at_once, rows - first);
         const size_t chunks = (n + kFp8TileRows - 1) / kFp8TileRows * row_chunks;
         k_fp8_repack<<<dim3(static_cast<unsigned>((chunks + 255) / 256)), dim3(256), 0, s>>>(
-            codes + first * cols, reinterpret_cast<uint4 *>(tiles + first / kFp8TileRows * stride * kFp8TileBytes), n, cols,
-            stride, chunks);
+            codes + first * cols, reinterpret_cast<uint4 *>(tiles + first / kFp8TileRows * nb * kFp8TileBytes), n, cols, nb,
+            chunks);
     }
     return hipGetLastError();
 }
@@ -94,13 +95,13 @@ hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, 
 namespace {
 
 template<bool Tiles>
-hipError_t launch_quantize(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes, int tile_stride,
+hipError_t launch_quantize(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
                            float *scales, int64_t scale_stride, int *error, hipStream_t s) {
     const int nb = (width + kFp8Block - 1) / kFp8Block;
     const size_t groups = Tiles ? static_cast<size_t>((columns + 15) / 16) * nb : (static_cast<size_t>(columns) * nb + 15) / 16;
     const dim3 grid(static_cast<unsigned>(groups)), block(256);
     const auto launch = [&](auto kernel) {
-        kernel<<<grid, block, 0, s>>>(x, stride, width, nb, columns, codes, tile_stride, scales, scale_stride, error);
+        kernel<<<grid, block, 0, s>>>(x, stride, width, nb, columns, codes, scales, scale_stride, error);
     };
     if (type == kF32) launch(k_quantize_e4m3<kF32, Tiles>);
     else if (type == kBF16) launch(k_quantize_e4m3<kBF16, Tiles>);
@@ -112,24 +113,23 @@ hipError_t launch_quantize(const void *x, int type, int64_t stride, int width, i
 
 hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
                                 float *scales, int *error, hipStream_t s) {
-    return launch_quantize<false>(x, type, stride, width, columns, codes, 0, scales, 0, error, s);
+    return launch_quantize<false>(x, type, stride, width, columns, codes, scales, 0, error, s);
 }
 
 namespace {
 
 struct Fp8LinearArgs {
-    const uint8_t *tiles;    // [ceil(M/16)][tile_stride] tiles, nb of each used
+    const uint8_t *tiles;    // [ceil(M/16)][nb] tiles
     const float *wscale;     // [ceil(M/128)][nb]
     const void *x;           // rows of a type (few columns), or unused
     int64_t x_stride;
-    const uint8_t *codes;    // e4m3 columns: rows [N][K], or tiles [ceil(N/16)][tile_stride]
+    const uint8_t *codes;    // e4m3 columns: rows [N][K], or tiles [ceil(N/16)][nb]
     const float *xscale;     // scale of column n, block b at n scale_n + b scale_b
     int scale_n, scale_b;
     void *y;
     int64_t y_stride;
     int y_type;
     int M, N, K, nb;
-    int tile_stride;         // tiles from one 16 rows to the next: nb, made odd
     int *error;
 };
 
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int mt = min(static_cast<int>(blockIdx.x) * RT + r, row_tiles - 1);   // past the end: the last one again
-        row[r] = a.tiles + static_cast<size_t>(mt) * a.tile_stride * kFp8TileBytes;
+        row[r] = a.tiles + static_cast<size_t>(mt) * a.nb * kFp8TileBytes;
         wscale[r] = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
     }
     const int kl = (lane >> 4) * 32;
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
                 float sx;
                 if constexpr (IN == kTiles) {
                     const int tile = min(n0 / 16 + t, (a.N - 1) / 16);
-                    x = load_tile(a.codes + (static_cast<size_t>(tile) * a.tile_stride + b) * kFp8TileBytes, lane);
+                    x = load_tile(a.codes + (static_cast<size_t>(tile) * a.nb + b) * kFp8TileBytes, lane);
                 } else if constexpr (IN == kCodes) {
                     const int k = b * kFp8Block + kl;
                     x = Frag{};
@@ -306,11 +306,11 @@ __global__ __launch_bounds__(64 * W) void k_fp8_split(Fp8LinearArgs a, int tiles
     const float *xscale[TN], *wscale = a.wscale + static_cast<size_t>(mt * kFp8TileRows / kFp8Block) * a.nb;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
-        row[i] = a.tiles + static_cast<size_t>(min(mt + i, row_tiles - 1)) * a.tile_stride * kFp8TileBytes;
+        row[i] = a.tiles + static_cast<size_t>(min(mt + i, row_tiles - 1)) * a.nb * kFp8TileBytes;
 #pragma unroll
     for (int t = 0; t < TN; ++t) {
         const int n = min((nt + t) * 16 + (lane & 15), a.N - 1);
-        if constexpr (Tiles) col[t] = a.codes + static_cast<size_t>(min(nt + t, col_tiles - 1)) * a.tile_stride * kFp8TileBytes;
+        if constexpr (Tiles) col[t] = a.codes + static_cast<size_t>(min(nt + t, col_tiles - 1)) * a.nb * kFp8TileBytes;
         else col[t] = a.codes + static_cast<size_t>(n) * a.K + kl;
         xscale[t] = a.xscale + static_cast<size_t>(n) * a.scale_n;
     }
@@ -387,10 +387,7 @@ __global__ __launch_bounds__(64 * W) void k_fp8_split(Fp8LinearArgs a, int tiles
 // Otherwise they are canonical rows with scales [column][block], of which four
 // blocks' are loaded at once where a row's lie on 16 bytes: a block at a time,
 // the columns' scales take as many memory requests as their codes (8192 x 8192
-// at 16,384 columns 1.15 ms, in fours 1.08).  The tiles of 16 rows are an odd
-// number of tiles apart: at a power-of-two width a step's rows would lie a
-// multiple of the L2's channel period apart and queue up at one channel (1.31
-// against 1.15 ms).
+// at 16,384 columns 1.09 ms, in fours 1.01).
 template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles>
 struct GemmTile {
     static constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
@@ -422,7 +419,7 @@ struct GemmTile {
         nb = a.nb;
         // Rows of the matrix and columns past the end are read as zeros.
         const int row_tiles = (a.M + 15) / 16, cols = min(a.N - n0, BN);
-        tile_row = static_cast<uint32_t>(a.tile_stride) * kFp8TileBytes;   // bytes of 16 rows
+        tile_row = static_cast<uint32_t>(a.nb) * kFp8TileBytes;   // bytes of 16 rows
         ar = buffer_rsrc(a.tiles + static_cast<size_t>(m0 / 16) * tile_row,
                          static_cast<uint32_t>(min(row_tiles - m0 / 16, BM / 16)) * tile_row);
         aoff = lane * 16;
@@ -717,7 +714,7 @@ __global__ __launch_bounds__(512) void k_fp8_gemm_wide(Fp8LinearArgs a, int tile
 // ------------------------------------------------------------------ C ABI ---
 struct moe_fp8_linear {
     int input = 0, output = 0, max_columns = 0, device = 0;
-    int nb = 0, tile_stride = 0;
+    int nb = 0;
     uint8_t *mem = nullptr;       // tiles, scales
     const float *scales = nullptr;
     uint8_t *ws = nullptr;        // columns as tiles, then scales [nb][columns]
@@ -752,7 +749,6 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     a.N = columns;
     a.K = L->input;
     a.nb = L->nb;
-    a.tile_stride = L->tile_stride;
     return a;
 }
 
@@ -906,8 +902,7 @@ int moe_fp8_linear_create(int input, int output, int max_columns, const void *co
     L->nb = (input + moe::kFp8Block - 1) / moe::kFp8Block;
     const size_t code_bytes = static_cast<size_t>(output) * input;
     const size_t scale_bytes = static_cast<size_t>((output + 127) / 128) * L->nb * 4;
-    L->tile_stride = L->nb | 1;
-    const auto tile_bytes = [&](int rows) { return static_cast<size_t>((rows + 15) / 16) * L->tile_stride * moe::kFp8TileBytes; };
+    const auto tile_bytes = [&](int rows) { return static_cast<size_t>((rows + 15) / 16) * L->nb * moe::kFp8TileBytes; };
     const size_t tiles = tile_bytes(output);
     const size_t scale_at = round_up(tiles, 256);
     void *staging = nullptr;
@@ -922,8 +917,7 @@ int moe_fp8_linear_create(int input, int output, int max_columns, const void *co
         if (r == hipSuccess) r = hipMemcpy(staging, codes, code_bytes, hipMemcpyHostToDevice);
         device_codes = staging;
     }
-    if (r == hipSuccess) r = moe::launch_fp8_repack(static_cast<const uint8_t *>(device_codes), L->mem, output, input,
-                                                       L->tile_stride, nullptr);
+    if (r == hipSuccess) r = moe::launch_fp8_repack(static_cast<const uint8_t *>(device_codes), L->mem, output, input, nullptr);
     if (r == hipSuccess)
         r = hipMemcpy(L->mem + scale_at, scales, scale_bytes, weights_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);
     if (r == hipSuccess) r = hipDeviceSynchronize();
@@ -990,8 +984,8 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
         if (x_type == MOE_BF16) return launch_stream<moe::kBF16, 1, 1>(a, s);
         return launch_stream<moe::kF16, 1, 1>(a, s);
     }
-    auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>((columns + 15) / 16) * L->tile_stride * moe::kFp8TileBytes);
-    const hipError_t r = moe::launch_quantize<true>(x, x_type, x_stride, L->input, columns, L->ws, L->tile_stride, scales, columns,
+    auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>((columns + 15) / 16) * L->nb * moe::kFp8TileBytes);
+    const hipError_t r = moe::launch_quantize<true>(x, x_type, x_stride, L->input, columns, L->ws, scales, columns,
                                                     error, s);
     if (r != hipSuccess) return r;
     a.codes = L->ws;
