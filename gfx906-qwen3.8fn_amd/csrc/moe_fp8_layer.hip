@@ -350,7 +350,7 @@ inline constexpr int kDownPiece = 8, kDownTiles = 16;
 template<int T_>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(6))) void k_fp8_down_fold(Fp8LayerArgs a, int tiles) {
     extern __shared__ __attribute__((aligned(16))) float part[];   // [rank][16 tiles]
-    __shared__ __attribute__((aligned(16))) uint8_t codes[16][kDownPiece * kFp8Block];
+    __shared__ __attribute__((aligned(16))) _Float16 codes[16][kDownPiece * kFp8Block];   // widened, once for all of the rows
     __shared__ float scales[16][kDownPiece];
     constexpr int U = 2;
     const int R = 16 * tiles;
@@ -397,7 +397,8 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(6))) void 
                 float v[8];
                 unpack8<kF32>(raw, v);
                 const GroupScale g = group_scale(max16(v));
-                *reinterpret_cast<uint2 *>(&codes[wave][h * 512 + lane * 8]) = quantize8(v, g);
+                const uint2 c = quantize8(v, g);
+                *reinterpret_cast<f16x8 *>(&codes[wave][h * 512 + lane * 8]) = e4m3_to_f16(c.x, c.y);
                 if ((lane & 15) == 0) scales[wave][4 * h + (lane >> 4)] = g.s;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -412,8 +413,8 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(6))) void 
                 for (int u = 0; u < U; ++u) {
                     const int b = q * U + u;
                     if (b >= kb) break;
-                    const uint4 *c = reinterpret_cast<const uint4 *>(&codes[wave][b * kFp8Block + (lane >> 4) * 32]);
-                    const f32x4 p = block_dot(to_f16(f[u]), to_f16(Frag{c[0], c[1]}));
+                    const f16x8 *c = reinterpret_cast<const f16x8 *>(&codes[wave][b * kFp8Block + (lane >> 4) * 32]);
+                    const f32x4 p = block_dot(to_f16(f[u]), FragF16{{c[0], c[1], c[2], c[3]}});
                     const float sc = scales[wave][b] * sw[b];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) acc[i] = fmaf(p[i], sc, acc[i]);

@@ -82,7 +82,8 @@ def check(y, x, ids, w, bank, gate):
 # and of 128 (which gate/up takes in pieces); 1 to 32 routes a token.
 CASES = [(1, 64, 32, 4, 2, True), (1, 2048, 512, 64, 10, True), (3, 96, 160, 8, 8, False), (64, 128, 96, 1, 1, True),
          (64, 256, 352, 5, 2, False), (17, 416, 64, 40, 32, True), (33, 640, 288, 16, 3, True), (2, 16384, 32, 3, 1, True),
-         (9, 32, 16384, 3, 2, False), (20, 4128, 128, 6, 6, True), (8, 2048, 512, 512, 10, True), (5, 2560, 640, 48, 10, True)]
+         (9, 32, 16384, 3, 2, False), (20, 4128, 128, 6, 6, True), (8, 2048, 512, 512, 10, True), (5, 2560, 640, 48, 10, True),
+         (64, 4096, 64, 40, 32, True)]
 
 
 @pytest.mark.parametrize("T,H,I,E,k,shared", CASES)
