@@ -176,8 +176,9 @@ __device__ __forceinline__ void quantize_columns(const void *x, Rows rows, int c
 // items in turn, each with its first tiles on their way before the last one's
 // sums are done.  64 tokens, 2048/512, layer time in us with top-10 of 512
 // uniform / Zipf(1.1): 274 / 205 with a workgroup per route and slice, of
-// which those of an expert's later routes end at once, 244 / 170 so; with
-// eight or two waves a tile 258 / 191 and 251 / 178.  Four waves a SIMD (two
+// which those of an expert's later routes end at once, 244 / 170 so (235 / 165
+// with the down kernel as it is now); with eight or two waves a tile 258 / 191
+// and 251 / 178.  Four waves a SIMD (two
 // workgroups a CU): with two blocks a round in flight the kernel needs 167
 // registers and one fits (268 / 185).
 template<int T_>
@@ -345,7 +346,11 @@ __device__ __forceinline__ int route(const Fp8LayerArgs &a, int t, int r, float 
 // their way.  All 16 columns of its MFMA hold the one token, so every lane has
 // its results.
 // Six waves a SIMD: two workgroups of eleven waves (top-10 and the shared
-// expert) fit a CU, one streaming while the other starts or sums up.
+// expert) fit a CU, one streaming while the other starts or sums up.  2048/512,
+// 1 / 8 / 64 tokens 6.1 / 19.6 / 65 us: bound by latency, then by HBM (79 MB at
+// 4.0 TB/s), then by the tiles' way from L2 (720 MB) and their conversions.  The
+// middle's codes lie in LDS as fp16 already: widened again for every row tile,
+// they were half of the conversions (6.9 / 20.7 / 67).
 inline constexpr int kDownPiece = 8, kDownTiles = 16;
 template<int T_>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(6))) void k_fp8_down_fold(Fp8LayerArgs a, int tiles) {
@@ -458,8 +463,8 @@ hipError_t launch_layer(const Fp8LayerArgs &a, hipStream_t s) {
     const int row_tiles = a.H / 16;
     // Row tiles a workgroup: the fewest on the busiest CU, and of such choices
     // one workgroup a CU for few tokens, two (which fit at once) for more: us a
-    // layer of 2048/512 with 2 / 4 / 8 / 16, 8 tokens 56.1 / 53.9 / 62.1 / 80.8,
-    // 32 tokens 172 / 163 / 157 / 159, 64 tokens 277 / 263 / 255 / 242.
+    // layer of 2048/512 with 2 / 4 / 8 / 16, 8 tokens 53.7 / 52.7 / 60.6 / 80.3,
+    // 32 tokens 166 / 157 / 151 / 155, 64 tokens 271 / 253 / 249 / 235.
     int tiles = 1, best = INT_MAX, best_off = 0;
     for (int n = 1; n <= kDownTiles; ++n) {
         const int rounds = (a.T * ((row_tiles + n - 1) / n) + 255) / 256, off = std::abs(rounds - (a.T <= 8 ? 1 : 2));
