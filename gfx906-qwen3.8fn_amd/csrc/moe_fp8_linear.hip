@@ -385,7 +385,7 @@ __global__ __launch_bounds__(64 * W) void k_fp8_split(Fp8LinearArgs a, int tiles
 //
 // Tiles: the columns lie in tiles as the rows do, their scales [block][column].
 // Otherwise they are canonical rows with scales [column][block], of which four
-// blocks' are loaded at once where a row's lie on 16 bytes: a block at a time,
+// blocks' are loaded at once where a row has that many: a block at a time,
 // the columns' scales take as many memory requests as their codes (8192 x 8192
 // at 16,384 columns 1.09 ms, in fours 1.01).
 template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles>
@@ -437,7 +437,7 @@ struct GemmTile {
         sr = buffer_rsrc(a.xscale + static_cast<size_t>(n0) * a.scale_n,
                          (static_cast<uint32_t>(cols - 1) * a.scale_n + static_cast<uint32_t>(a.nb - 1) * a.scale_b + 1) * 4);
         soff = static_cast<uint32_t>(wave % (BN / 64) * 64 + lane) * a.scale_n * 4;
-        fours = !Tiles && a.nb % 4 == 0 && reinterpret_cast<uintptr_t>(a.xscale) % 16 == 0;
+        fours = !Tiles && a.nb >= 4;
         sstep = static_cast<uint32_t>(a.scale_b) * 4;
         if (wave % (BN / 64) * 64 + lane >= cols) soff = kPastEnd;
         lds0 = lds_offset(lds);
@@ -480,15 +480,18 @@ struct GemmTile {
         if (!Tiles && fours) {
             // Of the group's blocks b, b + G, .. the first of each four.
             if ((b & 3) < G)
-                load_to_lds(sr, b < nb ? soff + (b & ~3) * 4 : kPastEnd, lds0 + S * Buffer + (b >> 2 & 1) * (BN * 16) + part * 1024);
+                load_to_lds(sr, b < nb ? soff + first_of_four(b) * 4 : kPastEnd, lds0 + S * Buffer + (b >> 2 & 1) * (BN * 16) + part * 1024);
         } else {
             load_word_to_lds(sr, b < nb ? soff + b * sstep : kPastEnd, lds0 + buf * Buffer + ABytes + BBytes + part * 256);
         }
     }
+    // The first of the four blocks whose scales are loaded with block b's: the
+    // last four of a row end with it.
+    __device__ __forceinline__ int first_of_four(int b) const { return min(b & ~3, nb - 4); }
     // The scale of column l % 16 of column tile t in block b, whose buffer is buf of lds.
     __device__ __forceinline__ float scale(const uint8_t *lds, const uint8_t *buf, int b, int t) const {
         if (!Tiles && fours)
-            return *reinterpret_cast<const float *>(lds + S * Buffer + (b >> 2 & 1) * (BN * 16) + (wc * TN * 16 + t * 16 + (lane & 15)) * 16 + (b & 3) * 4);
+            return *reinterpret_cast<const float *>(lds + S * Buffer + (b >> 2 & 1) * (BN * 16) + (wc * TN * 16 + t * 16 + (lane & 15)) * 16 + (b - first_of_four(b) & 3) * 4);
         return *reinterpret_cast<const float *>(buf + sread + t * 64);
     }
     __device__ __forceinline__ Frag column(const uint8_t *buf, int t) const {

@@ -386,3 +386,20 @@ def test_overlapping_forwards_of_one_handle():
     torch.cuda.synchronize()
     assert all(same(y, want[i % 2]) for i, y in enumerate(got))
     lin.close()
+
+
+@pytest.mark.parametrize("K,M,N", [(640, 4090, 4090), (896, 1500, 1500), (1056, 600, 900), (2048, 512, 16), (512, 1000, 60)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_scales_at_any_start(K, M, N, dtype):
+    """Scales of the rows one element behind a 16-byte boundary, and rows of
+    scales of which not every four lie within a row."""
+    g = R.generator(K + N)
+    codes, scales = R.random_matrix(M, K, g)
+    qc, qs = R.quantise(torch.randn((N, K), generator=g, device=DEV))
+    lin = moe_ffn.MoeFp8Linear(K, M, codes, scales)
+    want = lin.forward(qc, qs, dtype=dtype)
+    moved = torch.full((qs.numel() + 2,), float("nan"), device=DEV)
+    moved[1:-1] = qs.flatten()
+    assert same(lin.forward(qc, moved[1:-1].view_as(qs), dtype=dtype), want)
+    check(want, qc, qs, R.matrix(codes, scales), dtype, N > 64)
+    lin.close()
