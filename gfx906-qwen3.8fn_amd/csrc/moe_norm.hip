@@ -51,12 +51,15 @@ __device__ __forceinline__ void store8_any(void *p, size_t at, int valid, const 
 
 // 1 / (1 + e^-g).  e^-g = 2^t (1 + r ln 2) with t the rounded product -g log2 e
 // and r what rounding it left out; 2^t and the quotient are the hardware's, an
-// ulp each, so that the whole is within 8 half ulps.  Infinite g: 0 or 1.
+// ulp each, so that the whole is within 8 half ulps.  Beyond |t| = 127 there is
+// nothing to correct: 2^t is infinite from t = 128 on (and r times it NaN), 1 +
+// 2^t is 1 below -25, and a quotient below 2^-126, from t = 126 on, is 0 or
+// itself.  Infinite g: 0 or 1.
 __device__ __forceinline__ float sigmoid(float g) {
     constexpr float log2e = 0x1.715476p+0f, log2e_rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;
     const float t = -g * log2e;
     float e = __builtin_amdgcn_exp2f(t);
-    if (fabsf(t) < 200.0f) e = fmaf(e, fmaf(-g, log2e_rest, fmaf(-g, log2e, -t)) * ln2, e);
+    if (fabsf(t) < 127.0f) e = fmaf(e, fmaf(-g, log2e_rest, fmaf(-g, log2e, -t)) * ln2, e);
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 

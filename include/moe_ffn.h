@@ -454,7 +454,8 @@ enum { MOE_GATE_NONE = 0, MOE_GATE_TOKEN = 1, MOE_GATE_CHANNEL = 2, MOE_GATE_ELE
 
 /* All pointers are device memory; strides are the elements between rows.
  *   b = post_weight ? rms(block) * (weight_offset + post_weight) : block
- *   b = b * gate, or b * sigmoid(gate) with gate_sigmoid
+ *   b = b * gate, or b * sigmoid(gate) with gate_sigmoid (below 2^-126, gates
+ *       under -87.3, it may count as 0)
  *   h = residual_scale * residual + block_scale * b   (no block: the first term)
  *   n = rms(h) * (weight_offset + pre_weight)
  * with rms(v) = v / sqrt(mean(v^2) + eps) over a row, in fp32 throughout.
