@@ -293,10 +293,12 @@ __global__ __launch_bounds__(512) void k_fp8_stream(Fp8LinearArgs a) {
 // rows, a power of two apart and with a scale load each, do not come fast enough
 // for more: 2048 x 2048 at 1,032 columns, fp32, in 32 x 48 tiles 34.5 us against
 // 20.9.
-template<int TM, int TN, int W, bool Tiles, int Y>
+// Y: type of y; Sums32: fp32 sums within a block (block_dot), as fp32 results always have.
+template<int TM, int TN, int W, bool Tiles, int Y, bool Sums32>
 __global__ __launch_bounds__(64 * W) void k_fp8_split(Fp8LinearArgs a, int tiles_m) {
     static_assert(kFp8Block % (16 * TM) == 0, "the rows share one scale block");
-    using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
+    static_assert(Sums32 || Y != kF32);
+    using Operand = std::conditional_t<Sums32, FragF16, Frag>;
     __shared__ f32x4 red[W][TM * TN][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int mt = static_cast<int>(blockIdx.x) % tiles_m * TM, nt = static_cast<int>(blockIdx.x) / tiles_m * TN;
@@ -550,12 +552,13 @@ struct GemmTile {
 
 // G groups of WR x WC waves share the tile, group g taking blocks g, g + G, ..
 // through a ring of its own; their sums meet in LDS at the end, in group order.
-// Y: type of y; fp32 results on fp16 operands, the others on e4m3 ones.
-template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, int Y>
+// Y, Sums32: as for k_fp8_split.
+template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, int Y, bool Sums32>
 __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, int tiles_m) {
     using Tile = GemmTile<WR, WC, TM, TN, S, G, Tiles>;
     constexpr int Sums = TM * TN * Tile::W * 64 * 16;   // bytes of one group's sums
     static_assert(G == 1 || Sums <= G * Tile::Lds);
+    static_assert(Sums32 || Y != kF32);
     __shared__ __attribute__((aligned(1024))) uint8_t lds[G][Tile::Lds];
     const int group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / Tile::W;
     const Tile g(a, blockIdx.x % tiles_m, blockIdx.x / tiles_m, lds[group]);
@@ -583,7 +586,7 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
         const uint8_t *buf = lds[group] + at * Tile::Buffer;
         at = at + 1 == S ? 0 : at + 1;
         const float sw = g.wscale[G == 1 ? b : min(b, a.nb - 1)];   // a group's block past the last: zeros
-        using Operand = std::conditional_t<Y == kF32, FragF16, Frag>;
+        using Operand = std::conditional_t<Sums32, FragF16, Frag>;
         Operand x[TN];
         float s[TN];
 #pragma unroll
@@ -721,6 +724,7 @@ struct moe_fp8_linear {
     uint8_t *mem = nullptr;       // tiles, scales
     const float *scales = nullptr;
     uint8_t *ws = nullptr;        // columns as tiles, then scales [nb][columns]
+    int sums = MOE_SUMS_AUTO;
 };
 
 namespace {
@@ -741,6 +745,8 @@ void release(moe_fp8_linear *L) {
     delete L;
 }
 
+bool sums32(const moe_fp8_linear *L, int y_type) { return y_type == MOE_F32 || L->sums == MOE_SUMS_F32; }
+
 moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int y_type, int64_t y_stride) {
     moe::Fp8LinearArgs a{};
     a.tiles = L->mem;
@@ -755,24 +761,37 @@ moe::Fp8LinearArgs base_args(const moe_fp8_linear *L, int columns, void *y, int 
     return a;
 }
 
-template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, bool F32>
+// Sums32: sums within a block in fp32, for y of any type; else y is of 16 bits.
+template<int WR, int WC, int TM, int TN, int S, int G, bool Tiles, bool Sums32>
 int launch_gemm(const moe::Fp8LinearArgs &a, hipStream_t s) {
     using Tile = moe::GemmTile<WR, WC, TM, TN, S, G, Tiles>;
     const int tm = (a.M + Tile::BM - 1) / Tile::BM, tn = (a.N + Tile::BN - 1) / Tile::BN;
     const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * Tile::W * G);
-    if constexpr (F32) moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
-    else if (a.y_type == MOE_BF16) moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
-    else moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
+    const auto launch = [&](auto kernel) { kernel<<<grid, block, 0, s>>>(a, tm); };
+    if constexpr (Sums32) {
+        if (a.y_type == MOE_F32) {
+            launch(moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF32, true>);
+            return hipGetLastError();
+        }
+    }
+    if (a.y_type == MOE_BF16) launch(moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kBF16, Sums32>);
+    else launch(moe::k_fp8_gemm<WR, WC, TM, TN, S, G, Tiles, moe::kF16, Sums32>);
     return hipGetLastError();
 }
 
-template<int TM, int TN, int W, bool Tiles, bool F32>
+template<int TM, int TN, int W, bool Tiles, bool Sums32>
 int launch_split(const moe::Fp8LinearArgs &a, hipStream_t s) {
     const int tm = (a.M + 16 * TM - 1) / (16 * TM), tn = (a.N + 16 * TN - 1) / (16 * TN);
     const dim3 grid(static_cast<unsigned>(tm) * tn), block(64 * W);
-    if constexpr (F32) moe::k_fp8_split<TM, TN, W, Tiles, moe::kF32><<<grid, block, 0, s>>>(a, tm);
-    else if (a.y_type == MOE_BF16) moe::k_fp8_split<TM, TN, W, Tiles, moe::kBF16><<<grid, block, 0, s>>>(a, tm);
-    else moe::k_fp8_split<TM, TN, W, Tiles, moe::kF16><<<grid, block, 0, s>>>(a, tm);
+    const auto launch = [&](auto kernel) { kernel<<<grid, block, 0, s>>>(a, tm); };
+    if constexpr (Sums32) {
+        if (a.y_type == MOE_F32) {
+            launch(moe::k_fp8_split<TM, TN, W, Tiles, moe::kF32, true>);
+            return hipGetLastError();
+        }
+    }
+    if (a.y_type == MOE_BF16) launch(moe::k_fp8_split<TM, TN, W, Tiles, moe::kBF16, Sums32>);
+    else launch(moe::k_fp8_split<TM, TN, W, Tiles, moe::kF16, Sums32>);
     return hipGetLastError();
 }
 
@@ -840,7 +859,7 @@ int launch_stream(const moe::Fp8LinearArgs &a, hipStream_t s) {
 // So the larger tiles take what fills the CUs, by how much of their last round of
 // 256 tiles is used, and the smaller ones the rest.
 template<bool Tiles>
-int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
+int launch_product(const moe::Fp8LinearArgs &a, bool sums32, hipStream_t s) {
     constexpr int IN = Tiles ? moe::kTiles : moe::kCodes;
     const auto tiles = [&](long m, long n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
     if (a.N <= 64 || static_cast<long>(a.M) * a.N <= 320 * 1024) {
@@ -850,7 +869,7 @@ int launch_product(const moe::Fp8LinearArgs &a, hipStream_t s) {
         return a.N <= 64 ? launch_stream<IN, 2, 1>(a, s) : launch_stream<IN, 2, 2>(a, s);
     }
     const long t64 = tiles(64, 64), t128 = tiles(128, 128), rounds128 = (t128 + 255) / 256;
-    if (a.y_type == MOE_F32) {
+    if (sums32) {
         if (tiles(64, 32) <= 256) return launch_split<4, 2, 8, Tiles, true>(a, s);
         // The two forms of a number of groups give the same sums, and so do apply and forward.
         const bool fills = t64 <= 512 && 10 * static_cast<long>(a.M) * a.N >= 9 * 4096 * 256 * ((t64 + 255) / 256);
@@ -944,6 +963,12 @@ int moe_fp8_linear_bytes(const moe_fp8_linear *L, size_t *weight_bytes) {
     return 0;
 }
 
+int moe_fp8_linear_set_sums(moe_fp8_linear *L, int sums) {
+    if (!L || (sums != MOE_SUMS_AUTO && sums != MOE_SUMS_F32)) return kInvalid;
+    L->sums = sums;
+    return 0;
+}
+
 int moe_fp8_linear_forward(moe_fp8_linear *L, const void *x_codes, const float *x_scales, int columns, void *y, int y_type,
                            int64_t y_stride, void *stream) {
     if (!L || !aligned(x_codes, 16) || !aligned(x_scales, 4) || columns < 1 || columns > 65536 ||
@@ -956,7 +981,7 @@ int moe_fp8_linear_forward(moe_fp8_linear *L, const void *x_codes, const float *
     a.xscale = x_scales;
     a.scale_n = L->nb;
     a.scale_b = 1;
-    return launch_product<false>(a, static_cast<hipStream_t>(stream));
+    return launch_product<false>(a, sums32(L, y_type), static_cast<hipStream_t>(stream));
 }
 
 int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x_stride, int columns, void *y, int y_type,
@@ -995,7 +1020,7 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
     a.xscale = scales;
     a.scale_n = 1;
     a.scale_b = columns;
-    return launch_product<true>(a, s);
+    return launch_product<true>(a, sums32(L, y_type), s);
 }
 
 }  // extern "C"

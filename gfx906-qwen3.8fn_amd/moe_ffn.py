@@ -29,6 +29,7 @@ PATH_AUTO, PATH_STREAM, PATH_MFMA = 0, 1, 2
 TYPE_Q4_0, TYPE_Q4_1 = 2, 3     # MOE_TYPE_Q4_0 / MOE_TYPE_Q4_1 (the reference's TensorType ids)
 F32, BF16, F16 = 0, 1, 2        # MOE_F32 / MOE_BF16 / MOE_F16
 GATE_NONE, GATE_TOKEN, GATE_CHANNEL, GATE_ELEMENT = 0, 1, 2, 3   # MOE_GATE_*
+SUMS_AUTO, SUMS_F32 = 0, 1      # MOE_SUMS_*
 E4M3_GROUP = 128                # elements per scale of an e4m3 row
 STAGE_PREPARE, STAGE_GATE_UP, STAGE_DOWN, STAGE_FOLD = 0, 1, 2, 3
 
@@ -126,6 +127,7 @@ def library():
         lib.moe_fp8_linear_create.argtypes = [_I, _I, _I, _P, _P, _I, _I, ctypes.POINTER(_P)]
         lib.moe_fp8_linear_destroy.argtypes = [_P]
         lib.moe_fp8_linear_bytes.argtypes = [_P, ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_fp8_linear_set_sums.argtypes = [_P, _I]
         lib.moe_fp8_linear_forward.argtypes = [_P, _P, _P, _I, _P, _I, _L, _P]
         lib.moe_fp8_linear_apply.argtypes = [_P, _P, _I, _L, _I, _P, _I, _L, _P, _P]
         lib.moe_fp8_layer_memory_bytes.argtypes = [ctypes.POINTER(Fp8LayerConfig), ctypes.POINTER(ctypes.c_size_t),
@@ -669,15 +671,18 @@ class MoeFp8Linear:
     128 (moe_fp8_linear_create): codes float8_e4m3fn (or uint8) and scales
     float32 [ceil(output/128)][ceil(input/128)], both torch tensors on a GPU
     or both numpy arrays.  forward takes e4m3 rows, apply rows of float32,
-    bfloat16 or float16."""
+    bfloat16 or float16.  sums: SUMS_F32 for fp32 sums within every block, also
+    of wide batches with 16-bit results, which otherwise (SUMS_AUTO) come from
+    the faster e4m3 instruction (moe_fp8_linear_forward says what it drops)."""
 
-    def __init__(self, input, output, codes, scales, max_columns=0, device=0):
+    def __init__(self, input, output, codes, scales, max_columns=0, device=0, sums=SUMS_AUTO):
         self.K, self.M, self.max_columns, self.device = input, output, max_columns, device
         c, s, on_device, _keep = _e4m3_matrices(codes, scales, (output, input), "weights", device)
         handle = ctypes.c_void_p()
         _check(library().moe_fp8_linear_create(input, output, max_columns, c, s, on_device, device,
                                                ctypes.byref(handle)), "moe_fp8_linear_create")
         self.handle = handle
+        self.set_sums(sums)
 
     def close(self):
         if getattr(self, "handle", None):
@@ -689,6 +694,10 @@ class MoeFp8Linear:
             self.close()
         except Exception:
             pass
+
+    def set_sums(self, sums):
+        """SUMS_AUTO or SUMS_F32 for the calls made from here on."""
+        _check(library().moe_fp8_linear_set_sums(self.handle, sums), "moe_fp8_linear_set_sums")
 
     def weight_bytes(self):
         n = ctypes.c_size_t()

@@ -375,14 +375,27 @@ int moe_fp8_linear_destroy(moe_fp8_linear *linear);
 /* Bytes of the codes and scales the handle was created from. */
 int moe_fp8_linear_bytes(const moe_fp8_linear *linear, size_t *weight_bytes);
 
+/* Sums within a block, see forward. */
+enum { MOE_SUMS_AUTO = 0, MOE_SUMS_F32 = 1 };
+
+/* MOE_SUMS_F32: fp32 sums whatever y's type and the number of columns, at about
+ * twice the time for wide batches with 16-bit results.  MOE_SUMS_AUTO, as
+ * created: as forward says.  Host state of the handle, read by the calls made
+ * after it; a captured call keeps the sums it was recorded with.  Not to be set
+ * while another thread makes a call on the handle. */
+int moe_fp8_linear_set_sums(moe_fp8_linear *linear, int sums);
+
 /* y[n][m] = sum over the matrix row of x * W, for e4m3 rows x_codes
  * [columns][input] (16-byte aligned) with x_scales; y rows are y_stride
  * elements of y_type apart.  Each block's sum is multiplied by both scales
  * into an fp32 sum over the blocks, rounded once to y_type.  The sum within a
- * block is fp32 when y_type is MOE_F32 or columns <= 64; larger products with
- * 16-bit results use the e4m3 matrix instructions, which drop what is more
- * than about 14 bits below a block's largest product.  columns 1..65536.  No
- * workspace: calls on one handle may overlap.  What lies between y's rows is
+ * block is fp32 when y_type is MOE_F32, columns <= 64 or output * columns <=
+ * 327,680, and for every call after moe_fp8_linear_set_sums(MOE_SUMS_F32).
+ * Larger products with 16-bit results otherwise use the e4m3 matrix
+ * instruction, which cuts, toward zero, the products of eight neighbouring
+ * columns of the matrix (8 i .. 8 i + 7) at 2^-13 of their largest (2^-10 where
+ * that one has a subnormal code); all other sums are fp32.  columns 1..65536.
+ * No workspace: calls on one handle may overlap.  What lies between y's rows is
  * left as it is.  y may not overlap the rows or their scales.  NaN codes give
  * NaN results.  Enqueue only; the handle's device need not be current. */
 int moe_fp8_linear_forward(moe_fp8_linear *linear, const void *x_codes, const float *x_scales, int columns, void *y,
