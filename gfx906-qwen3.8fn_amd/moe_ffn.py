@@ -191,6 +191,15 @@ def _stream(stream):
     return ctypes.c_void_p(s.cuda_stream)
 
 
+def _making(stream):
+    """Context in which a call makes the tensors it was not given: on the stream
+    that it launches on, so that an error word's zeros come before the kernels'
+    flags and no other stream's pending work still uses the memory."""
+    import contextlib
+    import torch
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+
+
 def _on_device(device):
     """Context in which `device` is current, for the calls without a handle."""
     import torch
@@ -309,18 +318,19 @@ class MoeLayer:
         return dict(stream_items=a.value, mfma_items=b.value, active_experts=c.value)
 
     # ------------------------------------------------------------ forward --
-    def _io_check(self, n, dev, ids, weights, shared_gate, y, error):
+    def _io_check(self, n, dev, ids, weights, shared_gate, y, error, stream=None):
         import torch
         if not 1 <= n <= self.max_tokens:
             raise ValueError(f"tokens {n} outside 1..{self.max_tokens}")
         _routes_check(ids, weights, n, self.k, dev)
         if shared_gate is not None:
             _need(shared_gate, "shared_gate", torch.float32, (n,), dev)
-        if y is None:
-            y = torch.empty((n, self.H), dtype=torch.float32, device=dev)
+        with _making(stream):
+            if y is None:
+                y = torch.empty((n, self.H), dtype=torch.float32, device=dev)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=dev)
         _need(y, "y", torch.float32, (n, self.H), dev)
-        if error is None:
-            error = torch.zeros(1, dtype=torch.int32, device=dev)
         _need(error, "error", torch.int32, (1,), dev)
         return y, error
 
@@ -328,7 +338,7 @@ class MoeLayer:
         import torch
         n = x.shape[0]
         _need(x, "x", torch.float32, (n, self.H), x.device)
-        y, error = self._io_check(n, x.device, ids, weights, shared_gate, y, error)
+        y, error = self._io_check(n, x.device, ids, weights, shared_gate, y, error, stream)
         _check(library().moe_ffn_forward(self.handle, _ptr(x), _ptr(ids), _ptr(weights), n, _ptr(shared_gate),
                                          _ptr(y), _ptr(error), _stream(stream)), "moe_ffn_forward")
         return y, error
@@ -357,7 +367,7 @@ class MoeLayer:
         import torch
         n = ids.shape[0]
         _need(x_q8, "x_q8", torch.uint8, (n, self.H // 32 * Q8_BLOCK), ids.device)
-        y, error = self._io_check(n, ids.device, ids, weights, shared_gate, y, error)
+        y, error = self._io_check(n, ids.device, ids, weights, shared_gate, y, error, stream)
         _check(library().moe_ffn_forward_q8(self.handle, _ptr(x_q8), _ptr(ids), _ptr(weights), n, _ptr(shared_gate),
                                             _ptr(y), _ptr(error), _stream(stream)), "moe_ffn_forward_q8")
         return y, error
@@ -380,10 +390,11 @@ class MoeLayer:
         import torch
         P = tokens * self.k + (tokens if self.has_shared else 0)
         dev = f"cuda:{self.device}"
-        xq = torch.empty((tokens, self.H // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
-        mq = torch.empty((P, self.I // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
-        rt = torch.empty(tokens * self.k, dtype=torch.int32, device=dev)
-        rr = torch.empty(tokens * self.k, dtype=torch.int32, device=dev)
+        with _making(stream):
+            xq = torch.empty((tokens, self.H // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+            mq = torch.empty((P, self.I // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+            rt = torch.empty(tokens * self.k, dtype=torch.int32, device=dev)
+            rr = torch.empty(tokens * self.k, dtype=torch.int32, device=dev)
         _check(library().moe_ffn_debug_last(self.handle, _ptr(xq), _ptr(mq), _ptr(rt), _ptr(rr), _stream(stream)),
                "moe_ffn_debug_last")
         return dict(x_q8=xq, middle_q8=mq, route_token=rt, route_rank=rr)
@@ -395,11 +406,12 @@ class MoeLayer:
         if not 1 <= n <= self.max_tokens:
             raise ValueError(f"tokens {n} outside 1..{self.max_tokens}")
         _routes_check(ids, weights, n, self.k, dev)
-        counts = torch.empty(self.E, dtype=torch.int32, device=dev)
-        offsets = torch.empty(self.E + 1, dtype=torch.int32, device=dev)
-        rt = torch.empty(n * self.k, dtype=torch.int32, device=dev)
-        rr = torch.empty(n * self.k, dtype=torch.int32, device=dev)
-        error = torch.zeros(1, dtype=torch.int32, device=dev)
+        with _making(stream):
+            counts = torch.empty(self.E, dtype=torch.int32, device=dev)
+            offsets = torch.empty(self.E + 1, dtype=torch.int32, device=dev)
+            rt = torch.empty(n * self.k, dtype=torch.int32, device=dev)
+            rr = torch.empty(n * self.k, dtype=torch.int32, device=dev)
+            error = torch.zeros(1, dtype=torch.int32, device=dev)
         _check(library().moe_ffn_group_routes(self.handle, _ptr(ids), _ptr(weights), n, _ptr(counts), _ptr(offsets),
                                               _ptr(rt), _ptr(rr), _ptr(error), _stream(stream)),
                "moe_ffn_group_routes")
@@ -408,13 +420,14 @@ class MoeLayer:
     def expert_gate_up(self, expert, x_q8, columns, path=PATH_AUTO, dots=False, stream=None):
         import torch
         dev = x_q8.device
-        middle = torch.empty((columns, self.I), dtype=torch.float32, device=dev)
-        mq = torch.empty((columns, self.I // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
         gd = ud = None
-        if dots:
-            gd = torch.full((columns, self.I, self.H // 32), -2**31, dtype=torch.int32, device=dev)
-            ud = torch.full((columns, self.I, self.H // 32), -2**31, dtype=torch.int32, device=dev)
-        error = torch.zeros(1, dtype=torch.int32, device=dev)
+        with _making(stream):
+            middle = torch.empty((columns, self.I), dtype=torch.float32, device=dev)
+            mq = torch.empty((columns, self.I // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+            if dots:
+                gd = torch.full((columns, self.I, self.H // 32), -2**31, dtype=torch.int32, device=dev)
+                ud = torch.full((columns, self.I, self.H // 32), -2**31, dtype=torch.int32, device=dev)
+            error = torch.zeros(1, dtype=torch.int32, device=dev)
         _check(library().moe_ffn_expert_gate_up(self.handle, expert, _ptr(x_q8), columns, _ptr(middle), _ptr(mq),
                                                 _ptr(gd), _ptr(ud), path, _ptr(error), _stream(stream)),
                "moe_ffn_expert_gate_up")
@@ -423,11 +436,12 @@ class MoeLayer:
     def expert_down(self, expert, middle_q8, columns, path=PATH_AUTO, dots=False, stream=None):
         import torch
         dev = middle_q8.device
-        y = torch.empty((columns, self.H), dtype=torch.float32, device=dev)
         dd = None
-        if dots:
-            dd = torch.full((columns, self.H, self.I // 32), -2**31, dtype=torch.int32, device=dev)
-        error = torch.zeros(1, dtype=torch.int32, device=dev)
+        with _making(stream):
+            y = torch.empty((columns, self.H), dtype=torch.float32, device=dev)
+            if dots:
+                dd = torch.full((columns, self.H, self.I // 32), -2**31, dtype=torch.int32, device=dev)
+            error = torch.zeros(1, dtype=torch.int32, device=dev)
         _check(library().moe_ffn_expert_down(self.handle, expert, _ptr(middle_q8), columns, _ptr(y), _ptr(dd), path,
                                              _ptr(error), _stream(stream)), "moe_ffn_expert_down")
         return dict(y=y, down_dots=dd, error=error)
@@ -465,7 +479,8 @@ def expf_host(x):
 def expf_device(x, stream=None):
     """The kernels' expf on the GPU: float32 device tensor in, out."""
     import torch
-    y = torch.empty_like(x)
+    with _making(stream):
+        y = torch.empty_like(x)
     _check(library().moe_expf_device(_ptr(x), _ptr(y), x.numel(), _stream(stream)), "moe_expf_device")
     return y
 
@@ -478,13 +493,14 @@ def router_select(logits, top_k=10, probabilities=False, error=None, stream=None
     n, e = logits.shape
     dev = logits.device
     _need(logits, "logits", torch.float32, (n, e), dev)
-    if ids is None:
-        ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
-    w = weights if weights is not None else torch.empty((n, top_k), dtype=torch.float32, device=dev)
+    with _making(stream):
+        if ids is None:
+            ids = torch.empty((n, top_k), dtype=torch.int32, device=dev)
+        w = weights if weights is not None else torch.empty((n, top_k), dtype=torch.float32, device=dev)
+        p = torch.empty((n, e), dtype=torch.float32, device=dev) if probabilities else None
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=dev)
     _routes_check(ids, w, n, top_k, dev)
-    p = torch.empty((n, e), dtype=torch.float32, device=dev) if probabilities else None
-    if error is None:
-        error = torch.zeros(1, dtype=torch.int32, device=dev)
     _need(error, "error", torch.int32, (1,), dev)
     _check(library().moe_router_select(_ptr(logits), n, e, top_k, _ptr(p), _ptr(ids), _ptr(w), _ptr(error),
                                        _stream(stream)), "moe_router_select")
@@ -502,9 +518,10 @@ def quantize_q8_1(x, error=None, stream=None):
     import torch
     cols, width = x.shape
     _need(x, "x", torch.float32, (cols, width), x.device)
-    out = torch.empty((cols, width // 32 * Q8_BLOCK), dtype=torch.uint8, device=x.device)
-    if error is None:
-        error = torch.zeros(1, dtype=torch.int32, device=x.device)
+    with _making(stream):
+        out = torch.empty((cols, width // 32 * Q8_BLOCK), dtype=torch.uint8, device=x.device)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=x.device)
     _need(error, "error", torch.int32, (1,), x.device)
     _check(library().moe_quantize_q8_1(_ptr(x), _ptr(out), width, cols, _ptr(error), _stream(stream)),
            "moe_quantize_q8_1")
@@ -521,8 +538,9 @@ def combine(contributions, weights, shared=None, shared_gate=None, stream=None):
         _need(shared, "shared", torch.float32, (n, h), dev)
     if shared_gate is not None:
         _need(shared_gate, "shared_gate", torch.float32, (n,), dev)
-    y = torch.empty((n, h), dtype=torch.float32, device=contributions.device)
-    error = torch.zeros(1, dtype=torch.int32, device=contributions.device)
+    with _making(stream):
+        y = torch.empty((n, h), dtype=torch.float32, device=contributions.device)
+        error = torch.zeros(1, dtype=torch.int32, device=contributions.device)
     _check(library().moe_combine(_ptr(contributions), _ptr(weights), _ptr(shared), _ptr(shared_gate), n, k, h,
                                  _ptr(y), _ptr(error), _stream(stream)), "moe_combine")
     return y, error
@@ -576,7 +594,8 @@ class MoeLinear:
         if x_q8.dtype != torch.uint8 or not x_q8.is_contiguous() or x_q8.numel() < columns * (self.K // 32) * Q8_BLOCK:
             raise ValueError("x_q8 must be contiguous uint8 holding columns x input/32 Q8_1 blocks")
         if y is None:
-            y = torch.empty((columns, self.M), dtype=torch.float32, device=x_q8.device)
+            with _making(stream):
+                y = torch.empty((columns, self.M), dtype=torch.float32, device=x_q8.device)
         _need(y, "y", torch.float32, (columns, self.M), x_q8.device)
         _check(library().moe_linear_forward_q8(self.handle, _ptr(x_q8), columns, _ptr(y), _stream(stream)),
                "moe_linear_forward_q8")
@@ -586,11 +605,12 @@ class MoeLinear:
         import torch
         n = x.shape[0]
         _need(x, "x", torch.float32, (n, self.K), x.device)
-        if y is None:
-            y = torch.empty((n, self.M), dtype=torch.float32, device=x.device)
+        with _making(stream):
+            if y is None:
+                y = torch.empty((n, self.M), dtype=torch.float32, device=x.device)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x.device)
         _need(y, "y", torch.float32, (n, self.M), x.device)
-        if error is None:
-            error = torch.zeros(1, dtype=torch.int32, device=x.device)
         _need(error, "error", torch.int32, (1,), x.device)
         _check(library().moe_linear_apply(self.handle, _ptr(x), n, _ptr(y), _ptr(error), _stream(stream)),
                "moe_linear_apply")
@@ -651,14 +671,15 @@ def quantize_e4m3(x, codes=None, scales=None, error=None, stream=None):
         raise ValueError("x must be a two-dimensional torch tensor")
     n, width = x.shape
     type_, stride = _need_rows(x, "x", (n, width))
-    if codes is None:
-        codes = torch.empty((n, width), dtype=torch.float8_e4m3fn, device=x.device)
-    if scales is None:
-        scales = torch.empty((n, _blocks(width)), dtype=torch.float32, device=x.device)
+    with _making(stream):
+        if codes is None:
+            codes = torch.empty((n, width), dtype=torch.float8_e4m3fn, device=x.device)
+        if scales is None:
+            scales = torch.empty((n, _blocks(width)), dtype=torch.float32, device=x.device)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=x.device)
     _e4m3(codes, "codes", (n, width), x.device)
     _need(scales, "scales", torch.float32, (n, _blocks(width)), x.device)
-    if error is None:
-        error = torch.zeros(1, dtype=torch.int32, device=x.device)
     _need(error, "error", torch.int32, (1,), x.device)
     with _on_device(x.device):
         _check(library().moe_quantize_e4m3(_ptr(x), type_, stride, width, n, _ptr(codes), _ptr(scales), _ptr(error),
@@ -729,7 +750,8 @@ class MoeFp8Linear:
         said) from e4m3 rows."""
         import torch
         if y is None:
-            y = torch.empty((x_codes.shape[0], self.M), dtype=dtype or torch.float32, device=x_codes.device)
+            with _making(stream):
+                y = torch.empty((x_codes.shape[0], self.M), dtype=dtype or torch.float32, device=x_codes.device)
         self.bind_forward(x_codes, x_scales, y, stream)()
         return y
 
@@ -753,10 +775,11 @@ class MoeFp8Linear:
     def apply(self, x, y=None, error=None, dtype=None, stream=None):
         """(y, error) from rows x [n][input]; y in x's type unless given."""
         import torch
-        if y is None:
-            y = torch.empty((x.shape[0], self.M), dtype=dtype or x.dtype, device=x.device)
-        if error is None:
-            error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        with _making(stream):
+            if y is None:
+                y = torch.empty((x.shape[0], self.M), dtype=dtype or x.dtype, device=x.device)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x.device)
         self.bind_apply(x, y, error, stream)()
         return y, error
 
@@ -831,10 +854,11 @@ class MoeFp8Layer:
         """(y, error) for x [n][H] of float32, bfloat16 or float16; y has x's
         type."""
         import torch
-        if y is None:
-            y = torch.empty_like(x)
-        if error is None:
-            error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        with _making(stream):
+            if y is None:
+                y = torch.empty_like(x)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x.device)
         self.bind_forward(x, ids, weights, y, error, shared_gate, stream)()
         return y, error
 
@@ -962,18 +986,19 @@ class BlockNorm:
         if unknown:
             raise ValueError(f"unknown outputs {sorted(unknown)}")
         n, h, dev = residual.shape[0], self.hidden, residual.device
-        if error is None:
-            error = torch.zeros(1, dtype=torch.int32, device=dev)
         made = {}
-        if "residual" in outputs:
-            made["residual_out"] = torch.empty((n, h), dtype=residual.dtype, device=dev)
-        if "out" in outputs and self.pre_weight is not None:
-            made["out"] = torch.empty((n, h), dtype=(block if block is not None else residual).dtype, device=dev)
-        if "q8" in outputs:
-            made["q8"] = torch.empty((n, h // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
-        if "e4m3" in outputs:
-            made["codes"] = torch.empty((n, h), dtype=torch.float8_e4m3fn, device=dev)
-            made["scales"] = torch.empty((n, _blocks(h)), dtype=torch.float32, device=dev)
+        with _making(stream):
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=dev)
+            if "residual" in outputs:
+                made["residual_out"] = torch.empty((n, h), dtype=residual.dtype, device=dev)
+            if "out" in outputs and self.pre_weight is not None:
+                made["out"] = torch.empty((n, h), dtype=(block if block is not None else residual).dtype, device=dev)
+            if "q8" in outputs:
+                made["q8"] = torch.empty((n, h // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
+            if "e4m3" in outputs:
+                made["codes"] = torch.empty((n, h), dtype=torch.float8_e4m3fn, device=dev)
+                made["scales"] = torch.empty((n, _blocks(h)), dtype=torch.float32, device=dev)
         self.bind(residual, block=block, gate=gate, error=error, stream=stream, **made)()
         if "residual_out" in made:
             made["residual"] = made.pop("residual_out")
