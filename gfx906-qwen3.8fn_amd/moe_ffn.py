@@ -1018,6 +1018,7 @@ class MoeStack:
     per layer) the layer input is h = projection.apply(x); with `routers` (H ->
     E per layer) the routes are chosen on the device from router.apply(h) by
     router_select; otherwise fixed device ids / weights are given to bind().
+    Fewer batches than layers run the first layers.
 
     With `norms` (len(layers) + 1 BlockNorms) the layers run on one residual
     stream, xs = [x]: norms[0] makes the first layer's input from x, norms[l]
@@ -1050,8 +1051,8 @@ class MoeStack:
         self.steps = []
         if self.norms is not None and len(xs) != 1:
             raise ValueError("a stack with norms takes one input batch")
-        for l, L in enumerate(self.layers):
-            x = xs[0] if self.norms is not None else xs[l]
+        batches = xs if self.norms is None else list(xs) * len(self.layers)
+        for l, (L, x) in enumerate(zip(self.layers, batches)):
             n, kind = x.shape[0], x.dtype if dtype is None or self.norms is None else dtype
             st = {"y": torch.empty((n, L.H), dtype=kind, device=dev)}
             if self.norms is not None:
