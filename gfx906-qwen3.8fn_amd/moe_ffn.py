@@ -1038,22 +1038,37 @@ class MoeStack:
         if norms is not None:
             if len(norms) != len(self.layers) + 1:
                 raise ValueError("norms: one before the first layer and one after each")
+            if not self.layers:
+                raise ValueError("a stack with norms needs a layer")
             if any(n.pre_weight is None for n in norms[:-1]):
                 raise ValueError("norms before a layer need a pre_weight")
+            if any(n.hidden != L.H for n in norms for L in self.layers):
+                raise ValueError("norms and layers need one hidden size")
         self.graph = None
 
     def bind(self, xs, ids=None, weights=None, dtype=None):
-        """Allocate every buffer for the input batches xs.  dtype (with norms):
-        type of the layers' inputs and outputs, that of x unless said."""
+        """Allocate every buffer for the input batches xs, on the current stream
+        (a run on another one has to wait for it).  dtype (with norms): type of
+        the layers' inputs and outputs, that of x unless said; x, the residual
+        stream, is of that type or float32.  The Q4 handles take float32 rows
+        alone."""
         import torch
+        if self.norms is not None:
+            if len(xs) != 1:
+                raise ValueError("a stack with norms takes one input batch")
+            if dtype is not None and xs[0].dtype not in (torch.float32, dtype):
+                raise TypeError(f"the residual stream must be float32 or {dtype}, got {xs[0].dtype}")
+        batches = xs if self.norms is None else list(xs) * len(self.layers)
+        kinds = [x.dtype if dtype is None or self.norms is None else dtype for _, x in zip(self.layers, batches)]
+        for l, kind in enumerate(kinds):
+            step = [self.layers[l]] + [handles[l] for handles in (self.projections, self.routers) if handles]
+            if kind != torch.float32 and any(isinstance(m, (MoeLayer, MoeLinear)) for m in step):
+                raise TypeError(f"layer {l}: Q4 layers, projections and routers take float32 rows, got {kind}")
         dev = xs[0].device
         self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         self.steps = []
-        if self.norms is not None and len(xs) != 1:
-            raise ValueError("a stack with norms takes one input batch")
-        batches = xs if self.norms is None else list(xs) * len(self.layers)
-        for l, (L, x) in enumerate(zip(self.layers, batches)):
-            n, kind = x.shape[0], x.dtype if dtype is None or self.norms is None else dtype
+        for l, (L, x, kind) in enumerate(zip(self.layers, batches, kinds)):
+            n = x.shape[0]
             st = {"y": torch.empty((n, L.H), dtype=kind, device=dev)}
             if self.norms is not None:
                 st["x"] = torch.empty((n, L.H), dtype=kind, device=dev)
