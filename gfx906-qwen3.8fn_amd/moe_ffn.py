@@ -1070,18 +1070,18 @@ class MoeStack:
         for l, (L, x, kind) in enumerate(zip(self.layers, batches, kinds)):
             n = x.shape[0]
             st = {"y": torch.empty((n, L.H), dtype=kind, device=dev)}
-            if self.norms is not None:
+            if self.norms is None:
+                st["x"] = x
+            elif self.projections and isinstance(self.projections[l], MoeFp8Linear):
+                st["codes"] = torch.empty((n, L.H), dtype=torch.float8_e4m3fn, device=dev)
+                st["scales"] = torch.empty((n, _blocks(L.H)), dtype=torch.float32, device=dev)
+                st["norm"] = {"codes": st["codes"], "scales": st["scales"]}
+            else:
                 st["x"] = torch.empty((n, L.H), dtype=kind, device=dev)
                 st["norm"] = {"out": st["x"]}
-                if self.projections and isinstance(self.projections[l], MoeFp8Linear):
-                    st["codes"] = torch.empty((n, L.H), dtype=torch.float8_e4m3fn, device=dev)
-                    st["scales"] = torch.empty((n, _blocks(L.H)), dtype=torch.float32, device=dev)
-                    st["norm"] = {"codes": st["codes"], "scales": st["scales"]}
-                elif not self.projections and isinstance(L, MoeLayer):
+                if not self.projections and isinstance(L, MoeLayer):
                     st["q8"] = torch.empty((n, L.H // 32 * Q8_BLOCK), dtype=torch.uint8, device=dev)
                     st["norm"]["q8"] = st["q8"]
-            else:
-                st["x"] = x
             st["h"] = torch.empty((n, L.H), dtype=kind, device=dev) if self.projections else st["x"]
             if self.routers:
                 st["logits"] = torch.empty((n, L.E), dtype=torch.float32, device=dev)

@@ -77,6 +77,19 @@ def test_dtype_and_stream():
         moe_ffn.MoeStack(q4(), norms=[norm() for _ in range(3)]).bind([torch.zeros((3, H))], [ids] * 2, [w] * 2, dtype=BF16)
 
 
+def test_rows_of_norms():
+    """Only the rows that a layer reads are made: e4m3 rows alone for an e4m3
+    projection."""
+    ids, w = routes(3)
+    norms = [norm() for _ in range(3)]
+    S = moe_ffn.MoeStack(fp8(), [shell(moe_ffn.MoeFp8Linear) for _ in range(2)], norms=norms)
+    S.bind([torch.zeros((3, H))], [ids] * 2, [w] * 2)
+    assert all("x" not in st and set(st["norm"]) == {"codes", "scales"} for st in S.steps)
+    S = moe_ffn.MoeStack(q4(), norms=norms)
+    S.bind([torch.zeros((3, H))], [ids] * 2, [w] * 2)
+    assert all(set(st["norm"]) == {"out", "q8"} for st in S.steps)
+
+
 def test_norms_that_do_not_fit():
     with pytest.raises(ValueError):
         moe_ffn.MoeStack([], norms=[norm()])
