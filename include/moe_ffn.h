@@ -448,9 +448,12 @@ int moe_fp8_layer_destroy(moe_fp8_layer *layer);
  * shared_gate and the sum as in moe_ffn_forward.  x's rows and the experts'
  * middle rows SiLU(gate) * up are quantised as moe_quantize_e4m3 does; sums
  * are fp32, y is rounded once.  Flags in `error` as in moe_ffn_forward:
- * routes with a bad id or an id of an earlier rank are dropped and set bit 1,
- * as do a negative or nonfinite weight (which stays in the sum, a nonfinite
- * one as 0) and nonfinite input, whose group of 128 counts as zeros.  x is
+ * routes with a bad id or an id of an earlier rank are dropped and set bit 1.
+ * So do nonfinite input, whose group of 128 counts as zeros, a negative weight,
+ * which stays in the sum, and a nonfinite weight, which gives up the token's
+ * routed sum: what is left is the shared expert.  An expert's output or a
+ * partial sum that is not finite gives up its own element of the routed sum,
+ * a nonfinite shared output or shared_gate its element of y (0).  x is
  * aligned to 16 bytes and may not overlap y.  tokens in 1..max_tokens.
  * Enqueue only; calls on one layer must not overlap (they share the
  * workspace).  The layer's device need not be current. */
