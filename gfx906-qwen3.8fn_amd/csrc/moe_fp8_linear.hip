@@ -585,7 +585,8 @@ __global__ __launch_bounds__(64 * WR * WC * G) void k_fp8_gemm(Fp8LinearArgs a, 
         g.stage_columns(b + (S - 1) * G, next);
         const uint8_t *buf = lds[group] + at * Tile::Buffer;
         at = at + 1 == S ? 0 : at + 1;
-        const float sw = g.wscale[G == 1 ? b : min(b, a.nb - 1)];   // a group's block past the last: zeros
+        if (G > 1 && b >= a.nb) break;   // the group's share has ended: only the others' barriers were left
+        const float sw = g.wscale[b];
         using Operand = std::conditional_t<Sums32, FragF16, Frag>;
         Operand x[TN];
         float s[TN];

@@ -53,3 +53,25 @@ def test_weights_and_gates_out_of_range(gated):
     assert flag(e) == 1
     check(y, x, ids, v, bank, gate)
     layer.close()
+
+
+# Seven blocks a row: two groups of waves share them unevenly, and the last
+# group's step past the end meets an earlier block's scale (16-bit results of
+# 64 x 64 tiles, whose form with half as many waves takes 1,300 x 1,500); four
+# groups and two for fp32 results; a single group and canonical rows for more.
+@pytest.mark.parametrize("M,N", [(1000, 900), (1300, 1500), (2000, 1700), (2047, 1500)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("K", [640, 672, 896])
+def test_scales_of_other_blocks_do_not_meet(K, M, N, dtype):
+    g = R.generator(43)
+    nb = R.blocks(K)
+    codes, scales = R.random_matrix(M, K, g)
+    qc, qs = R.quantise(torch.randn((N, K), generator=g, device=DEV))
+    want = moe_ffn.MoeFp8Linear(K, M, codes, scales).forward(qc, qs, dtype=dtype)
+    for b in range(nb - 1):   # block b's rows are scaled up and its matrix down, the last block's the other way round
+        up, down = torch.ones(nb, device=DEV), torch.ones(nb, device=DEV)
+        up[b], down[b] = 2.0 ** 110, 2.0 ** -110
+        up[nb - 1], down[nb - 1] = 2.0 ** -60, 2.0 ** 60
+        lin = moe_ffn.MoeFp8Linear(K, M, codes, scales * down)
+        assert same(lin.forward(qc, (qs * up).contiguous(), dtype=dtype), want), b
+        lin.close()
