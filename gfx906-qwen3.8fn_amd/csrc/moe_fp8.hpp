@@ -33,27 +33,6 @@ hipError_t launch_fp8_repack(const uint8_t *codes, uint8_t *tiles, size_t rows, 
 hipError_t launch_quantize_e4m3(const void *x, int type, int64_t stride, int width, int columns, uint8_t *codes,
                                 float *scales, int *error, hipStream_t s);
 
-// Makes the device of a handle current for a launch, and the caller's again
-// afterwards; no HIP call beyond the query where it is current already.
-class LaunchDevice {
-public:
-    explicit LaunchDevice(int device) {
-        if (hipGetDevice(&prev_) != hipSuccess) { prev_ = -1; return; }
-        if (prev_ == device) { prev_ = -1; ok_ = true; return; }
-        ok_ = hipSetDevice(device) == hipSuccess;
-    }
-    ~LaunchDevice() {
-        if (prev_ >= 0) (void)hipSetDevice(prev_);
-    }
-    LaunchDevice(const LaunchDevice &) = delete;
-    LaunchDevice &operator=(const LaunchDevice &) = delete;
-    bool ok() const { return ok_; }
-
-private:
-    int prev_ = -1;
-    bool ok_ = false;
-};
-
 namespace {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));

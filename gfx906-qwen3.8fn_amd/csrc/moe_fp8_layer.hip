@@ -39,6 +39,7 @@ struct Fp8LayerArgs {
 };
 
 inline constexpr int kTileWaves = 4, kRowTiles = 8 / kTileWaves;   // waves of a row tile, row tiles of a gate_up item
+static_assert(32 % (16 * kRowTiles) == 0, "the intermediate size is a multiple of 32");
 inline constexpr int kGateUpGroups = 512;   // workgroups of gate_up: two a CU
 inline constexpr int kChunk = 24;   // blocks of K whose columns a workgroup holds in LDS: 50 KB
 
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     constexpr int KW = kTileWaves, RW = kRowTiles;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int kw = wave % KW, rw = wave / KW;
-    const int row_tiles = a.I / 16, S = (row_tiles + RW - 1) / RW;
+    const int row_tiles = a.I / 16, S = row_tiles / RW;   // I is a multiple of 32
     for (int t = blockIdx.x; t < a.T; t += gridDim.x) {
         // A token's input flags, whatever becomes of its routes.
         bool bad = false;
@@ -198,21 +199,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     }
     const Routes routes(a);
     const int items = list_experts(a, routes, reinterpret_cast<int *>(lds), list) * S;
-    constexpr int U = 1;   // blocks a round; the next round's loads are on their way during one
-    Frag gf[2][U], uf[2][U];
+    Frag gf[2], uf[2];   // a block's, and the next one's on their way
     const uint8_t *gw = a.gate, *uw = a.up;
-    // Blocks k0 + b0, + KW, .. of an item's tile; past the chunk its last block again, not used.
-    auto load = [&](int k0, int kb, int b0, Frag (&g)[U], Frag (&v)[U]) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t b = k0 + min(b0 + u * KW, kb - 1);
-            g[u] = load_tile(gw + b * kFp8TileBytes, lane);
-            v[u] = load_tile(uw + b * kFp8TileBytes, lane);
-        }
+    // Block k0 + b of an item's tile; past the chunk its last block again, not used.
+    auto load = [&](int k0, int kb, int b, Frag &g, Frag &v) {
+        const size_t at = static_cast<size_t>(k0 + min(b, kb - 1)) * kFp8TileBytes;
+        g = load_tile(gw + at, lane);
+        v = load_tile(uw + at, lane);
     };
-    // The last slice may have fewer tiles: its other waves take the last one again.
     auto select = [&](int item) {
-        const int e = __builtin_amdgcn_readfirstlane(list[item / S]), tile = min(item % S * RW + rw, row_tiles - 1);
+        const int e = __builtin_amdgcn_readfirstlane(list[item / S]), tile = item % S * RW + rw;
         const size_t at = (static_cast<size_t>(e) * row_tiles + tile) * a.nbh * kFp8TileBytes;
         gw = a.gate + at;
         uw = a.up + at;
@@ -221,7 +217,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     };
     int flags = 0, e = static_cast<int>(blockIdx.x) < items ? select(blockIdx.x) : 0;
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int s = item % S, tile = min(s * RW + rw, row_tiles - 1);
+        const int s = item % S, tile = s * RW + rw;
         const int count = find_members(a, routes, e, m);
         const size_t scale0 = (static_cast<size_t>(e) * ((a.I + kFp8Block - 1) / kFp8Block) + tile * 16 / kFp8Block) * a.nbh;
         const float *gs = a.gate_s + scale0, *us = a.up_s + scale0;
@@ -231,30 +227,25 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
             for (int k0 = 0; k0 < a.nbh; k0 += kChunk) {
                 const int kb = min(kChunk, a.nbh - k0);
                 float *xs = reinterpret_cast<float *>(lds + kb * kFp8TileBytes);
-                auto multiply = [&](int b0, const Frag (&g)[U], const Frag (&v)[U]) {
+                auto multiply = [&](int b, const Frag &g, const Frag &v) {
+                    const FragF16 x = to_f16(load_tile(lds + b * kFp8TileBytes, lane));
+                    const float sx = xs[b * 16 + (lane & 15)];
+                    const f32x4 gp = block_dot(to_f16(g), x), up = block_dot(to_f16(v), x);
+                    const float sg = sx * gs[k0 + b], su = sx * us[k0 + b];
 #pragma unroll
-                    for (int u = 0; u < U; ++u) {
-                        const int b = b0 + u * KW;
-                        if (b >= kb) break;
-                        const FragF16 x = to_f16(load_tile(lds + b * kFp8TileBytes, lane));
-                        const float sx = xs[b * 16 + (lane & 15)];
-                        const f32x4 gp = block_dot(to_f16(g[u]), x), up = block_dot(to_f16(v[u]), x);
-                        const float sg = sx * gs[k0 + b], su = sx * us[k0 + b];
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            ga[q] = fmaf(gp[q], sg, ga[q]);
-                            ua[q] = fmaf(up[q], su, ua[q]);
-                        }
+                    for (int q = 0; q < 4; ++q) {
+                        ga[q] = fmaf(gp[q], sg, ga[q]);
+                        ua[q] = fmaf(up[q], su, ua[q]);
                     }
                 };
                 if (c0 > 0 || k0 > 0) load(k0, kb, kw, gf[0], uf[0]);
                 quantize_columns<T_>(a.x, [&](int c) { return static_cast<size_t>(m.token[c0 + c]) * a.H; }, cols, a.H, k0, kb, lds, xs);
                 __syncthreads();
-                for (int b0 = kw; b0 < kb; b0 += 2 * KW * U) {
-                    if (b0 + KW * U < kb) load(k0, kb, b0 + KW * U, gf[1], uf[1]);
-                    multiply(b0, gf[0], uf[0]);
-                    if (b0 + 2 * KW * U < kb) load(k0, kb, b0 + 2 * KW * U, gf[0], uf[0]);
-                    multiply(b0 + KW * U, gf[1], uf[1]);
+                for (int b = kw; b < kb; b += 2 * KW) {
+                    if (b + KW < kb) load(k0, kb, b + KW, gf[1], uf[1]);
+                    multiply(b, gf[0], uf[0]);
+                    if (b + 2 * KW < kb) load(k0, kb, b + 2 * KW, gf[0], uf[0]);
+                    if (b + KW < kb) multiply(b + KW, gf[1], uf[1]);
                 }
                 __syncthreads();   // the columns are used up
             }
@@ -267,7 +258,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
             const float *sum = reinterpret_cast<const float *>(lds);
             for (int i = threadIdx.x; i < 256 * RW; i += 512) {
                 const int r = i >> 8, j = i & 255, c = (j >> 2) & 15, row = (s * RW + r) * 16 + (j >> 6) * 4 + (j & 3);
-                if (c >= cols || row >= a.I) continue;
+                if (c >= cols) continue;
                 const float *w = sum + r * KW * 512 + j;
                 float g = w[0], u = w[256];
 #pragma unroll
@@ -450,7 +441,7 @@ size_t column_bytes(int blocks) { return static_cast<size_t>(std::min(blocks, kC
 template<int T_>
 hipError_t launch_gate_up(const Fp8LayerArgs &a, hipStream_t s) {
     const int experts = std::min(a.T * a.k, a.E) + (a.P1 > a.k ? 1 : 0);   // at most
-    const int slices = (a.I / 16 + kRowTiles - 1) / kRowTiles, grid = std::min(experts * slices, kGateUpGroups);
+    const int slices = a.I / 16 / kRowTiles, grid = std::min(experts * slices, kGateUpGroups);
     const size_t lds = std::max({column_bytes(a.nbh), size_t{8 * 2048}, static_cast<size_t>(a.E) * 4});
     k_fp8_gate_up<T_><<<dim3(grid), dim3(512), lds, s>>>(a);
     return hipGetLastError();
@@ -631,7 +622,7 @@ int moe_fp8_layer_forward(moe_fp8_layer *L, const void *x, int type, const int32
         !aligned(x, 16) || !aligned(ids, 4) || !aligned(weights, 4) || (shared_gate && !aligned(shared_gate, 4)) ||
         !aligned(y, moe::elem_bytes(type)) || !aligned(error, 4))
         return kInvalid;
-    moe::LaunchDevice device(L->device);
+    moe::DeviceScope device(L->device);
     if (!device.ok()) return hipErrorInvalidDevice;
     moe::Fp8LayerArgs a = L->args;
     a.x = x;

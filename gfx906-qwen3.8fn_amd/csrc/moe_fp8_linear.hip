@@ -975,7 +975,7 @@ int moe_fp8_linear_forward(moe_fp8_linear *L, const void *x_codes, const float *
     if (!L || !aligned(x_codes, 16) || !aligned(x_scales, 4) || columns < 1 || columns > 65536 ||
         !valid_rows(y, y_type, y_stride, L->output))
         return kInvalid;
-    moe::LaunchDevice device(L->device);
+    moe::DeviceScope device(L->device);
     if (!device.ok()) return hipErrorInvalidDevice;
     moe::Fp8LinearArgs a = base_args(L, columns, y, y_type, y_stride);
     a.codes = static_cast<const uint8_t *>(x_codes);
@@ -990,7 +990,7 @@ int moe_fp8_linear_apply(moe_fp8_linear *L, const void *x, int x_type, int64_t x
     if (!L || columns < 1 || columns > L->max_columns || !valid_rows(x, x_type, x_stride, L->input) ||
         !valid_rows(y, y_type, y_stride, L->output) || !aligned(error, 4))
         return kInvalid;
-    moe::LaunchDevice device(L->device);
+    moe::DeviceScope device(L->device);
     if (!device.ok()) return hipErrorInvalidDevice;
     const auto s = static_cast<hipStream_t>(stream);
     moe::Fp8LinearArgs a = base_args(L, columns, y, y_type, y_stride);

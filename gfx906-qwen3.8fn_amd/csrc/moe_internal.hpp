@@ -19,13 +19,19 @@
 namespace moe {
 
 // Makes `device` current for one host call of the C ABI and restores the
-// caller's current device on every return path (the calls that allocate,
-// copy or synchronise need their handle's device current; the caller's
-// choice of device must survive them).
+// caller's current device on every return path (calls that allocate, copy,
+// synchronise or launch need their handle's device current; the caller's choice
+// of device must survive them).  No HIP call beyond the query where it is
+// current already.
 class DeviceScope {
 public:
     explicit DeviceScope(int device) {
         if (hipGetDevice(&prev_) != hipSuccess) prev_ = -1;
+        if (prev_ == device) {
+            prev_ = -1;
+            ok_ = true;
+            return;
+        }
         ok_ = hipSetDevice(device) == hipSuccess;
     }
     ~DeviceScope() {
