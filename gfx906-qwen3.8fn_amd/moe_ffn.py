@@ -1060,10 +1060,17 @@ class MoeStack:
                 raise TypeError(f"the residual stream must be float32 or {dtype}, got {xs[0].dtype}")
         batches = xs if self.norms is None else list(xs) * len(self.layers)
         kinds = [x.dtype if dtype is None or self.norms is None else dtype for _, x in zip(self.layers, batches)]
-        for l, kind in enumerate(kinds):
-            step = [self.layers[l]] + [handles[l] for handles in (self.projections, self.routers) if handles]
-            if kind != torch.float32 and any(isinstance(m, (MoeLayer, MoeLinear)) for m in step):
+        for l, (x, kind) in enumerate(zip(batches, kinds)):
+            L, linears = self.layers[l], [handles[l] for handles in (self.projections, self.routers) if handles]
+            if kind != torch.float32 and any(isinstance(m, (MoeLayer, MoeLinear)) for m in [L] + linears):
                 raise TypeError(f"layer {l}: Q4 layers, projections and routers take float32 rows, got {kind}")
+            if x.dim() != 2 or x.shape[1] != L.H:
+                raise ValueError(f"layer {l}: expected rows of {L.H}, got {tuple(x.shape)}")
+            if self.norms is not None and self.projections and isinstance(self.projections[l], MoeFp8Linear):
+                linears = linears[1:]   # takes the norm's rows as they are
+            most = min([L.max_tokens] + [m.max_columns for m in linears])
+            if not 1 <= x.shape[0] <= most:
+                raise ValueError(f"layer {l}: tokens {x.shape[0]} outside 1..{most}")
         dev = xs[0].device
         self.error = torch.zeros(1, dtype=torch.int32, device=dev)
         self.steps = []

@@ -100,3 +100,26 @@ def test_norms_that_do_not_fit():
     ids, w = routes(3)
     with pytest.raises(ValueError):
         moe_ffn.MoeStack(fp8(1), norms=[norm(), norm()]).bind([torch.zeros((3, H))] * 2, [ids], [w])
+
+
+def test_batches_past_the_handles_are_refused():
+    """A batch larger than a layer's, a projection's or a router's capacity, and
+    rows of another width, before anything runs."""
+    ids, w = routes(9)
+    small = dict(max_tokens=8, max_columns=8)
+    linears = lambda **a: [shell(moe_ffn.MoeFp8Linear, **a)]  # noqa: E731
+    for layers, projections, routers in (([shell(moe_ffn.MoeFp8Layer, **small)], None, None),
+                                         ([shell(moe_ffn.MoeLayer, **small)], None, None),
+                                         (fp8(1), linears(**small), None), (fp8(1), None, linears(**small)),
+                                         (fp8(1), [shell(moe_ffn.MoeLinear, **small)], None)):
+        S = moe_ffn.MoeStack(layers, projections, routers)
+        with pytest.raises(ValueError):
+            S.bind([torch.zeros((9, H))], [ids], [w])
+        S.bind([torch.zeros((8, H))], [ids[:8]], [w[:8]])
+        with pytest.raises(ValueError):
+            S.bind([torch.zeros((8, H + 1))], [ids[:8]], [w[:8]])
+        with pytest.raises(ValueError):
+            S.bind([torch.zeros((0, H))], [ids[:0]], [w[:0]])
+    # A projection that takes the norm's e4m3 rows needs no workspace.
+    S = moe_ffn.MoeStack(fp8(1), linears(max_columns=0), norms=[norm(), norm()])
+    S.bind([torch.zeros((9, H))], [ids], [w])
