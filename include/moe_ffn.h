@@ -357,7 +357,8 @@ enum { MOE_F32 = 0, MOE_BF16 = 1, MOE_F16 = 2 };
  * codes [columns][width], scales [columns][ceil(width/128)].  A group that
  * holds an infinity or NaN is written as zero codes with scale 0 and sets bit
  * 1 of `error`.  width 1..16384, columns 1..65536; x, scales and error aligned
- * to their elements; x_stride >= width.  x may not overlap the outputs. */
+ * to their elements; x_stride >= width.  x may not overlap the outputs.  Launches
+ * on the current device. */
 int moe_quantize_e4m3(const void *x, int x_type, int64_t x_stride, int width, int columns, void *codes, float *scales,
                       int *error, void *stream);
 
@@ -508,9 +509,11 @@ typedef struct moe_block_norm_args {
 /* One launch; no workspace, so calls may overlap.  q8 rows and flags are
  * those of moe_quantize_q8_1, codes, scales and flags those of
  * moe_quantize_e4m3, for the fp32 n.  Values that are not finite carry
- * through to h and n.  residual_out may be residual and out may be block, with
- * the same stride; other overlaps are not allowed.  A block's post_weight and
- * gate need a block; pre_weight needs an output, and an output pre_weight. */
+ * through to h and n; rms is 0 for a row whose sum of squares passes fp32's
+ * range (elements of 10^17 and more).  residual_out may be residual and out may
+ * be block, with the same stride; other overlaps are not allowed.  A block's
+ * post_weight and gate need a block; pre_weight needs an output, and an output
+ * pre_weight.  Launches on the current device. */
 int moe_block_norm(const moe_block_norm_args *args, void *stream);
 
 #ifdef __cplusplus

@@ -101,3 +101,20 @@ def test_nan_gates_stay_in_their_rows(h):
     assert bool(got["out"][2].isnan().all())
     for k in ("residual", "out"):
         assert torch.equal(got[k][[0, 1, 3]], want[k][[0, 1, 3]])
+
+
+@pytest.mark.parametrize("h", [640, 8200])
+def test_rows_whose_squares_overflow(h):
+    """Finite rows of 10^20: the sum is what it is, its norm 0, as are its
+    quantised rows, without a flag; other rows are not touched."""
+    g = R.generator(h)
+    norm = make(g, h, post=False)
+    x, block = (torch.randn((3, h), generator=g, device=DEV) for _ in range(2))
+    outputs = ("residual", "out", "e4m3")
+    want = norm(x, block=block, outputs=outputs)
+    x[1] *= 1e20
+    got = norm(x, block=block, outputs=outputs)
+    assert bool(got["residual"][1].isfinite().all()) and flag(got["error"]) == 0
+    assert bool((got["out"][1] == 0).all()) and bool((got["codes"].view(torch.uint8)[1] & 0x7f == 0).all())
+    for k in outputs[:2] + ("scales",):
+        assert torch.equal(got[k][[0, 2]], want[k][[0, 2]])
