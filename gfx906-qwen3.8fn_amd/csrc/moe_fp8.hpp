@@ -218,9 +218,9 @@ __device__ __forceinline__ Operand operand(const Frag &f) {
 // its eight is about 2^7 times as large, and less than 2^-13 of that one (2^-10
 // where it has a subnormal code).  2-norm of the error: 1.5e-5 of the result's
 // on normal data, 5.5e-5 with an element of each group of 128 two hundred times
-// the others' deviation, 5e-5 on codes drawn evenly.  Fit for results that are rounded to
-// 16 bits (2^-9 and 2^-12 on either side), where the caller has not asked for
-// fp32 sums, not for fp32 ones.
+// the others' deviation, 5e-5 on codes drawn evenly.  Fit for results that are
+// rounded to 16 bits (by up to 2^-8 or 2^-11 of themselves), where the caller has
+// not asked for fp32 sums, not for fp32 ones.
 __device__ __forceinline__ f32x4 block_dot(const FragF16 &w, const FragF16 &x) {
     f32x4 p = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

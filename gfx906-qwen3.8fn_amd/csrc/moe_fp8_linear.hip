@@ -506,7 +506,9 @@ struct GemmTile {
     // fills any more), so that a wave's stores run along the rows of y: straight
     // from the accumulators they are pieces of four elements of 16 rows each
     // (96 x 2047 at 16,000 columns 41 us, 22 so; 96 x 2048 26 and 21; 8192 x 8192 at
-    // 16,384 1,012 and 985).  fp32 pieces are twice as long and gain nothing.
+    // 16,384 1,012 and 985).  fp32 pieces are twice as long: through LDS they took
+    // the same time within 4 % in rows of aligned length.  Rows of odd length cost
+    // them up to half more (96 x 2047 at 16,000 columns 51 us, 2048 36).
     template<int Y>
     __device__ __forceinline__ void store_along_rows(const Fp8LinearArgs &a, const f32x4 (&acc)[TM][TN], uint8_t *lds) const {
         constexpr int Pitch = BM * 2 + 8, Lanes = BM / 4;   // lanes of a row
@@ -872,7 +874,11 @@ int launch_product(const moe::Fp8LinearArgs &a, bool sums32, hipStream_t s) {
     const long t64 = tiles(64, 64), t128 = tiles(128, 128), rounds128 = (t128 + 255) / 256;
     if (sums32) {
         if (tiles(64, 32) <= 256) return launch_split<4, 2, 8, Tiles, true>(a, s);
-        // The two forms of a number of groups give the same sums, and so do apply and forward.
+        // The two forms of a number of groups give the same sums, and so do apply
+        // and forward.  That has a price: above 256 tiles 32 x 48 among four waves
+        // would be faster at some sizes (1,032 columns 18.2 against 19.3, 2,500 35.1
+        // against 37.5), but rows have its sums in four groups of 64 x 64 alone (26.4
+        // and 44.3 against 21.8 and 36.5).
         const bool fills = t64 <= 512 && 10 * static_cast<long>(a.M) * a.N >= 9 * 4096 * 256 * ((t64 + 255) / 256);
         if (t64 <= 256) {
             if constexpr (Tiles)

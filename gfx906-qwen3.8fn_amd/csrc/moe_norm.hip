@@ -54,7 +54,9 @@ __device__ __forceinline__ void store8_any(void *p, size_t at, int valid, const 
 // ulp each, so that the whole is within 8 half ulps.  Beyond |t| = 127 there is
 // nothing to correct: 2^t is infinite from t = 128 on (and r times it NaN), 1 +
 // 2^t is 1 below -25, and a quotient below 2^-126, from t = 126 on, is 0 or
-// itself.  Infinite g: 0 or 1.
+// itself.  Infinite g: 0 or 1.  With the exact expf of the layers' SiLU and a
+// division, 16,384 rows of 2,560 bf16 channels with an element gate take 189 us
+// instead of 88, 1,032 rows 15.9 instead of 10.1.
 __device__ __forceinline__ float sigmoid(float g) {
     constexpr float log2e = 0x1.715476p+0f, log2e_rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;
     const float t = -g * log2e;
@@ -147,8 +149,10 @@ __device__ __forceinline__ void store_e4m3(uint8_t *codes, size_t at, float *sca
 // and all of a row in registers.  Weights and a gate per channel stay in
 // registers and a row is on its way while the last one is reduced (NV = 1; with
 // 16 elements a thread the registers do not suffice for that, and an element
-// gate is read where it is used: 2,000 rows of 16,384 bf16 channels 70 us, 3.7
-// TB/s, and 84 with such a gate; 80 and 117 when it was read with the rest).
+// gate is read where it is used: 2,000 rows of 16,384 bf16 channels 72 us, 3.6
+// TB/s, and 87 with such a gate; 80 and 117 when it was read with the rest.  fp16
+// 72 and 88, fp32 120 and 136 us, 4.4 and 4.8 TB/s, though fp16 spills seven
+// registers there and fp32 three).
 // TB: type of block, out and an element gate; TR: of the residual.
 template<int TB, int TR, int NV>
 __global__ __launch_bounds__(1024) void k_block_norm(NormArgs a) {
