@@ -57,6 +57,17 @@ class Fp8Matrix(ctypes.Structure):
     _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
 
 
+class I8LayerConfig(ctypes.Structure):
+    """moe_i8_layer_config."""
+    _fields_ = [("hidden", ctypes.c_int), ("intermediate", ctypes.c_int), ("experts", ctypes.c_int),
+                ("top_k", ctypes.c_int), ("has_shared", ctypes.c_int), ("max_tokens", ctypes.c_int)]
+
+
+class I8Matrix(ctypes.Structure):
+    """moe_i8_matrix."""
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p)]
+
+
 class BlockNormArgs(ctypes.Structure):
     """moe_block_norm_args."""
     _fields_ = ([(n, ctypes.c_int) for n in ("hidden", "tokens", "type", "residual_type")] +
@@ -137,6 +148,22 @@ def library():
         lib.moe_fp8_layer_destroy.argtypes = [_P]
         lib.moe_fp8_layer_forward.argtypes = [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P]
         lib.moe_block_norm.argtypes = [ctypes.POINTER(BlockNormArgs), _P]
+        lib.moe_quantize_i8.argtypes = [_P, _I, _L, _I, _I, _P, _P, _P, _P]
+        lib.moe_i8_linear_create.argtypes = [_I, _I, _I, _P, _P, _I, _I, ctypes.POINTER(_P)]
+        lib.moe_i8_linear_destroy.argtypes = [_P]
+        lib.moe_i8_linear_bytes.argtypes = [_P, ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_i8_linear_forward.argtypes = [_P, _P, _P, _I, _P, _I, _L, _P]
+        lib.moe_i8_linear_apply.argtypes = [_P, _P, _I, _L, _I, _P, _I, _L, _P, _P]
+        lib.moe_i8_bank_create.argtypes = [_I, _I, _I, _P, _P, _I, _I, ctypes.POINTER(_P)]
+        lib.moe_i8_bank_destroy.argtypes = [_P]
+        lib.moe_i8_bank_bytes.argtypes = [_P, ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_i8_bank_forward.argtypes = [_P, _P, _P, _I, _P, _P, _I, _P, _I, _L, _P, _P]
+        lib.moe_i8_layer_memory_bytes.argtypes = [ctypes.POINTER(I8LayerConfig), ctypes.POINTER(ctypes.c_size_t),
+                                                  ctypes.POINTER(ctypes.c_size_t)]
+        lib.moe_i8_layer_create.argtypes = [ctypes.POINTER(I8LayerConfig), ctypes.POINTER(I8Matrix),
+                                            ctypes.POINTER(I8Matrix), _I, _I, ctypes.POINTER(_P)]
+        lib.moe_i8_layer_destroy.argtypes = [_P]
+        lib.moe_i8_layer_forward.argtypes = [_P, _P, _I, _P, _P, _I, _P, _P, _P, _P]
         _lib = lib
     return _lib
 
@@ -863,6 +890,312 @@ class MoeFp8Layer:
         return y, error
 
 
+def bind_quantize_i8(x, codes, scales, error, stream=None):
+    """Validate the tensors of a quantize_i8() once and return a no-argument
+    callable that enqueues it with no per-call checks; the tensors must stay
+    alive and keep their shapes while the callable is used."""
+    import torch
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a two-dimensional torch tensor")
+    n, width = x.shape
+    dev = x.device
+    type_, stride = _need_rows(x, "x", (n, width))
+    _need(codes, "codes", torch.int8, (n, width), dev)
+    _need(scales, "scales", torch.float32, (n,), dev)
+    _need(error, "error", torch.int32, (1,), dev)
+    fn = library().moe_quantize_i8
+    args = (_ptr(x), type_, stride, width, n, _ptr(codes), _ptr(scales), _ptr(error), _stream_on(stream, dev))
+    current, switch = torch.cuda.current_device, dev.index
+
+    def call():
+        if current() != switch:
+            with _on_device(dev):
+                st = fn(*args)
+        else:
+            st = fn(*args)
+        if st != 0:
+            raise MoeError("moe_quantize_i8", st)
+    return call
+
+
+def quantize_i8(x, codes=None, scales=None, error=None, stream=None):
+    """Rows x [n][width] (float32, bfloat16 or float16; rows may be strided)
+    -> (codes int8 [n][width], scales float32 [n], error)."""
+    import torch
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError("x must be a two-dimensional torch tensor")
+    with _making(stream):
+        if codes is None:
+            codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        if scales is None:
+            scales = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+        if error is None:
+            error = torch.zeros(1, dtype=torch.int32, device=x.device)
+    bind_quantize_i8(x, codes, scales, error, stream)()
+    return codes, scales, error
+
+
+def _i8_matrices(codes, scales, shape, name, device):
+    """(code pointer, scale pointer, on device, kept alive) of int8 matrices of
+    `shape` [..][rows][cols] with scales [..][rows], torch tensors on `device`
+    or numpy arrays."""
+    import torch
+    shape = tuple(shape)
+    if isinstance(codes, np.ndarray):
+        c, s = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+        if c.dtype != np.int8 or s.dtype != np.float32:
+            raise TypeError(f"{name}: numpy codes are int8 and scales float32, got {c.dtype} and {s.dtype}")
+        if c.shape != shape or s.shape != shape[:-1]:
+            raise ValueError(f"{name}: expected codes {shape} and scales {shape[:-1]}, got {c.shape} and {s.shape}")
+        return ctypes.c_void_p(c.ctypes.data), ctypes.c_void_p(s.ctypes.data), 0, (c, s)
+    dev = torch.device("cuda", device)
+    _need(codes, f"{name} codes", torch.int8, shape, dev)
+    _need(scales, f"{name} scales", torch.float32, shape[:-1], dev)
+    return _ptr(codes), _ptr(scales), 1, (codes, scales)
+
+
+class MoeI8Linear:
+    """One resident int8 matrix [output][input] with a scale per output channel
+    (moe_i8_linear_create): codes int8 and scales float32 [output], both torch
+    tensors on a GPU or both numpy arrays.  forward takes int8 rows with a scale
+    each, apply rows of float32, bfloat16 or float16.  The sums are exact."""
+
+    def __init__(self, input, output, codes, scales, max_columns=0, device=0):
+        self.K, self.M, self.max_columns, self.device = input, output, max_columns, device
+        c, s, on_device, _keep = _i8_matrices(codes, scales, (output, input), "weights", device)
+        handle = ctypes.c_void_p()
+        _check(library().moe_i8_linear_create(input, output, max_columns, c, s, on_device, device,
+                                              ctypes.byref(handle)), "moe_i8_linear_create")
+        self.handle = handle
+
+    def close(self):
+        if getattr(self, "handle", None):
+            library().moe_i8_linear_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def weight_bytes(self):
+        n = ctypes.c_size_t()
+        _check(library().moe_i8_linear_bytes(self.handle, ctypes.byref(n)), "moe_i8_linear_bytes")
+        return n.value
+
+    def bind_forward(self, x_codes, x_scales, y, stream=None):
+        """Validate the tensors of a forward() once and return a no-argument
+        callable that enqueues it with no per-call checks; the tensors must
+        stay alive and keep their shapes while the callable is used.  It keeps
+        the matrix alive, and raises after close()."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x_codes.shape[0]
+        _need(x_codes, "x_codes", torch.int8, (n, self.K), dev)
+        _need(x_scales, "x_scales", torch.float32, (n,), dev)
+        type_, stride = _need_rows(y, "y", (n, self.M), dev)
+        fn = library().moe_i8_linear_forward
+        args = (_ptr(x_codes), _ptr(x_scales), n, _ptr(y), type_, stride, _stream_on(stream, dev))
+
+        def call():
+            st = fn(self.handle, *args)
+            if st != 0:
+                raise MoeError("moe_i8_linear_forward", st)
+        return call
+
+    def forward(self, x_codes, x_scales, y=None, dtype=None, stream=None):
+        """y [n][output] (given, or a new tensor of `dtype`, float32 unless
+        said) from int8 rows."""
+        import torch
+        if y is None:
+            with _making(stream):
+                y = torch.empty((x_codes.shape[0], self.M), dtype=dtype or torch.float32, device=x_codes.device)
+        self.bind_forward(x_codes, x_scales, y, stream)()
+        return y
+
+    def bind_apply(self, x, y, error, stream=None):
+        """bind_forward's counterpart for apply()."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x.shape[0]
+        x_type, x_stride = _need_rows(x, "x", (n, self.K), dev)
+        y_type, y_stride = _need_rows(y, "y", (n, self.M), dev)
+        _need(error, "error", torch.int32, (1,), dev)
+        fn = library().moe_i8_linear_apply
+        args = (_ptr(x), x_type, x_stride, n, _ptr(y), y_type, y_stride, _ptr(error), _stream_on(stream, dev))
+
+        def call():
+            st = fn(self.handle, *args)
+            if st != 0:
+                raise MoeError("moe_i8_linear_apply", st)
+        return call
+
+    def apply(self, x, y=None, error=None, dtype=None, stream=None):
+        """(y, error) from rows x [n][input]; y in x's type unless given."""
+        import torch
+        with _making(stream):
+            if y is None:
+                y = torch.empty((x.shape[0], self.M), dtype=dtype or x.dtype, device=x.device)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        self.bind_apply(x, y, error, stream)()
+        return y, error
+
+
+class MoeI8Bank:
+    """Resident int8 matrices of a number of experts (moe_i8_bank_create): codes
+    int8 [experts][output][input] and scales float32 [experts][output], both
+    torch tensors on a GPU or both numpy arrays.  forward multiplies rows that
+    are grouped by expert, in groups of any sizes that only the device knows."""
+
+    def __init__(self, experts, input, output, codes, scales, device=0):
+        self.E, self.K, self.M, self.device = experts, input, output, device
+        c, s, on_device, _keep = _i8_matrices(codes, scales, (experts, output, input), "weights", device)
+        handle = ctypes.c_void_p()
+        _check(library().moe_i8_bank_create(experts, input, output, c, s, on_device, device, ctypes.byref(handle)),
+               "moe_i8_bank_create")
+        self.handle = handle
+
+    def close(self):
+        if getattr(self, "handle", None):
+            library().moe_i8_bank_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def weight_bytes(self):
+        n = ctypes.c_size_t()
+        _check(library().moe_i8_bank_bytes(self.handle, ctypes.byref(n)), "moe_i8_bank_bytes")
+        return n.value
+
+    def bind_forward(self, x_codes, x_scales, offsets, y, error, index=None, stream=None):
+        """Validate the tensors of a forward() once and return a no-argument
+        callable that enqueues it with no per-call checks; the tensors must
+        stay alive and keep their shapes while the callable is used.  It keeps
+        the bank alive, and raises after close()."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x_codes.shape[0]
+        _need(x_codes, "x_codes", torch.int8, (n, self.K), dev)
+        _need(x_scales, "x_scales", torch.float32, (n,), dev)
+        _need(offsets, "offsets", torch.int32, (self.E + 1,), dev)
+        if not isinstance(y, torch.Tensor) or y.dim() != 2:
+            raise ValueError("y must be a two-dimensional torch tensor")
+        rows = y.shape[0]
+        if index is not None:
+            _need(index, "index", torch.int32, (rows,), dev)
+        elif rows > n:
+            raise ValueError(f"y has {rows} rows, x_codes {n}; without an index they are the same rows")
+        type_, stride = _need_rows(y, "y", (rows, self.M), dev)
+        _need(error, "error", torch.int32, (1,), dev)
+        fn = library().moe_i8_bank_forward
+        args = (_ptr(x_codes), _ptr(x_scales), n, _ptr(index), _ptr(offsets), rows, _ptr(y), type_, stride, _ptr(error),
+                _stream_on(stream, dev))
+
+        def call():
+            st = fn(self.handle, *args)
+            if st != 0:
+                raise MoeError("moe_i8_bank_forward", st)
+        return call
+
+    def forward(self, x_codes, x_scales, offsets, y=None, error=None, index=None, dtype=None, stream=None):
+        """(y, error): rows offsets[e] .. offsets[e + 1] - 1 of y (given, or new
+        zeros of `dtype`, float32 unless said) are x_codes' rows, or its rows
+        index[i], times expert e's matrix.  Rows of no group stay as they are."""
+        import torch
+        with _making(stream):
+            if y is None:
+                rows = (index if index is not None else x_codes).shape[0]
+                y = torch.zeros((rows, self.M), dtype=dtype or torch.float32, device=x_codes.device)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x_codes.device)
+        self.bind_forward(x_codes, x_scales, offsets, y, error, index, stream)()
+        return y, error
+
+
+class MoeI8Layer:
+    """One MoE layer of int8 matrices, for one token as for whole prompts
+    (moe_i8_layer_create).  gate and up are (codes [E][I][H], scales [E][I]),
+    down is (codes [E][H][I], scales [E][H]) and shared, for a layer with a
+    shared expert, its (gate, up, down) of the same without E; all torch tensors
+    on the layer's GPU or all numpy arrays."""
+
+    def __init__(self, hidden, intermediate, experts, top_k, has_shared, max_tokens, gate, up, down, shared=None, device=0):
+        self.cfg = I8LayerConfig(hidden, intermediate, experts, top_k, 1 if has_shared else 0, max_tokens)
+        self.H, self.I, self.E, self.k = hidden, intermediate, experts, top_k
+        self.has_shared, self.max_tokens, self.device = bool(has_shared), max_tokens, device
+        if self.has_shared != (shared is not None) or (self.has_shared and len(shared) != 3):
+            raise ValueError("shared: three matrices where the layer has a shared expert, None where not")
+        gate_up, down_shape = (intermediate, hidden), (hidden, intermediate)
+        parts = [_i8_matrices(*m, (experts, *shape), name, device)
+                 for m, shape, name in ((gate, gate_up, "gate"), (up, gate_up, "up"), (down, down_shape, "down"))]
+        if self.has_shared:
+            parts += [_i8_matrices(*m, shape, f"shared {name}", device)
+                      for m, shape, name in zip(shared, (gate_up, gate_up, down_shape), ("gate", "up", "down"))]
+        if len({p[2] for p in parts}) != 1:
+            raise ValueError("the matrices must be all torch tensors or all numpy arrays")
+        banks = [(I8Matrix * 3)(*[I8Matrix(p[0], p[1]) for p in parts[i:i + 3]]) for i in range(0, len(parts), 3)]
+        handle = ctypes.c_void_p()
+        _check(library().moe_i8_layer_create(ctypes.byref(self.cfg), banks[0], banks[1] if self.has_shared else None,
+                                             parts[0][2], device, ctypes.byref(handle)), "moe_i8_layer_create")
+        self.handle = handle
+
+    def close(self):
+        if getattr(self, "handle", None):
+            library().moe_i8_layer_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def bind_forward(self, x, ids, weights, y, error, shared_gate=None, stream=None):
+        """Validate the tensors of a forward() once and return a no-argument
+        callable that enqueues it with no per-call checks (as
+        MoeLayer.bind_forward); it keeps the layer alive, and raises after
+        close()."""
+        import torch
+        dev = torch.device("cuda", self.device)
+        n = x.shape[0]
+        if not 1 <= n <= self.max_tokens:
+            raise ValueError(f"tokens {n} outside 1..{self.max_tokens}")
+        type_ = _elem_type(x, "x")
+        _need(x, "x", x.dtype, (n, self.H), dev)
+        _routes_check(ids, weights, n, self.k, dev)
+        if shared_gate is not None:
+            _need(shared_gate, "shared_gate", torch.float32, (n,), dev)
+        _need(y, "y", x.dtype, (n, self.H), dev)
+        _need(error, "error", torch.int32, (1,), dev)
+        fn = library().moe_i8_layer_forward
+        args = (_ptr(x), type_, _ptr(ids), _ptr(weights), n, _ptr(shared_gate), _ptr(y), _ptr(error),
+                _stream_on(stream, dev))
+
+        def call():
+            st = fn(self.handle, *args)
+            if st != 0:
+                raise MoeError("moe_i8_layer_forward", st)
+        return call
+
+    def forward(self, x, ids, weights, shared_gate=None, y=None, error=None, stream=None):
+        """(y, error) for x [n][H] of float32, bfloat16 or float16; y has x's
+        type."""
+        import torch
+        with _making(stream):
+            if y is None:
+                y = torch.empty_like(x)
+            if error is None:
+                error = torch.zeros(1, dtype=torch.int32, device=x.device)
+        self.bind_forward(x, ids, weights, y, error, shared_gate, stream)()
+        return y, error
+
+
 class BlockNorm:
     """The norm after a block and the norm before the next one, with the gate,
     the scales and the residual sum between them (moe_block_norm):
@@ -1010,11 +1343,11 @@ class MoeStack:
     or replayed from one captured HIP graph (torch.cuda.CUDAGraph over the
     library's launches).
 
-    Layers, projections and routers may be Q4 (MoeLayer, MoeLinear) or e4m3
-    (MoeFp8Layer, MoeFp8Linear) handles.
+    Layers, projections and routers may be Q4 (MoeLayer, MoeLinear), e4m3
+    (MoeFp8Layer, MoeFp8Linear) or int8 (MoeI8Layer, MoeI8Linear) handles.
 
     Without `norms`, layer l takes its own input batch x[l] (fp32 [N_l][H],
-    device; e4m3 layers also bfloat16 or float16).  With `projections` (H -> H
+    device; e4m3 and int8 layers also bfloat16 or float16).  With `projections` (H -> H
     per layer) the layer input is h = projection.apply(x); with `routers` (H ->
     E per layer) the routes are chosen on the device from router.apply(h) by
     router_select; otherwise fixed device ids / weights are given to bind().

@@ -462,6 +462,139 @@ int moe_fp8_layer_forward(moe_fp8_layer *layer, const void *x, int type, const i
                           int tokens, const float *shared_gate, void *y, int *error, void *stream);
 
 /* ------------------------------------------------------------------------
+ * 8-bit integers: int8 matrices with one fp32 scale per output channel, on
+ * activations quantised with one fp32 scale per row (token), for checkpoints
+ * that store their matrices so.  No counterpart in the reference, whose
+ * matrices are Q4.
+ *
+ *   matrix   codes [rows][cols] int8 (-128 .. 127), scales [rows] fp32: element
+ *            (r, c) = codes[r][c] * scales[r]
+ *   rows     (activations) codes [n][width] int8, scales [n]: a row x with a =
+ *            max(|x|max, 2^-100) has the scale a / 127 and the codes
+ *            rint(x * (127 / a)), nearest even, every operation rounded to fp32
+ * A product is the whole number sum_k cx cw, exact, made fp32 and multiplied by
+ * the product of both scales, then rounded to the type of the result: the same
+ * bits whatever the number of rows and from every entry point.  Where the
+ * product of the scales leaves fp32's normal range (beyond 2^128, below 2^-126)
+ * so do the results.
+ * ---------------------------------------------------------------------- */
+
+/* x [columns] rows of `width` elements of x_type, x_stride elements apart ->
+ * codes [columns][width], scales [columns].  A row that holds an infinity or NaN
+ * is written as zero codes with scale 0 and sets bit 1 of `error`.  width
+ * 1..16384, columns 1..65536; x, scales and error aligned to their elements;
+ * x_stride >= width.  x may not overlap the outputs.  Launches on the current
+ * device. */
+int moe_quantize_i8(const void *x, int x_type, int64_t x_stride, int width, int columns, void *codes, float *scales,
+                    int *error, void *stream);
+
+typedef struct moe_i8_linear moe_i8_linear;
+
+/* One resident int8 matrix [output][input] with its scales [output], on the host
+ * or (weights_on_device = 1) on `device`; they are copied into the handle's own
+ * layout, so the caller may free them afterwards.  input: multiple of 32,
+ * 32..16384; output 1..262144.  max_columns (0..65536) sizes the workspace of
+ * moe_i8_linear_apply.  Allocates; waits for the device before it reads the
+ * weights and before it returns. */
+int moe_i8_linear_create(int input, int output, int max_columns, const void *codes, const float *scales,
+                         int weights_on_device, int device, moe_i8_linear **out);
+int moe_i8_linear_destroy(moe_i8_linear *linear);
+/* Bytes of the codes and scales the handle was created from. */
+int moe_i8_linear_bytes(const moe_i8_linear *linear, size_t *weight_bytes);
+
+/* y[n][m] = sum over the matrix row of x * W, for int8 rows x_codes
+ * [columns][input] (16-byte aligned) with x_scales [columns]; y rows are y_stride
+ * elements of y_type apart.  columns 1..65536.  No workspace: calls on one handle
+ * may overlap.  What lies between y's rows is left as it is.  y may not overlap
+ * the rows or their scales.  Enqueue only; the handle's device need not be
+ * current. */
+int moe_i8_linear_forward(moe_i8_linear *linear, const void *x_codes, const float *x_scales, int columns, void *y,
+                          int y_type, int64_t y_stride, void *stream);
+
+/* moe_quantize_i8 (same codes, same flags), then forward, with the rows in the
+ * handle's workspace or, for a few columns, in the product's kernel.  columns
+ * 1..max_columns.  x and y may overlap: all of x is read before any of y is
+ * written.  Calls on one handle must not overlap (they share the workspace). */
+int moe_i8_linear_apply(moe_i8_linear *linear, const void *x, int x_type, int64_t x_stride, int columns, void *y,
+                        int y_type, int64_t y_stride, int *error, void *stream);
+
+typedef struct moe_i8_bank moe_i8_bank;
+
+/* `experts` (1..4096) resident int8 matrices: codes [experts][output][input],
+ * scales [experts][output].  Otherwise as moe_i8_linear_create; output
+ * 1..65536. */
+int moe_i8_bank_create(int experts, int input, int output, const void *codes, const float *scales, int weights_on_device,
+                       int device, moe_i8_bank **out);
+int moe_i8_bank_destroy(moe_i8_bank *bank);
+int moe_i8_bank_bytes(const moe_i8_bank *bank, size_t *weight_bytes);
+
+/* Products of rows grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of y
+ * [rows] belong to expert e, for offsets [experts + 1] on the DEVICE, and row i is
+ * the product of x's row index[i] (int32, device), or i without an index, with
+ * that expert's matrix.  x_codes [x_rows][input] (16-byte aligned) with x_scales
+ * [x_rows]; x_rows and rows 1..4194304; with an index x_rows * input <= 2^31,
+ * without one rows <= x_rows.  Groups may be empty; rows before the first offset
+ * and from the last one on are left as they are, and so is what lies between y's
+ * rows.  Offsets that leave 0 .. rows or that decrease set bit 1 of `error`: they
+ * are drawn into 0 .. rows, and a group whose end is not after its begin is empty
+ * (a row that two groups then claim is one of their products).  A row whose index
+ * leaves 0 .. x_rows - 1 is zero and sets bit 1.  No workspace: calls on one
+ * handle may overlap.  y may not overlap the inputs.  Enqueue only; the handle's
+ * device need not be current. */
+int moe_i8_bank_forward(moe_i8_bank *bank, const void *x_codes, const float *x_scales, int x_rows, const int32_t *index,
+                        const int32_t *offsets, int rows, void *y, int y_type, int64_t y_stride, int *error, void *stream);
+
+/* ------------------------------------------------------------------------
+ * A routed-expert layer of int8 matrices: moe_ffn_forward's operator for an
+ * int8 checkpoint, from one token to whole prompts.
+ * ---------------------------------------------------------------------- */
+
+typedef struct moe_i8_layer_config {
+    int hidden;        /* H: multiple of 32, 32..16384 */
+    int intermediate;  /* I: multiple of 32, 32..16384 */
+    int experts;       /* E: routed experts, 1..4096 with the shared one */
+    int top_k;         /* routes per token, 1..32, <= experts */
+    int has_shared;    /* 1: one shared expert, always routed */
+    int max_tokens;    /* capacity of forward(), 1..65536 */
+} moe_i8_layer_config;
+
+/* int8 matrices of one kind, one after the other: codes [n][rows][cols], scales
+ * [n][rows]. */
+typedef struct moe_i8_matrix {
+    const void *codes;
+    const float *scales;
+} moe_i8_matrix;
+
+typedef struct moe_i8_layer moe_i8_layer;
+
+/* Device bytes held by a layer (weights, workspace for max_tokens). */
+int moe_i8_layer_memory_bytes(const moe_i8_layer_config *config, size_t *weight_bytes, size_t *workspace_bytes);
+
+/* `experts` = gate [E][I][H], up [E][I][H], down [E][H][I]; `shared` = the
+ * shared expert's three matrices (n = 1), NULL when the layer has none.  All
+ * on the host or all on `device`; they are copied into the handle's own
+ * layout.  Allocates; waits for the device before it reads the weights and
+ * before it returns. */
+int moe_i8_layer_create(const moe_i8_layer_config *config, const moe_i8_matrix *experts, const moe_i8_matrix *shared,
+                        int weights_on_device, int device, moe_i8_layer **layer);
+int moe_i8_layer_destroy(moe_i8_layer *layer);
+
+/* x, y [tokens][H] of `type` (MOE_F32, MOE_BF16, MOE_F16); ids, weights,
+ * shared_gate and the sum as in moe_ffn_forward.  x's rows and the experts'
+ * middle rows SiLU(gate) * up are quantised as moe_quantize_i8 does; the weighted
+ * sum is fp32, y is rounded once.  Flags in `error` as in moe_ffn_forward: routes
+ * with a bad id or an id of an earlier rank are dropped and set bit 1.  So do
+ * nonfinite input, whose token counts as zeros, a negative weight, which stays in
+ * the sum, and a nonfinite weight, which gives up the token's routed sum: what is
+ * left is the shared expert.  An expert's output or a partial sum that is not
+ * finite gives up its own element of the routed sum, a nonfinite shared output or
+ * shared_gate its element of y (0).  x may not overlap y.  tokens in
+ * 1..max_tokens.  Enqueue only; calls on one layer must not overlap (they share
+ * the workspace).  The layer's device need not be current. */
+int moe_i8_layer_forward(moe_i8_layer *layer, const void *x, int type, const int32_t *ids, const float *weights,
+                         int tokens, const float *shared_gate, void *y, int *error, void *stream);
+
+/* ------------------------------------------------------------------------
  * The norms around a block, with its gate, the scales and the residual sum.
  * ---------------------------------------------------------------------- */
 

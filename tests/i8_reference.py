@@ -1,0 +1,95 @@
+"""Restatement of the 8-bit integer formats and operators for the tests: codes,
+scales and middle rows as the formats define them (fp32 operations, each rounded
+on its own), everything after them in 64 bits."""
+import numpy as np
+import torch
+
+import moe_ffn
+
+EPS = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}   # half a step, relative
+TINY = {torch.float32: 2.0 ** -149, torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}   # a subnormal's step
+
+
+def generator(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def quantise(x):
+    """(codes int8, scales fp32) of finite rows.  Divisions of fp32 numbers in 64
+    bits, rounded, are the correctly rounded fp32 quotients."""
+    v = x.float()
+    a = v.abs().amax(dim=1).clamp_min(2.0 ** -100).double()
+    return (v * (127.0 / a).float()[:, None]).round().to(torch.int8), (a / 127.0).float()
+
+
+def weights(count, rows, cols, seed):
+    """int8 matrices over the whole range of codes, -128 among them, with scales
+    over two powers of ten."""
+    g = generator(seed)
+    codes = torch.randint(-128, 128, (count, rows, cols), generator=g, device="cuda", dtype=torch.int32).to(torch.int8)
+    scales = 1e-3 * torch.exp(4.6 * torch.rand((count, rows), generator=g, device="cuda"))
+    return codes, scales
+
+
+def sums(x, w):
+    """The whole-number sums, in 64 bits."""
+    return x.double() @ w.double().T
+
+
+def product(x, sx, w, sw):
+    return sums(x, w) * sx.double()[:, None] * sw.double()
+
+
+def product_bound(ref, dtype):
+    """|y - ref| of a product: the sum made fp32, the product of the scales, their
+    product (2^-24 each, and second-order terms), y's own rounding."""
+    return ref.abs() * (3.01 * 2.0 ** -24 + EPS[dtype] * (1 + 2.0 ** -20)) + TINY[dtype]
+
+
+def close(y, ref, dtype):
+    assert y.dtype == dtype
+    d = (y.double() - ref).abs()
+    assert bool((d <= product_bound(ref, dtype)).all()), float((d / product_bound(ref, dtype)).max())
+
+
+def middle(x, sx, gate, up):
+    """fp32 SiLU(g) u with every operation rounded as the kernels round it."""
+    def rows(w):
+        s = sx.float()[:, None].cpu() * w[1].float().cpu()
+        return sums(x, w[0]).cpu().float() * s
+    g, u = rows(gate), rows(up)
+    e = torch.from_numpy(moe_ffn.expf_host((-g).numpy().astype(np.float32)))
+    return ((g / (1.0 + e)) * u).to(x.device)
+
+
+def expert(x, sx, gate, up, down):
+    """One expert's output in 64 bits, from its middle row's codes."""
+    m, sm = quantise(middle(x, sx, gate, up))
+    return product(m, sm, *down)
+
+
+def layer(x, bank, shared, ids, w, gate):
+    """(y in 64 bits, sum of the magnitudes that it adds up)."""
+    q, s = quantise(x)
+    n, k = ids.shape
+    y = torch.zeros((n, x.shape[1]), dtype=torch.float64, device=x.device)
+    size = torch.zeros_like(y)
+    for e in torch.unique(ids).tolist():
+        t, r = torch.nonzero(ids == e, as_tuple=True)
+        c = w[t, r].double()[:, None] * expert(q[t], s[t], *[(codes[e], scales[e]) for codes, scales in bank])
+        y.index_add_(0, t, c)
+        size.index_add_(0, t, c.abs())
+    if shared is not None:
+        c = expert(q, s, *shared)
+        if gate is not None:
+            c = c * torch.sigmoid(gate.double())[:, None]
+        y, size = y + c, size + c.abs()
+    return y, size
+
+
+def layer_bound(y, size, k, dtype):
+    """A contribution has three roundings of its own, one of its weight and up to
+    five in its gate's sigmoid; each of k + 1 sums has one."""
+    return size * ((k + 11) * 2.0 ** -24) + y.abs() * EPS[dtype] * (1 + 2.0 ** -10) + TINY[dtype]
