@@ -528,6 +528,40 @@ __device__ __forceinline__ float silu_mul(float g, float u, int &flags) {
     return silu_mul(g, u, flags, MoeExpfTable{});
 }
 
+// y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags
+// of moe_ffn_forward's sum.  c(r): rank r's output, of the routes that count.
+template<class C>
+__device__ __forceinline__ float fold(int k, bool shared, bool gated, const int *valid, const float *weight, C c, int &flags) {
+    int f = 0;
+    float v = 0.0f;
+    for (int r = 0; r < k; ++r) {
+        if (!valid[r]) continue;
+        float x = c(r), w = weight[r];
+        if (!isfinite(x)) { f |= 1; x = 0.0f; }
+        if (!isfinite(w)) { f |= 1; w = 0.0f; }
+        float q = w * x;
+        if (!isfinite(q)) { f |= 2; q = 0.0f; }
+        v = v + q;
+        if (!isfinite(v)) { f |= 2; v = 0.0f; }
+    }
+    if (f) v = 0.0f;
+    int sf = 0;
+    if (shared) {
+        float x = c(k), scale = 1.0f;
+        if (!isfinite(x)) { sf |= 1; x = 0.0f; }
+        if (gated) {
+            float g = weight[k];
+            if (!isfinite(g)) { sf |= 1; g = 0.0f; }
+            scale = 1.0f / (1.0f + moe_expf(-g));
+            if (!isfinite(scale)) { sf |= 2; scale = 0.0f; }
+        }
+        v = v + scale * x;
+        if (!isfinite(v)) { sf |= 2; v = 0.0f; }
+    }
+    flags |= f | sf;
+    return sf ? 0.0f : v;
+}
+
 // -------------------------------------------------------- buffer loads ---
 // Raw buffer loads: a uniform base in a buffer resource (SGPRs), a 32-bit
 // per-lane offset and a uniform SGPR offset.  A wave's row loads then share

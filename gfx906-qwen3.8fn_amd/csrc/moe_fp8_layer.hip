@@ -275,40 +275,6 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     if (flags) atomicOr(a.error, flags);
 }
 
-// y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags
-// of moe_ffn_forward's sum.  c(r): rank r's output, of the routes that count.
-template<class C>
-__device__ __forceinline__ float fold(int k, bool shared, bool gated, const int *valid, const float *weight, C c, int &flags) {
-    int f = 0;
-    float v = 0.0f;
-    for (int r = 0; r < k; ++r) {
-        if (!valid[r]) continue;
-        float x = c(r), w = weight[r];
-        if (!isfinite(x)) { f |= 1; x = 0.0f; }
-        if (!isfinite(w)) { f |= 1; w = 0.0f; }
-        float q = w * x;
-        if (!isfinite(q)) { f |= 2; q = 0.0f; }
-        v = v + q;
-        if (!isfinite(v)) { f |= 2; v = 0.0f; }
-    }
-    if (f) v = 0.0f;
-    int sf = 0;
-    if (shared) {
-        float x = c(k), scale = 1.0f;
-        if (!isfinite(x)) { sf |= 1; x = 0.0f; }
-        if (gated) {
-            float g = weight[k];
-            if (!isfinite(g)) { sf |= 1; g = 0.0f; }
-            scale = 1.0f / (1.0f + moe_expf(-g));
-            if (!isfinite(scale)) { sf |= 2; scale = 0.0f; }
-        }
-        v = v + scale * x;
-        if (!isfinite(v)) { sf |= 2; v = 0.0f; }
-    }
-    flags |= f | sf;
-    return sf ? 0.0f : v;
-}
-
 inline constexpr int kMaxPairs = 33;   // 32 routes and the shared expert
 
 // Route r of token t, by a whole wave: its expert (the shared one for r = k),

@@ -7,109 +7,155 @@
 #include "moe_i8.hpp"
 
 #include <algorithm>
+#include <cstdlib>
 #include <new>
 
 namespace moe {
 namespace {
 
-// The groups' row tiles, in LDS: first[e] = row tiles before group e, row[e] = its
-// first row, both of E + 1 entries.  Offsets outside 0 .. N, or below the one
+// The groups' row tiles, in LDS: group list[p] has the row tiles from first[p] to
+// first[p + 1], and its rows begin at row[e].  Groups of more than one tile come
+// first, with `big` tiles between them.  Offsets outside 0 .. N, or below the one
 // before, are drawn into that range and set bit 1; a group ends where the next
 // begins, and is empty where that is not after its own begin.
-__device__ __forceinline__ int group_tiles(const I8Args &a, int BN, int *first, int *row) {
-    __shared__ int sums[16];
-    __shared__ int total;
-    const int T = blockDim.x, per = (a.experts + T - 1) / T, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int lo = min(a.experts, static_cast<int>(threadIdx.x) * per), hi = min(a.experts, lo + per);
-    int bad = 0, mine = 0;
-    for (int e = lo; e < hi; ++e) {
-        const int from = a.offsets[e], to = a.offsets[e + 1], f = max(0, min(from, a.N)), t = max(0, min(to, a.N));
-        if (f != from || t != to || t < f) bad = 1;
-        row[e] = f;
-        if (e + 1 == a.experts) row[e + 1] = t;
-        first[e] = mine;
-        mine += (max(t - f, 0) + BN - 1) / BN;
-    }
-    int incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int v = __shfl_up(incl, d, 64);
-        if (lane >= d) incl += v;
-    }
-    if (lane == 63) sums[wave] = incl;
-    __syncthreads();
-    int before = incl - mine, all = 0;
-    for (int w = 0; w < T / 64; ++w) {
-        if (w < wave) before += sums[w];
-        all += sums[w];
-    }
-    for (int e = lo; e < hi; ++e) first[e] += before;
-    if (threadIdx.x == 0) {
-        first[a.experts] = all;
-        total = all;
-    }
-    if (bad && blockIdx.x == 0) atomicOr(a.error, 1);
-    __syncthreads();
-    return total;
-}
-// The last group e with first[e] <= t, which is the one that has row tile t: 64
-// lanes look at every `step`-th entry and then at those between.
-__device__ __forceinline__ int group_of(const int *first, int E, int t) {
-    const int lane = threadIdx.x & 63, step = (E + 63) / 64;   // at most 64: E <= 4096
-    int e = lane * step;
-    const int s = __builtin_popcountll(__builtin_amdgcn_ballot_w64(e < E && first[min(e, E - 1)] <= t)) - 1;
-    const int base = __builtin_amdgcn_readfirstlane(s) * step;
-    e = base + lane;
-    const int n = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < step && e < E && first[min(e, E - 1)] <= t)) - 1;
-    return __builtin_amdgcn_readfirstlane(base + n);
-}
+struct GroupTable {
+    int *first, *list, *row;   // [E + 1], [E], [E + 1]
+    int experts, tiles, big;
 
-// Workgroups take (row tile, matrix tile) items in turn; those of one XCD a run of
-// their own, in which the matrix tiles of a row tile follow each other, so that an
-// expert's matrix and its rows come from that XCD's L2 after the first time.
+    static size_t bytes(int experts) { return (static_cast<size_t>(experts) * 3 + 2) * 4; }
+
+    __device__ __forceinline__ GroupTable(const I8Args &a, int BN, int *lds) : experts(a.experts) {
+        __shared__ int sums[16][4];
+        first = lds;
+        row = first + experts + 1;
+        list = row + experts + 1;
+        const int T = blockDim.x, per = (experts + T - 1) / T, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int lo = min(experts, static_cast<int>(threadIdx.x) * per), hi = min(experts, lo + per);
+        int bad = 0, mine[4] = {};   // big groups, their tiles, other groups, their tiles
+        for (int e = lo; e < hi; ++e) {
+            const int from = a.offsets[e], to = a.offsets[e + 1], f = max(0, min(from, a.N)), t = max(0, min(to, a.N));
+            if (f != from || t != to || t < f) bad = 1;
+            row[e] = f;
+            if (e + 1 == experts) row[e + 1] = t;
+            const int n = (max(t - f, 0) + BN - 1) / BN, c = n > 1 ? 0 : 2;
+            mine[c] += 1;
+            mine[c + 1] += n;
+        }
+        int incl[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            incl[c] = mine[c];
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int v = __shfl_up(incl[c], d, 64);
+                if (lane >= d) incl[c] += v;
+            }
+            if (lane == 63) sums[wave][c] = incl[c];
+        }
+        __syncthreads();
+        int all[4] = {};
+        for (int w = 0; w < T / 64; ++w) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (w < wave) incl[c] += sums[w][c];
+                all[c] += sums[w][c];
+            }
+        }
+        int at[2] = {incl[0] - mine[0], all[0] + incl[2] - mine[2]}, tile[2] = {incl[1] - mine[1], all[1] + incl[3] - mine[3]};
+        for (int e = lo; e < hi; ++e) {
+            const int n = (max(row[e + 1] - row[e], 0) + BN - 1) / BN, c = n > 1 ? 0 : 1;
+            list[at[c]] = e;
+            first[at[c]] = tile[c];
+            ++at[c];
+            tile[c] += n;
+        }
+        tiles = __builtin_amdgcn_readfirstlane(all[1] + all[3]);
+        big = __builtin_amdgcn_readfirstlane(all[1]);
+        if (threadIdx.x == 0) first[experts] = tiles;
+        if (bad && blockIdx.x == 0) atomicOr(a.error, 1);
+        __syncthreads();
+    }
+    // The last place p with first[p] <= t, whose group has row tile t: 64 lanes look
+    // at every `step`-th place and then at those between.
+    __device__ __forceinline__ int place(int t) const {
+        const int lane = threadIdx.x & 63, step = (experts + 63) / 64;   // at most 64
+        const auto before = [&](int p, bool in) { return in && p < experts && first[min(p, experts - 1)] <= t; };
+        const int base = (__builtin_popcountll(__builtin_amdgcn_ballot_w64(before(lane * step, true))) - 1) * step;
+        return base + __builtin_popcountll(__builtin_amdgcn_ballot_w64(before(base + lane, lane < step))) - 1;
+    }
+    __device__ __forceinline__ I8Item item(int t, int m0, int BN) const {
+        const int p = __builtin_amdgcn_readfirstlane(place(t)), e = __builtin_amdgcn_readfirstlane(list[p]);
+        const int r = __builtin_amdgcn_readfirstlane(row[e] + (t - first[p]) * BN);
+        return I8Item{e, m0, r, __builtin_amdgcn_readfirstlane(min(BN, row[e + 1] - r)), t >= big};
+    }
+};
+
+// Workgroups take (row tile, matrix tile) items in turn; those of one XCD a share
+// of their own, in which the matrix tiles of a row tile follow each other, so that
+// an expert's matrix and its rows come from that XCD's L2 after the first time.
+// Where there are both, half of an XCD's workgroups begin with the groups of many
+// tiles, whose products keep the matrix cores busy, and the other half with those
+// whose matrices are read for a few rows; each has as many of either.
 template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y>
 __global__ __launch_bounds__(64 * WR * WC) void k_i8_grouped(I8Args a) {
-    using Tile = I8Tile<WR, WC, TM, TN, S, KS>;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[Tile::Lds];
+    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, true>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Stream::Lds];
     extern __shared__ int table[];
-    int *first = table, *row = table + a.experts + 1;
-    const int items = group_tiles(a, Tile::BN, first, row) * a.tiles_m;
-    const int each = (items + 7) / 8, end = min(items, static_cast<int>((blockIdx.x & 7) + 1) * each);
-    int flags = 0;
-    Tile g(lds);
-    for (int i = static_cast<int>(blockIdx.x & 7) * each + static_cast<int>(blockIdx.x >> 3); i < end; i += gridDim.x >> 3) {
-        const int t = i / a.tiles_m, m0 = i % a.tiles_m * Tile::BM;
-        const int e = group_of(first, a.experts, t);
-        const int r = __builtin_amdgcn_readfirstlane((t - first[e]) * Tile::BN + row[e]);
-        const int cols = __builtin_amdgcn_readfirstlane(min(Tile::BN, row[e + 1] - r));
-        g.start(a, e, m0, r, cols, flags);
-        i32x4 acc[TM][TN];
-        g.product(lds, acc);
-        if constexpr (Form == kStoreMiddle) g.store_middle(a, e, m0, r, cols, acc, flags);
-        else g.template store_rows<Y>(a, e, m0, r, cols, acc, lds);
-        if constexpr (Form == kStoreRows && Y != kF32) __syncthreads();   // the results have left the buffers
+    const GroupTable groups(a, Stream::BN, table);
+    const int xcd = static_cast<int>(blockIdx.x & 7), q = static_cast<int>(blockIdx.x >> 3), W = static_cast<int>(gridDim.x >> 3);
+    // The XCD's share of the items of either kind: `big` and `rest` of them.
+    const auto part = [](int n, int x) { return static_cast<int>(static_cast<int64_t>(n) * x / 8); };
+    const int bigs = groups.big * a.tiles_m, rests = groups.tiles * a.tiles_m - bigs;
+    int big0 = part(bigs, xcd), big = part(bigs, xcd + 1) - big0;
+    int rest0 = bigs + part(rests, xcd), rest = bigs + part(rests, xcd + 1) - rest0;
+    // Every other workgroup takes the second half of both kinds, the rest first.
+    int from = q, step = W;
+    bool rest_first = false;
+    if (W > 1 && 8 * big >= rest && 8 * rest >= big) {
+        const int half = q & 1;
+        rest_first = half;
+        from = q >> 1;
+        step = (W + 1 - half) / 2;
+        big0 += half * (big / 2);
+        big = half ? big - big / 2 : big / 2;
+        rest0 += half * (rest / 2);
+        rest = half ? rest - rest / 2 : rest / 2;
     }
-    if (flags) atomicOr(a.error, flags);
+    const auto fetch = [&](int i) {
+        const int j = rest_first ? (i < rest ? rest0 + i : big0 + i - rest) : (i < big ? big0 + i : rest0 + i - big);
+        return groups.item(j / a.tiles_m, j % a.tiles_m * Stream::BM, Stream::BN);
+    };
+    Stream g(a, lds);
+    g.run(from, step, big + rest, fetch,
+          [&](const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) {
+              if constexpr (Form == kStoreMiddle) g.store_middle(it, params, acc);
+              else g.template store_rows<Y>(it, params, acc);
+          });
+    if (g.flags) atomicOr(a.error, g.flags);
 }
 
 template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y>
 hipError_t launch_tile(I8Args a, hipStream_t s) {
-    using Tile = I8Tile<WR, WC, TM, TN, S, KS>;
-    a.tiles_m = (a.M + Tile::BM - 1) / Tile::BM;
-    const size_t lds = static_cast<size_t>(a.experts + 1) * 8;
-    const int resident = std::max(1, static_cast<int>(160 * 1024 / (Tile::Lds + lds + 256)));
-    const size_t items = (static_cast<size_t>(a.N) / Tile::BN + std::min(a.N, a.experts)) * a.tiles_m;   // at most
-    const size_t grid = std::min((items + 7) / 8 * 8, static_cast<size_t>(256) * std::min(resident, 4));
-    k_i8_grouped<WR, WC, TM, TN, S, KS, Form, Y><<<dim3(static_cast<unsigned>(grid)), dim3(64 * Tile::W), lds, s>>>(a);
+    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, true>;
+    a.tiles_m = (a.rows + Stream::BM - 1) / Stream::BM;
+    const size_t lds = GroupTable::bytes(a.experts);
+    const int resident = std::max(1, static_cast<int>(160 * 1024 / (Stream::Lds + lds + 256)));
+    const size_t items = (static_cast<size_t>(a.N) / Stream::BN + std::min(a.N, a.experts)) * a.tiles_m;   // at most
+    const size_t grid = std::min((items + 7) / 8 * 8, static_cast<size_t>(256) * std::min(resident, 8));
+    k_i8_grouped<WR, WC, TM, TN, S, KS, Form, Y><<<dim3(static_cast<unsigned>(grid)), dim3(64 * Stream::W), lds, s>>>(a);
     return hipGetLastError();
 }
 
 template<int Form, int Y>
 hipError_t launch_grouped(const I8Args &a, hipStream_t s) {
     const int mean = a.N / a.experts;
-    if (mean <= 12) return launch_tile<4, 1, 2, 1, 3, 4, Form, Y>(a, s);
-    if (mean <= 64) return launch_tile<2, 2, 2, 2, 3, 2, Form, Y>(a, s);
-    return launch_tile<2, 2, 4, 4, 4, 1, Form, Y>(a, s);
+    if (mean <= 2) {
+        if constexpr (Form == kStoreMiddle) return launch_tile<2, 1, 2, 1, 4, 2, Form, Y>(a, s);
+        else return launch_tile<4, 1, 1, 1, 4, 4, Form, Y>(a, s);
+    }
+    if (mean <= 10) return launch_tile<4, 1, 2, 2, 4, 2, Form, Y>(a, s);
+    if (mean <= 64) return launch_tile<4, 1, 2, 4, 4, 1, Form, Y>(a, s);
+    return launch_tile<4, 2, 4, 4, 4, 1, Form, Y>(a, s);
 }
 
 hipError_t launch_grouped_rows(const I8Args &a, int y_type, hipStream_t s) {
@@ -118,42 +164,247 @@ hipError_t launch_grouped_rows(const I8Args &a, int y_type, hipStream_t s) {
     return launch_grouped<kStoreRows, kF16>(a, s);
 }
 
-// y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags of
-// moe_ffn_forward's sum, rounded once; four elements a thread.  c: grouped rows.
+// ------------------------------------------------------------- grouping ---
+// Rows of the product ("pairs" of a token and one of its ranks) grouped by expert,
+// the shared expert's behind the last.  Their order within a group is that in
+// which LDS counted them, which nothing depends on: a row's result is the same
+// wherever it stands, and the sum finds it by its place.
+struct I8Groups {
+    int32_t *offsets;   // [E' + 1]
+    int32_t *token;     // [pairs]: token of a place
+    int32_t *place;     // [tokens * k]: place of a route; -1: dropped
+    int32_t *counts;    // [blocks][E']: routes of a block of tokens, for batches of many
+};
+struct I8GroupArgs {
+    const int32_t *ids;
+    const float *weights;
+    I8Groups g;
+    int tokens, k, E, Ep;
+    int per, blocks;    // tokens of a block, blocks
+    int *error;
+};
+inline constexpr int kGroupThreads = 256;
+
+// The routes of tokens t0 .. t0 + n - 1, as they stand in sid (LDS): each one's
+// number among the block's of its expert, or -1 for a bad id or an id of an earlier
+// rank, to local(i, number); counts (LDS, zeroed) get the experts' numbers.
+template<class Local>
+__device__ __forceinline__ void count_routes(const I8GroupArgs &a, int t0, int n, int32_t *sid, int32_t *counts, const Local &local) {
+    const size_t at = static_cast<size_t>(t0) * a.k;
+    int flags = 0;
+    for (int e = threadIdx.x; e < a.Ep; e += kGroupThreads) counts[e] = 0;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n * a.k; i += kGroupThreads) {
+        sid[i] = a.ids[at + i];
+        const float w = a.weights[at + i];
+        if (!isfinite(w) || w < 0.0f) flags |= 1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * a.k; i += kGroupThreads) {
+        const int r = i % a.k, e = sid[i];
+        bool valid = e >= 0 && e < a.E;
+        for (int q = 1; q <= r; ++q) valid &= sid[i - q] != e;
+        if (!valid) flags |= 1;
+        local(i, valid ? atomicAdd(&counts[e], 1) : -1);
+    }
+    if (flags) atomicOr(a.error, flags);
+}
+// Exclusive sums over the experts' numbers n(e); base(e, sum) takes them, and the
+// offsets are written by `writer`.
+template<class Number, class Base>
+__device__ __forceinline__ void scan_experts(const I8GroupArgs &a, bool writer, const Number &number, const Base &base) {
+    __shared__ int sums[kGroupThreads / 64];
+    const int per = (a.Ep + kGroupThreads - 1) / kGroupThreads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lo = min(a.Ep, static_cast<int>(threadIdx.x) * per), hi = min(a.Ep, lo + per);
+    int mine = 0;
+    for (int e = lo; e < hi; ++e) mine += number(e);
+    int incl = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int v = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += v;
+    }
+    if (lane == 63) sums[wave] = incl;
+    __syncthreads();
+    int run = incl - mine;
+    for (int w = 0; w < wave; ++w) run += sums[w];
+    for (int e = lo; e < hi; ++e) {
+        const int n = number(e);
+        base(e, run);
+        if (writer) a.g.offsets[e] = run;
+        run += n;
+        if (writer && e + 1 == a.Ep) a.g.offsets[a.Ep] = run;
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void place_route(const I8GroupArgs &a, int i, int place) {
+    a.g.place[i] = place;
+    if (place >= 0) a.g.token[place] = i / a.k;
+}
+
+// Up to kSmallRoutes routes: the first workgroup groups them, the others quantise x.
+inline constexpr int kSmallRoutes = 2048;
+template<int T, int L, int V>
+__global__ __launch_bounds__(kGroupThreads) void k_i8_prepare_small(I8GroupArgs a, I8Rows x) {
+    extern __shared__ int32_t group_lds[];
+    if (blockIdx.x > 0) {
+        quantize_rows<T, L, V>(x, blockIdx.x - 1);
+        return;
+    }
+    int32_t *sid = group_lds, *counts = sid + a.tokens * a.k;
+    int number[kSmallRoutes / kGroupThreads];
+#pragma unroll
+    for (int j = 0; j < kSmallRoutes / kGroupThreads; ++j) number[j] = -1;
+    count_routes(a, 0, a.tokens, sid, counts, [&](int i, int n) {
+#pragma unroll
+        for (int j = 0; j < kSmallRoutes / kGroupThreads; ++j)
+            if (i / kGroupThreads == j) number[j] = n;
+    });
+    __syncthreads();
+    scan_experts(a, true, [&](int e) { return e < a.E ? counts[e] : a.tokens; }, [&](int e, int run) { counts[e] = run; });
+#pragma unroll
+    for (int j = 0; j < kSmallRoutes / kGroupThreads; ++j) {
+        const int i = j * kGroupThreads + threadIdx.x;
+        if (i < a.tokens * a.k) place_route(a, i, number[j] < 0 ? -1 : counts[sid[i]] + number[j]);
+    }
+    if (a.Ep > a.E)
+        for (int t = threadIdx.x; t < a.tokens; t += kGroupThreads) a.g.token[counts[a.E] + t] = t;
+}
+
+// More routes: blocks of tokens count theirs (place holds a route's number in its
+// block) beside the workgroups that quantise x; then each block sums up the counts
+// of those before it.
+template<int T, int L, int V>
+__global__ __launch_bounds__(kGroupThreads) void k_i8_count(I8GroupArgs a, I8Rows x) {
+    extern __shared__ int32_t group_lds[];
+    if (static_cast<int>(blockIdx.x) >= a.blocks) {
+        quantize_rows<T, L, V>(x, blockIdx.x - a.blocks);
+        return;
+    }
+    const int t0 = blockIdx.x * a.per, n = min(a.per, a.tokens - t0);
+    int32_t *counts = group_lds, *sid = counts + a.Ep;
+    count_routes(a, t0, n, sid, counts, [&](int i, int number) { a.g.place[static_cast<size_t>(t0) * a.k + i] = number; });
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += kGroupThreads) a.g.counts[static_cast<size_t>(blockIdx.x) * a.Ep + e] = counts[e];
+}
+__global__ __launch_bounds__(kGroupThreads) void k_i8_place(I8GroupArgs a) {
+    extern __shared__ int32_t group_lds[];
+    int32_t *all = group_lds, *before = all + a.Ep;
+    for (int e = threadIdx.x; e < a.Ep; e += kGroupThreads) {
+        int n = 0, b = 0;
+        if (e < a.E) {
+#pragma unroll 8
+            for (int j = 0; j < a.blocks; ++j) {
+                const int c = a.g.counts[static_cast<size_t>(j) * a.Ep + e];
+                n += c;
+                if (j < static_cast<int>(blockIdx.x)) b += c;
+            }
+        } else {
+            n = a.tokens;
+        }
+        all[e] = n;
+        before[e] = b;
+    }
+    __syncthreads();
+    scan_experts(a, blockIdx.x == 0, [&](int e) { return all[e]; }, [&](int e, int run) { before[e] += run; });
+    const int t0 = blockIdx.x * a.per, n = min(a.per, a.tokens - t0);
+    const size_t at = static_cast<size_t>(t0) * a.k;
+    for (int i = threadIdx.x; i < n * a.k; i += kGroupThreads) {
+        const int number = a.g.place[at + i];
+        if (number >= 0) place_route(a, static_cast<int>(at) + i, before[a.ids[at + i]] + number);
+    }
+    if (a.Ep > a.E)
+        for (int i = threadIdx.x; i < n; i += kGroupThreads) a.g.token[before[a.E] + t0 + i] = t0 + i;
+}
+
+hipError_t launch_prepare_i8(I8GroupArgs a, const I8Rows &x, int type, hipStream_t s) {
+    const bool small = a.tokens * a.k <= kSmallRoutes;
+    a.per = small ? a.tokens : std::max(64, (a.tokens + 127) / 128);
+    a.blocks = (a.tokens + a.per - 1) / a.per;
+    const size_t lds = (static_cast<size_t>(a.per) * a.k + a.Ep) * 4;
+    with_quantizer(type, x.width, [&](auto t, auto l, auto v) {
+        const dim3 grid(a.blocks + quantize_blocks(x.rows, l)), block(kGroupThreads);
+        if (small) k_i8_prepare_small<t, l, v><<<grid, block, lds, s>>>(a, x);
+        else k_i8_count<t, l, v><<<grid, block, lds, s>>>(a, x);
+    });
+    hipError_t r = hipGetLastError();
+    if (r != hipSuccess || small) return r;
+    k_i8_place<<<dim3(a.blocks), dim3(kGroupThreads), static_cast<size_t>(a.Ep) * 8, s>>>(a);
+    return hipGetLastError();
+}
+
+// ------------------------------------------------------------------- sums ---
 struct I8FoldArgs {
-    const float *c;            // [pairs][H]
-    const int32_t *pos_of;     // [tokens * k] row of c, -1 for a route that was dropped
-    const int32_t *offsets;    // [E + 2]; the shared expert's rows begin at offsets[E]
+    const void *c;             // [pairs][H] outputs of the experts: fp32, or fp16 as k_i8_expert_scale says
+    const float *c_scale;      // fp16: [pairs] scales of the rows
+    const float *expert_scale; // fp16: [E'] scales of the experts
+    const int32_t *ids;
+    I8Groups g;
     const float *weights, *shared_gate;
     void *y;
     int tokens, H, k, E, shared;
     int *error;
 };
-template<int T>
+// fp16 for the experts' outputs, where y is bf16: half the bytes of the largest
+// tensor of a long prompt.  An output is (whole number) * sw[m] * sx; what is stored
+// is (whole number) * sw[m] * 2^p with the largest p that keeps 127 * 128 * I *
+// max |sw| of its expert within fp16, and the sum multiplies by sx * 2^-p in fp32.
+// So nothing overflows, and a value is off by at most 2^-11 of itself down to
+// 2^-30 of that bound, an eighth of what y's own rounding may cost.
+// One workgroup an expert: scale = 2^-p.
+__global__ __launch_bounds__(256) void k_i8_expert_scale(const float *sw, float *scale, int rows, int M, int I) {
+    __shared__ uint32_t most[4];
+    const float *s = sw + static_cast<size_t>(blockIdx.x) * rows;
+    uint32_t m = 0;
+    for (int i = threadIdx.x; i < M; i += 256)
+        if (isfinite(s[i])) m = max(m, magnitude(s[i]));
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = max(max(most[0], most[1]), max(most[2], most[3]));
+    // max |sw| < 2^e, and 127 * 128 * I < 2^q: within fp16 where 2^(e + q + p) <= 2^15.
+    const int e = m ? static_cast<int>(m >> 23) - 126 : 0, q = 14 + 32 - __builtin_clz(I);
+    if (threadIdx.x == 0) scale[blockIdx.x] = ldexpf(1.0f, m ? min(max(e + q - 15, -100), 100) : 0);
+}
+
+// y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags of
+// moe_ffn_forward's sum, rounded once; four elements a thread.
+template<int T, bool Halves>
 __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
     const size_t i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
     if (i >= static_cast<size_t>(a.tokens) * a.H) return;
     const size_t t = i / a.H, h = i % a.H;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    const auto load = [&](size_t row) { return __builtin_nontemporal_load(reinterpret_cast<const f4 *>(a.c + row * a.H + h)); };
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    using Row = std::conditional_t<Halves, h4, f4>;
+    using Value = std::conditional_t<Halves, _Float16, float>;
+    const auto load = [&](size_t row) {
+        return __builtin_nontemporal_load(reinterpret_cast<const Row *>(static_cast<const Value *>(a.c) + row * a.H + h));
+    };
     int flags[4] = {};
     float v[4] = {};
     for (int r0 = 0; r0 < a.k; r0 += 8) {
-        f4 x[8];
-        float w[8];
-        int pos[8];
+        Row x[8];
+        float w[8], scale[8];
+        int place[8];
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            pos[q] = r0 + q < a.k ? a.pos_of[t * a.k + r0 + q] : -1;
-            if (pos[q] >= 0) x[q] = load(pos[q]);
-            w[q] = r0 + q < a.k ? a.weights[t * a.k + r0 + q] : 0.0f;
+            const size_t route = t * a.k + r0 + q;
+            place[q] = r0 + q < a.k ? a.g.place[route] : -1;
+            scale[q] = 1.0f;
+            if (place[q] >= 0) {
+                x[q] = load(place[q]);
+                if constexpr (Halves) scale[q] = a.c_scale[place[q]] * a.expert_scale[a.ids[route]];
+            }
+            w[q] = r0 + q < a.k ? a.weights[route] : 0.0f;
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) {
-            if (pos[q] < 0) continue;
+            if (place[q] < 0) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                float c = x[q][e], s = w[q];
+                float c = static_cast<float>(x[q][e]), s = w[q];
+                if constexpr (Halves) c = c * scale[q];
                 if (!isfinite(c)) { flags[e] |= 1; c = 0.0f; }
                 if (!isfinite(s)) { flags[e] |= 1; s = 0.0f; }
                 float p = s * c;
@@ -164,16 +415,18 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
         }
     }
     int any = 0;
-    f4 sx = {0.0f, 0.0f, 0.0f, 0.0f};
-    float scale = 1.0f;
+    Row sx = {};
+    float scale = 1.0f, gate = 1.0f;
     int gate_flags = 0;
     if (a.shared) {
-        sx = load(a.offsets[a.E] + t);
+        const size_t row = a.g.offsets[a.E] + t;
+        sx = load(row);
+        if constexpr (Halves) scale = a.c_scale[row] * a.expert_scale[a.E];
         if (a.shared_gate) {
             float g = a.shared_gate[t];
             if (!isfinite(g)) { gate_flags |= 1; g = 0.0f; }
-            scale = 1.0f / (1.0f + moe_expf(-g));
-            if (!isfinite(scale)) { gate_flags |= 2; scale = 0.0f; }
+            gate = 1.0f / (1.0f + moe_expf(-g));
+            if (!isfinite(gate)) { gate_flags |= 2; gate = 0.0f; }
         }
     }
 #pragma unroll
@@ -182,9 +435,10 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
         int sf = 0;
         if (a.shared) {
             sf = gate_flags;
-            float c = sx[e];
+            float c = static_cast<float>(sx[e]);
+            if constexpr (Halves) c = c * scale;
             if (!isfinite(c)) { sf |= 1; c = 0.0f; }
-            v[e] = v[e] + scale * c;
+            v[e] = v[e] + gate * c;
             if (!isfinite(v[e])) { sf |= 2; v[e] = 0.0f; }
             if (sf) v[e] = 0.0f;
         }
@@ -194,14 +448,145 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
     if (any) atomicOr(a.error, any);
 }
 
+// ------------------------------------- few tokens: down and the sum in one ---
+// Workgroup (t, slice of `tiles` tiles of 16 rows); wave w takes ranks w, w + W, ..
+// It quantises the rank's middle row into LDS in pieces of eight chunks and streams
+// the expert's tiles past it, a tile's chunks of a piece at a time with the next
+// tile's on their way.  All 16 columns of its MFMA hold the one token.
+struct I8DownArgs {
+    const uint8_t *blocks;     // [E'][H / 64][chunks]
+    const float *sw;           // [E'][rows]
+    const float *middle;       // [pairs][I]
+    const int32_t *ids;
+    I8Groups g;
+    const float *weights, *shared_gate;
+    void *y;
+    int T, H, I, E, k, P1;     // P1 = k + shared
+    int rows, chunks;
+    int *error;
+};
+inline constexpr int kDownPiece = 8, kDownTiles = 16, kDownPairs = 33;
+template<int Y>
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void k_i8_down_fold(I8DownArgs a, int tiles) {
+    extern __shared__ __attribute__((aligned(16))) int part[];   // [rank][16 tiles]: sums, then outputs
+    __shared__ __attribute__((aligned(16))) uint8_t codes[16][kDownPiece * kI8Chunk];
+    __shared__ float weight[kDownPairs];
+    __shared__ int valid[kDownPairs];
+    const int R = 16 * tiles;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = blockDim.x >> 6;
+    // Workgroup i runs on XCD i % 8: all tokens of one slice on one XCD, one after the
+    // other, so that experts they share come from its L2.
+    const int row_tiles = a.rows / 16, S = (row_tiles + tiles - 1) / tiles;
+    const int j = blockIdx.x >> 3, t = j % a.T, s = (blockIdx.x & 7) + 8 * (j / a.T);
+    if (s >= S) return;
+    const int tile0 = s * tiles, here = min(tiles, row_tiles - tile0);
+    for (int r = wave; r < a.P1; r += W) {
+        const int place = r < a.k ? a.g.place[t * a.k + r] : a.g.offsets[a.E] + t;
+        const int e = r < a.k ? a.ids[t * a.k + r] : a.E;
+        if (lane == 0) {
+            weight[r] = r < a.k ? a.weights[t * a.k + r] : a.shared_gate ? a.shared_gate[t] : 1.0f;
+            valid[r] = place >= 0;
+        }
+        const int at = __builtin_amdgcn_readfirstlane(place), expert = __builtin_amdgcn_readfirstlane(e);
+        if (at < 0) continue;
+        const float *mid = a.middle + static_cast<size_t>(at) * a.I;
+        const uint8_t *w = a.blocks + static_cast<size_t>(expert) * a.rows / kI8Block * a.chunks * kI8BlockBytes;
+        const float *sw = a.sw + static_cast<size_t>(expert) * a.rows;
+        uint4 f[2][kDownPiece];
+        // Tile n's chunks k0 .. + kb - 1.
+        const auto load = [&](int n, int k0, int kb, uint4 (&to)[kDownPiece]) {
+            const int tile = tile0 + min(n, here - 1);
+            const uint4 *p = reinterpret_cast<const uint4 *>(w + (static_cast<size_t>(tile >> 2) * a.chunks + k0) * kI8BlockBytes + (tile & 3) * 1024) + lane;
+#pragma unroll
+            for (int u = 0; u < kDownPiece; ++u) to[u] = p[min(u, kb - 1) * (kI8BlockBytes / 16)];   // past the piece: the last again, not used
+        };
+        load(0, 0, min(kDownPiece, a.chunks), f[0]);
+        uint32_t m = 0;
+        for (int c = lane * 8; c < a.I; c += 512) {
+            float v[8];
+            unpack8<kF32>(load8_raw<kF32>(mid, c), v);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) m = max(m, magnitude(v[q]));
+        }
+        const GroupScale scale = row_scale(wave_max(m));
+        for (int k0 = 0; k0 < a.chunks; k0 += kDownPiece) {
+            const int kb = min(kDownPiece, a.chunks - k0), col = k0 * kI8Chunk + lane * 8;
+            if (k0 > 0) load(0, k0, kb, f[0]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // the last piece's reads are done
+            Raw8 raw{};
+            if (col < a.I) raw = load8_raw<kF32>(mid, col);
+            float v[8];
+            unpack8<kF32>(raw, v);
+            *reinterpret_cast<uint2 *>(&codes[wave][lane * 8]) = quantize8_i8(v, scale);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            uint4 x[kDownPiece];
+#pragma unroll
+            for (int u = 0; u < kDownPiece; ++u) x[u] = *reinterpret_cast<const uint4 *>(&codes[wave][u * kI8Chunk + (lane >> 4) * 16]);
+            const auto multiply = [&](int n, const uint4 (&from)[kDownPiece]) {
+                // Lanes 16 g .. + 15 have rows 16 g + 4 i + q of tile i's block.
+                const int tile = tile0 + n, row = n * 16 + (lane >> 4) * 4;
+                i32x4 *out = reinterpret_cast<i32x4 *>(&part[r * R + row]);
+                i32x4 acc = k0 > 0 ? *out : i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int u = 0; u < kDownPiece; ++u)
+                    if (u < kb) acc = i8_dot(from[u], x[u], acc);
+                if (k0 + kDownPiece >= a.chunks) {
+                    const float *c = sw + (tile >> 2) * kI8Block + (lane >> 4) * 16 + (tile & 3) * 4;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) acc[q] = __float_as_int(static_cast<float>(acc[q]) * (scale.s * c[q]));
+                }
+                if ((lane & 15) == 0) *out = acc;
+            };
+            for (int n = 0; n < here; n += 2) {
+                load(n + 1, k0, kb, f[1]);
+                multiply(n, f[0]);
+                if (n + 1 >= here) break;
+                load(n + 2, k0, kb, f[0]);
+                multiply(n + 1, f[1]);
+            }
+        }
+    }
+    __syncthreads();
+    int flags = 0;
+    for (int i = threadIdx.x; i < here * 16; i += blockDim.x) {
+        const int tile = tile0 + (i >> 4), row = (tile >> 2) * kI8Block + (i >> 2 & 3) * 16 + (tile & 3) * 4 + (i & 3);
+        if (row >= a.H) continue;
+        const float v = fold(a.k, a.P1 > a.k, a.shared_gate != nullptr, valid, weight, [&](int r) { return __int_as_float(part[r * R + i]); }, flags);
+        store1<Y>(a.y, static_cast<size_t>(t) * a.H + row, v);
+    }
+    if (flags) atomicOr(a.error, flags);
+}
+
+hipError_t launch_down_fold(const I8DownArgs &a, int type, hipStream_t s) {
+    const int row_tiles = a.rows / 16;
+    // Row tiles a workgroup: the fewest on the busiest CU, and of such choices one
+    // workgroup a CU for few tokens, two (which fit at once) for more.
+    int tiles = 1, best = 1 << 30, best_off = 0;
+    for (int n = 1; n <= kDownTiles; ++n) {
+        const int rounds = (a.T * ((row_tiles + n - 1) / n) + 255) / 256, off = std::abs(rounds - (a.T <= 8 ? 1 : 2));
+        if (rounds * n < best || (rounds * n == best && off < best_off)) {
+            tiles = n;
+            best = rounds * n;
+            best_off = off;
+        }
+    }
+    const dim3 grid(static_cast<unsigned>((row_tiles + tiles - 1) / tiles + 7) / 8 * 8 * a.T), block(64 * std::min(16, a.P1));
+    const size_t lds = static_cast<size_t>(a.P1) * tiles * 64;
+    if (type == kF32) k_i8_down_fold<kF32><<<grid, block, lds, s>>>(a, tiles);
+    else if (type == kBF16) k_i8_down_fold<kBF16><<<grid, block, lds, s>>>(a, tiles);
+    else k_i8_down_fold<kF16><<<grid, block, lds, s>>>(a, tiles);
+    return hipGetLastError();
+}
+
 }  // namespace
 }  // namespace moe
 
 // ------------------------------------------------------------------ C ABI ---
 struct moe_i8_bank {
     int experts = 0, input = 0, output = 0, device = 0;
-    uint8_t *mem = nullptr;   // tiles, scales
-    const float *scales = nullptr;
+    uint8_t *mem = nullptr;   // blocks, scales
+    float *scales = nullptr;
 };
 
 struct moe_i8_layer {
@@ -214,9 +599,11 @@ struct moe_i8_layer {
     int64_t x_pitch = 0, m_pitch = 0;
     int8_t *x = nullptr, *m = nullptr;             // quantised rows of x and of the middle
     float *x_s = nullptr, *m_s = nullptr;
-    float *middle = nullptr, *contrib = nullptr;   // [pairs][I], [pairs][H]
+    float *middle = nullptr;                       // [pairs][I]
+    void *contrib = nullptr;                       // [pairs][H]
+    float *expert_scale = nullptr;                 // [E']
     int *dropped = nullptr;                        // flags of rows that are not used
-    moe::RouteOut routes{};
+    moe::I8Groups groups{};
 };
 
 namespace {
@@ -227,16 +614,31 @@ bool aligned(const void *p, size_t a) { return p && reinterpret_cast<uintptr_t>(
 size_t round_up(size_t v, size_t m) { return (v + m - 1) / m * m; }
 bool is_type(int t) { return t == MOE_F32 || t == MOE_BF16 || t == MOE_F16; }
 int64_t odd_pitch(int width) { return static_cast<int64_t>(moe::i8_chunks(width) | 1) * moe::kI8Chunk; }
-size_t tile_bytes(int rows, int cols) { return static_cast<size_t>((rows + 15) / 16) * moe::i8_chunks(cols) * moe::kI8TileBytes; }
+size_t block_bytes(int rows, int cols) { return static_cast<size_t>(moe::i8_rows(rows)) * moe::i8_chunks(cols) * moe::kI8Chunk; }
 
-// `count` matrices of codes on the host or the device into tiles at `to`.
-hipError_t upload(const void *codes, uint8_t *to, size_t count, int rows, int cols, bool pairs, int shift, bool on_device) {
-    if (on_device) return moe::launch_i8_repack(static_cast<const int8_t *>(codes), to, count, rows, cols, pairs, shift, nullptr);
-    void *staging = nullptr;
+// `count` matrices on the host or the device into blocks and scales.
+hipError_t upload(const moe_i8_matrix &m, uint8_t *to, float *scales, size_t count, int rows, int cols, int part, bool on_device) {
     const size_t bytes = count * rows * cols;
-    hipError_t r = hipMalloc(&staging, bytes);
-    if (r == hipSuccess) r = hipMemcpy(staging, codes, bytes, hipMemcpyHostToDevice);
-    if (r == hipSuccess) r = moe::launch_i8_repack(static_cast<const int8_t *>(staging), to, count, rows, cols, pairs, shift, nullptr);
+    const int8_t *codes = static_cast<const int8_t *>(m.codes);
+    void *staging = nullptr;
+    hipError_t r = hipSuccess;
+    if (!on_device) {
+        if ((r = hipMalloc(&staging, bytes)) != hipSuccess) return r;
+        r = hipMemcpy(staging, m.codes, bytes, hipMemcpyHostToDevice);
+        codes = static_cast<const int8_t *>(staging);
+    }
+    if (r == hipSuccess) r = moe::launch_i8_repack(codes, to, count, rows, cols, part, nullptr);
+    const hipMemcpyKind kind = on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+    const size_t width = static_cast<size_t>(rows) * 4, padded = static_cast<size_t>(moe::i8_rows(rows)) * 4;
+    if (part == moe::kI8Whole) {
+        if (r == hipSuccess) r = hipMemcpy2D(scales, padded, m.scales, width, width, count, kind);
+    } else if (rows % 64 == 0) {
+        // 64 of gate, 64 of up in turn.
+        if (r == hipSuccess) r = hipMemcpy2D(scales + part * 64, 512, m.scales, 256, 256, count * (rows / 64), kind);
+    } else {
+        for (int at = 0; at < rows && r == hipSuccess; at += 64)
+            r = hipMemcpy2D(scales + at * 2 + part * 64, 2 * padded, m.scales + at, width, std::min(64, rows - at) * 4, count, kind);
+    }
     if (r == hipSuccess) r = hipDeviceSynchronize();
     if (staging) (void)hipFree(staging);
     return r;
@@ -249,10 +651,11 @@ bool valid_config(const moe_i8_layer_config *c) {
            c->max_tokens <= 65536;
 }
 
+inline constexpr int kFewTokens = 32;   // tokens up to which down and the sum are one launch
+
 struct LayerLayout {
     size_t gate_up, down, gate_up_s, down_s, weights;   // offsets and end of the weights
-    size_t x, x_s, m, m_s, middle, contrib, counts, offsets, token, rank, pos, stream_items, mfma_items, item_counts, dropped, bitmap,
-        prefix, workspace;
+    size_t x, x_s, m, m_s, middle, contrib, offsets, token, place, counts, expert_scale, dropped, workspace;
 };
 LayerLayout layout(const moe_i8_layer_config &c) {
     LayerLayout l{};
@@ -263,11 +666,11 @@ LayerLayout layout(const moe_i8_layer_config &c) {
         return here;
     };
     const size_t H = c.hidden, I = c.intermediate, Ep = static_cast<size_t>(c.experts) + c.has_shared, T = c.max_tokens;
-    const size_t P = T * (c.top_k + c.has_shared), W = (T + 31) / 32;
-    l.gate_up = take(Ep * 2 * tile_bytes(c.intermediate, c.hidden));
-    l.down = take(Ep * tile_bytes(c.hidden, c.intermediate));
-    l.gate_up_s = take(Ep * 2 * I * 4);
-    l.down_s = take(Ep * H * 4);
+    const size_t P = T * (c.top_k + c.has_shared);
+    l.gate_up = take(Ep * 2 * block_bytes(c.intermediate, c.hidden));
+    l.down = take(Ep * block_bytes(c.hidden, c.intermediate));
+    l.gate_up_s = take(Ep * 2 * moe::i8_rows(c.intermediate) * 4);
+    l.down_s = take(Ep * moe::i8_rows(c.hidden) * 4);
     l.weights = at;
     at = 0;
     l.x = take(T * odd_pitch(c.hidden));
@@ -276,17 +679,12 @@ LayerLayout layout(const moe_i8_layer_config &c) {
     l.m_s = take(P * 4);
     l.middle = take(P * I * 4);
     l.contrib = take(P * H * 4);
-    l.counts = take(Ep * 4);
     l.offsets = take((Ep + 1) * 4);
     l.token = take(P * 4);
-    l.rank = take(P * 4);
-    l.pos = take(T * c.top_k * 4);
-    l.stream_items = take(sizeof(moe::Item));
-    l.mfma_items = take((P / moe::kMfmaTile + std::min(P, Ep)) * sizeof(moe::Item));
-    l.item_counts = take(16);
+    l.place = take(T * c.top_k * 4);
+    l.counts = take(std::min<size_t>(128, (T + 63) / 64) * Ep * 4);
+    l.expert_scale = take(Ep * 4);
     l.dropped = take(4);
-    l.bitmap = take(W * Ep * 4);
-    l.prefix = take(W * Ep * 4);
     l.workspace = at;
     return l;
 }
@@ -320,16 +718,14 @@ int moe_i8_bank_create(int experts, int input, int output, const void *codes, co
     B->input = input;
     B->output = output;
     B->device = device;
-    const size_t scale_at = round_up(tile_bytes(output, input) * experts, 256), scale_bytes = static_cast<size_t>(experts) * output * 4;
+    const size_t scale_at = block_bytes(output, input) * experts, scale_bytes = static_cast<size_t>(experts) * moe::i8_rows(output) * 4;
     // Weights that another stream is still writing are complete after this.
     hipError_t r = hipDeviceSynchronize();
     if (r == hipSuccess) r = hipMalloc(&B->mem, scale_at + scale_bytes);
-    if (r == hipSuccess) r = upload(codes, B->mem, experts, output, input, false, 0, weights_on_device != 0);
+    B->scales = reinterpret_cast<float *>(B->mem + scale_at);
     if (r == hipSuccess)
-        r = hipMemcpy(B->mem + scale_at, scales, scale_bytes, weights_on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice);
-    if (r == hipSuccess) r = hipDeviceSynchronize();
+        r = upload(moe_i8_matrix{codes, scales}, B->mem, B->scales, experts, output, input, moe::kI8Whole, weights_on_device != 0);
     if (r != hipSuccess) { release(B); return r; }
-    B->scales = reinterpret_cast<const float *>(B->mem + scale_at);
     *out = B;
     return 0;
 }
@@ -358,7 +754,7 @@ int moe_i8_bank_forward(moe_i8_bank *B, const void *x_codes, const float *x_scal
     moe::DeviceScope device(B->device);
     if (!device.ok()) return hipErrorInvalidDevice;
     moe::I8Args a{};
-    a.tiles = B->mem;
+    a.blocks = B->mem;
     a.sw = B->scales;
     a.x = static_cast<const int8_t *>(x_codes);
     a.sx = x_scales;
@@ -370,6 +766,7 @@ int moe_i8_bank_forward(moe_i8_bank *B, const void *x_codes, const float *x_scal
     a.y = y;
     a.y_stride = y_stride;
     a.M = B->output;
+    a.rows = moe::i8_rows(B->output);
     a.N = rows;
     a.K = B->input;
     a.chunks = moe::i8_chunks(B->input);
@@ -405,48 +802,41 @@ int moe_i8_layer_create(const moe_i8_layer_config *c, const moe_i8_matrix *exper
     const LayerLayout l = layout(*c);
     const bool on_device = weights_on_device != 0;
     const int H = c->hidden, I = c->intermediate;
-    const size_t E = c->experts, one = tile_bytes(I, H), half = static_cast<size_t>(I) * 4;
-    const hipMemcpyKind kind = on_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice;
+    const size_t E = c->experts;
     // Weights that another stream is still writing are complete after this.
     hipError_t r = hipDeviceSynchronize();
     if (r == hipSuccess) r = hipMalloc(&L->mem, l.weights);
     if (r == hipSuccess) r = hipMalloc(&L->ws, l.workspace);
     const auto bank = [&](const moe_i8_matrix *m, size_t at, size_t count) {
-        for (int i = 0; i < 2 && r == hipSuccess; ++i) {
-            r = upload(m[i].codes, L->mem + l.gate_up + at * 2 * one, count, I, H, true, i, on_device);
-            // Scales in the order of the rows: 16 of gate, 16 of up.
-            if (r == hipSuccess)
-                r = hipMemcpy2D(L->mem + l.gate_up_s + at * 2 * half + i * 64, 128, m[i].scales, 64, 64, count * (I / 16), kind);
-        }
-        if (r == hipSuccess) r = upload(m[2].codes, L->mem + l.down + at * tile_bytes(H, I), count, H, I, false, 0, on_device);
-        if (r == hipSuccess) r = hipMemcpy(L->mem + l.down_s + at * H * 4, m[2].scales, count * H * 4, kind);
+        uint8_t *gate_up = L->mem + l.gate_up + at * 2 * block_bytes(I, H), *down = L->mem + l.down + at * block_bytes(H, I);
+        float *gate_up_s = reinterpret_cast<float *>(L->mem + l.gate_up_s) + at * 2 * moe::i8_rows(I);
+        float *down_s = reinterpret_cast<float *>(L->mem + l.down_s) + at * moe::i8_rows(H);
+        if (r == hipSuccess) r = upload(m[0], gate_up, gate_up_s, count, I, H, moe::kI8Gate, on_device);
+        if (r == hipSuccess) r = upload(m[1], gate_up, gate_up_s, count, I, H, moe::kI8Up, on_device);
+        if (r == hipSuccess) r = upload(m[2], down, down_s, count, H, I, moe::kI8Whole, on_device);
     };
     if (r == hipSuccess) bank(experts, 0, E);
     if (r == hipSuccess && c->has_shared) bank(shared, E, 1);
-    if (r == hipSuccess) r = hipDeviceSynchronize();
+    if (r == hipSuccess) {
+        moe::k_i8_expert_scale<<<dim3(static_cast<unsigned>(E) + c->has_shared), dim3(256)>>>(
+            reinterpret_cast<const float *>(L->mem + l.down_s), reinterpret_cast<float *>(L->ws + l.expert_scale), moe::i8_rows(H), H, I);
+        r = hipDeviceSynchronize();
+    }
     if (r != hipSuccess) { release(L); return r; }
     L->gate_up = L->mem + l.gate_up;
     L->down = L->mem + l.down;
     L->gate_up_s = reinterpret_cast<const float *>(L->mem + l.gate_up_s);
     L->down_s = reinterpret_cast<const float *>(L->mem + l.down_s);
+    L->expert_scale = reinterpret_cast<float *>(L->ws + l.expert_scale);
     L->x = reinterpret_cast<int8_t *>(L->ws + l.x);
     L->m = reinterpret_cast<int8_t *>(L->ws + l.m);
     L->x_s = reinterpret_cast<float *>(L->ws + l.x_s);
     L->m_s = reinterpret_cast<float *>(L->ws + l.m_s);
     L->middle = reinterpret_cast<float *>(L->ws + l.middle);
-    L->contrib = reinterpret_cast<float *>(L->ws + l.contrib);
+    L->contrib = L->ws + l.contrib;
     const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(L->ws + at); };
     L->dropped = ints(l.dropped);
-    L->routes.counts = ints(l.counts);
-    L->routes.offsets = ints(l.offsets);
-    L->routes.pair_token = ints(l.token);
-    L->routes.pair_rank = ints(l.rank);
-    L->routes.pos_of = ints(l.pos);
-    L->routes.stream_items = reinterpret_cast<moe::Item *>(L->ws + l.stream_items);
-    L->routes.mfma_items = reinterpret_cast<moe::Item *>(L->ws + l.mfma_items);
-    L->routes.item_counts = ints(l.item_counts);
-    L->routes.bitmap = reinterpret_cast<uint32_t *>(L->ws + l.bitmap);
-    L->routes.wprefix = reinterpret_cast<uint32_t *>(L->ws + l.prefix);
+    L->groups = moe::I8Groups{ints(l.offsets), ints(l.token), ints(l.place), ints(l.counts)};
     *out = L;
     return 0;
 }
@@ -469,37 +859,43 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     const auto s = static_cast<hipStream_t>(stream);
     const moe_i8_layer_config &c = L->cfg;
     const int Ep = c.experts + c.has_shared, pairs = tokens * (c.top_k + c.has_shared);
-    hipError_t r = moe::launch_quantize_i8(x, type, c.hidden, c.hidden, tokens, L->x, L->x_pitch, L->x_s, error, s);
-    if (r != hipSuccess) return r;
-    const moe::Shape shape{c.hidden, c.intermediate, c.experts, Ep, c.top_k};
-    // Every group an item of the matrix kernels, of which only counts and positions are read.
-    r = moe::launch_prepare(nullptr, ids, weights, tokens, shape, moe::ActOut{}, L->routes, 1, error, s);
+    const moe::I8GroupArgs ga{ids, weights, L->groups, tokens, c.top_k, c.experts, Ep, 0, 0, error};
+    const moe::I8Rows xr{x, c.hidden, c.hidden, static_cast<size_t>(tokens), L->x, L->x_pitch, L->x_s, error};
+    hipError_t r = moe::launch_prepare_i8(ga, xr, type, s);
     if (r != hipSuccess) return r;
     moe::I8Args a{};
-    a.tiles = L->gate_up;
+    a.blocks = L->gate_up;
     a.sw = L->gate_up_s;
     a.x = L->x;
     a.sx = L->x_s;
     a.pitch = L->x_pitch;
-    a.index = L->routes.pair_token;
+    a.index = L->groups.token;
     a.x_rows = tokens;
-    a.offsets = L->routes.offsets;
+    a.offsets = L->groups.offsets;
     a.experts = Ep;
     a.y = L->middle;
     a.y_stride = c.intermediate;
-    a.M = 2 * c.intermediate;
+    a.M = c.intermediate;
+    a.rows = 2 * moe::i8_rows(c.intermediate);
     a.N = pairs;
     a.K = c.hidden;
     a.chunks = moe::i8_chunks(c.hidden);
     a.error = error;
     if ((r = moe::launch_grouped<moe::kStoreMiddle, moe::kF32>(a, s)) != hipSuccess) return r;
+    if (tokens <= kFewTokens) {
+        const moe::I8DownArgs d{L->down, L->down_s, L->middle, ids, L->groups, weights, shared_gate, y, tokens, c.hidden,
+                                c.intermediate, c.experts, c.top_k, c.top_k + c.has_shared, moe::i8_rows(c.hidden),
+                                moe::i8_chunks(c.intermediate), error};
+        return moe::launch_down_fold(d, type, s);
+    }
     // Rows that no group took (dropped routes) are quantised as well, and not used;
     // what they hold raises no flag of this call, and SiLU(g) u is always finite.
-    r = moe::launch_quantize_i8(L->middle, moe::kF32, c.intermediate, c.intermediate, pairs, L->m, L->m_pitch, L->m_s,
-                                L->dropped, s);
-    if (r != hipSuccess) return r;
-    a.tiles = L->down;
+    const moe::I8Rows mr{L->middle, c.intermediate, c.intermediate, static_cast<size_t>(pairs), L->m, L->m_pitch, L->m_s, L->dropped};
+    if ((r = moe::launch_quantize_i8(mr, moe::kF32, s)) != hipSuccess) return r;
+    const bool halves = type == MOE_BF16;
+    a.blocks = L->down;
     a.sw = L->down_s;
+    a.expert_scale = L->expert_scale;
     a.x = L->m;
     a.sx = L->m_s;
     a.pitch = L->m_pitch;
@@ -508,15 +904,17 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     a.y = L->contrib;
     a.y_stride = c.hidden;
     a.M = c.hidden;
+    a.rows = moe::i8_rows(c.hidden);
     a.K = c.intermediate;
     a.chunks = moe::i8_chunks(c.intermediate);
-    if ((r = moe::launch_grouped<moe::kStoreRows, moe::kF32>(a, s)) != hipSuccess) return r;
-    const moe::I8FoldArgs f{L->contrib, L->routes.pos_of, L->routes.offsets, weights, shared_gate, y,
-                            tokens,     c.hidden,         c.top_k,           c.experts, c.has_shared, error};
+    r = halves ? moe::launch_grouped<moe::kStoreHalves, moe::kF16>(a, s) : moe::launch_grouped<moe::kStoreRows, moe::kF32>(a, s);
+    if (r != hipSuccess) return r;
+    const moe::I8FoldArgs f{L->contrib, L->m_s, L->expert_scale, ids, L->groups, weights, shared_gate, y,
+                            tokens, c.hidden, c.top_k, c.experts, c.has_shared, error};
     const dim3 grid(static_cast<unsigned>((static_cast<size_t>(tokens) * c.hidden / 4 + 255) / 256)), block(256);
-    if (type == MOE_F32) moe::k_i8_fold<moe::kF32><<<grid, block, 0, s>>>(f);
-    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16><<<grid, block, 0, s>>>(f);
-    else moe::k_i8_fold<moe::kF16><<<grid, block, 0, s>>>(f);
+    if (type == MOE_F32) moe::k_i8_fold<moe::kF32, false><<<grid, block, 0, s>>>(f);
+    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16, true><<<grid, block, 0, s>>>(f);
+    else moe::k_i8_fold<moe::kF16, false><<<grid, block, 0, s>>>(f);
     return hipGetLastError();
 }
 

@@ -70,26 +70,38 @@ def expert(x, sx, gate, up, down):
     return product(m, sm, *down)
 
 
+def half_step(x, sx, gate, up, down):
+    """Half a step of the smallest fp16 numbers in which an expert's output may be
+    held on the way to a bf16 sum: 2^-25 sx 2^-p with 2^-p < 2 I max |sw|."""
+    _, sm = quantise(middle(x, sx, gate, up))
+    return (2.0 ** -24 * up[0].shape[0] * float(down[1].abs().max())) * sm.double()[:, None]
+
+
 def layer(x, bank, shared, ids, w, gate):
-    """(y in 64 bits, sum of the magnitudes that it adds up)."""
+    """(y in 64 bits, sum of the magnitudes that it adds up, sum of their half steps)."""
     q, s = quantise(x)
     n, k = ids.shape
     y = torch.zeros((n, x.shape[1]), dtype=torch.float64, device=x.device)
-    size = torch.zeros_like(y)
+    size, steps = torch.zeros_like(y), torch.zeros((n, 1), dtype=torch.float64, device=x.device)
     for e in torch.unique(ids).tolist():
         t, r = torch.nonzero(ids == e, as_tuple=True)
-        c = w[t, r].double()[:, None] * expert(q[t], s[t], *[(codes[e], scales[e]) for codes, scales in bank])
+        args = (q[t], s[t], *[(codes[e], scales[e]) for codes, scales in bank])
+        f = w[t, r].double()[:, None]
+        c = f * expert(*args)
         y.index_add_(0, t, c)
         size.index_add_(0, t, c.abs())
+        steps.index_add_(0, t, f.abs() * half_step(*args))
     if shared is not None:
-        c = expert(q, s, *shared)
-        if gate is not None:
-            c = c * torch.sigmoid(gate.double())[:, None]
-        y, size = y + c, size + c.abs()
-    return y, size
+        f = 1.0 if gate is None else torch.sigmoid(gate.double())[:, None]
+        c = f * expert(q, s, *shared)
+        y, size, steps = y + c, size + c.abs(), steps + f * half_step(q, s, *shared)
+    return y, size, steps
 
 
-def layer_bound(y, size, k, dtype):
+def layer_bound(y, size, k, dtype, steps=0.0):
     """A contribution has three roundings of its own, one of its weight and up to
-    five in its gate's sigmoid; each of k + 1 sums has one."""
-    return size * ((k + 11) * 2.0 ** -24) + y.abs() * EPS[dtype] * (1 + 2.0 ** -10) + TINY[dtype]
+    five in its gate's sigmoid; each of k + 1 sums has one.  Where y is bf16 the
+    contributions may have been fp16, each rounded by 2^-11 of itself or half a
+    step."""
+    half = size * (2.0 ** -11 + 2.0 ** -22) + steps if dtype == torch.bfloat16 else 0.0
+    return size * ((k + 11) * 2.0 ** -24) + half + (y.abs() + half) * EPS[dtype] * (1 + 2.0 ** -10) + TINY[dtype]

@@ -46,8 +46,8 @@ class Case:
         x = self.x.to(dtype)
         y, e = self.layer.forward(x, self.ids, self.w, shared_gate=self.gate if gate else None)
         assert flag(e) == 0
-        ref, size = R.layer(x, self.bank, self.shared, self.ids, self.w, self.gate if gate else None)
-        bound = R.layer_bound(ref, size, self.k, dtype)
+        ref, size, steps = R.layer(x, self.bank, self.shared, self.ids, self.w, self.gate if gate else None)
+        bound = R.layer_bound(ref, size, self.k, dtype, steps)
         d = (y.double() - ref).abs()
         assert bool((d <= bound).all()), float((d / bound).max())
         return y
@@ -97,7 +97,7 @@ def test_bad_routes(n):
     assert flag(e) == 1
     w2 = w.clone()
     w2[1, 2] = w2[2, 0] = w2[3, 3] = w2[4, 1] = 0.0     # the dropped routes
-    ref, size = R.layer(c.x, c.bank, c.shared, c.ids, w2, None)
+    ref, size, _ = R.layer(c.x, c.bank, c.shared, c.ids, w2, None)
     assert bool(((y.double() - ref).abs() <= R.layer_bound(ref, size, 4, F32)).all())
     keep = torch.tensor([i for i in range(n) if i not in (1, 2, 3, 4)], device=DEV)
     assert torch.equal(y[keep], good[keep])
@@ -132,7 +132,7 @@ def test_nonfinite_values(n):
     w = c.w.clone()
     w[2, 0] = -0.25                                 # flagged, and stays in the sum
     y, e = c.layer.forward(c.x, c.ids, w, shared_gate=c.gate)
-    ref, size = R.layer(c.x, c.bank, c.shared, c.ids, w, c.gate)
+    ref, size, _ = R.layer(c.x, c.bank, c.shared, c.ids, w, c.gate)
     assert flag(e) == 1 and bool(((y.double() - ref).abs() <= R.layer_bound(ref, size, 4, F32)).all())
 
 
