@@ -334,6 +334,7 @@ hipError_t launch_prepare_i8(I8GroupArgs a, const I8Rows &x, int type, hipStream
 }
 
 // ------------------------------------------------------------------- sums ---
+inline constexpr int kDownPairs = 33;   // 32 routes and the shared expert
 struct I8FoldArgs {
     const void *c;             // [pairs][H] outputs of the experts: fp32, or fp16 as k_i8_expert_scale says
     const float *c_scale;      // fp16: [pairs] scales of the rows
@@ -368,84 +369,102 @@ __global__ __launch_bounds__(256) void k_i8_expert_scale(const float *sw, float 
 }
 
 // y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags of
-// moe_ffn_forward's sum, rounded once; four elements a thread.
+// moe_ffn_forward's sum, rounded once: a workgroup a token, V elements (16 bytes of
+// the contributions) a thread, eight rows' loads in flight.
 template<int T, bool Halves>
 __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
-    const size_t i = (static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
-    if (i >= static_cast<size_t>(a.tokens) * a.H) return;
-    const size_t t = i / a.H, h = i % a.H;
+    constexpr int V = Halves ? 8 : 4;
     typedef float f4 __attribute__((ext_vector_type(4)));
-    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-    using Row = std::conditional_t<Halves, h4, f4>;
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+    using Row = std::conditional_t<Halves, h8, f4>;
     using Value = std::conditional_t<Halves, _Float16, float>;
-    const auto load = [&](size_t row) {
-        return __builtin_nontemporal_load(reinterpret_cast<const Row *>(static_cast<const Value *>(a.c) + row * a.H + h));
-    };
-    int flags[4] = {};
-    float v[4] = {};
-    for (int r0 = 0; r0 < a.k; r0 += 8) {
-        Row x[8];
-        float w[8], scale[8];
-        int place[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const size_t route = t * a.k + r0 + q;
-            place[q] = r0 + q < a.k ? a.g.place[route] : -1;
-            scale[q] = 1.0f;
-            if (place[q] >= 0) {
-                x[q] = load(place[q]);
-                if constexpr (Halves) scale[q] = a.c_scale[place[q]] * a.expert_scale[a.ids[route]];
+    __shared__ int place[kDownPairs];
+    __shared__ float weight[kDownPairs], scale[kDownPairs];
+    const size_t t = blockIdx.x;
+    int flags = 0;
+    if (threadIdx.x <= static_cast<unsigned>(a.k)) {
+        const int r = threadIdx.x;
+        const size_t route = t * a.k + r;
+        int at = -1;
+        float w = 1.0f, s = 1.0f;
+        if (r < a.k) {
+            at = a.g.place[route];
+            w = a.weights[route];
+            if (at >= 0) {
+                if (!isfinite(w)) { flags |= 1; w = 0.0f; }
+                if constexpr (Halves) s = a.c_scale[at] * a.expert_scale[a.ids[route]];
             }
-            w[q] = r0 + q < a.k ? a.weights[route] : 0.0f;
-        }
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            if (place[q] < 0) continue;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float c = static_cast<float>(x[q][e]), s = w[q];
-                if constexpr (Halves) c = c * scale[q];
-                if (!isfinite(c)) { flags[e] |= 1; c = 0.0f; }
-                if (!isfinite(s)) { flags[e] |= 1; s = 0.0f; }
-                float p = s * c;
-                if (!isfinite(p)) { flags[e] |= 2; p = 0.0f; }
-                v[e] = v[e] + p;
-                if (!isfinite(v[e])) { flags[e] |= 2; v[e] = 0.0f; }
+        } else if (a.shared) {
+            at = a.g.offsets[a.E] + static_cast<int>(t);
+            if constexpr (Halves) s = a.c_scale[at] * a.expert_scale[a.E];
+            if (a.shared_gate) {
+                float g = a.shared_gate[t];
+                if (!isfinite(g)) { flags |= 1; g = 0.0f; }
+                w = 1.0f / (1.0f + moe_expf(-g));
+                if (!isfinite(w)) { flags |= 2; w = 0.0f; }
             }
         }
+        place[r] = at;
+        weight[r] = w;
+        scale[r] = s;
     }
-    int any = 0;
-    Row sx = {};
-    float scale = 1.0f, gate = 1.0f;
-    int gate_flags = 0;
-    if (a.shared) {
-        const size_t row = a.g.offsets[a.E] + t;
-        sx = load(row);
-        if constexpr (Halves) scale = a.c_scale[row] * a.expert_scale[a.E];
-        if (a.shared_gate) {
-            float g = a.shared_gate[t];
-            if (!isfinite(g)) { gate_flags |= 1; g = 0.0f; }
-            gate = 1.0f / (1.0f + moe_expf(-g));
-            if (!isfinite(gate)) { gate_flags |= 2; gate = 0.0f; }
-        }
-    }
+    // A weight that is not finite gives up the routed sum, such a gate all of it.
+    const uint64_t first = __builtin_amdgcn_ballot_w64(flags != 0);   // of the first wave, which has them all
+    __shared__ uint64_t lost_ranks;
+    if (threadIdx.x == 0) lost_ranks = first;
+    __syncthreads();
+    const uint64_t lost = lost_ranks;
+    const bool no_routes = (lost & ((uint64_t{1} << a.k) - 1)) != 0, no_shared = (lost >> a.k & 1) != 0;
+    for (int h = threadIdx.x * V; h < a.H; h += 256 * V) {
+        const auto load = [&](int r) {
+            return __builtin_nontemporal_load(reinterpret_cast<const Row *>(static_cast<const Value *>(a.c) + static_cast<size_t>(place[r]) * a.H + h));
+        };
+        int f[V] = {};
+        float v[V] = {};
+        Row shared = {};
+        if (a.shared) shared = load(a.k);
+        for (int r0 = 0; r0 < a.k; r0 += 8) {
+            Row x[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        if (flags[e]) v[e] = 0.0f;
-        int sf = 0;
-        if (a.shared) {
-            sf = gate_flags;
-            float c = static_cast<float>(sx[e]);
-            if constexpr (Halves) c = c * scale;
-            if (!isfinite(c)) { sf |= 1; c = 0.0f; }
-            v[e] = v[e] + gate * c;
-            if (!isfinite(v[e])) { sf |= 2; v[e] = 0.0f; }
-            if (sf) v[e] = 0.0f;
+            for (int q = 0; q < 8; ++q)
+                if (r0 + q < a.k && place[r0 + q] >= 0) x[q] = load(r0 + q);
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                if (r0 + q >= a.k || place[r0 + q] < 0) continue;
+                const float w = weight[r0 + q], s = scale[r0 + q];
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float c = static_cast<float>(x[q][e]);
+                    if constexpr (Halves) c = c * s;
+                    if (!isfinite(c)) { f[e] |= 1; c = 0.0f; }
+                    float p = w * c;
+                    if (!isfinite(p)) { f[e] |= 2; p = 0.0f; }
+                    v[e] = v[e] + p;
+                    if (!isfinite(v[e])) { f[e] |= 2; v[e] = 0.0f; }
+                }
+            }
         }
-        any |= flags[e] | sf;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (f[e] || no_routes) v[e] = 0.0f;
+            flags |= f[e];
+            if (a.shared) {
+                int sf = no_shared ? 1 : 0;
+                float c = static_cast<float>(shared[e]);
+                if constexpr (Halves) c = c * scale[a.k];
+                if (!isfinite(c)) { sf |= 1; flags |= 1; c = 0.0f; }
+                v[e] = v[e] + weight[a.k] * c;
+                if (!isfinite(v[e])) { sf |= 2; flags |= 2; v[e] = 0.0f; }
+                if (sf) v[e] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; e += 4) {
+            const float o[4] = {v[e], v[e + 1], v[e + 2], v[e + 3]};
+            store4<T>(a.y, t * a.H + h + e, o);
+        }
     }
-    store4<T>(a.y, i, v);
-    if (any) atomicOr(a.error, any);
+    if (flags) atomicOr(a.error, flags);
 }
 
 // ------------------------------------- few tokens: down and the sum in one ---
@@ -465,7 +484,7 @@ struct I8DownArgs {
     int rows, chunks;
     int *error;
 };
-inline constexpr int kDownPiece = 8, kDownTiles = 16, kDownPairs = 33;
+inline constexpr int kDownPiece = 8, kDownTiles = 16;
 template<int Y>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void k_i8_down_fold(I8DownArgs a, int tiles) {
     extern __shared__ __attribute__((aligned(16))) int part[];   // [rank][16 tiles]: sums, then outputs
@@ -911,7 +930,7 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     if (r != hipSuccess) return r;
     const moe::I8FoldArgs f{L->contrib, L->m_s, L->expert_scale, ids, L->groups, weights, shared_gate, y,
                             tokens, c.hidden, c.top_k, c.experts, c.has_shared, error};
-    const dim3 grid(static_cast<unsigned>((static_cast<size_t>(tokens) * c.hidden / 4 + 255) / 256)), block(256);
+    const dim3 grid(tokens), block(256);
     if (type == MOE_F32) moe::k_i8_fold<moe::kF32, false><<<grid, block, 0, s>>>(f);
     else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16, true><<<grid, block, 0, s>>>(f);
     else moe::k_i8_fold<moe::kF16, false><<<grid, block, 0, s>>>(f);
