@@ -76,6 +76,137 @@ __global__ __launch_bounds__(64 * WR * WC) void k_i8_gemm(I8Args a) {
           [&](const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) { g.template store_rows<Y>(it, params, acc); });
 }
 
+// Few rows of x (at most 16): a workgroup takes 16 results of each, one tile of every
+// chunk, and its waves share out the chunks (wave w: chunks w, w + W, ..), the
+// matrix straight from memory into registers.  IN: x's type, quantised here by
+// every workgroup while its first tiles are on their way; or kCodes.  What bounds
+// it: the launch and one trip to memory, then HBM.
+struct I8FewArgs {
+    const uint8_t *blocks;
+    const float *sw;
+    const void *x;        // rows of IN, x_stride elements apart, or codes
+    int64_t x_stride;
+    const float *sx;      // kCodes
+    void *y;
+    int64_t y_stride;
+    int y_type, M, N, K, chunks;
+    int *error;
+};
+inline constexpr int kFewRows = 16, kFewWaves = 8, kFewVectors = 4;   // vectors of 8 that a thread quantises
+template<int IN, int Y>
+__global__ __launch_bounds__(64 * kFewWaves) void k_i8_few(I8FewArgs a) {
+    constexpr bool Quantize = IN != kCodes;
+    constexpr int U = 4, T = 64 * kFewWaves;   // chunks of a wave in flight
+    __shared__ i32x4 red[kFewWaves][64];
+    __shared__ uint32_t most[kFewRows];
+    extern __shared__ __attribute__((aligned(16))) uint8_t codes[];   // Quantize: [piece of 16][row][16]
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = blockIdx.x;
+    const uint8_t *w = a.blocks + static_cast<size_t>(tile >> 2) * a.chunks * kI8BlockBytes + (tile & 3) * 1024 + lane * 16;
+    uint4 f[U];
+    const auto load = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = min(c0 + u * kFewWaves, a.chunks - 1);   // past the last one: it again, not used
+            f[u] = load_once(w + static_cast<size_t>(c) * kI8BlockBytes);
+        }
+    };
+    load(wave);
+    if constexpr (Quantize) {
+        // A thread's vectors stay in registers between their row's maximum and the codes.
+        const int per = a.K / 8;
+        if (threadIdx.x < kFewRows) most[threadIdx.x] = 0;
+        Raw8 raw[kFewVectors];
+#pragma unroll
+        for (int j = 0; j < kFewVectors; ++j) {
+            const int i = j * T + threadIdx.x, n = i / per;
+            raw[j] = load8_any<IN>(a.x, static_cast<size_t>(n) * a.x_stride + i % per * 8, n < a.N ? 8 : 0);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kFewVectors; ++j) {
+            const int n = (j * T + threadIdx.x) / per;
+            float v[8];
+            unpack8<IN>(raw[j], v);
+            uint32_t m = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) m = max(m, magnitude(v[q]));
+            // Four neighbouring threads have one row's vectors (K is a multiple of 32).
+            m = max(m, static_cast<uint32_t>(lane_xor<1>(static_cast<int>(m))));
+            m = max(m, static_cast<uint32_t>(lane_xor<2>(static_cast<int>(m))));
+            if ((threadIdx.x & 3) == 0 && n < a.N) atomicMax(&most[n], m);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kFewVectors; ++j) {
+            const int i = j * T + threadIdx.x, n = i / per, k = i % per;
+            if (n >= a.N) break;
+            float v[8];
+            unpack8<IN>(raw[j], v);
+            *reinterpret_cast<uint2 *>(codes + (static_cast<size_t>(k >> 1) * a.N + n) * 16 + (k & 1) * 8) = quantize8_i8(v, row_scale(most[n]));
+        }
+        if (a.K % kI8Chunk) {   // the last chunk's second half meets zeros of the matrix, as whole numbers
+            for (int i = threadIdx.x; i < a.N * 8; i += T)
+                reinterpret_cast<uint32_t *>(codes + static_cast<size_t>(a.K / 16) * a.N * 16)[i] = 0;
+        }
+        __syncthreads();
+    }
+    const int n = min(lane & 15, a.N - 1);
+    const int8_t *rows = static_cast<const int8_t *>(a.x) + (Quantize ? 0 : static_cast<size_t>(n) * a.x_stride + (lane >> 4) * 16);
+    i32x4 acc = {0, 0, 0, 0};
+    for (int c0 = wave; c0 < a.chunks; c0 += kFewWaves * U) {
+        if (c0 != wave) load(c0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int c = c0 + u * kFewWaves;
+            if (c >= a.chunks) break;
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (Quantize) x = *reinterpret_cast<const uint4 *>(codes + (static_cast<size_t>(c * 4 + (lane >> 4)) * a.N + n) * 16);
+            else if (c * kI8Chunk + (lane >> 4) * 16 < a.K) x = *reinterpret_cast<const uint4 *>(rows + c * kI8Chunk);
+            acc = i8_dot(f[u], x, acc);
+        }
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int j = 1; j < kFewWaves; ++j) acc += red[j][lane];
+    const int row = lane & 15;
+    if (row >= a.N) return;
+    float sx;
+    if constexpr (Quantize) {
+        const GroupScale s = row_scale(most[row]);
+        sx = s.s;
+        if (s.bad && blockIdx.x == 0 && lane < 16) atomicOr(a.error, 1);
+    } else {
+        sx = a.sx[row];
+    }
+    const int m = (tile >> 2) * kI8Block + (lane >> 4) * 16 + (tile & 3) * 4;
+    if (m >= a.M) return;
+    float v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = static_cast<float>(acc[q]) * (sx * a.sw[m + q]);   // there up to i8_rows(M)
+    const size_t at = static_cast<size_t>(row) * a.y_stride + m;
+    if (m + 3 < a.M) {
+        store4<Y>(a.y, at, v);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (m + q < a.M) store1<Y>(a.y, at + q, v[q]);
+    }
+}
+
+template<int IN>
+hipError_t launch_few(const I8FewArgs &a, hipStream_t s) {
+    const dim3 block(64 * kFewWaves);
+    const size_t lds = IN == kCodes ? 0 : static_cast<size_t>(a.N) * a.chunks * kI8Chunk;
+    const dim3 blocks(static_cast<unsigned>(i8_rows(a.M) / 16));
+    if (a.y_type == kF32) k_i8_few<IN, kF32><<<blocks, block, lds, s>>>(a);
+    else if (a.y_type == kBF16) k_i8_few<IN, kBF16><<<blocks, block, lds, s>>>(a);
+    else k_i8_few<IN, kF16><<<blocks, block, lds, s>>>(a);
+    return hipGetLastError();
+}
+
 }  // namespace
 }  // namespace moe
 
@@ -105,6 +236,8 @@ void release(moe_i8_linear *L) {
     delete L;
 }
 
+inline constexpr int kFewElements = moe::kFewVectors * 64 * moe::kFewWaves * 8;   // of x, quantised inside the product
+
 template<int WR, int WC, int TM, int TN, int S, int KS>
 int launch_gemm(moe::I8Args a, int y_type, hipStream_t s) {
     using Stream = moe::I8Stream<WR, WC, TM, TN, S, KS, moe::kStoreRows, false>;
@@ -116,6 +249,12 @@ int launch_gemm(moe::I8Args a, int y_type, hipStream_t s) {
     else if (y_type == MOE_BF16) moe::k_i8_gemm<WR, WC, TM, TN, S, KS, moe::kBF16><<<grid, block, 0, s>>>(a);
     else moe::k_i8_gemm<WR, WC, TM, TN, S, KS, moe::kF16><<<grid, block, 0, s>>>(a);
     return hipGetLastError();
+}
+
+moe::I8FewArgs few_args(const moe_i8_linear *L, const void *x, int64_t x_stride, const float *sx, int columns, void *y, int y_type,
+                        int64_t y_stride, int *error) {
+    return moe::I8FewArgs{L->mem, L->scales, x, x_stride, sx, y, y_stride, y_type, L->output, columns, L->input,
+                          moe::i8_chunks(L->input), error};
 }
 
 int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, const float *scales, int columns, void *y,
@@ -136,10 +275,13 @@ int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, c
     a.K = L->input;
     a.chunks = moe::i8_chunks(L->input);
     const auto tiles = [&](long m, long n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
-    if (a.N <= 16) return launch_gemm<4, 1, 1, 1, 3, 4>(a, y_type, s);
-    if (tiles(128, 128) < 400) return launch_gemm<2, 2, 2, 2, 3, 2>(a, y_type, s);
-    if (tiles(256, 256) < 256) return launch_gemm<2, 2, 4, 4, 4, 1>(a, y_type, s);
-    return launch_gemm<2, 2, 8, 8, 4, 1>(a, y_type, s);
+    if (a.N <= moe::kFewRows) return moe::launch_few<moe::kCodes>(few_args(L, codes, pitch, scales, columns, y, y_type, y_stride, nullptr), s);
+    const long t256 = tiles(256, 256);
+    if (t256 * 5 >= 3 * 256 * ((t256 + 255) / 256)) return launch_gemm<2, 4, 8, 4, 4, 1>(a, y_type, s);
+    if (tiles(128, 128) >= 144) return launch_gemm<4, 2, 2, 4, 4, 1>(a, y_type, s);
+    if (tiles(64, 64) >= 192) return launch_gemm<4, 2, 1, 2, 4, 2>(a, y_type, s);
+    if (tiles(64, 32) >= 128) return launch_gemm<2, 2, 2, 1, 4, 2>(a, y_type, s);
+    return launch_gemm<4, 1, 1, 1, 4, 4>(a, y_type, s);
 }
 
 }  // namespace
@@ -231,6 +373,19 @@ int moe_i8_linear_apply(moe_i8_linear *L, const void *x, int x_type, int64_t x_s
     moe::DeviceScope device(L->device);
     if (!device.ok()) return hipErrorInvalidDevice;
     const auto s = static_cast<hipStream_t>(stream);
+    const auto extent = [&](int64_t stride, int width, int type) {
+        return (static_cast<size_t>(columns - 1) * stride + width) * moe::elem_bytes(type);
+    };
+    const char *xb = static_cast<const char *>(x), *yb = static_cast<const char *>(y);
+    const bool apart = xb + extent(x_stride, L->input, x_type) <= yb || yb + extent(y_stride, L->output, y_type) <= xb;
+    // Every workgroup quantises all of the rows: in the product's kernel where each
+    // thread has few vectors of them.
+    if (columns <= moe::kFewRows && apart && columns * L->input <= kFewElements) {
+        const moe::I8FewArgs f = few_args(L, x, x_stride, nullptr, columns, y, y_type, y_stride, error);
+        if (x_type == MOE_F32) return moe::launch_few<moe::kF32>(f, s);
+        if (x_type == MOE_BF16) return moe::launch_few<moe::kBF16>(f, s);
+        return moe::launch_few<moe::kF16>(f, s);
+    }
     auto *scales = reinterpret_cast<float *>(L->ws + static_cast<size_t>(columns) * L->pitch);
     const moe::I8Rows rows{x, x_stride, L->input, static_cast<size_t>(columns), L->ws, L->pitch, scales, error};
     const hipError_t r = moe::launch_quantize_i8(rows, x_type, s);
