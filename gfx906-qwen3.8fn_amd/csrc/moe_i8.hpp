@@ -8,15 +8,16 @@
 // KiB, zero past its edges), [ceil(M/64)][ceil(K/64)], each as four tiles of 16
 // rows in the order in which a wave's lanes take them as an operand of
 // v_mfma_i32_16x16x64_i8: lane l holds tile row l % 16, columns 16 (l / 16) .. +
-// 15.  Row 4 g + q of tile i is row 16 g + 4 i + q of the block: the product
-// leaves rows 4 g .. + 3 of each tile in lanes 16 g .. + 15, so that a lane's
-// results of the four tiles are 16 neighbours in a row of y, and the stores of
-// four lanes 64 of them.  What a product reads past a row of activations meets the
-// zeros past the matrix row, so rows need no padding.
+// 15.  The product leaves rows 4 g .. + 3 of a tile in lanes 16 g .. + 15; row 4 g +
+// q of tile i is row 32 (i / 2) + 8 g + 4 (i % 2) + q of the block, so that a lane's
+// results of two tiles are eight neighbours in a row of y and a store of 16-bit
+// ones fills 64 bytes of each row; with 16 neighbours in a lane, and stores that fill
+// every other 16 bytes, 2048 x 2048 at 1,032 fp32 rows took 19.8 us instead of 18.1.  What a product reads past a row of activations
+// meets the zeros past the matrix row, so rows need no padding.
 //
 // Gate and up matrices of an expert lie together as one of 2 I rows (I rounded up
-// to 64), in which 64 rows of both make two blocks: tile 2 i holds gate's tile i,
-// tile 2 i + 1 up's.
+// to 64), in which 64 rows of both make two blocks: tile 2 i holds rows 16 i .. + 15
+// of gate, tile 2 i + 1 those of up.
 #pragma once
 
 #include "moe_fp8.hpp"   // element types, loads into LDS
@@ -172,6 +173,17 @@ __device__ __forceinline__ i32x4 i8_dot(const uint4 &w, const uint4 &x, const i3
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, w), __builtin_bit_cast(i32x4, x), acc, 0, 0, 0);
 }
 
+// SiLU(g) * u by the hardware's exponential and reciprocal (8 half ulps): with the Q4
+// layers' exact expf, whose table lies in memory, 4,096 tokens of 2048/512 take 559
+// us instead of 516.  0, with a flag, where it is not finite: bit 1 where g or u is
+// not, bit 2 where their product is not.
+__device__ __forceinline__ float silu_product(float g, float u, int &flags) {
+    const float v = g * sigmoid(g) * u;
+    if (isfinite(v)) return v;
+    flags |= isfinite(g) && isfinite(u) ? 2 : 1;
+    return 0.0f;
+}
+
 // What a product writes: rows of y; SiLU(gate) * up in fp32 from pairs of gate and up;
 // or rows with 1 / expert_scale[e] in place of the row's scale.
 enum { kStoreRows = 0, kStoreMiddle = 1, kStoreHalves = 2 };
@@ -213,8 +225,9 @@ struct I8Item {
 // The rows' and channels' scales come with an item's first stage into a ring of
 // their own, and so do, one item ahead, the indices of its rows: nothing but
 // loads into LDS is in flight, and a wait for one of them waits for no later one.
-template<int WR, int WC, int TM, int TN, int S, int KS, int Form, bool Grouped>
+template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y, bool Grouped>
 struct I8Stream {
+    static constexpr int Bytes = elem_bytes(Y);
     static constexpr int W = WR * WC, BM = 16 * TM * WR, BN = 16 * TN * WC;
     static constexpr int ATiles = BM / 16, BTiles = BN / 16;
     static constexpr int ABytes = ATiles * KS * 1024, Stage = ABytes + BTiles * KS * 1024;
@@ -344,6 +357,12 @@ struct I8Stream {
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     }
+    // An item every result of which is stored: `Stores` instructions of a wave at least,
+    // 16 bytes a lane each.
+    static constexpr int Stores = TM * TN * (Form == kStoreMiddle ? 8 : Bytes * 4) / 16;
+    __device__ __forceinline__ bool whole(const I8Item &t) const {
+        return t.cols == BN && (Form == kStoreMiddle ? (t.m0 + BM + 127) / 128 * 64 : t.m0 + BM) <= a.M;
+    }
     // All items first, first + step, .. below end; item(i) says which that is.
     template<class Fetch, class Store>
     __device__ __forceinline__ void run(int first, int step, int end, const Fetch &fetch, const Store &store) {
@@ -384,8 +403,17 @@ struct I8Stream {
         // wave reads any more, takes the stage S - 1 ahead.  An item's indices were
         // on their way `stages` turns before it begins, and what was S - 2 turns ago
         // has arrived.
+        // A wave's memory operations complete in the order in which it issued them, so
+        // that for S - 2 turns the last item's stores, issued behind the loads waited
+        // for, may still be on their way (163,840 rows of 512 x 2048 matrices 373 -> 369 us).
+        int stored = 0;   // such turns left
         const auto turn = [&](Frags &into) {
-            wait_for_lds_loads<(S - 3) * Loads>();
+            if (stored > 0) {
+                --stored;
+                wait_for_lds_loads<(S - 3) * Loads + Stores>();
+            } else {
+                wait_for_lds_loads<(S - 3) * Loads>();
+            }
             barrier();
             advance(slot == 0 ? S - 1 : slot - 1, stages >= S - 2);
             slot = slot + 1 == S ? 0 : slot + 1;
@@ -416,43 +444,28 @@ struct I8Stream {
                     }
                 }
             }
-            store(fetch(i), reinterpret_cast<const float *>(lds + params_at(done)), acc);
+            const I8Item item = fetch(i);
+            store(item, reinterpret_cast<const float *>(lds + params_at(done)), acc);
+            if (whole(item)) stored = S - 2;
         }
         wait_for_lds_loads<0>();   // no load may outlive the buffers
     }
 
-    // R neighbours in row n of y from column m on.
-    template<int Y, int R>
-    __device__ __forceinline__ void store_run(size_t row, int m, const float (&v)[R]) const {
-        const size_t at = row * static_cast<size_t>(a.y_stride) + m;
-        if (m + R <= a.M) {
-            if constexpr (Y == kF32) {
+    __device__ __forceinline__ void store_each(size_t at, int m, const float *v, int count) const {
 #pragma unroll
-                for (int i = 0; i < R; i += 4) {
-                    const float w[4] = {v[i], v[i + 1], v[i + 2], v[i + 3]};
-                    store4<kF32>(a.y, at + i, w);
-                }
-            } else {
-                uint32_t w[R / 2];
-#pragma unroll
-                for (int i = 0; i < R / 2; ++i) w[i] = Y == kBF16 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_f16(v[2 * i], v[2 * i + 1]);
-                __builtin_memcpy(static_cast<uint16_t *>(a.y) + at, w, R * 2);
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i)
+        for (int i = 0; i < count; ++i)
             if (m + i < a.M) store1<Y>(a.y, at + i, v[i]);
     }
-    template<int Y>
     __device__ __forceinline__ void store_rows(const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) const {
-        constexpr int G = TM < 4 ? TM : 4, R = 4 * G;   // tiles of a run
+        constexpr int G = TM < 2 ? 1 : 2, R = 4 * G;   // tiles of a run, its length
+        const int g = lane >> 4;
         float halves = 1.0f;
         if constexpr (Form == kStoreHalves)   // a scalar load, which no wait for others counts
             halves = 1.0f / ((const __attribute__((address_space(4))) float *)a.expert_scale)[it.e];
 #pragma unroll
         for (int p = 0; p < TM; p += G) {
-            const int tile = wr * TM + p, m = (tile >> 2) * 64 + (lane >> 4) * 16 + (tile & 3) * 4;
+            const int tile = wr * TM + p, first = (tile >> 1) * 32, m = first + g * 8 + (tile & 1) * 4;
+            const bool inside = it.m0 + first + 32 <= a.M;
             float sw[R];
 #pragma unroll
             for (int i = 0; i < R; ++i) sw[i] = params[m + i];
@@ -464,20 +477,41 @@ struct I8Stream {
                 float v[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) v[i] = static_cast<float>(acc[p + i / 4][t][i % 4]) * (sx * sw[i]);
-                store_run<Y, R>(static_cast<size_t>(it.r) + n, it.m0 + m, v);
+                const size_t row = (static_cast<size_t>(it.r) + n) * static_cast<size_t>(a.y_stride) + it.m0;
+                if (!inside) {
+                    store_each(row + m, it.m0 + m, v, R);
+                } else if constexpr (G == 1) {
+                    store4<Y>(a.y, row + m, v);
+                } else if constexpr (Y == kF32) {
+                    // Half of a run for half of the partner's, 32 lanes away, of the same
+                    // row: 64 bytes of it a store here as well.
+                    float lo[4], hi[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[4 + i]), false, false);
+                        lo[i] = __uint_as_float(s[0]);
+                        hi[i] = __uint_as_float(s[1]);
+                    }
+                    const size_t at = row + first + (g & 1) * 8 + (g >> 1) * 4;
+                    store4<kF32>(a.y, at, lo);
+                    store4<kF32>(a.y, at + 16, hi);
+                } else {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = Y == kBF16 ? pack_bf16(v[2 * i], v[2 * i + 1]) : pack_f16(v[2 * i], v[2 * i + 1]);
+                    __builtin_memcpy(static_cast<uint16_t *>(a.y) + row + m, w, 16);
+                }
             }
         }
     }
-    // SiLU(gate) * up of pairs of tiles, [rows][I] in fp32, by the hardware's exponential
-    // and reciprocal (8 half ulps): with the Q4 layers' exact expf, whose table lies
-    // in memory, 4,096 tokens of 2048/512 take 516 us instead of 559.
+    // SiLU(gate) * up of pairs of tiles, [rows][I] in fp32.
     __device__ __forceinline__ void store_middle(const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) {
         static_assert(Form != kStoreMiddle || TM % 2 == 0);
 #pragma unroll
         for (int p = 0; p < TM; p += 2) {
-            const int tile = it.m0 / 16 + wr * TM + p, i4 = (tile & 7) >> 1, at = (tile >> 3) * 64 + (lane >> 4) * 16 + i4 * 4;
+            const int tile = it.m0 / 16 + wr * TM + p, in = (tile & 7) * 8 + (lane >> 4) * 4, at = (tile >> 3) * 64 + in;   // tile is even
             if (at >= a.M) continue;
-            const float *s = params + ((tile >> 3) - it.m0 / 128) * 128 + (lane >> 4) * 16 + i4 * 4;
+            const float *s = params + ((tile >> 3) - it.m0 / 128) * 128 + in;
 #pragma unroll
             for (int t = 0; t < TN; ++t) {
                 const int n = (wc * TN + t) * 16 + (lane & 15);
@@ -485,14 +519,9 @@ struct I8Stream {
                 const float sx = params[PA + n];
                 float v[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const float g = static_cast<float>(acc[p][t][q]) * (sx * s[q]), u = static_cast<float>(acc[p + 1][t][q]) * (sx * s[64 + q]);
-                    v[q] = g * sigmoid(g) * u;
-                    if (!isfinite(v[q])) {   // only where g or u is not, or their product
-                        flags |= isfinite(g) && isfinite(u) ? 2 : 1;
-                        v[q] = 0.0f;
-                    }
-                }
+                for (int q = 0; q < 4; ++q)
+                    v[q] = silu_product(static_cast<float>(acc[p][t][q]) * (sx * s[q]),
+                                        static_cast<float>(acc[p + 1][t][q]) * (sx * s[64 + q]), flags);
                 store4<kF32>(a.y, (static_cast<size_t>(it.r) + n) * static_cast<size_t>(a.y_stride) + at, v);
             }
         }

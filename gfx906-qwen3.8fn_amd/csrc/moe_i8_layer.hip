@@ -7,7 +7,6 @@
 #include "moe_i8.hpp"
 
 #include <algorithm>
-#include <cstdlib>
 #include <new>
 
 namespace moe {
@@ -18,11 +17,12 @@ namespace {
 // first, with `big` tiles between them.  Offsets outside 0 .. N, or below the one
 // before, are drawn into that range and set bit 1; a group ends where the next
 // begins, and is empty where that is not after its own begin.
+inline constexpr int kMostExperts = 4096;
 struct GroupTable {
     int *first, *list, *row;   // [E + 1], [E], [E + 1]
     int experts, tiles, big;
 
-    static size_t bytes(int experts) { return (static_cast<size_t>(experts) * 3 + 2) * 4; }
+    static constexpr size_t bytes(int experts) { return (static_cast<size_t>(experts) * 3 + 2) * 4; }
 
     __device__ __forceinline__ GroupTable(const I8Args &a, int BN, int *lds) : experts(a.experts) {
         __shared__ int sums[16][4];
@@ -98,7 +98,7 @@ struct GroupTable {
 // whose matrices are read for a few rows; each has as many of either.
 template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y>
 __global__ __launch_bounds__(64 * WR * WC) void k_i8_grouped(I8Args a) {
-    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, true>;
+    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, Y, true>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Stream::Lds];
     extern __shared__ int table[];
     const GroupTable groups(a, Stream::BN, table);
@@ -129,14 +129,15 @@ __global__ __launch_bounds__(64 * WR * WC) void k_i8_grouped(I8Args a) {
     g.run(from, step, big + rest, fetch,
           [&](const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) {
               if constexpr (Form == kStoreMiddle) g.store_middle(it, params, acc);
-              else g.template store_rows<Y>(it, params, acc);
+              else g.store_rows(it, params, acc);
           });
     if (g.flags) atomicOr(a.error, g.flags);
 }
 
 template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y>
 hipError_t launch_tile(I8Args a, hipStream_t s) {
-    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, true>;
+    using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, Y, true>;
+    static_assert(Stream::Lds + GroupTable::bytes(kMostExperts) + 256 <= 160 * 1024, "a CU's LDS");
     a.tiles_m = (a.rows + Stream::BM - 1) / Stream::BM;
     const size_t lds = GroupTable::bytes(a.experts);
     const int resident = std::max(1, static_cast<int>(160 * 1024 / (Stream::Lds + lds + 256)));
@@ -146,16 +147,30 @@ hipError_t launch_tile(I8Args a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// The tile by the mean number of rows of a group, which the host knows: few rows,
+// matrices read for them and workgroups enough to have many on their way; many
+// rows, tiles that read less.  us, bank of 512 2048 x 1024 matrices, bf16, at 10, 80,
+// 640, 2,560, 5,120 and 20,480 rows in even groups, then 10,320 of 2560 x 640 in uneven
+// ones, fp32:
+//   64 x 16     9.8 / 30.6 / 119 / 166 / 181 / 398 / 210
+//   64 x 32    11.8 / 31.3 / 114 / 164 / 176 / 276 / 162
+//   128 x 64   16.1 / 36.3 / 119 / 167 / 176 / 215 / 155
+//   256 x 128  21.0 / 42.0 / 125 / 172 / 183 / 209 / 179
+// The layer's gate and up, 64 x 32 / 128 x 32 / 128 x 64 / 256 x 128, all of the
+// layer: 128 tokens - / 258 / 262 / 275, 512 - / 313 / 316 / 327, 1,024 - / 353 / 347 / 361,
+// 4,096 - / 688 / 573 / 539; its down (K = 512, an item's start and end weigh more):
+// 128 tokens 271 / 273 / 261 / 269, 512 331 / 328 / 315 / 324, 4,096 688 / 699 / 576 / 519.
 template<int Form, int Y>
 hipError_t launch_grouped(const I8Args &a, hipStream_t s) {
     const int mean = a.N / a.experts;
-    if (mean <= 2) {
-        if constexpr (Form == kStoreMiddle) return launch_tile<2, 1, 2, 1, 4, 2, Form, Y>(a, s);
-        else return launch_tile<4, 1, 1, 1, 4, 4, Form, Y>(a, s);
+    if (mean > 64) return launch_tile<4, 2, 4, 4, 4, 1, Form, Y>(a, s);
+    if constexpr (Form == kStoreMiddle) {   // pairs of tiles
+        if (mean <= 12) return launch_tile<4, 1, 2, 2, 4, 2, Form, Y>(a, s);
+    } else {
+        if (a.N <= a.experts / 2) return launch_tile<4, 1, 1, 1, 4, 4, Form, Y>(a, s);
+        if (mean <= 12 && a.chunks > 16) return launch_tile<4, 1, 1, 2, 4, 2, Form, Y>(a, s);
     }
-    if (mean <= 10) return launch_tile<4, 1, 2, 2, 4, 2, Form, Y>(a, s);
-    if (mean <= 64) return launch_tile<4, 1, 2, 4, 4, 1, Form, Y>(a, s);
-    return launch_tile<4, 2, 4, 4, 4, 1, Form, Y>(a, s);
+    return launch_tile<4, 1, 2, 4, 4, 1, Form, Y>(a, s);
 }
 
 hipError_t launch_grouped_rows(const I8Args &a, int y_type, hipStream_t s) {
@@ -174,6 +189,8 @@ struct I8Groups {
     int32_t *token;     // [pairs]: token of a place
     int32_t *place;     // [tokens * k]: place of a route; -1: dropped
     int32_t *counts;    // [blocks][E']: routes of a block of tokens, for batches of many
+    int4 *active;       // few tokens: expert, first place and number of rows of each group that has any
+    int32_t *groups;    // and how many those are
 };
 struct I8GroupArgs {
     const int32_t *ids;
@@ -209,10 +226,10 @@ __device__ __forceinline__ void count_routes(const I8GroupArgs &a, int t0, int n
     }
     if (flags) atomicOr(a.error, flags);
 }
-// Exclusive sums over the experts' numbers n(e); base(e, sum) takes them, and the
-// offsets are written by `writer`.
-template<class Number, class Base>
-__device__ __forceinline__ void scan_experts(const I8GroupArgs &a, bool writer, const Number &number, const Base &base) {
+// Exclusive sums over the experts' numbers n(e); base(e, sum) takes them and
+// returns the sum with all of the experts up to e, last(sum) the total.
+template<class Number, class Base, class Last>
+__device__ __forceinline__ void scan_experts(const I8GroupArgs &a, const Number &number, const Base &base, const Last &last) {
     __shared__ int sums[kGroupThreads / 64];
     const int per = (a.Ep + kGroupThreads - 1) / kGroupThreads, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int lo = min(a.Ep, static_cast<int>(threadIdx.x) * per), hi = min(a.Ep, lo + per);
@@ -230,10 +247,9 @@ __device__ __forceinline__ void scan_experts(const I8GroupArgs &a, bool writer, 
     for (int w = 0; w < wave; ++w) run += sums[w];
     for (int e = lo; e < hi; ++e) {
         const int n = number(e);
-        base(e, run);
-        if (writer) a.g.offsets[e] = run;
+        base(e, run, n);
         run += n;
-        if (writer && e + 1 == a.Ep) a.g.offsets[a.Ep] = run;
+        if (e + 1 == a.Ep) last(run);
     }
     __syncthreads();
 }
@@ -261,7 +277,21 @@ __global__ __launch_bounds__(kGroupThreads) void k_i8_prepare_small(I8GroupArgs 
             if (i / kGroupThreads == j) number[j] = n;
     });
     __syncthreads();
-    scan_experts(a, true, [&](int e) { return e < a.E ? counts[e] : a.tokens; }, [&](int e, int run) { counts[e] = run; });
+    // Rows below bit 16 (at most 2,048 routes and as many of the shared expert),
+    // groups that have any above.
+    const auto number_of = [&](int e) {
+        const int n = e < a.E ? counts[e] : a.tokens;
+        return n > 0 ? n | 1 << 16 : 0;
+    };
+    scan_experts(a, number_of, [&](int e, int run, int n) {
+        const int first = run & 0xffff;
+        counts[e] = first;
+        a.g.offsets[e] = first;
+        if (n) a.g.active[run >> 16] = make_int4(e, first, n & 0xffff, 0);
+    }, [&](int all) {
+        a.g.offsets[a.Ep] = all & 0xffff;
+        *a.g.groups = all >> 16;
+    });
 #pragma unroll
     for (int j = 0; j < kSmallRoutes / kGroupThreads; ++j) {
         const int i = j * kGroupThreads + threadIdx.x;
@@ -293,7 +323,7 @@ __global__ __launch_bounds__(kGroupThreads) void k_i8_place(I8GroupArgs a) {
     for (int e = threadIdx.x; e < a.Ep; e += kGroupThreads) {
         int n = 0, b = 0;
         if (e < a.E) {
-#pragma unroll 8
+#pragma unroll 32
             for (int j = 0; j < a.blocks; ++j) {
                 const int c = a.g.counts[static_cast<size_t>(j) * a.Ep + e];
                 n += c;
@@ -306,7 +336,13 @@ __global__ __launch_bounds__(kGroupThreads) void k_i8_place(I8GroupArgs a) {
         before[e] = b;
     }
     __syncthreads();
-    scan_experts(a, blockIdx.x == 0, [&](int e) { return all[e]; }, [&](int e, int run) { before[e] += run; });
+    const bool writer = blockIdx.x == 0;
+    scan_experts(a, [&](int e) { return all[e]; }, [&](int e, int run, int) {
+        before[e] += run;
+        if (writer) a.g.offsets[e] = run;
+    }, [&](int rows) {
+        if (writer) a.g.offsets[a.Ep] = rows;
+    });
     const int t0 = blockIdx.x * a.per, n = min(a.per, a.tokens - t0);
     const size_t at = static_cast<size_t>(t0) * a.k;
     for (int i = threadIdx.x; i < n * a.k; i += kGroupThreads) {
@@ -467,6 +503,112 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
     if (flags) atomicOr(a.error, flags);
 }
 
+// ------------------------------------------- few tokens: gate and up ---
+// Work item (group, pair of tiles): 16 rows of gate and of up, whose chunks the eight
+// waves share out (wave w: chunks w, w + 8, ..), straight from memory into
+// registers, against all of the group's rows, 16 at a time; the sums meet in LDS.
+// A workgroup takes items in turn, each with its first tiles on their way before
+// the last one's sums are done.  2048/512, 1 / 8 / 32 tokens 8.3 / 28.9 / 84 us: bound by
+// three dependent trips to memory (group, its rows' numbers, the rows), then by HBM
+// (160 MB at 5.5 TB/s); the grouped products' kernel 14.8 / 32.2 / 81, at 64 tokens 120
+// against 129.
+struct I8GateUpArgs {
+    const uint8_t *blocks;
+    const float *sw;
+    const int8_t *x;
+    const float *sx;
+    int64_t pitch;
+    I8Groups g;
+    float *middle;             // [pairs][I]
+    int I, rows, K, chunks;    // rows: 2 i8_rows(I)
+    int *error;
+};
+inline constexpr int kFewTokens = 32;   // tokens up to which gate and up take this kernel
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k_i8_gate_up_few(I8GateUpArgs a) {
+    constexpr int U = 4, W = 8, Most = kFewTokens / 16;   // chunks in flight, waves, row tiles of x
+    __shared__ i32x4 red[W][2][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pairs = i8_rows(a.I) / 16, items = *a.g.groups * pairs;
+    uint4 f[U][2];
+    const uint8_t *w = a.blocks;
+    const auto load = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const size_t at = static_cast<size_t>(min(c0 + u * W, a.chunks - 1)) * kI8BlockBytes;   // past the last: it again, not used
+            f[u][0] = load_once(w + at);
+            f[u][1] = load_once(w + at + 1024);
+        }
+    };
+    const auto select = [&](int item) {
+        const int4 group = a.g.active[item / pairs];
+        const int pair = item % pairs, e = __builtin_amdgcn_readfirstlane(group.x);
+        w = a.blocks + (static_cast<size_t>(e) * (a.rows / kI8Block) + pair / 2) * a.chunks * kI8BlockBytes + (pair & 1) * 2048 + lane * 16;
+        load(wave);
+        return make_int4(e, __builtin_amdgcn_readfirstlane(group.y), __builtin_amdgcn_readfirstlane(group.z), pair);
+    };
+    int flags = 0;
+    int4 next = static_cast<int>(blockIdx.x) < items ? select(blockIdx.x) : int4{};
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        const int4 now = next;   // expert, first place, rows, pair
+        const int tiles = (now.z + 15) / 16;
+        const int8_t *x[Most];
+#pragma unroll
+        for (int t = 0; t < Most; ++t) {
+            const int n = min(t * 16 + (lane & 15), now.z - 1);
+            x[t] = a.x + static_cast<int64_t>(t < tiles ? a.g.token[now.y + n] : 0) * a.pitch + (lane >> 4) * 16;
+        }
+        i32x4 acc[Most][2];
+#pragma unroll
+        for (int t = 0; t < Most; ++t) acc[t][0] = acc[t][1] = i32x4{0, 0, 0, 0};
+        for (int c0 = wave; c0 < a.chunks; c0 += W * U) {
+            if (c0 != wave) load(c0);
+#pragma unroll
+            for (int t = 0; t < Most; ++t) {
+                if (t >= tiles) break;
+                uint4 v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int c = min(c0 + u * W, a.chunks - 1);
+                    v[u] = make_uint4(0u, 0u, 0u, 0u);
+                    if (c * kI8Chunk + (lane >> 4) * 16 < a.K) v[u] = *reinterpret_cast<const uint4 *>(x[t] + c * kI8Chunk);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    if (c0 + u * W >= a.chunks) break;
+                    acc[t][0] = i8_dot(f[u][0], v[u], acc[t][0]);
+                    acc[t][1] = i8_dot(f[u][1], v[u], acc[t][1]);
+                }
+            }
+        }
+        if (item + static_cast<int>(gridDim.x) < items) next = select(item + gridDim.x);
+#pragma unroll
+        for (int t = 0; t < Most; ++t) {
+            if (t >= tiles) break;
+            red[wave][0][lane] = acc[t][0];
+            red[wave][1][lane] = acc[t][1];
+            __syncthreads();
+            // Thread i < 256: result i % 4 of lane i / 4.
+            if (threadIdx.x < 256) {
+                const int l = threadIdx.x >> 2, q = threadIdx.x & 3, n = t * 16 + (l & 15), j = now.w * 16 + (l >> 4) * 4 + q;
+                int g = 0, u = 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    g += reinterpret_cast<const int *>(&red[i][0][l])[q];
+                    u += reinterpret_cast<const int *>(&red[i][1][l])[q];
+                }
+                if (n < now.z && j < a.I) {
+                    const float sx = a.sx[a.g.token[now.y + n]];
+                    const float *s = a.sw + static_cast<size_t>(now.x) * a.rows + (now.w >> 2) * 128 + (now.w & 3) * 16 + (l >> 4) * 4 + q;
+                    a.middle[static_cast<size_t>(now.y + n) * a.I + j] =
+                        silu_product(static_cast<float>(g) * (sx * s[0]), static_cast<float>(u) * (sx * s[64]), flags);
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (flags) atomicOr(a.error, flags);
+}
+
 // ------------------------------------- few tokens: down and the sum in one ---
 // Workgroup (t, slice of `tiles` tiles of 16 rows); wave w takes ranks w, w + W, ..
 // It quantises the rank's middle row into LDS in pieces of eight chunks and streams
@@ -543,7 +685,6 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
 #pragma unroll
             for (int u = 0; u < kDownPiece; ++u) x[u] = *reinterpret_cast<const uint4 *>(&codes[wave][u * kI8Chunk + (lane >> 4) * 16]);
             const auto multiply = [&](int n, const uint4 (&from)[kDownPiece]) {
-                // Lanes 16 g .. + 15 have rows 16 g + 4 i + q of tile i's block.
                 const int tile = tile0 + n, row = n * 16 + (lane >> 4) * 4;
                 i32x4 *out = reinterpret_cast<i32x4 *>(&part[r * R + row]);
                 i32x4 acc = k0 > 0 ? *out : i32x4{0, 0, 0, 0};
@@ -551,7 +692,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
                 for (int u = 0; u < kDownPiece; ++u)
                     if (u < kb) acc = i8_dot(from[u], x[u], acc);
                 if (k0 + kDownPiece >= a.chunks) {
-                    const float *c = sw + (tile >> 2) * kI8Block + (lane >> 4) * 16 + (tile & 3) * 4;
+                    const float *c = sw + (tile >> 1) * 32 + (lane >> 4) * 8 + (tile & 1) * 4;
 #pragma unroll
                     for (int q = 0; q < 4; ++q) acc[q] = __float_as_int(static_cast<float>(acc[q]) * (scale.s * c[q]));
                 }
@@ -569,7 +710,7 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
     __syncthreads();
     int flags = 0;
     for (int i = threadIdx.x; i < here * 16; i += blockDim.x) {
-        const int tile = tile0 + (i >> 4), row = (tile >> 2) * kI8Block + (i >> 2 & 3) * 16 + (tile & 3) * 4 + (i & 3);
+        const int tile = tile0 + (i >> 4), row = (tile >> 1) * 32 + (i >> 2 & 3) * 8 + (tile & 1) * 4 + (i & 3);
         if (row >= a.H) continue;
         const float v = fold(a.k, a.P1 > a.k, a.shared_gate != nullptr, valid, weight, [&](int r) { return __int_as_float(part[r * R + i]); }, flags);
         store1<Y>(a.y, static_cast<size_t>(t) * a.H + row, v);
@@ -579,15 +720,16 @@ __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(4))) void 
 
 hipError_t launch_down_fold(const I8DownArgs &a, int type, hipStream_t s) {
     const int row_tiles = a.rows / 16;
-    // Row tiles a workgroup: the fewest on the busiest CU, and of such choices one
-    // workgroup a CU for few tokens, two (which fit at once) for more.
-    int tiles = 1, best = 1 << 30, best_off = 0;
+    // Row tiles a workgroup: the fewest on the busiest CU, and of such choices the one
+    // with the fewest workgroups a CU (one / two / four first, us a layer of 2048/512:
+    // 4 tokens 33.2 / 37.5 / 37.3, 8 52.0 / 54.5 / 62.1, 64 226.5 / 227.1 / 229.3).
+    int tiles = 1, best = 1 << 30, fewest = 0;
     for (int n = 1; n <= kDownTiles; ++n) {
-        const int rounds = (a.T * ((row_tiles + n - 1) / n) + 255) / 256, off = std::abs(rounds - (a.T <= 8 ? 1 : 2));
-        if (rounds * n < best || (rounds * n == best && off < best_off)) {
+        const int rounds = (a.T * ((row_tiles + n - 1) / n) + 255) / 256;
+        if (rounds * n < best || (rounds * n == best && rounds < fewest)) {
             tiles = n;
             best = rounds * n;
-            best_off = off;
+            fewest = rounds;
         }
     }
     const dim3 grid(static_cast<unsigned>((row_tiles + tiles - 1) / tiles + 7) / 8 * 8 * a.T), block(64 * std::min(16, a.P1));
@@ -670,11 +812,11 @@ bool valid_config(const moe_i8_layer_config *c) {
            c->max_tokens <= 65536;
 }
 
-inline constexpr int kFewTokens = 32;   // tokens up to which down and the sum are one launch
+inline constexpr int kFewDown = 64;   // tokens up to which down and the sum are one launch
 
 struct LayerLayout {
     size_t gate_up, down, gate_up_s, down_s, weights;   // offsets and end of the weights
-    size_t x, x_s, m, m_s, middle, contrib, offsets, token, place, counts, expert_scale, dropped, workspace;
+    size_t x, x_s, m, m_s, middle, contrib, offsets, token, place, counts, expert_scale, active, groups, dropped, workspace;
 };
 LayerLayout layout(const moe_i8_layer_config &c) {
     LayerLayout l{};
@@ -703,6 +845,8 @@ LayerLayout layout(const moe_i8_layer_config &c) {
     l.place = take(T * c.top_k * 4);
     l.counts = take(std::min<size_t>(128, (T + 63) / 64) * Ep * 4);
     l.expert_scale = take(Ep * 4);
+    l.active = take(Ep * 16);
+    l.groups = take(4);
     l.dropped = take(4);
     l.workspace = at;
     return l;
@@ -855,7 +999,8 @@ int moe_i8_layer_create(const moe_i8_layer_config *c, const moe_i8_matrix *exper
     L->contrib = L->ws + l.contrib;
     const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(L->ws + at); };
     L->dropped = ints(l.dropped);
-    L->groups = moe::I8Groups{ints(l.offsets), ints(l.token), ints(l.place), ints(l.counts)};
+    L->groups = moe::I8Groups{ints(l.offsets), ints(l.token), ints(l.place), ints(l.counts),
+                              reinterpret_cast<int4 *>(L->ws + l.active), ints(l.groups)};
     *out = L;
     return 0;
 }
@@ -900,8 +1045,16 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     a.K = c.hidden;
     a.chunks = moe::i8_chunks(c.hidden);
     a.error = error;
-    if ((r = moe::launch_grouped<moe::kStoreMiddle, moe::kF32>(a, s)) != hipSuccess) return r;
-    if (tokens <= kFewTokens) {
+    if (tokens <= moe::kFewTokens) {
+        const moe::I8GateUpArgs u{a.blocks, a.sw, a.x, a.sx, a.pitch, L->groups, L->middle, a.M, a.rows, a.K, a.chunks, error};
+        const size_t items = static_cast<size_t>(std::min(tokens * c.top_k, c.experts) + c.has_shared) * (moe::i8_rows(a.M) / 16);   // at most
+        moe::k_i8_gate_up_few<<<dim3(static_cast<unsigned>(std::min<size_t>(items, 512))), dim3(512), 0, s>>>(u);
+        r = hipGetLastError();
+    } else {
+        r = moe::launch_grouped<moe::kStoreMiddle, moe::kF32>(a, s);
+    }
+    if (r != hipSuccess) return r;
+    if (tokens <= kFewDown) {
         const moe::I8DownArgs d{L->down, L->down_s, L->middle, ids, L->groups, weights, shared_gate, y, tokens, c.hidden,
                                 c.intermediate, c.experts, c.top_k, c.top_k + c.has_shared, moe::i8_rows(c.hidden),
                                 moe::i8_chunks(c.intermediate), error};

@@ -18,7 +18,8 @@ __global__ __launch_bounds__(256) void k_i8_repack(const int8_t *__restrict__ co
     const int lane = static_cast<int>(i & 63), tile = static_cast<int>(i >> 6) & 3, per = i8_rows(rows) / kI8Block;
     const size_t block = i >> 8, chunk = block % chunks, at = block / chunks;   // at: 64 rows, over all matrices
     const size_t matrix = at / per;
-    const int row = static_cast<int>(at % per) * kI8Block + (lane >> 2 & 3) * 16 + tile * 4 + (lane & 3);
+    const int r = lane & 15, in = part == kI8Whole ? (tile >> 1) * 32 + (r >> 2) * 8 + (tile & 1) * 4 + (r & 3) : tile * 16 + r;
+    const int row = static_cast<int>(at % per) * kI8Block + in;
     const int col = static_cast<int>(chunk) * kI8Chunk + (lane >> 4) * 16;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows && col < cols) __builtin_memcpy(&v, codes + (matrix * rows + row) * cols + col, 16);
@@ -61,7 +62,7 @@ namespace {
 // run of the output's tiles, in columns of eight tiles of the matrix.
 template<int WR, int WC, int TM, int TN, int S, int KS, int Y>
 __global__ __launch_bounds__(64 * WR * WC) void k_i8_gemm(I8Args a) {
-    using Stream = I8Stream<WR, WC, TM, TN, S, KS, kStoreRows, false>;
+    using Stream = I8Stream<WR, WC, TM, TN, S, KS, kStoreRows, Y, false>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[Stream::Lds];
     const int tn = (a.N + Stream::BN - 1) / Stream::BN, total = a.tiles_m * tn, each = (total + 7) / 8;
     const int xcd = static_cast<int>(blockIdx.x & 7);
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_i8_gemm(I8Args a) {
     };
     Stream g(a, lds);
     g.run(xcd * each + static_cast<int>(blockIdx.x >> 3), static_cast<int>(gridDim.x >> 3), min(total, (xcd + 1) * each), fetch,
-          [&](const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) { g.template store_rows<Y>(it, params, acc); });
+          [&](const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) { g.store_rows(it, params, acc); });
 }
 
 // Few rows of x (at most 16): a workgroup takes 16 results of each, one tile of every
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_i8_few(I8FewArgs a) {
     } else {
         sx = a.sx[row];
     }
-    const int m = (tile >> 2) * kI8Block + (lane >> 4) * 16 + (tile & 3) * 4;
+    const int m = (tile >> 1) * 32 + (lane >> 4) * 8 + (tile & 1) * 4;
     if (m >= a.M) return;
     float v[4];
 #pragma unroll
@@ -240,7 +241,7 @@ inline constexpr int kFewElements = moe::kFewVectors * 64 * moe::kFewWaves * 8; 
 
 template<int WR, int WC, int TM, int TN, int S, int KS>
 int launch_gemm(moe::I8Args a, int y_type, hipStream_t s) {
-    using Stream = moe::I8Stream<WR, WC, TM, TN, S, KS, moe::kStoreRows, false>;
+    using Stream = moe::I8Stream<WR, WC, TM, TN, S, KS, moe::kStoreRows, moe::kF32, false>;   // sizes are those of any type
     a.tiles_m = (a.M + Stream::BM - 1) / Stream::BM;
     const size_t total = static_cast<size_t>(a.tiles_m) * ((a.N + Stream::BN - 1) / Stream::BN);
     const size_t resident = 256 * std::min(4, 160 * 1024 / Stream::Lds);
