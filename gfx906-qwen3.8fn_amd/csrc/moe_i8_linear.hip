@@ -258,6 +258,21 @@ moe::I8FewArgs few_args(const moe_i8_linear *L, const void *x, int64_t x_stride,
                           moe::i8_chunks(L->input), error};
 }
 
+// The product for quantised rows.  The output tile grows with the number of tiles, by
+// how they fill the 256 CUs.  us for forward (MI355X, launches in a row), bf16, tiles
+// of 64 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / 128 x 128 / 256 x 256:
+//         2048 x 2048 at   64:   5.4 /  6.2 /  6.7 /   -  / 11.1 / 24.9
+//                         333:  10.5 /  8.1 /  7.1 /  8.8 / 12.0 / 27.2
+//                        1032:  25.9 / 14.4 / 13.3 / 15.0 / 12.3 / 26.8
+//                        2500:    -  /   -  / 22.6 / 20.9 / 19.0 /   -
+//                        4096:  86.0 / 39.8 / 34.1 / 27.8 / 22.4 / 30.4
+//         2560 x 2560 at  700:    -  / 14.8 / 12.0 / 10.7 / 14.5 /   -
+//         2048 of 8192, 600:      -  / 28.7 / 28.9 / 24.7 / 35.6 /   -   (fp32)
+//         8192 x 8192 at   64:  21.1 / 17.6 / 26.6 /   -  / 47.1 / 84.5
+//                         256:  72.6 / 38.1 / 29.0 / 25.1 / 35.4 / 96.9
+//                         512:    -  / 68.9 / 56.6 / 46.7 / 41.3 / 86.6
+//                        2048:    -  /   -  /  223 /   -  /  152 /  118
+//                        8192:    -  /   -  /  903 /   -  /  599 /  437 (a library int8 product 439)
 int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, const float *scales, int columns, void *y,
                    int y_type, int64_t y_stride, hipStream_t s) {
     moe::I8Args a{};
@@ -279,8 +294,10 @@ int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, c
     if (a.N <= moe::kFewRows) return moe::launch_few<moe::kCodes>(few_args(L, codes, pitch, scales, columns, y, y_type, y_stride, nullptr), s);
     const long t256 = tiles(256, 256);
     if (t256 * 5 >= 3 * 256 * ((t256 + 255) / 256)) return launch_gemm<2, 4, 8, 4, 4, 1>(a, y_type, s);
-    if (tiles(128, 128) >= 144) return launch_gemm<4, 2, 2, 4, 4, 1>(a, y_type, s);
-    if (tiles(64, 64) >= 192) return launch_gemm<4, 2, 1, 2, 4, 2>(a, y_type, s);
+    const long t128 = tiles(64, 128);
+    if (t128 > 256) return launch_gemm<4, 2, 2, 4, 4, 1>(a, y_type, s);
+    if (t128 >= 150) return launch_gemm<2, 4, 2, 2, 4, 2>(a, y_type, s);
+    if (tiles(64, 64) >= 160) return launch_gemm<2, 4, 2, 1, 4, 2>(a, y_type, s);
     if (tiles(64, 32) >= 128) return launch_gemm<2, 2, 2, 1, 4, 2>(a, y_type, s);
     return launch_gemm<4, 1, 1, 1, 4, 4>(a, y_type, s);
 }
@@ -380,7 +397,9 @@ int moe_i8_linear_apply(moe_i8_linear *L, const void *x, int x_type, int64_t x_s
     const char *xb = static_cast<const char *>(x), *yb = static_cast<const char *>(y);
     const bool apart = xb + extent(x_stride, L->input, x_type) <= yb || yb + extent(y_stride, L->output, y_type) <= xb;
     // Every workgroup quantises all of the rows: in the product's kernel where each
-    // thread has few vectors of them.
+    // thread has few vectors of them (us, so / in two launches: 2048 x 2048 at 1, 4, 8
+    // rows 3.8 / 6.1, 4.2 / 6.2, 4.8 / 6.2; 8192 x 8192 at 1, 2 14.7 / 17.2, 15.9 / 16.9;
+    // rows of 2,048 of 8,192 at 4, 8 6.4 / 7.1, 7.5 / 7.3).
     if (columns <= moe::kFewRows && apart && columns * L->input <= kFewElements) {
         const moe::I8FewArgs f = few_args(L, x, x_stride, nullptr, columns, y, y_type, y_stride, error);
         if (x_type == MOE_F32) return moe::launch_few<moe::kF32>(f, s);

@@ -87,7 +87,8 @@ def make(k, m, seed=1, columns=0):
 
 SIZES = [(32, 1, 1), (64, 16, 1), (96, 17, 3), (2048, 64, 1), (160, 100, 15), (2080, 1000, 16), (1024, 130, 17), (352, 257, 40),
          (640, 2560, 64), (2048, 48, 65), (96, 2047, 100), (512, 300, 333), (2080, 1000, 333), (16384, 33, 5), (16384, 16, 130),
-         (128, 4099, 700), (2048, 2048, 1032), (256, 8192, 900), (64, 520, 5000), (192, 3001, 2100), (320, 4096, 4100)]
+         (128, 4099, 700), (2048, 2048, 1032), (256, 8192, 900), (64, 520, 5000), (192, 3001, 2100), (320, 4096, 4100), (640, 2560, 700), (352, 2100, 330),
+         (160, 4001, 2700), (8192, 2, 2), (8192, 100, 3), (16384, 40, 1), (4064, 33, 4)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
