@@ -323,11 +323,15 @@ __global__ __launch_bounds__(kGroupThreads) void k_i8_place(I8GroupArgs a) {
     for (int e = threadIdx.x; e < a.Ep; e += kGroupThreads) {
         int n = 0, b = 0;
         if (e < a.E) {
-#pragma unroll 32
-            for (int j = 0; j < a.blocks; ++j) {
-                const int c = a.g.counts[static_cast<size_t>(j) * a.Ep + e];
-                n += c;
-                if (j < static_cast<int>(blockIdx.x)) b += c;
+            for (int j0 = 0; j0 < a.blocks; j0 += 16) {
+                int c[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) c[i] = a.g.counts[static_cast<size_t>(min(j0 + i, a.blocks - 1)) * a.Ep + e];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    n += j0 + i < a.blocks ? c[i] : 0;
+                    b += j0 + i < static_cast<int>(blockIdx.x) ? c[i] : 0;
+                }
             }
         } else {
             n = a.tokens;

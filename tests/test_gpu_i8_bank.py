@@ -206,3 +206,63 @@ def test_graph_replay_with_new_groups():
                 R.close(y[lo:hi], R.product(q[lo:hi], s[lo:hi], codes[i], scales[i]), BF16)
         eager, _ = bank.forward(q, s, offsets, dtype=BF16)
         assert torch.equal(eager, y) and flag(e) == 0
+
+
+def test_many_experts_with_many_rows_each():
+    """The largest table of groups beside the largest tile."""
+    experts, k, m = 4096, 32, 17
+    codes, scales = R.weights(experts, m, k, 9)
+    bank = moe_ffn.MoeI8Bank(experts, k, m, codes, scales)
+    g = R.generator(9)
+    sizes = 66 + torch.randint(0, 12, (experts,), generator=g, device=DEV)
+    sizes[100:300] = 0
+    sizes[7], sizes[4095] = 900, 8000
+    offsets = torch.zeros(experts + 1, dtype=torch.int32, device=DEV)
+    offsets[1:] = sizes.cumsum(0)
+    rows = int(offsets[-1])
+    assert rows // experts > 64
+    q, s = R.quantise(torch.randn((rows, k), generator=g, device=DEV))
+    y, e = bank.forward(q, s, offsets)
+    assert flag(e) == 0
+    owner = torch.repeat_interleave(torch.arange(experts, device=DEV), sizes)
+    for at in range(0, rows, 20000):
+        o = owner[at:at + 20000]
+        ref = (codes[o].double() * q[at:at + 20000].double()[:, None]).sum(2) * s[at:at + 20000].double()[:, None] * scales[o].double()
+        R.close(y[at:at + 20000], ref, F32)
+
+
+def test_rows_past_32_bits():
+    """x's codes beyond 2^32 bytes and y's rows beyond 2^31 elements."""
+    k, m, rows = 16384, 16, 270000
+    codes, scales = R.weights(3, m, k, 10)
+    bank = moe_ffn.MoeI8Bank(3, k, m, codes, scales)
+    q = torch.zeros((rows, k), dtype=torch.int8, device=DEV)
+    s = torch.ones(rows, device=DEV)
+    some = torch.tensor([0, 1, 129999, 130000, 262143, 262144, 262145, 269999], device=DEV)
+    q[some] = torch.randint(-127, 128, (8, k), generator=R.generator(1), device=DEV).to(torch.int8)
+    wide = torch.empty((rows, 10000), dtype=BF16, device=DEV)
+    y = wide[:, 9000:9016]
+    _, e = bank.forward(q, s, ints([0, 130000, 130000, rows]), y)
+    assert flag(e) == 0
+    for r in some.tolist():
+        i = 0 if r < 130000 else 2
+        R.close(y[r:r + 1], R.product(q[r:r + 1], s[r:r + 1], codes[i], scales[i]), BF16)
+    assert not y[2:129999].any() and not y[262146:269999].any()
+
+
+def test_calls_of_one_bank_overlap():
+    codes, scales = R.weights(16, 512, 1024, 11)
+    bank = moe_ffn.MoeI8Bank(16, 1024, 512, codes, scales)
+    calls = []
+    for i in range(2):
+        q, s = R.quantise(torch.randn((900, 1024), generator=R.generator(i), device=DEV))
+        cuts = torch.randint(0, 901, (15,), generator=R.generator(i), device=DEV).sort().values.to(torch.int32)
+        offsets = torch.cat([ints([0]), cuts, ints([900])])
+        want, _ = bank.forward(q, s, offsets)
+        calls.append((q, s, offsets, want, torch.zeros_like(want), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for q, s, offsets, _, y, st in calls:
+            bank.forward(q, s, offsets, y=y, stream=st)
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want) for _, _, _, want, y, _ in calls)

@@ -246,3 +246,42 @@ def test_stack(dtype, n):
         stack.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(stack.outputs(), eager))
+
+
+@pytest.mark.parametrize("tokens,k", [(65536, 32), (40000, 3)])
+def test_largest_batches(tokens, k):
+    """Rows, routes and groups at the ends of their ranges; the first and last
+    tokens against 64 bits, and the rest against the same tokens in a batch of
+    their own."""
+    c = Case(tokens, 32, 32, 40, k, True, seed=30)
+    y, e = c.layer.forward(c.x, c.ids, c.w, shared_gate=c.gate)
+    assert flag(e) == 0
+    for part in (slice(0, 300), slice(tokens // 2 - 50, tokens // 2 + 50), slice(tokens - 300, tokens)):
+        ref = R.layer(c.x[part], c.bank, c.shared, c.ids[part], c.w[part], c.gate[part])
+        assert bool(((y[part].double() - ref[0]).abs() <= R.layer_bound(*ref, k, F32)).all())
+        again, _ = c.layer.forward(c.x[part], c.ids[part], c.w[part], shared_gate=c.gate[part])
+        assert torch.equal(again, y[part])
+
+
+@pytest.mark.parametrize("n", [1, 2, 31, 32, 33, 63, 64, 65, 204, 205])
+def test_limits_between_kernels(n):
+    """Either side of the sizes at which other kernels take over: the same bits
+    for a token whatever its batch (fp32)."""
+    c = Case(210, 320, 96, 24, 10, True, seed=31)
+    whole, e = c.layer.forward(c.x, c.ids, c.w, shared_gate=c.gate)
+    part, f = c.layer.forward(c.x[:n], c.ids[:n], c.w[:n], shared_gate=c.gate[:n])
+    assert flag(e) == 0 and flag(f) == 0
+    ref = R.layer(c.x[:n], c.bank, c.shared, c.ids[:n], c.w[:n], c.gate[:n])
+    assert bool(((part.double() - ref[0]).abs() <= R.layer_bound(*ref, 10, F32)).all())
+    assert torch.equal(whole[:n], part)
+
+
+@pytest.mark.parametrize("n", [5, 300])
+def test_on_a_stream_of_its_own(n):
+    c = Case(n, 256, 96, 12, 4, True, seed=32)
+    want, _ = c.layer.forward(c.x, c.ids, c.w)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got, e = c.layer.forward(c.x, c.ids, c.w, stream=side)
+    side.synchronize()
+    assert torch.equal(got, want) and flag(e) == 0

@@ -231,3 +231,27 @@ def test_forwards_of_one_handle_overlap():
             matrix.forward(*q, y=y, stream=st)
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("n", [9, 300])
+def test_results_past_32_bits(n):
+    """Rows of y that begin beyond 2^31 elements."""
+    matrix, codes, scales = make(96, 40, 12, n)
+    stride = (1 << 32) // n + 40
+    wide = torch.empty(stride * n, dtype=BF16, device=DEV)
+    y = wide.as_strided((n, 40), (stride, 1), 5)
+    x = torch.randn((n, 96), generator=R.generator(2), device=DEV).to(BF16)
+    e = torch.zeros(1, dtype=torch.int32, device=DEV)
+    matrix.apply(x, y, e)
+    q, s = R.quantise(x)
+    R.close(y, R.product(q, s, codes, scales), BF16)
+
+
+def test_rows_on_a_stream_of_their_own():
+    x = torch.randn((300, 1000), device=DEV)
+    want = moe_ffn.quantize_i8(x)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = moe_ffn.quantize_i8(x, stream=side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
