@@ -14,30 +14,46 @@ namespace {
 
 // The groups' row tiles, in LDS: group list[p] has the row tiles from first[p] to
 // first[p + 1], and its rows begin at row[e].  Groups of more than one tile come
-// first, with `big` tiles between them.  Offsets outside 0 .. N, or below the one
-// before, are drawn into that range and set bit 1; a group ends where the next
-// begins, and is empty where that is not after its own begin.
+// first, with `big` tiles between them.  Offsets outside 0 .. N are drawn into that
+// range, those below one before up to it, so that no row has two groups and the
+// tiles are at most N / BN and one a group; they set bit 1.
 inline constexpr int kMostExperts = 4096;
 struct GroupTable {
     int *first, *list, *row;   // [E + 1], [E], [E + 1]
     int experts, tiles, big;
 
     static constexpr size_t bytes(int experts) { return (static_cast<size_t>(experts) * 3 + 2) * 4; }
+    static constexpr size_t kShared = 16 * 5 * 4;   // and of its own
 
     __device__ __forceinline__ GroupTable(const I8Args &a, int BN, int *lds) : experts(a.experts) {
-        __shared__ int sums[16][4];
+        __shared__ int sums[16][4], wrong[16];
         first = lds;
         row = first + experts + 1;
         list = row + experts + 1;
         const int T = blockDim.x, per = (experts + T - 1) / T, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         const int lo = min(experts, static_cast<int>(threadIdx.x) * per), hi = min(experts, lo + per);
-        int bad = 0, mine[4] = {};   // big groups, their tiles, other groups, their tiles
+        bool bad = false;
         for (int e = lo; e < hi; ++e) {
-            const int from = a.offsets[e], to = a.offsets[e + 1], f = max(0, min(from, a.N)), t = max(0, min(to, a.N));
-            if (f != from || t != to || t < f) bad = 1;
-            row[e] = f;
-            if (e + 1 == experts) row[e + 1] = t;
-            const int n = (max(t - f, 0) + BN - 1) / BN, c = n > 1 ? 0 : 2;
+            const int from = a.offsets[e], to = a.offsets[e + 1];
+            bad |= from < 0 || to < from || to > a.N;
+            row[e] = max(0, min(from, a.N));
+            if (e + 1 == experts) row[e + 1] = max(0, min(to, a.N));
+        }
+        const uint64_t any = __builtin_amdgcn_ballot_w64(bad);
+        if (lane == 0) wrong[wave] = any != 0;
+        __syncthreads();
+        bad = false;
+        for (int w = 0; w < T / 64; ++w) bad |= wrong[w] != 0;
+        if (bad) {
+            if (threadIdx.x == 0) {
+                for (int e = 0; e < experts; ++e) row[e + 1] = max(row[e + 1], row[e]);
+                if (blockIdx.x == 0) atomicOr(a.error, 1);
+            }
+            __syncthreads();
+        }
+        int mine[4] = {};   // big groups, their tiles, other groups, their tiles
+        for (int e = lo; e < hi; ++e) {
+            const int n = (row[e + 1] - row[e] + BN - 1) / BN, c = n > 1 ? 0 : 2;
             mine[c] += 1;
             mine[c + 1] += n;
         }
@@ -63,7 +79,7 @@ struct GroupTable {
         }
         int at[2] = {incl[0] - mine[0], all[0] + incl[2] - mine[2]}, tile[2] = {incl[1] - mine[1], all[1] + incl[3] - mine[3]};
         for (int e = lo; e < hi; ++e) {
-            const int n = (max(row[e + 1] - row[e], 0) + BN - 1) / BN, c = n > 1 ? 0 : 1;
+            const int n = (row[e + 1] - row[e] + BN - 1) / BN, c = n > 1 ? 0 : 1;
             list[at[c]] = e;
             first[at[c]] = tile[c];
             ++at[c];
@@ -72,7 +88,6 @@ struct GroupTable {
         tiles = __builtin_amdgcn_readfirstlane(all[1] + all[3]);
         big = __builtin_amdgcn_readfirstlane(all[1]);
         if (threadIdx.x == 0) first[experts] = tiles;
-        if (bad && blockIdx.x == 0) atomicOr(a.error, 1);
         __syncthreads();
     }
     // The last place p with first[p] <= t, whose group has row tile t: 64 lanes look
@@ -137,10 +152,10 @@ __global__ __launch_bounds__(64 * WR * WC) void k_i8_grouped(I8Args a) {
 template<int WR, int WC, int TM, int TN, int S, int KS, int Form, int Y>
 hipError_t launch_tile(I8Args a, hipStream_t s) {
     using Stream = I8Stream<WR, WC, TM, TN, S, KS, Form, Y, true>;
-    static_assert(Stream::Lds + GroupTable::bytes(kMostExperts) + 256 <= 160 * 1024, "a CU's LDS");
+    static_assert(Stream::Lds + GroupTable::bytes(kMostExperts) + GroupTable::kShared <= 160 * 1024, "a CU's LDS");
     a.tiles_m = (a.rows + Stream::BM - 1) / Stream::BM;
     const size_t lds = GroupTable::bytes(a.experts);
-    const int resident = std::max(1, static_cast<int>(160 * 1024 / (Stream::Lds + lds + 256)));
+    const int resident = std::max(1, static_cast<int>(160 * 1024 / (Stream::Lds + lds + GroupTable::kShared)));
     const size_t items = (static_cast<size_t>(a.N) / Stream::BN + std::min(a.N, a.experts)) * a.tiles_m;   // at most
     const size_t grid = std::min((items + 7) / 8 * 8, static_cast<size_t>(256) * std::min(resident, 8));
     k_i8_grouped<WR, WC, TM, TN, S, KS, Form, Y><<<dim3(static_cast<unsigned>(grid)), dim3(64 * Stream::W), lds, s>>>(a);
@@ -390,9 +405,10 @@ struct I8FoldArgs {
 // tensor of a long prompt.  An output is (whole number) * sw[m] * sx; what is stored
 // is (whole number) * sw[m] * 2^p with the largest p that keeps 127 * 128 * I *
 // max |sw| of its expert within fp16, and the sum multiplies by sx * 2^-p in fp32.
-// So nothing overflows, and a value is off by at most 2^-11 of itself down to
-// 2^-30 of that bound, an eighth of what y's own rounding may cost.
-// One workgroup an expert: scale = 2^-p.
+// So nothing overflows, and a value is off by at most 2^-11 of itself, an eighth of
+// what y's own rounding may cost, down to 2^-26 of that bound, and by 2^-37 of it below.
+// One workgroup an expert: scale = 2^-p, or 0 where p is beyond +-100, whose layer
+// keeps fp32.
 __global__ __launch_bounds__(256) void k_i8_expert_scale(const float *sw, float *scale, int rows, int M, int I) {
     __shared__ uint32_t most[4];
     const float *s = sw + static_cast<size_t>(blockIdx.x) * rows;
@@ -405,7 +421,8 @@ __global__ __launch_bounds__(256) void k_i8_expert_scale(const float *sw, float 
     m = max(max(most[0], most[1]), max(most[2], most[3]));
     // max |sw| < 2^e, and 127 * 128 * I < 2^q: within fp16 where 2^(e + q + p) <= 2^15.
     const int e = m ? static_cast<int>(m >> 23) - 126 : 0, q = 14 + 32 - __builtin_clz(I);
-    if (threadIdx.x == 0) scale[blockIdx.x] = ldexpf(1.0f, m ? min(max(e + q - 15, -100), 100) : 0);
+    const int p = m ? e + q - 15 : 0;
+    if (threadIdx.x == 0) scale[blockIdx.x] = p < -100 || p > 100 ? 0.0f : ldexpf(1.0f, p);
 }
 
 // y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags of
@@ -767,6 +784,7 @@ struct moe_i8_layer {
     float *middle = nullptr;                       // [pairs][I]
     void *contrib = nullptr;                       // [pairs][H]
     float *expert_scale = nullptr;                 // [E']
+    bool halves = true;                            // contributions may be fp16
     int *dropped = nullptr;                        // flags of rows that are not used
     moe::I8Groups groups{};
 };
@@ -988,6 +1006,12 @@ int moe_i8_layer_create(const moe_i8_layer_config *c, const moe_i8_matrix *exper
         moe::k_i8_expert_scale<<<dim3(static_cast<unsigned>(E) + c->has_shared), dim3(256)>>>(
             reinterpret_cast<const float *>(L->mem + l.down_s), reinterpret_cast<float *>(L->ws + l.expert_scale), moe::i8_rows(H), H, I);
         r = hipDeviceSynchronize();
+        float scales[256];
+        for (size_t e = 0, n; e < E + c->has_shared && r == hipSuccess; e += n) {
+            n = std::min<size_t>(E + c->has_shared - e, 256);
+            r = hipMemcpy(scales, L->ws + l.expert_scale + e * 4, n * 4, hipMemcpyDeviceToHost);
+            if (r == hipSuccess) L->halves &= std::find(scales, scales + n, 0.0f) == scales + n;
+        }
     }
     if (r != hipSuccess) { release(L); return r; }
     L->gate_up = L->mem + l.gate_up;
@@ -1068,7 +1092,7 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     // what they hold raises no flag of this call, and SiLU(g) u is always finite.
     const moe::I8Rows mr{L->middle, c.intermediate, c.intermediate, static_cast<size_t>(pairs), L->m, L->m_pitch, L->m_s, L->dropped};
     if ((r = moe::launch_quantize_i8(mr, moe::kF32, s)) != hipSuccess) return r;
-    const bool halves = type == MOE_BF16;
+    const bool halves = type == MOE_BF16 && L->halves;
     a.blocks = L->down;
     a.sw = L->down_s;
     a.expert_scale = L->expert_scale;
@@ -1089,7 +1113,8 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
                             tokens, c.hidden, c.top_k, c.experts, c.has_shared, error};
     const dim3 grid(tokens), block(256);
     if (type == MOE_F32) moe::k_i8_fold<moe::kF32, false><<<grid, block, 0, s>>>(f);
-    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16, true><<<grid, block, 0, s>>>(f);
+    else if (halves) moe::k_i8_fold<moe::kBF16, true><<<grid, block, 0, s>>>(f);
+    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16, false><<<grid, block, 0, s>>>(f);
     else moe::k_i8_fold<moe::kF16, false><<<grid, block, 0, s>>>(f);
     return hipGetLastError();
 }

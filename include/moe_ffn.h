@@ -536,8 +536,7 @@ int moe_i8_bank_bytes(const moe_i8_bank *bank, size_t *weight_bytes);
  * without one rows <= x_rows.  Groups may be empty; rows before the first offset
  * and from the last one on are left as they are, and so is what lies between y's
  * rows.  Offsets that leave 0 .. rows or that decrease set bit 1 of `error`: they
- * are drawn into 0 .. rows, and a group whose end is not after its begin is empty
- * (a row that two groups then claim is one of their products).  A row whose index
+ * are drawn into 0 .. rows and up to the largest before them.  A row whose index
  * leaves 0 .. x_rows - 1 is zero and sets bit 1.  No workspace: calls on one
  * handle may overlap.  y may not overlap the inputs.  Enqueue only; the handle's
  * device need not be current. */
@@ -581,8 +580,12 @@ int moe_i8_layer_destroy(moe_i8_layer *layer);
 
 /* x, y [tokens][H] of `type` (MOE_F32, MOE_BF16, MOE_F16); ids, weights,
  * shared_gate and the sum as in moe_ffn_forward.  x's rows and the experts'
- * middle rows SiLU(gate) * up are quantised as moe_quantize_i8 does; the weighted
- * sum is fp32, y is rounded once.  Flags in `error` as in moe_ffn_forward: routes
+ * middle rows SiLU(gate) * up (the sigmoid within 8 half ulps) are quantised as
+ * moe_quantize_i8 does; the weighted sum is fp32, y is rounded once.  With bf16 y
+ * and more than 64 tokens an expert's output is held in fp16 with a scale of its own
+ * before the sum: off by at most 2^-11 of itself, or by 2^-24 I
+ * max |down scale of its expert| times its row's scale.  Otherwise a token's results
+ * are the same bits whatever its batch.  Flags in `error` as in moe_ffn_forward: routes
  * with a bad id or an id of an earlier rank are dropped and set bit 1.  So do
  * nonfinite input, whose token counts as zeros, a negative weight, which stays in
  * the sum, and a nonfinite weight, which gives up the token's routed sum: what is

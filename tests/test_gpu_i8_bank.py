@@ -121,6 +121,20 @@ def test_bad_offsets_flag():
         assert bool((out[0] == 3.0).all()) and bool((out[101] == 3.0).all())
 
 
+def test_offsets_that_go_back_and_forth():
+    """Offsets of which every other one decreases: no row is computed for two
+    groups, so that the work stays that of the rows."""
+    for experts, rows in ((6, 1000), (4096, 270000), (1025, 300)):
+        codes, scales = R.weights(experts, 17, 32, 12)
+        bank = moe_ffn.MoeI8Bank(experts, 32, 17, codes, scales)
+        q, s = R.quantise(torch.randn((rows, 32), generator=R.generator(experts), device=DEV))
+        offsets = torch.zeros(experts + 1, dtype=torch.int32, device=DEV)
+        offsets[1::2] = rows
+        y, e = bank.forward(q, s, offsets)
+        assert flag(e) == 1
+        R.close(y, R.product(q, s, codes[0], scales[0]), F32)
+
+
 def test_bad_index_gives_zero_rows():
     codes, scales = R.weights(2, 130, 96, 5)
     bank = moe_ffn.MoeI8Bank(2, 96, 130, codes, scales)

@@ -156,6 +156,29 @@ def test_nonfinite_weight_scales():
         assert flag(e) & 1 and bool(torch.isfinite(y).all()) and torch.equal(y[~hit], good[~hit])
 
 
+@pytest.mark.parametrize("down,up", [(120, -60), (-120, 40), (100, -60), (-95, 40)])
+def test_scales_at_the_ends_of_their_range(down, up):
+    """Scales of the down matrices, or of one expert's, far from 1: bf16 results
+    within the bound, and as the fp32 ones where fp16 cannot hold an output on the
+    way."""
+    n = 100
+    c = Case(n, 256, 96, 12, 4, True, seed=33)
+    x = c.x.to(BF16)
+    some = torch.zeros((12, 1), device=DEV)
+    some[3] = 1.0
+    for d in (torch.ones_like(some), some):
+        bank = [c.bank[0], (c.bank[1][0], c.bank[1][1] * 2.0 ** (up * d)), (c.bank[2][0], c.bank[2][1] * 2.0 ** (down * d))]
+        layer = moe_ffn.MoeI8Layer(256, 96, 12, 4, True, n, *bank, shared=c.shared)
+        y, e = layer.forward(x, c.ids, c.w)
+        full, f = layer.forward(x.float(), c.ids, c.w)
+        assert flag(e) == 0 and flag(f) == 0
+        ref = R.layer(x, bank, c.shared, c.ids, c.w, None)
+        assert bool(((y.double() - ref[0]).abs() <= R.layer_bound(*ref, 4, BF16)).all())
+        assert bool(((full.double() - ref[0]).abs() <= R.layer_bound(*ref, 4, F32)).all())
+        if abs(down) == 120:
+            assert torch.equal(y, full.to(BF16))
+
+
 def test_host_weights():
     c = Case(12, 96, 64, 6, 2, True, seed=11)
     host = lambda m: tuple(np.ascontiguousarray(t.cpu().numpy()) for t in m)  # noqa: E731
