@@ -12,8 +12,9 @@
 // q of tile i is row 32 (i / 2) + 8 g + 4 (i % 2) + q of the block, so that a lane's
 // results of two tiles are eight neighbours in a row of y and a store of 16-bit
 // ones fills 64 bytes of each row; with 16 neighbours in a lane, and stores that fill
-// every other 16 bytes, 2048 x 2048 at 1,032 fp32 rows took 19.8 us instead of 18.1.  What a product reads past a row of activations
-// meets the zeros past the matrix row, so rows need no padding.
+// every other 16 bytes, 2048 x 2048 at 1,032 fp32 rows took 19.8 us instead of 18.1.
+// What a product reads past a row of activations meets the zeros past the matrix
+// row, so rows need no padding.
 //
 // Gate and up matrices of an expert lie together as one of 2 I rows (I rounded up
 // to 64), in which 64 rows of both make two blocks: tile 2 i holds rows 16 i .. + 15
