@@ -259,20 +259,30 @@ moe::I8FewArgs few_args(const moe_i8_linear *L, const void *x, int64_t x_stride,
 }
 
 // The product for quantised rows.  The output tile grows with the number of tiles, by
-// how they fill the 256 CUs.  us for forward (MI355X, launches in a row), bf16, tiles
-// of 64 x 16 / 64 x 32 / 64 x 64 / 64 x 128 / 128 x 128 / 256 x 256:
-//         2048 x 2048 at   64:   5.4 /  6.2 /  6.7 /   -  / 11.1 / 24.9
-//                         333:  10.5 /  8.1 /  7.1 /  8.8 / 12.0 / 27.2
-//                        1032:  25.9 / 14.4 / 13.3 / 15.0 / 12.3 / 26.8
-//                        2500:    -  /   -  / 22.6 / 20.9 / 19.0 /   -
-//                        4096:  86.0 / 39.8 / 34.1 / 27.8 / 22.4 / 30.4
-//         2560 x 2560 at  700:    -  / 14.8 / 12.0 / 10.7 / 14.5 /   -
-//         2048 of 8192, 600:      -  / 28.7 / 28.9 / 24.7 / 35.6 /   -   (fp32)
-//         8192 x 8192 at   64:  21.1 / 17.6 / 26.6 /   -  / 47.1 / 84.5
-//                         256:  72.6 / 38.1 / 29.0 / 25.1 / 35.4 / 96.9
-//                         512:    -  / 68.9 / 56.6 / 46.7 / 41.3 / 86.6
-//                        2048:    -  /   -  /  223 /   -  /  152 /  118
-//                        8192:    -  /   -  /  903 /   -  /  599 /  437 (a library int8 product 439)
+// how they fill the 256 CUs, and is no wider than the rows of x.  us for forward (MI355X,
+// launches in a row), bf16, tiles of 64 x 16 / 64 x 32 in stages of four chunks / of two /
+// 64 x 64 / 64 x 128 / 128 x 128 / 256 x 256:
+//         2048 x 2048 at   40:   5.6 /  5.9 /  6.5 /   -  /   -  /   -  /   -
+//                         130:   8.9 /  6.0 /  6.6 /  7.0 /   -  /   -  /   -
+//                         300:    -  /  9.8 /  8.2 /  7.1 /   -  /   -  /   -
+//                         333:  10.5 /   -  /  8.1 /  7.1 /  8.8 / 12.0 / 27.2
+//                        1032:  25.9 /   -  / 14.4 / 13.3 / 15.0 / 12.3 / 26.8
+//                        2500:    -  /   -  /   -  / 22.6 / 20.9 / 19.0 /   -
+//                        4096:  86.0 /   -  / 39.8 / 34.1 / 27.8 / 22.4 / 30.4
+//         2560 x 2560 at  700:    -  /   -  / 14.8 / 12.0 / 10.7 / 14.5 /   -
+//         2048 of 8192, 200:      -  / 14.8 / 17.8 / 16.8 /   -  /   -  /   -
+//                       600:      -  /   -  / 28.7 / 28.9 / 24.7 / 35.6 /   -   (fp32)
+//         8192 x 8192 at   20:  14.4 / 17.9 / 26.3 / 27.0 /   -  /   -  /   -
+//                          64:  21.1 /   -  / 17.6 / 26.6 /   -  / 47.1 / 84.5
+//                         256:  72.6 /   -  / 38.1 / 29.0 / 25.1 / 35.4 / 96.9
+//                         512:    -  /   -  / 68.9 / 56.6 / 46.7 / 41.3 / 86.6
+//                        2048:    -  /   -  /   -  /  223 /   -  /  152 /  118
+//                        8192:    -  /   -  /   -  /  903 /   -  /  599 /  437 (a library int8 product 439)
+//         28,672 of 8192,  20:  62.1 / 39.3 / 36.5 / 39.6 / 59.0 / 51.0 / 83.5
+//         151,936 of 2048, 20:  86.0 / 53.2 / 52.2 / 57.1 / 78.9 / 55.8 / 78.4
+//                          64:   145 / 91.2 / 90.5 / 80.3 / 86.5 / 72.4 / 94.4   (fp32)
+//                         128:   261 /  150 /  135 /  107 / 90.4 / 83.6 / 92.5
+//                         200:   404 /  234 /  198 /  177 /  144 /  119 /  105
 int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, const float *scales, int columns, void *y,
                    int y_type, int64_t y_stride, hipStream_t s) {
     moe::I8Args a{};
@@ -293,13 +303,14 @@ int launch_product(const moe_i8_linear *L, const int8_t *codes, int64_t pitch, c
     const auto tiles = [&](long m, long n) { return ((a.M + m - 1) / m) * ((a.N + n - 1) / n); };
     if (a.N <= moe::kFewRows) return moe::launch_few<moe::kCodes>(few_args(L, codes, pitch, scales, columns, y, y_type, y_stride, nullptr), s);
     const long t256 = tiles(256, 256);
-    if (t256 * 5 >= 3 * 256 * ((t256 + 255) / 256)) return launch_gemm<2, 4, 8, 4, 4, 1>(a, y_type, s);
+    if (a.N > 128 && t256 * 5 >= 3 * 256 * ((t256 + 255) / 256)) return launch_gemm<2, 4, 8, 4, 4, 1>(a, y_type, s);
     const long t128 = tiles(64, 128);
-    if (t128 > 256) return launch_gemm<4, 2, 2, 4, 4, 1>(a, y_type, s);
-    if (t128 >= 150) return launch_gemm<2, 4, 2, 2, 4, 2>(a, y_type, s);
-    if (tiles(64, 64) >= 160) return launch_gemm<2, 4, 2, 1, 4, 2>(a, y_type, s);
-    if (tiles(64, 32) >= 128) return launch_gemm<2, 2, 2, 1, 4, 2>(a, y_type, s);
-    return launch_gemm<4, 1, 1, 1, 4, 4>(a, y_type, s);
+    if (a.N > 32 && t128 > 256) return launch_gemm<4, 2, 2, 4, 4, 1>(a, y_type, s);
+    if (a.N > 64 && t128 >= 150) return launch_gemm<2, 4, 2, 2, 4, 2>(a, y_type, s);
+    if (tiles(64, 16) <= 256) return launch_gemm<4, 1, 1, 1, 4, 4>(a, y_type, s);
+    if (tiles(64, 32) <= 256) return launch_gemm<2, 2, 2, 1, 4, 4>(a, y_type, s);
+    if (a.N <= 32) return launch_gemm<2, 2, 2, 1, 4, 2>(a, y_type, s);
+    return launch_gemm<2, 4, 2, 1, 4, 2>(a, y_type, s);
 }
 
 }  // namespace

@@ -121,6 +121,24 @@ def test_codes_at_their_ends_sum_exactly():
     assert torch.equal(y.double(), R.sums(x, codes).float().double())
 
 
+# 64 x 16, 64 x 32 in stages of four chunks and of two, 64 x 64, 64 x 128, 128 x 128, 256 x 256
+TILES = [(1000, 40), (1000, 300), (16999, 21), (8970, 40), (10230, 70), (16641, 33), (40960, 129)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [32, 96, 416])
+@pytest.mark.parametrize("m,n", TILES)
+def test_every_tile(dtype, k, m, n):
+    """Every tile on short rows, whose last stage is cut."""
+    codes, scales = R.weights(1, m, k, m + k)
+    q, s = R.quantise(0.1 * torch.randn((n, k), generator=R.generator(n), device=DEV))
+    matrix = moe_ffn.MoeI8Linear(k, m, codes[0], scales[0])
+    y = torch.full((n + 1, m), 7.0, dtype=dtype, device=DEV)
+    matrix.forward(q, s, y[:n])
+    R.close(y[:n], R.product(q, s, codes[0], scales[0]), dtype)
+    assert bool((y[n] == 7.0).all())
+
+
 @pytest.mark.parametrize("n", [2, 50, 700])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strided_rows(dtype, n):
