@@ -7,6 +7,7 @@
 #include "moe_i8.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <new>
 
 namespace moe {
@@ -175,14 +176,27 @@ hipError_t launch_tile(I8Args a, hipStream_t s) {
 // layer: 128 tokens - / 258 / 262 / 275, 512 - / 313 / 316 / 327, 1,024 - / 353 / 347 / 361,
 // 4,096 - / 688 / 573 / 539; its down (K = 512, an item's start and end weigh more):
 // 128 tokens 271 / 273 / 261 / 269, 512 331 / 328 / 315 / 324, 4,096 688 / 699 / 576 / 519.
+// A few experts: smaller tiles where larger ones leave CUs without any.  Bank of 8
+// such matrices at 100, 300, 1,000 and 4,000 rows, bf16:
+//   64 x 16                          7.7 / 10.7 / 24.1 / 64.2
+//   64 x 32, stages of four chunks   8.0 / 10.4 / 18.9 / 42.3
+//   64 x 32                          8.6 / 11.8 / 19.5 / 38.6
+//   128 x 64                        10.9 / 15.2 / 13.7 / 24.8
+//   256 x 128                       15.6 / 21.5 / 25.6 / 23.9
+// Layer of 8 experts, 2048/512, top-2, gate and up by 64 x 32 / 128 x 32 / 128 x 64 / 256 x 128:
+// 33 tokens 28.6 / 31.0 / 33.9 / 39.4, 400 37.0 / 34.4 / 38.5 / 47.9, 1,000 59.1 / 56.6 / 48.6 / 54.4.
 template<int Form, int Y>
 hipError_t launch_grouped(const I8Args &a, hipStream_t s) {
     const int mean = a.N / a.experts;
-    if (mean > 64) return launch_tile<4, 2, 4, 4, 4, 1, Form, Y>(a, s);
+    // Tiles of groups that end, on average, in the middle of one.
+    const auto tiles = [&](int m, int n) { return static_cast<int64_t>((a.rows + m - 1) / m) * (a.N / n + (std::min(a.N, a.experts) + 1) / 2); };
+    if (mean > 64 && tiles(256, 128) >= 128) return launch_tile<4, 2, 4, 4, 4, 1, Form, Y>(a, s);
     if constexpr (Form == kStoreMiddle) {   // pairs of tiles
-        if (mean <= 12) return launch_tile<4, 1, 2, 2, 4, 2, Form, Y>(a, s);
+        if (tiles(64, 32) <= 256) return launch_tile<2, 2, 2, 1, 4, 4, Form, Y>(a, s);
+        if (mean <= 12 || tiles(128, 64) <= 256) return launch_tile<4, 1, 2, 2, 4, 2, Form, Y>(a, s);
     } else {
-        if (a.N <= a.experts / 2) return launch_tile<4, 1, 1, 1, 4, 4, Form, Y>(a, s);
+        if (a.N <= a.experts / 2 || tiles(64, 16) <= 256) return launch_tile<4, 1, 1, 1, 4, 4, Form, Y>(a, s);
+        if (tiles(64, 32) <= 256) return launch_tile<2, 2, 2, 1, 4, 4, Form, Y>(a, s);
         if (mean <= 12 && a.chunks > 16) return launch_tile<4, 1, 1, 2, 4, 2, Form, Y>(a, s);
     }
     return launch_tile<4, 1, 2, 4, 4, 1, Form, Y>(a, s);
@@ -401,8 +415,8 @@ struct I8FoldArgs {
     int tokens, H, k, E, shared;
     int *error;
 };
-// fp16 for the experts' outputs, where y is bf16: half the bytes of the largest
-// tensor of a long prompt.  An output is (whole number) * sw[m] * sx; what is stored
+// fp16 for the experts' outputs, where y is bf16 and the tokens are more than 64: half
+// the bytes of the largest tensor of a long prompt.  An output is (whole number) * sw[m] * sx; what is stored
 // is (whole number) * sw[m] * 2^p with the largest p that keeps 127 * 128 * I *
 // max |sw| of its expert within fp16, and the sum multiplies by sx * 2^-p in fp32.
 // So nothing overflows, and a value is off by at most 2^-11 of itself, an eighth of
@@ -630,7 +644,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     if (flags) atomicOr(a.error, flags);
 }
 
-// ------------------------------------- few tokens: down and the sum in one ---
+// ----------------- few tokens an expert (down_in_one): down and the sum in one ---
 // Workgroup (t, slice of `tiles` tiles of 16 rows); wave w takes ranks w, w + W, ..
 // It quantises the rank's middle row into LDS in pieces of eight chunks and streams
 // the expert's tiles past it, a tile's chunks of a piece at a time with the next
@@ -743,7 +757,7 @@ hipError_t launch_down_fold(const I8DownArgs &a, int type, hipStream_t s) {
     const int row_tiles = a.rows / 16;
     // Row tiles a workgroup: the fewest on the busiest CU, and of such choices the one
     // with the fewest workgroups a CU (one / two / four first, us a layer of 2048/512:
-    // 4 tokens 33.2 / 37.5 / 37.3, 8 52.0 / 54.5 / 62.1, 64 226.5 / 227.1 / 229.3).
+    // 4 tokens 33.2 / 37.5 / 37.3, 8 52.0 / 54.5 / 62.1).
     int tiles = 1, best = 1 << 30, fewest = 0;
     for (int n = 1; n <= kDownTiles; ++n) {
         const int rounds = (a.T * ((row_tiles + n - 1) / n) + 255) / 256;
@@ -834,7 +848,22 @@ bool valid_config(const moe_i8_layer_config *c) {
            c->max_tokens <= 65536;
 }
 
-inline constexpr int kFewDown = 64;   // tokens up to which down and the sum are one launch
+// Down and the sum in one launch, which reads an expert again, from L2, for each of its
+// tokens, or down grouped by expert, in three.  The first where what it reads again
+// of the routed experts is less than 100 MB of an evenly routed batch (the shared one's
+// reads are cheap: all tokens' are near each other); us a layer, one launch / three:
+//   2048/512, top-10 of 512      16 tokens 88.3 / 106   24 122 / 136   32 148 / 150   48 183 / 176
+//   2048/768, top-8 of 128       16        91.0 / 96.3  24 118 / 109   32 123 / 117   48 139 / 118
+//   2048/1024, top-6 of 64       16        71.9 / 76.0  24 95.8 / 87.4 32 92.7 / 86.7 48 108 / 84.8
+//   4096/2048, top-2 of 8         8        49.9 / 53.6  16 61.6 / 55.7 32 65.6 / 56.2 48 70.7 / 55.5
+//   2048/512, top-2 of 8          8        16.1 / 23.0  16 18.6 / 23.2 48 25.5 / 27.8 64 29.2 / 28.2
+// Up to 64 tokens, so that results of bf16 batches up to there have the same bits.
+inline constexpr int kFewDown = 64;
+bool down_in_one(const moe_i8_layer_config &c, int tokens) {
+    const double E = c.experts, pairs = static_cast<double>(tokens) * c.top_k;
+    const double reached = E * (1.0 - std::pow(1.0 - c.top_k / E, tokens));
+    return tokens <= kFewDown && (pairs - reached) * c.hidden * c.intermediate <= 100e6;
+}
 
 struct LayerLayout {
     size_t gate_up, down, gate_up_s, down_s, weights;   // offsets and end of the weights
@@ -1082,7 +1111,7 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
         r = moe::launch_grouped<moe::kStoreMiddle, moe::kF32>(a, s);
     }
     if (r != hipSuccess) return r;
-    if (tokens <= kFewDown) {
+    if (down_in_one(c, tokens)) {
         const moe::I8DownArgs d{L->down, L->down_s, L->middle, ids, L->groups, weights, shared_gate, y, tokens, c.hidden,
                                 c.intermediate, c.experts, c.top_k, c.top_k + c.has_shared, moe::i8_rows(c.hidden),
                                 moe::i8_chunks(c.intermediate), error};
@@ -1092,7 +1121,7 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     // what they hold raises no flag of this call, and SiLU(g) u is always finite.
     const moe::I8Rows mr{L->middle, c.intermediate, c.intermediate, static_cast<size_t>(pairs), L->m, L->m_pitch, L->m_s, L->dropped};
     if ((r = moe::launch_quantize_i8(mr, moe::kF32, s)) != hipSuccess) return r;
-    const bool halves = type == MOE_BF16 && L->halves;
+    const bool halves = type == MOE_BF16 && L->halves && tokens > kFewDown;
     a.blocks = L->down;
     a.sw = L->down_s;
     a.expert_scale = L->expert_scale;

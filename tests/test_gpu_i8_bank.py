@@ -68,6 +68,25 @@ def test_ragged(dtype, case):
     check(bank, codes, scales, sizes, dtype, gather=max(1, sum(sizes) // 3), seed=case + 50)
 
 
+# Every tile: 64 x 16, 64 x 32 in stages of four chunks and of two, 128 x 64, 256 x 128.
+TILES = [(4, 96, 1000, 50), (4, 416, 1000, 400), (64, 1088, 1000, 500), (8, 416, 1000, 600), (8, 96, 1000, 600), (4, 96, 4000, 900),
+         (4, 416, 4001, 1000)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("experts,k,m,rows", TILES)
+def test_every_tile(dtype, experts, k, m, rows):
+    codes, scales = R.weights(experts, m, k, rows)
+    bank = moe_ffn.MoeI8Bank(experts, k, m, codes, scales)
+    g = torch.Generator().manual_seed(rows + k)
+    share = torch.rand(experts, generator=g) ** 2
+    share[1] = 0.0
+    sizes = [int(v) for v in (share / share.sum() * rows).floor()]
+    sizes[0] += rows - sum(sizes)
+    check(bank, codes, scales, sizes, dtype, seed=k, lead=3, extra=5)
+    check(bank, codes, scales, sizes, dtype, gather=77, seed=k)
+
+
 def test_rows_outside_the_groups_stay():
     codes, scales = R.weights(3, 80, 64, 1)
     bank = moe_ffn.MoeI8Bank(3, 64, 80, codes, scales)

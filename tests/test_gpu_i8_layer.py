@@ -67,6 +67,25 @@ def test_layer(dtype, shape):
         c.check(dtype, gate=True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("shape", [(40, 160, 512, 64, 4, True), (600, 160, 512, 16, 4, True), (1000, 160, 544, 16, 4, False),
+                                   (1000, 2048, 160, 16, 4, True), (100, 512, 1056, 64, 4, True)])
+def test_every_tile(dtype, shape):
+    """The tiles of the grouped products that the shapes above do not reach."""
+    Case(*shape, seed=34).check(dtype, gate=shape[5])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_shared_experts_of_a_small_batch(dtype):
+    """Few tokens whose experts are read once for all of them: the same bits for a
+    token as in a batch in which its experts are its own."""
+    c = Case(64, 4096, 2048, 8, 2, True, seed=35)
+    y = c.check(dtype, gate=True)
+    for n in (1, 4, 33):
+        part, e = c.layer.forward(c.x[:n].to(dtype), c.ids[:n], c.w[:n], shared_gate=c.gate[:n])
+        assert flag(e) == 0 and torch.equal(part, y[:n])
+
+
 def test_one_handle_takes_batches_of_all_sizes():
     """Rows and routes of an earlier, larger batch change nothing."""
     big = Case(600, 256, 64, 16, 4, True, seed=3)
