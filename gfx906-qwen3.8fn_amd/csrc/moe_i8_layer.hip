@@ -567,11 +567,20 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
     uint4 f[U][2];
     const uint8_t *w = a.blocks;
     const auto load = [&](int c0) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const size_t at = static_cast<size_t>(min(c0 + u * W, a.chunks - 1)) * kI8BlockBytes;   // past the last: it again, not used
+        const auto one = [&](int u) {
+            const size_t at = static_cast<size_t>(c0 + u * W) * kI8BlockBytes;
             f[u][0] = load_once(w + at);
             f[u][1] = load_once(w + at + 1024);
+        };
+        // All at once, without a branch between them; where there are fewer, no others
+        // in their place (2560/640, 40 chunks, 8 tokens 88.4 -> 81.1 us a layer).
+        if (c0 + (U - 1) * W < a.chunks) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) one(u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c0 + u * W < a.chunks) one(u);
         }
     };
     const auto select = [&](int item) {
@@ -601,11 +610,18 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4))) void k
             for (int t = 0; t < Most; ++t) {
                 if (t >= tiles) break;
                 uint4 v[U];
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    const int c = min(c0 + u * W, a.chunks - 1);
+                const auto part = [&](int u) {
+                    const int c = c0 + u * W;
                     v[u] = make_uint4(0u, 0u, 0u, 0u);
                     if (c * kI8Chunk + (lane >> 4) * 16 < a.K) v[u] = *reinterpret_cast<const uint4 *>(x[t] + c * kI8Chunk);
+                };
+                if (c0 + (U - 1) * W < a.chunks) {
+#pragma unroll
+                    for (int u = 0; u < U; ++u) part(u);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (c0 + u * W < a.chunks) part(u);
                 }
 #pragma unroll
                 for (int u = 0; u < U; ++u) {

@@ -106,10 +106,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_i8_few(I8FewArgs a) {
     const uint8_t *w = a.blocks + static_cast<size_t>(tile >> 2) * a.chunks * kI8BlockBytes + (tile & 3) * 1024 + lane * 16;
     uint4 f[U];
     const auto load = [&](int c0) {
+        const auto one = [&](int u) { f[u] = load_once(w + static_cast<size_t>(c0 + u * kFewWaves) * kI8BlockBytes); };
+        // All at once, without a branch between them; where there are fewer, no others
+        // in their place (8192 of 2560 at 8 rows 9.4 -> 8.7 us).
+        if (c0 + (U - 1) * kFewWaves < a.chunks) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int c = min(c0 + u * kFewWaves, a.chunks - 1);   // past the last one: it again, not used
-            f[u] = load_once(w + static_cast<size_t>(c) * kI8BlockBytes);
+            for (int u = 0; u < U; ++u) one(u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (c0 + u * kFewWaves < a.chunks) one(u);
         }
     };
     load(wave);
