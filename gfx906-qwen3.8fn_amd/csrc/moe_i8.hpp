@@ -185,9 +185,8 @@ __device__ __forceinline__ float silu_product(float g, float u, int &flags) {
     return 0.0f;
 }
 
-// What a product writes: rows of y; SiLU(gate) * up in fp32 from pairs of gate and up;
-// or rows with 1 / expert_scale[e] in place of the row's scale.
-enum { kStoreRows = 0, kStoreMiddle = 1, kStoreHalves = 2 };
+// What a product writes: rows of y, or SiLU(gate) * up in fp32 from pairs of gate and up.
+enum { kStoreRows = 0, kStoreMiddle = 1 };
 
 struct I8Args {
     const uint8_t *blocks;    // [experts][rows / 64][chunks] blocks
@@ -204,7 +203,6 @@ struct I8Args {
     int M, N, K, chunks;      // results in a row (kStoreMiddle: of either half), rows of the product
     int rows;                 // of the blocks: i8_rows(M), twice that for pairs
     int tiles_m;
-    const float *expert_scale;   // [experts], kStoreHalves
     int *error;
 };
 
@@ -460,9 +458,6 @@ struct I8Stream {
     __device__ __forceinline__ void store_rows(const I8Item &it, const float *params, const i32x4 (&acc)[TM][TN]) const {
         constexpr int G = TM < 2 ? 1 : 2, R = 4 * G;   // tiles of a run, its length
         const int g = lane >> 4;
-        float halves = 1.0f;
-        if constexpr (Form == kStoreHalves)   // a scalar load, which no wait for others counts
-            halves = 1.0f / ((const __attribute__((address_space(4))) float *)a.expert_scale)[it.e];
 #pragma unroll
         for (int p = 0; p < TM; p += G) {
             const int tile = wr * TM + p, first = (tile >> 1) * 32, m = first + g * 8 + (tile & 1) * 4;
@@ -474,7 +469,7 @@ struct I8Stream {
             for (int t = 0; t < TN; ++t) {
                 const int n = (wc * TN + t) * 16 + (lane & 15);
                 if (n >= it.cols) continue;
-                const float sx = Form == kStoreHalves ? halves : params[PA + n];
+                const float sx = params[PA + n];
                 float v[R];
 #pragma unroll
                 for (int i = 0; i < R; ++i) v[i] = static_cast<float>(acc[p + i / 4][t][i % 4]) * (sx * sw[i]);

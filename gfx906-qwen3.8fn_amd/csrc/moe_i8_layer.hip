@@ -405,69 +405,35 @@ hipError_t launch_prepare_i8(I8GroupArgs a, const I8Rows &x, int type, hipStream
 // ------------------------------------------------------------------- sums ---
 inline constexpr int kDownPairs = 33;   // 32 routes and the shared expert
 struct I8FoldArgs {
-    const void *c;             // [pairs][H] outputs of the experts: fp32, or fp16 as k_i8_expert_scale says
-    const float *c_scale;      // fp16: [pairs] scales of the rows
-    const float *expert_scale; // fp16: [E'] scales of the experts
-    const int32_t *ids;
+    const float *c;            // [pairs][H] outputs of the experts
     I8Groups g;
     const float *weights, *shared_gate;
     void *y;
     int tokens, H, k, E, shared;
     int *error;
 };
-// fp16 for the experts' outputs, where y is bf16 and the tokens are more than 64: half
-// the bytes of the largest tensor of a long prompt.  An output is (whole number) * sw[m] * sx; what is stored
-// is (whole number) * sw[m] * 2^p with the largest p that keeps 127 * 128 * I *
-// max |sw| of its expert within fp16, and the sum multiplies by sx * 2^-p in fp32.
-// So nothing overflows, and a value is off by at most 2^-11 of itself, an eighth of
-// what y's own rounding may cost, down to 2^-26 of that bound, and by 2^-37 of it below.
-// One workgroup an expert: scale = 2^-p, or 0 where p is beyond +-100, whose layer
-// keeps fp32.
-__global__ __launch_bounds__(256) void k_i8_expert_scale(const float *sw, float *scale, int rows, int M, int I) {
-    __shared__ uint32_t most[4];
-    const float *s = sw + static_cast<size_t>(blockIdx.x) * rows;
-    uint32_t m = 0;
-    for (int i = threadIdx.x; i < M; i += 256)
-        if (isfinite(s[i])) m = max(m, magnitude(s[i]));
-    m = wave_max(m);
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = max(max(most[0], most[1]), max(most[2], most[3]));
-    // max |sw| < 2^e, and 127 * 128 * I < 2^q: within fp16 where 2^(e + q + p) <= 2^15.
-    const int e = m ? static_cast<int>(m >> 23) - 126 : 0, q = 14 + 32 - __builtin_clz(I);
-    const int p = m ? e + q - 15 : 0;
-    if (threadIdx.x == 0) scale[blockIdx.x] = p < -100 || p > 100 ? 0.0f : ldexpf(1.0f, p);
-}
-
 // y = +0 + w_0 c_0 + .. in rank order, + sigmoid(gate) shared, with the flags of
 // moe_ffn_forward's sum, rounded once: a workgroup a token, V elements (16 bytes of
 // the contributions) a thread, eight rows' loads in flight.
-template<int T, bool Halves>
+template<int T>
 __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
-    constexpr int V = Halves ? 8 : 4;
-    typedef float f4 __attribute__((ext_vector_type(4)));
-    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-    using Row = std::conditional_t<Halves, h8, f4>;
-    using Value = std::conditional_t<Halves, _Float16, float>;
+    constexpr int V = 4;
+    typedef float Row __attribute__((ext_vector_type(4)));
     __shared__ int place[kDownPairs];
-    __shared__ float weight[kDownPairs], scale[kDownPairs];
+    __shared__ float weight[kDownPairs];
     const size_t t = blockIdx.x;
     int flags = 0;
     if (threadIdx.x <= static_cast<unsigned>(a.k)) {
         const int r = threadIdx.x;
         const size_t route = t * a.k + r;
         int at = -1;
-        float w = 1.0f, s = 1.0f;
+        float w = 1.0f;
         if (r < a.k) {
             at = a.g.place[route];
             w = a.weights[route];
-            if (at >= 0) {
-                if (!isfinite(w)) { flags |= 1; w = 0.0f; }
-                if constexpr (Halves) s = a.c_scale[at] * a.expert_scale[a.ids[route]];
-            }
+            if (at >= 0 && !isfinite(w)) { flags |= 1; w = 0.0f; }
         } else if (a.shared) {
             at = a.g.offsets[a.E] + static_cast<int>(t);
-            if constexpr (Halves) s = a.c_scale[at] * a.expert_scale[a.E];
             if (a.shared_gate) {
                 float g = a.shared_gate[t];
                 if (!isfinite(g)) { flags |= 1; g = 0.0f; }
@@ -477,7 +443,6 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
         }
         place[r] = at;
         weight[r] = w;
-        scale[r] = s;
     }
     // A weight that is not finite gives up the routed sum, such a gate all of it.
     const uint64_t first = __builtin_amdgcn_ballot_w64(flags != 0);   // of the first wave, which has them all
@@ -488,7 +453,7 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
     const bool no_routes = (lost & ((uint64_t{1} << a.k) - 1)) != 0, no_shared = (lost >> a.k & 1) != 0;
     for (int h = threadIdx.x * V; h < a.H; h += 256 * V) {
         const auto load = [&](int r) {
-            return __builtin_nontemporal_load(reinterpret_cast<const Row *>(static_cast<const Value *>(a.c) + static_cast<size_t>(place[r]) * a.H + h));
+            return __builtin_nontemporal_load(reinterpret_cast<const Row *>(a.c + static_cast<size_t>(place[r]) * a.H + h));
         };
         int f[V] = {};
         float v[V] = {};
@@ -502,11 +467,10 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
                 if (r0 + q >= a.k || place[r0 + q] < 0) continue;
-                const float w = weight[r0 + q], s = scale[r0 + q];
+                const float w = weight[r0 + q];
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    float c = static_cast<float>(x[q][e]);
-                    if constexpr (Halves) c = c * s;
+                    float c = x[q][e];
                     if (!isfinite(c)) { f[e] |= 1; c = 0.0f; }
                     float p = w * c;
                     if (!isfinite(p)) { f[e] |= 2; p = 0.0f; }
@@ -521,19 +485,14 @@ __global__ __launch_bounds__(256) void k_i8_fold(I8FoldArgs a) {
             flags |= f[e];
             if (a.shared) {
                 int sf = no_shared ? 1 : 0;
-                float c = static_cast<float>(shared[e]);
-                if constexpr (Halves) c = c * scale[a.k];
+                float c = shared[e];
                 if (!isfinite(c)) { sf |= 1; flags |= 1; c = 0.0f; }
                 v[e] = v[e] + weight[a.k] * c;
                 if (!isfinite(v[e])) { sf |= 2; flags |= 2; v[e] = 0.0f; }
                 if (sf) v[e] = 0.0f;
             }
         }
-#pragma unroll
-        for (int e = 0; e < V; e += 4) {
-            const float o[4] = {v[e], v[e + 1], v[e + 2], v[e + 3]};
-            store4<T>(a.y, t * a.H + h + e, o);
-        }
+        store4<T>(a.y, t * a.H + h, v);
     }
     if (flags) atomicOr(a.error, flags);
 }
@@ -812,9 +771,7 @@ struct moe_i8_layer {
     int8_t *x = nullptr, *m = nullptr;             // quantised rows of x and of the middle
     float *x_s = nullptr, *m_s = nullptr;
     float *middle = nullptr;                       // [pairs][I]
-    void *contrib = nullptr;                       // [pairs][H]
-    float *expert_scale = nullptr;                 // [E']
-    bool halves = true;                            // contributions may be fp16
+    float *contrib = nullptr;                      // [pairs][H]
     int *dropped = nullptr;                        // flags of rows that are not used
     moe::I8Groups groups{};
 };
@@ -873,7 +830,7 @@ bool valid_config(const moe_i8_layer_config *c) {
 //   2048/1024, top-6 of 64       16        71.9 / 76.0  24 95.8 / 87.4 32 92.7 / 86.7 48 108 / 84.8
 //   4096/2048, top-2 of 8         8        49.9 / 53.6  16 61.6 / 55.7 32 65.6 / 56.2 48 70.7 / 55.5
 //   2048/512, top-2 of 8          8        16.1 / 23.0  16 18.6 / 23.2 48 25.5 / 27.8 64 29.2 / 28.2
-// Up to 64 tokens, so that results of bf16 batches up to there have the same bits.
+// Up to 64 tokens, where three launches have caught up on every shape above.
 inline constexpr int kFewDown = 64;
 bool down_in_one(const moe_i8_layer_config &c, int tokens) {
     const double E = c.experts, pairs = static_cast<double>(tokens) * c.top_k;
@@ -883,7 +840,7 @@ bool down_in_one(const moe_i8_layer_config &c, int tokens) {
 
 struct LayerLayout {
     size_t gate_up, down, gate_up_s, down_s, weights;   // offsets and end of the weights
-    size_t x, x_s, m, m_s, middle, contrib, offsets, token, place, counts, expert_scale, active, groups, dropped, workspace;
+    size_t x, x_s, m, m_s, middle, contrib, offsets, token, place, counts, active, groups, dropped, workspace;
 };
 LayerLayout layout(const moe_i8_layer_config &c) {
     LayerLayout l{};
@@ -911,7 +868,6 @@ LayerLayout layout(const moe_i8_layer_config &c) {
     l.token = take(P * 4);
     l.place = take(T * c.top_k * 4);
     l.counts = take(std::min<size_t>(128, (T + 63) / 64) * Ep * 4);
-    l.expert_scale = take(Ep * 4);
     l.active = take(Ep * 16);
     l.groups = take(4);
     l.dropped = take(4);
@@ -1047,29 +1003,17 @@ int moe_i8_layer_create(const moe_i8_layer_config *c, const moe_i8_matrix *exper
     };
     if (r == hipSuccess) bank(experts, 0, E);
     if (r == hipSuccess && c->has_shared) bank(shared, E, 1);
-    if (r == hipSuccess) {
-        moe::k_i8_expert_scale<<<dim3(static_cast<unsigned>(E) + c->has_shared), dim3(256)>>>(
-            reinterpret_cast<const float *>(L->mem + l.down_s), reinterpret_cast<float *>(L->ws + l.expert_scale), moe::i8_rows(H), H, I);
-        r = hipDeviceSynchronize();
-        float scales[256];
-        for (size_t e = 0, n; e < E + c->has_shared && r == hipSuccess; e += n) {
-            n = std::min<size_t>(E + c->has_shared - e, 256);
-            r = hipMemcpy(scales, L->ws + l.expert_scale + e * 4, n * 4, hipMemcpyDeviceToHost);
-            if (r == hipSuccess) L->halves &= std::find(scales, scales + n, 0.0f) == scales + n;
-        }
-    }
     if (r != hipSuccess) { release(L); return r; }
     L->gate_up = L->mem + l.gate_up;
     L->down = L->mem + l.down;
     L->gate_up_s = reinterpret_cast<const float *>(L->mem + l.gate_up_s);
     L->down_s = reinterpret_cast<const float *>(L->mem + l.down_s);
-    L->expert_scale = reinterpret_cast<float *>(L->ws + l.expert_scale);
     L->x = reinterpret_cast<int8_t *>(L->ws + l.x);
     L->m = reinterpret_cast<int8_t *>(L->ws + l.m);
     L->x_s = reinterpret_cast<float *>(L->ws + l.x_s);
     L->m_s = reinterpret_cast<float *>(L->ws + l.m_s);
     L->middle = reinterpret_cast<float *>(L->ws + l.middle);
-    L->contrib = L->ws + l.contrib;
+    L->contrib = reinterpret_cast<float *>(L->ws + l.contrib);
     const auto ints = [&](size_t at) { return reinterpret_cast<int32_t *>(L->ws + at); };
     L->dropped = ints(l.dropped);
     L->groups = moe::I8Groups{ints(l.offsets), ints(l.token), ints(l.place), ints(l.counts),
@@ -1137,10 +1081,8 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     // what they hold raises no flag of this call, and SiLU(g) u is always finite.
     const moe::I8Rows mr{L->middle, c.intermediate, c.intermediate, static_cast<size_t>(pairs), L->m, L->m_pitch, L->m_s, L->dropped};
     if ((r = moe::launch_quantize_i8(mr, moe::kF32, s)) != hipSuccess) return r;
-    const bool halves = type == MOE_BF16 && L->halves && tokens > kFewDown;
     a.blocks = L->down;
     a.sw = L->down_s;
-    a.expert_scale = L->expert_scale;
     a.x = L->m;
     a.sx = L->m_s;
     a.pitch = L->m_pitch;
@@ -1152,15 +1094,12 @@ int moe_i8_layer_forward(moe_i8_layer *L, const void *x, int type, const int32_t
     a.rows = moe::i8_rows(c.hidden);
     a.K = c.intermediate;
     a.chunks = moe::i8_chunks(c.intermediate);
-    r = halves ? moe::launch_grouped<moe::kStoreHalves, moe::kF16>(a, s) : moe::launch_grouped<moe::kStoreRows, moe::kF32>(a, s);
-    if (r != hipSuccess) return r;
-    const moe::I8FoldArgs f{L->contrib, L->m_s, L->expert_scale, ids, L->groups, weights, shared_gate, y,
-                            tokens, c.hidden, c.top_k, c.experts, c.has_shared, error};
+    if ((r = moe::launch_grouped<moe::kStoreRows, moe::kF32>(a, s)) != hipSuccess) return r;
+    const moe::I8FoldArgs f{L->contrib, L->groups, weights, shared_gate, y, tokens, c.hidden, c.top_k, c.experts, c.has_shared, error};
     const dim3 grid(tokens), block(256);
-    if (type == MOE_F32) moe::k_i8_fold<moe::kF32, false><<<grid, block, 0, s>>>(f);
-    else if (halves) moe::k_i8_fold<moe::kBF16, true><<<grid, block, 0, s>>>(f);
-    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16, false><<<grid, block, 0, s>>>(f);
-    else moe::k_i8_fold<moe::kF16, false><<<grid, block, 0, s>>>(f);
+    if (type == MOE_F32) moe::k_i8_fold<moe::kF32><<<grid, block, 0, s>>>(f);
+    else if (type == MOE_BF16) moe::k_i8_fold<moe::kBF16><<<grid, block, 0, s>>>(f);
+    else moe::k_i8_fold<moe::kF16><<<grid, block, 0, s>>>(f);
     return hipGetLastError();
 }
 

@@ -581,11 +581,9 @@ int moe_i8_layer_destroy(moe_i8_layer *layer);
 /* x, y [tokens][H] of `type` (MOE_F32, MOE_BF16, MOE_F16); ids, weights,
  * shared_gate and the sum as in moe_ffn_forward.  x's rows and the experts'
  * middle rows SiLU(gate) * up (the sigmoid within 8 half ulps) are quantised as
- * moe_quantize_i8 does; the weighted sum is fp32, y is rounded once.  With bf16 y
- * and more than 64 tokens an expert's output is held in fp16 with a scale of its own
- * before the sum: off by at most 2^-11 of itself, or by 2^-24 I
- * max |down scale of its expert| times its row's scale.  Otherwise a token's results
- * are the same bits whatever its batch.  Flags in `error` as in moe_ffn_forward: routes
+ * moe_quantize_i8 does; the experts' outputs and their weighted sum are fp32, y is
+ * rounded once.  A token's results are the same bits whatever its batch, and in a
+ * 16-bit type those of the same x in fp32, rounded.  Flags in `error` as in moe_ffn_forward: routes
  * with a bad id or an id of an earlier rank are dropped and set bit 1.  So do
  * nonfinite input, whose token counts as zeros, a negative weight, which stays in
  * the sum, and a nonfinite weight, which gives up the token's routed sum: what is
