@@ -244,6 +244,7 @@ void release(moe_i8_linear *L) {
 }
 
 inline constexpr int kFewElements = moe::kFewVectors * 64 * moe::kFewWaves * 8;   // of x, quantised inside the product
+inline constexpr int kFewOutputs = 16 * 4 * 256;
 
 template<int WR, int WC, int TM, int TN, int S, int KS>
 int launch_gemm(moe::I8Args a, int y_type, hipStream_t s) {
@@ -413,11 +414,21 @@ int moe_i8_linear_apply(moe_i8_linear *L, const void *x, int x_type, int64_t x_s
     };
     const char *xb = static_cast<const char *>(x), *yb = static_cast<const char *>(y);
     const bool apart = xb + extent(x_stride, L->input, x_type) <= yb || yb + extent(y_stride, L->output, y_type) <= xb;
-    // Every workgroup quantises all of the rows: in the product's kernel where each
-    // thread has few vectors of them (us, so / in two launches: 2048 x 2048 at 1, 4, 8
-    // rows 3.8 / 6.1, 4.2 / 6.2, 4.8 / 6.2; 8192 x 8192 at 1, 2 14.7 / 17.2, 15.9 / 16.9;
-    // rows of 2,048 of 8,192 at 4, 8 6.4 / 7.1, 7.5 / 7.3).
-    if (columns <= moe::kFewRows && apart && columns * L->input <= kFewElements) {
+    // Every workgroup (16 outputs) quantises all of the rows: in the product's kernel where
+    // each thread has few vectors of them and all workgroups are on the chip at once (4 a
+    // CU), up to 16,384 outputs; with more than four rows, to 2^26 products.  us, so / in two
+    // launches, bf16:
+    //   outputs                2,048      8,192      16,384     32,768     65,536     151,936
+    //   input 512, 1 row     4.0 / 6.6  4.4 / 6.7  6.0 / 6.5  9.9 / 7.1  16.9 / 9.7  35.3 / 17.2
+    //              4         4.0 / 6.5  4.4 / 6.5  6.1 / 6.4  10.3 / 6.9 17.6 / 9.6  37.5 / 17.5
+    //             16         4.2 / 6.4  5.0 / 6.5  7.3 / 6.5  13.0 / 7.3 22.4 / 10.6 49.6 / 20.1
+    //   2,048,     1         4.1 / 6.6  5.7 / 6.8  8.7 / 9.3  14.4 / 15.1 24.0 / 25.0 49.9 / 49.2
+    //              4         4.4 / 6.4  6.3 / 6.9  9.3 / 9.4  16.5 / 15.3 27.9 / 25.4 59.5 / 50.9
+    //              8         4.9 / 6.5  7.5 / 7.1  11.5 / 9.6 20.1 / 15.7 34.7 / 26.2 75.9 / 53.7
+    //   8,192,     2         8.2 / 12.3 14.7 / 18.2 27.6 / 26.2 45.6 / 46.7 85.9 / 86.5 191 / 193
+    const bool in_one = columns * L->input <= kFewElements && L->output <= kFewOutputs &&
+                        (columns <= 4 || columns * L->input * L->output <= 1 << 26);
+    if (columns <= moe::kFewRows && apart && in_one) {
         const moe::I8FewArgs f = few_args(L, x, x_stride, nullptr, columns, y, y_type, y_stride, error);
         if (x_type == MOE_F32) return moe::launch_few<moe::kF32>(f, s);
         if (x_type == MOE_BF16) return moe::launch_few<moe::kBF16>(f, s);

@@ -1,10 +1,12 @@
 """A token's result from moe_i8_layer_forward: the same bits whatever its batch, and
-in a 16-bit type the fp32 result rounded once."""
+in a 16-bit type the fp32 result rounded once; moe_i8_linear_apply the same where
+it takes one launch and where it takes two."""
 import pytest
 
 import moe_ffn
 
 torch = pytest.importorskip("torch")
+import i8_reference as R  # noqa: E402
 from test_gpu_i8_layer import Case, flag  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +50,21 @@ def test_same_bits_in_every_batch(dtype, h, i, experts, k):
     for n in (1, 16, 33, 64, 65, 100):
         part, e = c.layer.forward(x[:n], c.ids[:n], c.w[:n], shared_gate=c.gate[:n])
         assert flag(e) == 0 and torch.equal(part, whole[:n]), n
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k,m", [(512, 16384), (512, 16385), (2048, 8192), (2048, 8193), (32, 40001), (8192, 8192)])
+def test_few_rows_in_one_launch_or_two(dtype, k, m):
+    """Both sides of the numbers of outputs and rows up to which the product's kernel
+    quantises x itself, with a row that is not finite."""
+    codes, scales = R.weights(1, m, k, m + k)
+    matrix = moe_ffn.MoeI8Linear(k, m, codes[0], scales[0] / 64, max_columns=17)
+    for n in (1, 2, 4, 5, 8, 9, 16, 17):
+        x = torch.randn((n, k), generator=R.generator(n), device=DEV).to(dtype)
+        q, s = R.quantise(x)
+        y, e = matrix.apply(x)
+        assert flag(e) == 0 and torch.equal(y, matrix.forward(q, s, dtype=dtype)), n
+        R.close(y, R.product(q, s, codes[0], scales[0] / 64), dtype)
+        x[n - 1, 17] = float("nan")
+        z, e = matrix.apply(x)
+        assert flag(e) == 1 and not z[n - 1].any() and torch.equal(z[:n - 1], y[:n - 1]), n
