@@ -174,8 +174,8 @@ hipError_t launch_tile(I8Args a, hipStream_t s) {
 //   256 x 128  21.0 / 42.0 / 125 / 172 / 183 / 209 / 179
 // The layer's gate and up, 64 x 32 / 128 x 32 / 128 x 64 / 256 x 128, all of the
 // layer: 128 tokens - / 258 / 262 / 275, 512 - / 313 / 316 / 327, 1,024 - / 353 / 347 / 361,
-// 4,096 - / 688 / 573 / 539; its down (K = 512, an item's start and end weigh more):
-// 128 tokens 271 / 273 / 261 / 269, 512 331 / 328 / 315 / 324, 4,096 688 / 699 / 576 / 519.
+// 4,096 - / 679 / 562 / 529; its down (K = 512, an item's start and end weigh more), 64 x 32 /
+// 128 x 64 / 256 x 128: 128 tokens 274 / 265 / 274, 512 335 / 321 / 329, 4,096 671 / 614 / 530.
 // A few experts: smaller tiles where larger ones leave CUs without any.  Bank of 8
 // such matrices at 100, 300, 1,000 and 4,000 rows, bf16:
 //   64 x 16                          7.7 / 10.7 / 24.1 / 64.2
